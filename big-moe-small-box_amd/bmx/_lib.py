@@ -15,6 +15,7 @@ STAGE_GATE_UP, STAGE_ACT, STAGE_DOWN, STAGE_COMBINE, STAGE_DOWN_OUT, STAGE_PREP 
 STAGE_GATE_UP_RESIDENT, STAGE_GATE_UP_STAGED = 6, 7
 STAGE_ROUTE = 8
 STAGE_DOWN_RESIDENT, STAGE_DOWN_STAGED = 9, 10
+DT_FP16, DT_BF16 = 0, 1
 LANE_VRAM, LANE_ADMIT, LANE_HOME, LANE_CPU = 0, 1, 2, 3
 PLAN_MAXP, PLAN_MAXT = 64, 8
 
@@ -58,6 +59,15 @@ class RouterDesc(ctypes.Structure):
     _fields_ = [("score_fn", ctypes.c_int32), ("renorm", ctypes.c_int32), ("n_group", ctypes.c_int32),
                 ("topk_group", ctypes.c_int32), ("scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("bias", _P),
                 ("weight", _P)]
+
+
+class FfnDesc(ctypes.Structure):
+    _fields_ = [("H", ctypes.c_int32), ("I", ctypes.c_int32), ("dtype", ctypes.c_int32), ("act", ctypes.c_int32),
+                ("act_limit", ctypes.c_float), ("reserved", ctypes.c_int32), ("gate", _P), ("up", _P), ("down", _P)]
+
+
+class FfnSaved(ctypes.Structure):
+    _fields_ = [("g", _P), ("u", _P), ("h", _P)]
 
 
 class Routes(ctypes.Structure):
@@ -120,6 +130,11 @@ SIGNATURES = {
     "bmx_copy_agent_plan_stats": (_I, [_P, _P]),
     "bmx_slot_stage_async": (_I, [_P, _P, _P, _I, _P]),
     "bmx_slot_stage_rows": (_I, [ctypes.POINTER(SlotTable), _I, _P, _I, ctypes.c_uint64, _I, _P]),
+    "bmx_ffn_workspace": (_SZ, [ctypes.POINTER(FfnDesc), _I]),
+    "bmx_ffn_backward_workspace": (_SZ, [ctypes.POINTER(FfnDesc), _I]),
+    "bmx_ffn_forward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, ctypes.POINTER(FfnSaved), _P, _SZ, _P]),
+    "bmx_ffn_add": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, _P, _P, _SZ, _P]),
+    "bmx_ffn_backward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, ctypes.POINTER(FfnSaved), _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "bmx_host_device_ptr": (_I, [_P, ctypes.POINTER(ctypes.c_uint64)]),
 }
 

@@ -1,0 +1,160 @@
+"""GatedFFN: the gated feed-forward block y = act(x Wg^T, x Wu^T) Wd^T outside the routed experts (a model's leading dense
+layers, a shared expert that the checkpoint keeps out of the trellis records), forward and backward, on the HIP library.
+
+The reference runs these modules as exllamav3 MLPs beside its BlockSparseMLP hooks (engine/tiers.py:703-739 wraps the routed
+experts only); here the block is a MoELayer's shared_ffn or a module of its own. Every call enqueues on torch's current
+stream of the input's device; nothing synchronises."""
+import ctypes
+
+import torch
+
+from . import _lib as L
+
+DTYPES = {torch.float16: L.DT_FP16, torch.bfloat16: L.DT_BF16}
+
+
+def rows_of(x, K, dtype, device, name):
+    """x [..., K] as contiguous 16-byte aligned rows [T, K] (a copy only where x is neither)."""
+    if not x.is_cuda or x.device != device:
+        raise ValueError(f"{name}: expected a tensor on {device}, got {x.device}")
+    if x.dtype != dtype:
+        raise ValueError(f"{name}: expected {dtype}, got {x.dtype}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"{name}: expected [..., {K}], got {tuple(x.shape)}")
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
+    if not x.is_contiguous():
+        x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+class on_device:
+    """The call's device as the current one, and its current stream (entered with the stream's handle)."""
+
+    def __init__(self, device):
+        self.device = device
+
+    def __enter__(self):
+        self.ctx = None
+        if torch.cuda.current_device() != self.device.index:
+            self.ctx = torch.cuda.device(self.device)
+            self.ctx.__enter__()
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def __exit__(self, *e):
+        if self.ctx is not None:
+            self.ctx.__exit__(*e)
+
+
+class GatedFFN:
+    """gate, up [I, H] and down [H, I]: contiguous fp16 or bf16 device tensors of one type (H, I multiples of 8); act:
+    ACT_SILU, ACT_GELU (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
+
+    forward(x) -> y, x [..., H] of the weights' type. Where autograd records (x or a weight requires grad), y carries the
+    gradients of x and of the three weights; the forward pass then keeps x, g, u and h ([T, I] each, 16 bits)."""
+
+    def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
+        if gate.dim() != 2 or gate.dtype not in DTYPES:
+            raise ValueError(f"GatedFFN: gate must be fp16 or bf16 [I, H], got {gate.dtype} {tuple(gate.shape)}")
+        I, H = gate.shape
+        for name, w, shape in (("gate", gate, (I, H)), ("up", up, (I, H)), ("down", down, (H, I))):
+            if tuple(w.shape) != shape or w.dtype != gate.dtype or not w.is_cuda or w.device != gate.device:
+                raise ValueError(f"GatedFFN: {name} must be {gate.dtype} {list(shape)} on {gate.device}, got {w.dtype} "
+                                 f"{list(w.shape)} on {w.device}")
+            if not w.is_contiguous() or w.data_ptr() % 16:
+                raise ValueError(f"GatedFFN: {name} must be contiguous and 16-byte aligned")
+        if H <= 0 or I <= 0 or H % 8 or I % 8:
+            raise ValueError(f"GatedFFN: H ({H}) and I ({I}) must be positive multiples of 8")
+        if act not in (L.ACT_SILU, L.ACT_GELU, L.ACT_RELU2, L.ACT_SILU_OAI):
+            raise ValueError(f"GatedFFN: unknown activation {act}")
+        if not act_limit >= 0.0:
+            raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {act_limit}")
+        self.gate, self.up, self.down = gate, up, down
+        self.act, self.act_limit = act, float(act_limit)
+        self.hidden_size, self.intermediate_size = H, I
+        self.dtype, self.device = gate.dtype, gate.device
+
+    def desc(self):
+        return L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0,
+                         self.gate.data_ptr(), self.up.data_ptr(), self.down.data_ptr())
+
+    def _workspace(self, need):
+        if need == 0:
+            L.check(L.BMX_ERR_ARG, "GatedFFN")
+        return torch.empty(need, dtype=torch.uint8, device=self.device)
+
+    def forward(self, x):
+        if torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or self.up.requires_grad or
+                                        self.down.requires_grad):
+            return _GatedFFNFunction.apply(x, self.gate, self.up, self.down, self)
+        return self._forward(x, None)
+
+    __call__ = forward
+
+    def _forward(self, x, keep):
+        """y; keep: a list that receives x's rows and the saved g, u, h."""
+        r = rows_of(x, self.hidden_size, self.dtype, self.device, "GatedFFN: x")
+        T = r.shape[0]
+        y = torch.empty_like(r)
+        saved = None
+        if keep is not None:
+            g, u, h = (torch.empty((T, self.intermediate_size), dtype=self.dtype, device=self.device) for _ in range(3))
+            keep.extend((r, g, u, h))
+            saved = L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr())
+        if T:
+            d, lib = self.desc(), L.lib()
+            with on_device(self.device) as s:
+                ws = self._workspace(lib.bmx_ffn_workspace(d, T))
+                L.check(lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s),
+                        "bmx_ffn_forward")
+        return y if x.dim() == 2 else y.view(x.shape)
+
+    def add_to(self, out, x, gate_vec=None):
+        """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of the weights' type: the block
+        as a layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
+        r = rows_of(x.detach(), self.hidden_size, self.dtype, self.device, "GatedFFN: x")
+        T = r.shape[0]
+        if out.dtype != torch.float32 or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 or \
+                tuple(out.shape) != (T, self.hidden_size):
+            raise ValueError(f"GatedFFN: out must be contiguous fp32 [{T}, {self.hidden_size}] on {self.device}")
+        if gate_vec is not None and (gate_vec.dtype != self.dtype or gate_vec.device != self.device or
+                                     gate_vec.numel() != self.hidden_size or not gate_vec.is_contiguous() or
+                                     gate_vec.data_ptr() % 16):
+            raise ValueError(f"GatedFFN: gate_vec must be a contiguous {self.dtype} tensor of {self.hidden_size} elements")
+        if T:
+            d, lib = self.desc(), L.lib()
+            with on_device(self.device) as s:
+                ws = self._workspace(lib.bmx_ffn_workspace(d, T))
+                L.check(lib.bmx_ffn_add(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None,
+                                        out.data_ptr(), ws.data_ptr(), ws.numel(), s), "bmx_ffn_add")
+        return out
+
+
+class _GatedFFNFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, ffn):
+        keep = []
+        y = ffn._forward(x.detach(), keep)
+        ctx.save_for_backward(gate, up, down, *keep)
+        ctx.act, ctx.act_limit = ffn.act, ffn.act_limit
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        gate, up, down, x, g, u, h = ctx.saved_tensors
+        I, H = gate.shape
+        want = ctx.needs_input_grad
+        T, dev = x.shape[0], x.device
+        r = rows_of(dy, H, gate.dtype, dev, "GatedFFN: the gradient of y")
+        dx = torch.empty_like(x) if want[0] else None
+        dw = [torch.empty_like(w) if n else None for w, n in zip((gate, up, down), want[1:4])]
+        d, lib = L.FfnDesc(H, I, DTYPES[gate.dtype], ctx.act, ctx.act_limit, 0, gate.data_ptr(), up.data_ptr(),
+                           down.data_ptr()), L.lib()
+        ptr = lambda t: t.data_ptr() if t is not None else None
+        with on_device(dev) as s:
+            need = lib.bmx_ffn_backward_workspace(d, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
+            L.check(lib.bmx_ffn_backward(d, ptr(x), T, L.FfnSaved(ptr(g), ptr(u), ptr(h)), ptr(r), ptr(dx), ptr(dw[0]),
+                                         ptr(dw[1]), ptr(dw[2]), ptr(ws), need, s), "bmx_ffn_backward")
+        return dx.view(dy.shape) if dx is not None else None, dw[0], dw[1], dw[2], None

@@ -24,11 +24,23 @@ class MoELayer:
     score (SCORE_SOFTMAX / SCORE_SIGMOID / SCORE_SQRTSP), selection bias fp32 [E], group limit, renorm, scale
     (routed_scaling_factor); activation, gated, act_limit; router_weight: fp16 [E, H] gate weight (checkpoint layout),
     used when no logits are given; shared_gate: fp16 [H] gate vector of the shared expert (its output scaled by
-    sigmoid(x . shared_gate)) or None; slots / li: an ExpertSlots table and this layer's index in it."""
+    sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 weights as the layer's shared expert, for tables
+    without one (shared_gate then scales its output); slots / li: an ExpertSlots table and this layer's index in it."""
 
     def __init__(self, table, topk, first=0, score=L.SCORE_SIGMOID, bias=None, n_group=1, topk_group=1, renorm=True,
                  scale=1.0, act=L.ACT_SILU, gated=True, act_limit=0.0, router_weight=None, slots=None, li=0,
-                 shared_gate=None):
+                 shared_gate=None, shared_ffn=None):
+        if shared_ffn is not None:
+            if table.has_shared:
+                raise ValueError("shared_ffn: the table already has a shared expert")
+            if shared_ffn.hidden_size != table.H or shared_ffn.dtype != torch.float16 or shared_ffn.device != table.device:
+                raise ValueError(f"shared_ffn: expected fp16 weights of H = {table.H} on {table.device}")
+        self.shared_ffn, self.shared_ffn_gate = shared_ffn, None
+        if shared_ffn is not None and shared_gate is not None:
+            if (shared_gate.dtype != torch.float16 or shared_gate.numel() != table.H or not shared_gate.is_cuda or
+                    not shared_gate.is_contiguous()):
+                raise ValueError("shared_gate must be a contiguous fp16 device tensor of H elements")
+            self.shared_ffn_gate, shared_gate = shared_gate, None
         self.table = table
         self.num_experts_per_tok = topk
         self.routing_first = first
@@ -121,6 +133,10 @@ class MoELayer:
         return self._ws
 
     # ---- experts + combine ----
+    def _add_shared(self, out, x):
+        """out += the shared_ffn's output on the rows x, when there is one."""
+        return out if self.shared_ffn is None else self.shared_ffn.add_to(out, x, self.shared_ffn_gate)
+
     def run_bszN(self, z, sel, rw, path=L.PATH_AUTO):
         x = z.view(-1, self.hidden_size)
         if x.dtype != torch.float16 or not x.is_contiguous():
@@ -138,14 +154,14 @@ class MoELayer:
             self._workspace(need)
             self.out_bszn = ops.moe_forward(self.slot_desc, x, sel, rw, path, self._ws)
             self.slots.stage_restore(staged)
-            return self.out_bszn
+            return self._add_shared(self.out_bszn, x)
         if self.slots is not None:
             self.out_bszn = self._run_slots(x, sel, rw, path)
-            return self.out_bszn
+            return self._add_shared(self.out_bszn, x)
         need = L.lib().bmx_moe_workspace(self.desc, x.shape[0], path)
         self._workspace(need)
         self.out_bszn = ops.moe_forward(self.desc, x, sel, rw, path, self._ws)
-        return self.out_bszn
+        return self._add_shared(self.out_bszn, x)
 
     def _run_slots(self, x, sel, rw, path):
         """Expert products with the slot table: gate / up of the experts resident before this layer's step, then (after
@@ -271,7 +287,7 @@ class MoELayer:
             self._workspace(need)
             out, self.sel, self.w = ops.moe_layer(self.desc, self.router, x, lg, path, self._ws)
             self.out_bszn = out
-            return out
+            return self._add_shared(out, x)
         bsz = z.shape[0]
         sel, w = self.routing_fn(bsz, None, z, {"logits": logits} if logits is not None else {})
         sel, w, _ = self.layer(self.li, sel, w, z, bsz)

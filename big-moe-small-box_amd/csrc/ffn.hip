@@ -1,0 +1,316 @@
+// Gated feed-forward block with 16-bit weights: forward, the form that adds to a layer's output, and gradients. The products
+// are gemm16_k's; this file plans tiles and splits, lays out the workspace and checks arguments.
+#include "gemm16.hpp"
+
+namespace bmx {
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+
+static bool dtype_ok(int d) { return d == BMX_DT_FP16 || d == BMX_DT_BF16; }
+
+struct TilePlan { int big, splits; };
+
+// Tiles of a product with M x N results, `products` side by side, nk tiles of K: 256 x 256 where they fill the chip, else
+// 128 x 128, K split (partial sums joined by a second kernel) where even those leave compute units without work.
+static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split)
+{
+    auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b - 1) / b) * products; };
+    TilePlan p = {tiles(256) >= 192, 1};
+    if (p.big || !can_split) return p;
+    const int64_t t = tiles(128);
+    while (p.splits < 16 && t * p.splits * 2 <= 512 && nk / (p.splits * 2) >= 4) p.splits *= 2;
+    return p;
+}
+
+template <class T, bool AX, bool BX, int EPI>
+static int run_gemm(const GemmArgs& a, int big, hipStream_t s)
+{
+    GemmArgs p = a;
+    // EPI_GU: a tile's rows are half gate, half up
+    const int b = big ? 256 : 128, bm = EPI == EPI_GU ? b / 2 : b;
+    p.tm = (a.M + bm - 1) / bm;
+    p.tn = (a.N + b - 1) / b;
+    const dim3 grid((unsigned)(p.tm * p.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * a.batch : a.batch));
+    if (big) hipLaunchKernelGGL((gemm16_k<T, 256, 256, 2, 4, AX, BX, EPI>), grid, dim3(512), 0, s, p);
+    else hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, AX, BX, EPI>), grid, dim3(256), 0, s, p);
+    return check_launch("gemm16");
+}
+
+// One product, split or not; EPI: what becomes of the sums
+template <class T, bool AX, bool BX, int EPI>
+static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
+{
+    if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.big, s);
+    a.splits = tp.splits;
+    GemmArgs g = a;
+    g.batch = EPI == EPI_GU ? 2 : 1;
+    if (EPI == EPI_GU) g.b[1] = g.b[0];
+    int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.big, s);
+    if (rc) return rc;
+    const int64_t quads = (int64_t)a.M * a.N / 4;
+    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
+    return check_launch("gemm_finish");
+}
+
+// s_t = sigmoid(x[t] . v): one wave per token, fp32 sums
+template <class T>
+__global__ __launch_bounds__(256) void row_gate_k(const uint16_t* __restrict__ x, const uint16_t* __restrict__ v, int n, int H,
+                                                  float* __restrict__ out)
+{
+    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (t >= n) return;
+    float sum = 0.0f;
+    for (int k = lane * 8; k < H; k += 512)
+    {
+        const u32x4 a = ldg4(x + (int64_t)t * H + k), b = ldg4(v + k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            sum = __builtin_fmaf(from16<T>((uint16_t)a[i]), from16<T>((uint16_t)b[i]), sum);
+            sum = __builtin_fmaf(from16<T>((uint16_t)(a[i] >> 16)), from16<T>((uint16_t)(b[i] >> 16)), sum);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) out[t] = sigmoid_fixed(sum);
+}
+
+static int tiles_k(int K) { return (K + GK - 1) / GK; }
+
+struct FfnPlan {
+    TilePlan gu, down;
+    size_t h, part, gate, total;       // workspace offsets
+};
+
+static FfnPlan ffn_plan(const bmx_ffn_desc* d, int T)
+{
+    FfnPlan p;
+    p.gu = plan_product(2 * (int64_t)d->I, T, tiles_k(d->H), 1, true);
+    p.down = plan_product(d->H, T, tiles_k(d->I), 1, true);
+    size_t o = 0;
+    auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
+    p.h = take((size_t)T * d->I * 2);
+    p.gate = take((size_t)T * 4);
+    const size_t pg = p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d->I * 4 : 0;
+    const size_t pd = p.down.splits > 1 ? (size_t)p.down.splits * T * d->H * 4 : 0;
+    p.part = take(pg > pd ? pg : pd);
+    p.total = o + 256;
+    return p;
+}
+
+template <class T>
+static int ffn_forward(const bmx_ffn_desc* d, const void* x, int n, void* y, float* add, const void* gate_vec,
+                       const bmx_ffn_saved* sv, char* ws, hipStream_t s)
+{
+    const FfnPlan p = ffn_plan(d, n);
+    void* h = sv ? sv->h : ws + p.h;
+    float* scale = nullptr;
+    if (gate_vec)
+    {
+        scale = reinterpret_cast<float*>(ws + p.gate);
+        hipLaunchKernelGGL((row_gate_k<T>), dim3((n + 3) / 4), dim3(256), 0, s, static_cast<const uint16_t*>(x),
+                           static_cast<const uint16_t*>(gate_vec), n, d->H, scale);
+        const int rc = check_launch("row_gate");
+        if (rc) return rc;
+    }
+    GemmArgs a = {};
+    a.chain = a.batch = a.splits = 1;
+    a.part = reinterpret_cast<float*>(ws + p.part);
+    a.act = act_par(d->act, d->act_limit);
+    a.a[0] = d->gate; a.a[1] = d->up; a.b[0] = x; a.out[0] = h;
+    a.M = d->I; a.N = n; a.K = d->H; a.lda = a.ldb = d->H; a.ldo = d->I;
+    if (sv) { a.g = sv->g; a.u = sv->u; }
+    int rc = product<T, false, false, EPI_GU>(a, p.gu, s);
+    if (rc) return rc;
+    a.a[0] = d->down; a.a[1] = nullptr; a.b[0] = h; a.out[0] = add ? static_cast<void*>(add) : y;
+    a.M = d->H; a.K = d->I; a.lda = a.ldb = d->I; a.ldo = d->H;
+    a.scale = scale;
+    return add ? product<T, false, false, EPI_ADD>(a, p.down, s) : product<T, false, false, EPI_STORE>(a, p.down, s);
+}
+
+struct FfnBackPlan {
+    TilePlan dh, dx, dd, dw;
+    size_t dg, du, part, total;
+};
+
+static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
+{
+    FfnBackPlan p;
+    p.dh = plan_product(d->I, T, tiles_k(d->H), 1, true);
+    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true);
+    p.dd = plan_product(d->I, d->H, tiles_k(T), 1, false);
+    p.dw = plan_product(d->H, d->I, tiles_k(T), 2, false);
+    size_t o = 0;
+    auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
+    p.dg = take((size_t)T * d->I * 2);
+    p.du = take((size_t)T * d->I * 2);
+    const size_t ph = p.dh.splits > 1 ? (size_t)p.dh.splits * T * d->I * 4 : 0;
+    const size_t px = p.dx.splits > 1 ? (size_t)p.dx.splits * T * d->H * 4 : 0;
+    p.part = take(ph > px ? ph : px);
+    p.total = o + 256;
+    return p;
+}
+
+template <class T>
+static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_ffn_saved* sv, const void* dy, void* dx,
+                        void* dgate, void* dup, void* ddown, char* ws, hipStream_t s)
+{
+    const FfnBackPlan p = ffn_back_plan(d, n);
+    const int H = d->H, I = d->I;
+    GemmArgs z = {};
+    z.chain = z.batch = z.splits = 1;
+    z.part = reinterpret_cast<float*>(ws + p.part);
+    z.act = act_par(d->act, d->act_limit);
+    int rc = BMX_OK;
+    if (dx || dgate || dup)
+    {
+        GemmArgs a = z;                                            // dh = dy Wd, then dg, du
+        a.a[0] = d->down; a.b[0] = dy; a.out[0] = ws + p.dg; a.out[1] = ws + p.du;
+        a.g = sv->g; a.u = sv->u;
+        a.M = I; a.N = n; a.K = H; a.lda = I; a.ldb = H; a.ldo = I;
+        rc = product<T, true, false, EPI_DGU>(a, p.dh, s);
+    }
+    if (!rc && dx)
+    {
+        GemmArgs a = z;                                            // dx = dg Wg + du Wu
+        a.a[0] = d->gate; a.a[1] = d->up; a.b[0] = ws + p.dg; a.b[1] = ws + p.du; a.out[0] = dx;
+        a.chain = 2;
+        a.M = H; a.N = n; a.K = I; a.lda = H; a.ldb = I; a.ldo = H;
+        rc = product<T, true, false, EPI_STORE>(a, p.dx, s);
+    }
+    if (!rc && ddown)
+    {
+        GemmArgs a = z;                                            // dWd = dy^T h
+        a.a[0] = sv->h; a.b[0] = dy; a.out[0] = ddown;
+        a.M = I; a.N = H; a.K = n; a.lda = I; a.ldb = H; a.ldo = I;
+        rc = product<T, true, true, EPI_STORE>(a, p.dd, s);
+    }
+    if (!rc && (dgate || dup))
+    {
+        GemmArgs a = z;                                            // dWg = dg^T x, dWu = du^T x
+        a.batch = dgate && dup ? 2 : 1;
+        a.a[0] = a.a[1] = x;
+        a.b[0] = dgate ? ws + p.dg : ws + p.du; a.out[0] = dgate ? dgate : dup;
+        a.b[1] = ws + p.du; a.out[1] = dup;
+        a.M = H; a.N = I; a.K = n; a.lda = H; a.ldb = I; a.ldo = H;
+        rc = product<T, true, true, EPI_STORE>(a, p.dw, s);
+    }
+    return rc;
+}
+
+// ---- argument checks ----------------------------------------------------------------------------------------------------
+
+static bool odd16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; }
+
+static int check_ffn(const bmx_ffn_desc* d, int T, const char* who)
+{
+    if (!d) return set_error(BMX_ERR_ARG, "%s: null descriptor", who);
+    if (d->H <= 0 || d->I <= 0 || d->H % 8 || d->I % 8 || d->H > (1 << 20) || d->I > (1 << 20))
+        return set_error(BMX_ERR_ARG, "%s: H (%d) and I (%d) must be positive multiples of 8, at most 2^20", who, d->H, d->I);
+    if (!dtype_ok(d->dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", who, d->dtype);
+    if (d->act < BMX_ACT_SILU || d->act > BMX_ACT_SILU_OAI) return set_error(BMX_ERR_ARG, "%s: unknown activation %d", who, d->act);
+    if (!(d->act_limit >= 0.0f)) return set_error(BMX_ERR_ARG, "%s: act_limit must be 0 (off) or positive", who);
+    if (!d->gate || !d->up || !d->down) return set_error(BMX_ERR_ARG, "%s: null weight pointer", who);
+    if (odd16(d->gate) || odd16(d->up) || odd16(d->down)) return set_error(BMX_ERR_ARG, "%s: weights must be 16-byte aligned", who);
+    // launch sizes: the tiles of a product are one grid dimension
+    if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", who, T);
+    return BMX_OK;
+}
+
+static int check_saved(const bmx_ffn_saved* sv, const char* who)
+{
+    if (!sv->g || !sv->u || !sv->h || odd16(sv->g) || odd16(sv->u) || odd16(sv->h))
+        return set_error(BMX_ERR_ARG, "%s: g, u and h must be 16-byte aligned device arrays", who);
+    return BMX_OK;
+}
+
+static int check_ws(const void* ws, size_t have, size_t need, const char* who)
+{
+    if (!ws || odd16(ws)) return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", who);
+    if (have < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", who, have, need);
+    return BMX_OK;
+}
+
+template <class T> __global__ __launch_bounds__(256) void zero16_k(u32x4* p, int64_t n)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = u32x4{0, 0, 0, 0};
+}
+
+}  // namespace bmx
+
+using namespace bmx;
+
+extern "C" {
+
+size_t bmx_ffn_workspace(const bmx_ffn_desc* desc, int T)
+{
+    if (check_ffn(desc, T, "bmx_ffn_workspace")) return 0;
+    return ffn_plan(desc, T).total;
+}
+
+size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T)
+{
+    if (check_ffn(desc, T, "bmx_ffn_backward_workspace")) return 0;
+    return ffn_back_plan(desc, T).total;
+}
+
+int bmx_ffn_forward(const bmx_ffn_desc* desc, const void* x, int T, void* y, const bmx_ffn_saved* saved, void* workspace,
+                    size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_ffn_forward";
+    int rc = check_ffn(desc, T, fn);
+    if (rc || T == 0) return rc;
+    if (!x || !y || odd16(x) || odd16(y)) return set_error(BMX_ERR_ARG, "%s: x or y null or not 16-byte aligned", fn);
+    if (saved && (rc = check_saved(saved, fn))) return rc;
+    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(desc, T).total, fn))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    return desc->dtype == BMX_DT_FP16 ? ffn_forward<f16>(desc, x, T, y, nullptr, nullptr, saved, ws, s)
+                                      : ffn_forward<bf16>(desc, x, T, y, nullptr, nullptr, saved, ws, s);
+}
+
+int bmx_ffn_add(const bmx_ffn_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
+                size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_ffn_add";
+    int rc = check_ffn(desc, T, fn);
+    if (rc || T == 0) return rc;
+    if (!x || !out || odd16(x) || odd16(out)) return set_error(BMX_ERR_ARG, "%s: x or out null or not 16-byte aligned", fn);
+    if (odd16(gate_vec)) return set_error(BMX_ERR_ARG, "%s: gate_vec not 16-byte aligned", fn);
+    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(desc, T).total, fn))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    return desc->dtype == BMX_DT_FP16 ? ffn_forward<f16>(desc, x, T, nullptr, out, gate_vec, nullptr, ws, s)
+                                      : ffn_forward<bf16>(desc, x, T, nullptr, out, gate_vec, nullptr, ws, s);
+}
+
+int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_ffn_saved* saved, const void* dy, void* dx,
+                     void* dgate, void* dup, void* ddown, void* workspace, size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_ffn_backward";
+    int rc = check_ffn(desc, T, fn);
+    if (rc) return rc;
+    if (odd16(dx) || odd16(dgate) || odd16(dup) || odd16(ddown)) return set_error(BMX_ERR_ARG, "%s: gradients must be 16-byte aligned", fn);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (T == 0)
+    {
+        const int64_t n = (int64_t)desc->H * desc->I / 8;
+        for (void* w : {dgate, dup, ddown})
+            if (w)
+            {
+                hipLaunchKernelGGL((zero16_k<f16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, static_cast<u32x4*>(w), n);
+                if ((rc = check_launch(fn))) return rc;
+            }
+        return BMX_OK;
+    }
+    if (!x || !dy || odd16(x) || odd16(dy)) return set_error(BMX_ERR_ARG, "%s: x or dy null or not 16-byte aligned", fn);
+    if (!saved) return set_error(BMX_ERR_ARG, "%s: needs the forward pass's saved values", fn);
+    if ((rc = check_saved(saved, fn))) return rc;
+    if ((rc = check_ws(workspace, workspace_bytes, ffn_back_plan(desc, T).total, fn))) return rc;
+    char* ws = static_cast<char*>(workspace);
+    return desc->dtype == BMX_DT_FP16 ? ffn_backward<f16>(desc, x, T, saved, dy, dx, dgate, dup, ddown, ws, s)
+                                      : ffn_backward<bf16>(desc, x, T, saved, dy, dx, dgate, dup, ddown, ws, s);
+}
+
+}  // extern "C"

@@ -1,0 +1,362 @@
+// Tiled 16-bit matrix product for gfx950: D[n][m] = sum_k A(m, k) B(n, k), the products of the gated feed-forward block and
+// of its gradients (many tokens). A is the side whose index m is contiguous in the result's rows, so that a lane's four
+// neighbouring accumulators are four neighbouring values of one row.
+//
+// An operand is stored [rows][K] ("along K": weights of a forward product, activations) or [K][rows] ("across K": weights of
+// a product with their transpose, both sides of a weight gradient). Either way its tile goes from HBM to LDS by 16-byte
+// direct loads in the order in which it lies in memory; operands across K are transposed on the way to registers by
+// ds_read_b64_tr_b16. Rows and columns outside the matrices come from the buffer range check as zeros (last rows) or hold
+// neighbouring data whose results are never stored.
+#pragma once
+#include "ffn_act.hpp"
+#include "bmx_internal.hpp"
+
+typedef __bf16 bf16;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+namespace bmx {
+
+template <class T> struct Elem;
+template <> struct Elem<f16>
+{
+    typedef f16x8 v8;
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <> struct Elem<bf16>
+{
+    typedef bf16x8 v8;
+    static __device__ __forceinline__ f32x16 mfma32(v8 a, v8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ f32x4 mfma16(v8 a, v8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// 16-bit value of an fp32 one (round to nearest even) and back, as bits
+template <class T> __device__ __forceinline__ uint16_t to16(float v) { return __builtin_bit_cast(uint16_t, (T)v); }
+template <class T> __device__ __forceinline__ float from16(uint16_t b) { return (float)__builtin_bit_cast(T, b); }
+
+// What a product does with its sums
+enum GemmEpi {
+    EPI_STORE = 0,   // out[n][m], 16 bits
+    EPI_ADD = 1,     // out32[n][m] += scale[n] * sum
+    EPI_PART = 2,    // part[matrix * splits + split][n][m] fp32: K in several splits, joined by gemm_finish_k
+    EPI_GU = 3,      // the rows of A are gate and up rows in turn by 32: h = act(g, u) (and g, u for a backward pass)
+    EPI_DGU = 4,     // the sum is dh: dg = dh dh/dg, du = dh dh/du from the saved g, u
+};
+
+struct GemmArgs {
+    const void* a[2];       // second: the up matrix (EPI_GU), or the second product of a chain or batch
+    const void* b[2];
+    void* out[2];
+    int M, N, K;            // M: rows of A (EPI_GU: of each of its two matrices), N: rows of B
+    int lda, ldb, ldo;      // elements
+    int chain;              // 2: the two products are summed
+    int batch;              // 2: two products side by side (grid z)
+    int splits;             // of K (EPI_PART; grid z = product * splits + split)
+    int tm, tn;             // tiles along M and N
+    float* part;
+    const float* scale;     // EPI_ADD: [N] or null
+    ActPar act;
+    void *g, *u;            // EPI_GU: saved when not null; EPI_DGU: read
+};
+
+typedef __attribute__((address_space(3))) char* lds_ptr;
+
+template <class T> __device__ __forceinline__ u32x2 pack4(const f32x4 v)
+{
+    u32x2 w;
+    w[0] = (uint32_t)to16<T>(v[0]) | ((uint32_t)to16<T>(v[1]) << 16);
+    w[1] = (uint32_t)to16<T>(v[2]) | ((uint32_t)to16<T>(v[3]) << 16);
+    return w;
+}
+
+// What becomes of four neighbouring sums of a result row, at element o of the outputs
+template <class T> __device__ __forceinline__ void store_4(const GemmArgs& p, void* out, int64_t o, const f32x4 v)
+{
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + o) = pack4<T>(v);
+}
+
+__device__ __forceinline__ void add_4(const GemmArgs& p, int64_t o, int n, const f32x4 v)
+{
+    const float sc = p.scale ? p.scale[n] : 1.0f;
+    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p.out[0]) + o);
+    f32x4 c = *q;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(sc, v[t], c[t]);
+    *q = c;
+}
+
+template <class T> __device__ __forceinline__ void gu_4(const GemmArgs& p, int64_t o, const f32x4 g, const f32x4 u)
+{
+    f32x4 h;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) h[t] = act_h(p.act, g[t], u[t]);
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[0]) + o) = pack4<T>(h);
+    if (p.g)
+    {
+        uint16_t gb[4], ub[4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) save_gu<T>(p.act, g[t], u[t], gb[t], ub[t]);
+        u32x2 w;
+        w[0] = gb[0] | ((uint32_t)gb[1] << 16); w[1] = gb[2] | ((uint32_t)gb[3] << 16);
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.g) + o) = w;
+        w[0] = ub[0] | ((uint32_t)ub[1] << 16); w[1] = ub[2] | ((uint32_t)ub[3] << 16);
+        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.u) + o) = w;
+    }
+}
+
+template <class T> __device__ __forceinline__ void dgu_4(const GemmArgs& p, int64_t o, const f32x4 dh)
+{
+    const u32x2 gw = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.g) + o);
+    const u32x2 uw = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.u) + o);
+    f32x4 dg, du;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+    {
+        float hg, hu;
+        act_grad(p.act, from16<T>((uint16_t)(gw[t >> 1] >> ((t & 1) * 16))), from16<T>((uint16_t)(uw[t >> 1] >> ((t & 1) * 16))), hg, hu);
+        dg[t] = dh[t] * hg;
+        du[t] = dh[t] * hu;
+    }
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[0]) + o) = pack4<T>(dg);
+    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[1]) + o) = pack4<T>(du);
+}
+
+// ---- tiles --------------------------------------------------------------------------------------------------------------
+constexpr int GK = 64;      // K of a tile
+
+// LDS position of 16-byte chunk c of row r. Along K: a row is 64 values = 8 chunks; 16 rows at one chunk (a fragment read)
+// fall on 16 different 16-byte columns of the 64 banks. Across K: a row is W values; the 4 rows x 32 bytes that 16 lanes
+// read for a transposition fall on different banks, and so do those of rows 8 further (the next 16 lanes).
+__device__ __forceinline__ int swz_along(int r) { return (r >> 1) & 7; }
+__device__ __forceinline__ int swz_across(int r) { return ((r & 3) | ((r >> 1) & 4)) << 1; }
+
+// One operand's tile of ROWS rows x GK, loaded by NT threads. ACROSS: stored [K][rows].
+template <int ROWS, int NT, bool ACROSS>
+struct TileLoader {
+    static constexpr int INSTR = ROWS * GK * 2 / (NT * 16);
+    static constexpr int CPR = ACROSS ? ROWS / 8 : GK / 8;         // chunks of an LDS row
+    static constexpr int RPI = NT / CPR;                           // LDS rows of one load of all threads
+    uint32_t voff;      // of this lane's chunk in the first load (bytes from the tile's base)
+    uint32_t step;      // from one load to the next
+    int chunk;          // ... its column chunk in the matrix
+    __device__ __forceinline__ void init(int ld)
+    {
+        const int r = threadIdx.x / CPR, p = threadIdx.x % CPR;
+        chunk = p ^ (ACROSS ? swz_across(r) : swz_along(r));
+        voff = (uint32_t)r * ld * 2 + chunk * 16;
+        step = (uint32_t)RPI * ld * 2;
+        static_assert(RPI % 16 == 0 || ACROSS, "rows of later loads are swizzled as the first's");
+    }
+};
+
+template <class T, int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
+{
+    constexpr int NT = WM * WN * 64;
+    constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
+    constexpr int ABYTES = BM * GK * 2, BBYTES = BN * GK * 2;
+    typedef typename Elem<T>::v8 v8;
+    __shared__ __attribute__((aligned(1024))) char lds[2 * (ABYTES + BBYTES)];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+
+    // Tiles in an order that keeps an XCD (workgroups are dealt to the 8 XCDs in turn) on neighbouring tiles: each XCD takes
+    // one contiguous run, and a run walks N within groups of 8 tiles of M, so that its L2 holds the rows it shares
+    const int nwg = p.tm * p.tn;
+    int id = blockIdx.x;
+    {
+        const int q = nwg / 8, r = nwg % 8, x = id & 7;
+        id = x * q + (x < r ? x : r) + (id >> 3);
+    }
+    constexpr int GRP = 8;
+    const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
+    const int tm = g0 + (id % per) % gn, tn = (id % per) / gn;
+    const int m0 = EPI == EPI_GU ? tm * (BM / 2) : tm * BM, n0 = tn * BN;
+    const int z = blockIdx.z;
+
+    const int nk1 = (p.K + GK - 1) / GK;                           // K tiles of one product
+    int kt = 0, kt_end = nk1 * p.chain;
+    const int prod = EPI == EPI_PART ? z / p.splits : z;           // which of the products side by side
+    if (EPI == EPI_PART)
+    {
+        const int q = kt_end / p.splits, r = kt_end % p.splits, sp = z - prod * p.splits;
+        kt = sp * q + min(sp, r);
+        kt_end = kt + q + (sp < r);
+    }
+
+    TileLoader<BM, NT, AX> la;
+    TileLoader<BN, NT, BX> lb;
+    la.init(p.lda);
+    lb.init(p.ldb);
+
+    // Range of a tile's loads: the bytes from its first element to the matrix's last, at most 1 GiB (a tile spans half of
+    // that at the widest rows the entries take). Offsets past it load zeros; OUT is past any range.
+    constexpr uint32_t OUT = 0x7ffffff0u;
+    auto rsrc = [](const void* base, int64_t first, int64_t total) {
+        const int64_t left = (total - first) * 2;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + first * 2, 0,
+                                                 (int)(left < 0 ? 0 : left > 0x40000000 ? 0x40000000 : left), 0x00020000);
+    };
+    auto load_tile = [&](int t, int buf) {
+        const int second = t >= nk1;                                // of a chain
+        const int pi = prod | second;
+        const int k0 = (second ? t - nk1 : t) * GK;
+        lds_ptr base = (lds_ptr)lds + buf * (ABYTES + BBYTES) + wave * 1024;
+        const int tail = p.K - k0;                                  // < GK: the last tile along K
+#pragma unroll
+        for (int j = 0; j < la.INSTR; ++j)
+        {
+            uint32_t v;
+            __amdgpu_buffer_rsrc_t r;
+            if (EPI == EPI_GU)
+            {
+                // this load's rows (8 of one wave) lie in one block of 32, of the gate or of the up matrix
+                const int row = j * la.RPI + wave * 8, blk = row >> 5;
+                const int mi = (blk >> 1) * 32 + (row & 31);        // its first row within the tile's BM / 2
+                r = rsrc(p.a[blk & 1], (int64_t)(m0 + mi) * p.lda + k0, (int64_t)p.M * p.lda);
+                v = la.voff - (uint32_t)(wave * 8) * p.lda * 2;
+            }
+            else
+            {
+                r = AX ? rsrc(p.a[pi], (int64_t)k0 * p.lda + m0, (int64_t)p.K * p.lda)
+                       : rsrc(p.a[pi], (int64_t)m0 * p.lda + k0, (int64_t)p.M * p.lda);
+                v = la.voff + j * la.step;
+            }
+            if (!AX && tail < GK) v = la.chunk * 8 < tail ? v : OUT;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(base + j * NT * 16), 16, v, 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < lb.INSTR; ++j)
+        {
+            const __amdgpu_buffer_rsrc_t r = BX ? rsrc(p.b[pi], (int64_t)k0 * p.ldb + n0, (int64_t)p.K * p.ldb)
+                                                : rsrc(p.b[pi], (int64_t)n0 * p.ldb + k0, (int64_t)p.N * p.ldb);
+            uint32_t v = lb.voff + j * lb.step;
+            if (!BX && tail < GK) v = lb.chunk * 8 < tail ? v : OUT;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(base + ABYTES + j * NT * 16), 16, v, 0, 0, 0);
+        }
+    };
+
+    // A fragment (32 rows from row0, 16 of K from ks * 16): lane l holds row l % 32, K (l / 32) * 8 .. + 7
+    auto frag = [&](lds_ptr tile, int row0, int ks, bool across, int rows) -> v8 {
+        if (!across)
+        {
+            const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
+            return *(__attribute__((address_space(3))) v8*)(tile + r * (GK * 2) + ((c ^ swz_along(r)) << 4));
+        }
+        s16x8 v;
+        const int m = lane & 15, c = (row0 + ((lane >> 4) & 1) * 16 + (m & 3) * 4) >> 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            const int k = ks * 16 + (lane >> 5) * 8 + i * 4 + (m >> 2);
+            const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) s16x4*)(tile + k * (rows * 2) + ((c ^ swz_across(k)) << 4) + (m & 1) * 8));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[i * 4 + e] = t[e];
+        }
+        return __builtin_bit_cast(v8, v);
+    };
+
+    f32x16 acc[MF][NF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+
+    load_tile(kt, 0);
+    for (int buf = 0; kt < kt_end; ++kt, buf ^= 1)
+    {
+        __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt 0: this wave's loads of tile kt are in LDS
+        __syncthreads();                                            // everyone's are, and the other half is read
+        if (kt + 1 < kt_end) load_tile(kt + 1, buf ^ 1);
+        lds_ptr at = (lds_ptr)lds + buf * (ABYTES + BBYTES), bt = at + ABYTES;
+#pragma unroll
+        for (int ks = 0; ks < GK / 16; ++ks)
+        {
+            v8 a[MF], b[NF];
+#pragma unroll
+            for (int i = 0; i < MF; ++i) a[i] = frag(at, wm * (BM / WM) + i * 32, ks, AX, BM);
+#pragma unroll
+            for (int j = 0; j < NF; ++j) b[j] = frag(bt, wn * (BN / WN) + j * 32, ks, BX, BN);
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[i][j] = Elem<T>::mfma32(a[i], b[j], acc[i][j]);
+        }
+    }
+
+    // ---- results: lane l holds column n = l % 32 and rows m = (e / 4) * 8 + (l / 32) * 4 + e % 4 of a fragment ----
+    const int ml = (lane >> 5) * 4, nl = lane & 31;
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+    {
+        const int n = n0 + wn * (BN / WN) + j * 32 + nl;
+        if (n >= p.N) continue;
+        if (EPI == EPI_GU)
+        {
+#pragma unroll
+            for (int i = 0; i < MF; i += 2)
+#pragma unroll
+                for (int e = 0; e < 16; e += 4)
+                {
+                    const int m = m0 + (wm * (BM / WM) + i * 32) / 2 + e * 2 + ml;
+                    if (m >= p.M) continue;                         // M % 8 == 0: four values are in or out together
+                    const f32x4 g = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                    const f32x4 u = {acc[i + 1][j][e], acc[i + 1][j][e + 1], acc[i + 1][j][e + 2], acc[i + 1][j][e + 3]};
+                    gu_4<T>(p, (int64_t)n * p.ldo + m, g, u);
+                }
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+            {
+                const int m = m0 + wm * (BM / WM) + i * 32 + e * 2 + ml;
+                if (m >= p.M) continue;
+                const int64_t o = (int64_t)n * p.ldo + m;
+                const f32x4 v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+                if (EPI == EPI_PART) *reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.M + m) = v;
+                else if (EPI == EPI_ADD) add_4(p, o, n, v);
+                else if (EPI == EPI_DGU) dgu_4<T>(p, o, v);
+                else store_4<T>(p, p.out[prod], o, v);
+            }
+    }
+}
+
+// The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Four values per thread.
+template <class T, int EPI>
+__global__ __launch_bounds__(256) void gemm_finish_k(const GemmArgs p)
+{
+    const int64_t quads = (int64_t)p.N * p.M / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= quads) return;
+    const int64_t at = i * 4, plane = (int64_t)p.N * p.M;
+    const int n = (int)(at / p.M), m = (int)(at % p.M);
+    auto sum = [&](int prod) {
+        const float* q = p.part + prod * p.splits * plane + at;
+        f32x4 v = ldg4f(q);
+        for (int s = 1; s < p.splits; ++s)
+        {
+            const f32x4 w = ldg4f(q + s * plane);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) v[t] += w[t];
+        }
+        return v;
+    };
+    const int64_t o = (int64_t)n * p.ldo + m;
+    if (EPI == EPI_GU)
+    {
+        const f32x4 g = sum(0), u = sum(1);
+        gu_4<T>(p, o, g, u);
+    }
+    else if (EPI == EPI_ADD) add_4(p, o, n, sum(0));
+    else if (EPI == EPI_DGU) dgu_4<T>(p, o, sum(0));
+    else store_4<T>(p, p.out[0], o, sum(0));
+}
+
+}  // namespace bmx

@@ -463,6 +463,42 @@ int bmx_host_device_ptr(void* host, uint64_t* device_addr);
 int bmx_combine(const float* y_rows, const int32_t* inv, const void* w_fp16, const int32_t* offsets, int T, int topk,
                 int H, int E, int has_shared, float* out, bmx_stream_t stream);
 
+/* ---- gated feed-forward block ----
+ * y = act(x Wg^T, x Wu^T) Wd^T, the feed-forward block that checkpoints keep outside the routed experts' trellis records: a
+ * model's leading dense layers, or a layer's shared expert in 16 bits. x, y [T, H]; gate, up [I, H]; down [H, I]; row-major,
+ * contiguous, all of type dtype, 16-byte aligned; H and I multiples of 8; any T >= 0. act, act_limit as the routed experts'
+ * (enum bmx_act; h = min(act(g), limit) * clamp(u, +-limit), or for BMX_ACT_SILU_OAI the clamps first and (u + 1);
+ * act_limit 0 = off, else positive). Products accumulate in fp32; h = act(g, u) is rounded once to dtype between the two
+ * products, y once at the end. NaN and infinities pass through. */
+enum bmx_dtype { BMX_DT_FP16 = 0, BMX_DT_BF16 = 1 };
+typedef struct bmx_ffn_desc {
+    int32_t H, I;
+    int32_t dtype;
+    int32_t act;
+    float act_limit;
+    int32_t reserved;
+    const void *gate, *up, *down;    /* device */
+} bmx_ffn_desc;
+/* What a forward pass keeps for the backward pass: g, u, h [T, I] of dtype, device, 16-byte aligned. Values of g and u
+ * beyond a clamp are kept only as being beyond it. */
+typedef struct bmx_ffn_saved { void *g, *u, *h; } bmx_ffn_saved;
+/* Workspace bytes of the calls below for up to T tokens (0 and an error text when the descriptor is refused). */
+size_t bmx_ffn_workspace(const bmx_ffn_desc* desc, int T);
+size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T);
+/* y [T, H]; saved NULL: nothing kept. */
+int bmx_ffn_forward(const bmx_ffn_desc* desc, const void* x, int T, void* y, const bmx_ffn_saved* saved, void* workspace,
+                    size_t workspace_bytes, bmx_stream_t stream);
+/* out[t] += s_t * y[t] in fp32 (out fp32 [T, H]: a layer call's output): the block as a layer's shared expert. gate_vec NULL:
+ * s = 1; else dtype [H], 16-byte aligned: s_t = sigmoid(x[t] . gate_vec) (the gated shared expert, bmx_moe_desc.shared_gate). y
+ * is not rounded to dtype. */
+int bmx_ffn_add(const bmx_ffn_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
+                size_t workspace_bytes, bmx_stream_t stream);
+/* Gradients from dy [T, H] and a forward pass's x and saved values: dx [T, H], dgate, dup [I, H], ddown [H, I], of dtype,
+ * each NULL when it is not wanted (its products are then not computed). The gradient of h's two factors is rounded to
+ * dtype before the products that use it. T = 0: the wanted weight gradients are zeroed. */
+int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_ffn_saved* saved, const void* dy, void* dx,
+                     void* dgate, void* dup, void* ddown, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
