@@ -66,6 +66,16 @@ class FfnDesc(ctypes.Structure):
                 ("act_limit", ctypes.c_float), ("reserved", ctypes.c_int32), ("gate", _P), ("up", _P), ("down", _P)]
 
 
+class Q4(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_int32), ("K", ctypes.c_int32), ("group", ctypes.c_int32), ("scale_dtype", ctypes.c_int32),
+                ("codes", _P), ("scale", _P), ("zero", _P)]
+
+
+class Ffn4Desc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("act_limit", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("gate", ctypes.POINTER(Q4)), ("up", ctypes.POINTER(Q4)), ("down", ctypes.POINTER(Q4))]
+
+
 class FfnSaved(ctypes.Structure):
     _fields_ = [("g", _P), ("u", _P), ("h", _P)]
 
@@ -130,6 +140,15 @@ SIGNATURES = {
     "bmx_copy_agent_plan_stats": (_I, [_P, _P]),
     "bmx_slot_stage_async": (_I, [_P, _P, _P, _I, _P]),
     "bmx_slot_stage_rows": (_I, [ctypes.POINTER(SlotTable), _I, _P, _I, ctypes.c_uint64, _I, _P]),
+    "bmx_q4_code_bytes": (_SZ, [_I, _I]),
+    "bmx_q4_group_count": (_SZ, [_I, _I, _I]),
+    "bmx_q4_pack": (_I, [ctypes.POINTER(Q4), _P, _P, _P, _P]),
+    "bmx_q4_dequant": (_I, [ctypes.POINTER(Q4), _I, _P, _P]),
+    "bmx_q4_linear_workspace": (_SZ, [ctypes.POINTER(Q4), _I]),
+    "bmx_q4_linear": (_I, [ctypes.POINTER(Q4), _I, _P, _I, _P, _P, _SZ, _P]),
+    "bmx_ffn4_workspace": (_SZ, [ctypes.POINTER(Ffn4Desc), _I]),
+    "bmx_ffn4_forward": (_I, [ctypes.POINTER(Ffn4Desc), _P, _I, _P, _P, _SZ, _P]),
+    "bmx_ffn4_add": (_I, [ctypes.POINTER(Ffn4Desc), _P, _I, _P, _P, _P, _SZ, _P]),
     "bmx_ffn_workspace": (_SZ, [ctypes.POINTER(FfnDesc), _I]),
     "bmx_ffn_backward_workspace": (_SZ, [ctypes.POINTER(FfnDesc), _I]),
     "bmx_ffn_forward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, ctypes.POINTER(FfnSaved), _P, _SZ, _P]),

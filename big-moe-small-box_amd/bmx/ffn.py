@@ -47,13 +47,38 @@ class on_device:
 
 
 class GatedFFN:
-    """gate, up [I, H] and down [H, I]: contiguous fp16 or bf16 device tensors of one type (H, I multiples of 8); act:
-    ACT_SILU, ACT_GELU (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
+    """gate, up [I, H] and down [H, I]: contiguous fp16 or bf16 device tensors of one type (H, I multiples of 8), or three
+    Q4Matrix (gate and up of one group size; x may then be fp16 or bf16, and there are no gradients); act: ACT_SILU, ACT_GELU
+    (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
 
     forward(x) -> y, x [..., H] of the weights' type. Where autograd records (x or a weight requires grad), y carries the
     gradients of x and of the three weights; the forward pass then keeps x, g, u and h ([T, I] each, 16 bits)."""
 
     def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
+        self.quantized = not any(torch.is_tensor(w) for w in (gate, up, down))
+        if self.quantized:
+            I, H = gate.N, gate.K
+            for name, q, shape in (("gate", gate, (I, H)), ("up", up, (I, H)), ("down", down, (H, I))):
+                if (q.N, q.K) != shape or q.device != gate.device:
+                    raise ValueError(f"GatedFFN: {name} must be {list(shape)} on {gate.device}, got {[q.N, q.K]} on {q.device}")
+            if gate.group != up.group:
+                raise ValueError(f"GatedFFN: gate and up must have groups of one size, got {gate.group} and {up.group}")
+        else:
+            I, H = self._check_tensors(gate, up, down)
+        if act not in (L.ACT_SILU, L.ACT_GELU, L.ACT_RELU2, L.ACT_SILU_OAI):
+            raise ValueError(f"GatedFFN: unknown activation {act}")
+        if not act_limit >= 0.0:
+            raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {act_limit}")
+        self.gate, self.up, self.down = gate, up, down
+        self.act, self.act_limit = act, float(act_limit)
+        self.hidden_size, self.intermediate_size = H, I
+        self.device = gate.device
+        self.dtype = None if self.quantized else gate.dtype      # None: the input's
+
+    @staticmethod
+    def _check_tensors(gate, up, down):
+        if not all(torch.is_tensor(w) for w in (gate, up, down)):
+            raise ValueError("GatedFFN: three tensors or three Q4Matrix")
         if gate.dim() != 2 or gate.dtype not in DTYPES:
             raise ValueError(f"GatedFFN: gate must be fp16 or bf16 [I, H], got {gate.dtype} {tuple(gate.shape)}")
         I, H = gate.shape
@@ -65,18 +90,20 @@ class GatedFFN:
                 raise ValueError(f"GatedFFN: {name} must be contiguous and 16-byte aligned")
         if H <= 0 or I <= 0 or H % 8 or I % 8:
             raise ValueError(f"GatedFFN: H ({H}) and I ({I}) must be positive multiples of 8")
-        if act not in (L.ACT_SILU, L.ACT_GELU, L.ACT_RELU2, L.ACT_SILU_OAI):
-            raise ValueError(f"GatedFFN: unknown activation {act}")
-        if not act_limit >= 0.0:
-            raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {act_limit}")
-        self.gate, self.up, self.down = gate, up, down
-        self.act, self.act_limit = act, float(act_limit)
-        self.hidden_size, self.intermediate_size = H, I
-        self.dtype, self.device = gate.dtype, gate.device
+        return I, H
 
-    def desc(self):
+    def desc(self, dtype=None):
+        """The call descriptor for an input of dtype (default: the weights')."""
+        if self.quantized:
+            ref = lambda q: ctypes.pointer(q.struct)
+            return L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up), ref(self.down))
         return L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0,
                          self.gate.data_ptr(), self.up.data_ptr(), self.down.data_ptr())
+
+    def _rows(self, x):
+        if self.quantized and x.dtype not in DTYPES:
+            raise ValueError(f"GatedFFN: x must be fp16 or bf16, got {x.dtype}")
+        return rows_of(x, self.hidden_size, self.dtype or x.dtype, self.device, "GatedFFN: x")
 
     def _workspace(self, need):
         if need == 0:
@@ -84,16 +111,18 @@ class GatedFFN:
         return torch.empty(need, dtype=torch.uint8, device=self.device)
 
     def forward(self, x):
-        if torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or self.up.requires_grad or
-                                        self.down.requires_grad):
+        if not self.quantized and torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or
+                                                               self.up.requires_grad or self.down.requires_grad):
             return _GatedFFNFunction.apply(x, self.gate, self.up, self.down, self)
+        if self.quantized and x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("GatedFFN: 4-bit weights have no gradients (detach x, or torch.no_grad())")
         return self._forward(x, None)
 
     __call__ = forward
 
     def _forward(self, x, keep):
         """y; keep: a list that receives x's rows and the saved g, u, h."""
-        r = rows_of(x, self.hidden_size, self.dtype, self.device, "GatedFFN: x")
+        r = self._rows(x)
         T = r.shape[0]
         y = torch.empty_like(r)
         saved = None
@@ -102,31 +131,36 @@ class GatedFFN:
             keep.extend((r, g, u, h))
             saved = L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr())
         if T:
-            d, lib = self.desc(), L.lib()
+            d, lib = self.desc(r.dtype), L.lib()
             with on_device(self.device) as s:
-                ws = self._workspace(lib.bmx_ffn_workspace(d, T))
-                L.check(lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s),
-                        "bmx_ffn_forward")
+                if self.quantized:
+                    ws = self._workspace(lib.bmx_ffn4_workspace(d, T))
+                    rc = lib.bmx_ffn4_forward(d, r.data_ptr(), T, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
+                else:
+                    ws = self._workspace(lib.bmx_ffn_workspace(d, T))
+                    rc = lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s)
+                L.check(rc, "GatedFFN.forward")
         return y if x.dim() == 2 else y.view(x.shape)
 
     def add_to(self, out, x, gate_vec=None):
-        """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of the weights' type: the block
-        as a layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
-        r = rows_of(x.detach(), self.hidden_size, self.dtype, self.device, "GatedFFN: x")
+        """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
+        layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
+        r = self._rows(x.detach())
         T = r.shape[0]
         if out.dtype != torch.float32 or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 or \
                 tuple(out.shape) != (T, self.hidden_size):
             raise ValueError(f"GatedFFN: out must be contiguous fp32 [{T}, {self.hidden_size}] on {self.device}")
-        if gate_vec is not None and (gate_vec.dtype != self.dtype or gate_vec.device != self.device or
+        if gate_vec is not None and (gate_vec.dtype != r.dtype or gate_vec.device != self.device or
                                      gate_vec.numel() != self.hidden_size or not gate_vec.is_contiguous() or
                                      gate_vec.data_ptr() % 16):
-            raise ValueError(f"GatedFFN: gate_vec must be a contiguous {self.dtype} tensor of {self.hidden_size} elements")
+            raise ValueError(f"GatedFFN: gate_vec must be a contiguous {r.dtype} tensor of {self.hidden_size} elements")
         if T:
-            d, lib = self.desc(), L.lib()
+            d, lib = self.desc(r.dtype), L.lib()
             with on_device(self.device) as s:
-                ws = self._workspace(lib.bmx_ffn_workspace(d, T))
-                L.check(lib.bmx_ffn_add(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None,
-                                        out.data_ptr(), ws.data_ptr(), ws.numel(), s), "bmx_ffn_add")
+                ws = self._workspace(lib.bmx_ffn4_workspace(d, T) if self.quantized else lib.bmx_ffn_workspace(d, T))
+                call = lib.bmx_ffn4_add if self.quantized else lib.bmx_ffn_add
+                L.check(call(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None, out.data_ptr(),
+                             ws.data_ptr(), ws.numel(), s), "GatedFFN.add_to")
         return out
 
 

@@ -24,8 +24,8 @@ class MoELayer:
     score (SCORE_SOFTMAX / SCORE_SIGMOID / SCORE_SQRTSP), selection bias fp32 [E], group limit, renorm, scale
     (routed_scaling_factor); activation, gated, act_limit; router_weight: fp16 [E, H] gate weight (checkpoint layout),
     used when no logits are given; shared_gate: fp16 [H] gate vector of the shared expert (its output scaled by
-    sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 weights as the layer's shared expert, for tables
-    without one (shared_gate then scales its output); slots / li: an ExpertSlots table and this layer's index in it."""
+    sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 or 4-bit weights as the layer's shared expert, for
+    tables without one (shared_gate then scales its output); slots / li: an ExpertSlots table and this layer's index in it."""
 
     def __init__(self, table, topk, first=0, score=L.SCORE_SIGMOID, bias=None, n_group=1, topk_group=1, renorm=True,
                  scale=1.0, act=L.ACT_SILU, gated=True, act_limit=0.0, router_weight=None, slots=None, li=0,
@@ -33,8 +33,9 @@ class MoELayer:
         if shared_ffn is not None:
             if table.has_shared:
                 raise ValueError("shared_ffn: the table already has a shared expert")
-            if shared_ffn.hidden_size != table.H or shared_ffn.dtype != torch.float16 or shared_ffn.device != table.device:
-                raise ValueError(f"shared_ffn: expected fp16 weights of H = {table.H} on {table.device}")
+            if shared_ffn.hidden_size != table.H or shared_ffn.dtype not in (None, torch.float16) or \
+                    shared_ffn.device != table.device:
+                raise ValueError(f"shared_ffn: expected fp16 or 4-bit weights of H = {table.H} on {table.device}")
         self.shared_ffn, self.shared_ffn_gate = shared_ffn, None
         if shared_ffn is not None and shared_gate is not None:
             if (shared_gate.dtype != torch.float16 or shared_gate.numel() != table.H or not shared_gate.is_cuda or

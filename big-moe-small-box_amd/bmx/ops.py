@@ -6,6 +6,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check, lib
+from .ffn import DTYPES, on_device, rows_of
 
 
 def _stream():
@@ -56,6 +57,24 @@ def router_logits(z, weight):
     out = torch.empty((T, E), dtype=torch.float16, device=z.device)
     check(lib().bmx_router_logits(_ptr(z), _ptr(weight), T, H, E, _ptr(out), _stream()), "bmx_router_logits")
     return out
+
+
+def q4_linear(x, q):
+    """y [..., N] = x W^T for a Q4Matrix q, x [..., K] fp16 or bf16 on the matrix's device; fp32 sums, one rounding."""
+    dt = DTYPES.get(x.dtype)
+    if dt is None:
+        raise ValueError(f"q4_linear: x must be fp16 or bf16, got {x.dtype}")
+    r = rows_of(x, q.K, x.dtype, q.device, "q4_linear: x")
+    T = r.shape[0]
+    y = torch.empty((T, q.N), dtype=x.dtype, device=q.device)
+    if T:
+        L_ = lib()
+        with on_device(q.device) as s:
+            need = L_.bmx_q4_linear_workspace(q.struct, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+            check(L_.bmx_q4_linear(q.struct, dt, r.data_ptr(), T, y.data_ptr(), ws.data_ptr() if need else None, need, s),
+                  "bmx_q4_linear")
+    return y if x.dim() == 2 else y.view(x.shape[:-1] + (q.N,))
 
 
 class RoutesBuf:

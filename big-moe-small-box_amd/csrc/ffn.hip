@@ -1,6 +1,7 @@
-// Gated feed-forward block with 16-bit weights: forward, the form that adds to a layer's output, and gradients. The products
-// are gemm16_k's; this file plans tiles and splits, lays out the workspace and checks arguments.
-#include "gemm16.hpp"
+// Gated feed-forward block: forward and the form that adds to a layer's output (16-bit and 4-bit weights), gradients (16-bit).
+// The products are skinny_k's for few tokens and gemm16_k's for many (4-bit weights then decoded to 16 bits first); this file
+// plans tiles and splits, lays out the workspace and checks arguments.
+#include "skinny.hpp"
 
 namespace bmx {
 
@@ -42,12 +43,13 @@ static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
 {
     if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.big, s);
     a.splits = tp.splits;
+    a.ldp = (a.M + 3) / 4 * 4;
     GemmArgs g = a;
     g.batch = EPI == EPI_GU ? 2 : 1;
     if (EPI == EPI_GU) g.b[1] = g.b[0];
     int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.big, s);
     if (rc) return rc;
-    const int64_t quads = (int64_t)a.M * a.N / 4;
+    const int64_t quads = (int64_t)a.ldp / 4 * a.N;
     hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
     return check_launch("gemm_finish");
 }
@@ -77,54 +79,135 @@ __global__ __launch_bounds__(256) void row_gate_k(const uint16_t* __restrict__ x
 
 static int tiles_k(int K) { return (K + GK - 1) / GK; }
 
-struct FfnPlan {
-    TilePlan gu, down;
-    size_t h, part, gate, total;       // workspace offsets
+size_t product_part_bytes(int N, int T, int K)
+{
+    const TilePlan p = plan_product(N, T, tiles_k(K), 1, true);
+    return p.splits > 1 ? (size_t)p.splits * T * ((N + 3) / 4 * 4) * 4 : 0;
+}
+
+int launch_product(const void* w, const void* x, int T, int N, int K, int dtype, void* y, void* part, hipStream_t s)
+{
+    GemmArgs a = {};
+    a.chain = a.batch = a.splits = 1;
+    a.part = static_cast<float*>(part);
+    a.a[0] = w; a.b[0] = x; a.out[0] = y;
+    a.M = N; a.N = T; a.K = K; a.lda = a.ldb = K; a.ldo = N;
+    const TilePlan p = plan_product(N, T, tiles_k(K), 1, true);
+    return dtype == BMX_DT_FP16 ? product<f16, false, false, EPI_STORE>(a, p, s) : product<bf16, false, false, EPI_STORE>(a, p, s);
+}
+
+// A forward pass's weights: 16-bit, or q[3] (4-bit)
+struct FfnIn {
+    int H, I, dtype;
+    ActPar act;
+    const void* w[3];
+    const bmx_q4* q[3];
+    int group() const { return q[0] ? q[0]->group : 0; }
 };
 
-static FfnPlan ffn_plan(const bmx_ffn_desc* d, int T)
+static FfnIn ffn_in(const bmx_ffn_desc* d)
+{
+    return {d->H, d->I, d->dtype, act_par(d->act, d->act_limit), {d->gate, d->up, d->down}, {nullptr, nullptr, nullptr}};
+}
+
+static FfnIn ffn_in(const bmx_ffn4_desc* d)
+{
+    return {d->gate->K, d->gate->N, d->dtype, act_par(d->act, d->act_limit), {nullptr, nullptr, nullptr}, {d->gate, d->up, d->down}};
+}
+
+struct FfnPlan {
+    TilePlan gu, down;
+    bool skinny_gu, skinny_down;
+    size_t h, part, gate, deq, total;       // workspace offsets
+};
+
+static FfnPlan ffn_plan(const FfnIn& d, int T)
 {
     FfnPlan p;
-    p.gu = plan_product(2 * (int64_t)d->I, T, tiles_k(d->H), 1, true);
-    p.down = plan_product(d->H, T, tiles_k(d->I), 1, true);
+    p.skinny_gu = T <= skinny_tokens_max(d.group());
+    p.skinny_down = T <= skinny_tokens_max(d.q[2] ? d.q[2]->group : 0);
+    p.gu = plan_product(2 * (int64_t)d.I, T, tiles_k(d.H), 1, true);
+    p.down = plan_product(d.H, T, tiles_k(d.I), 1, true);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
-    p.h = take((size_t)T * d->I * 2);
+    p.h = take((size_t)T * d.I * 2);
     p.gate = take((size_t)T * 4);
-    const size_t pg = p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d->I * 4 : 0;
-    const size_t pd = p.down.splits > 1 ? (size_t)p.down.splits * T * d->H * 4 : 0;
+    const size_t pg = !p.skinny_gu && p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d.I * 4 : 0;
+    const size_t pd = !p.skinny_down && p.down.splits > 1 ? (size_t)p.down.splits * T * d.H * 4 : 0;
     p.part = take(pg > pd ? pg : pd);
+    p.deq = take(!d.q[0] ? 0 : !p.skinny_gu ? (size_t)d.H * d.I * 4 : !p.skinny_down ? (size_t)d.H * d.I * 2 : 0);
     p.total = o + 256;
     return p;
 }
 
 template <class T>
-static int ffn_forward(const bmx_ffn_desc* d, const void* x, int n, void* y, float* add, const void* gate_vec,
-                       const bmx_ffn_saved* sv, char* ws, hipStream_t s)
+static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add, const void* gate_vec, const bmx_ffn_saved* sv,
+                       char* ws, hipStream_t s)
 {
     const FfnPlan p = ffn_plan(d, n);
     void* h = sv ? sv->h : ws + p.h;
     float* scale = nullptr;
+    int rc = BMX_OK;
     if (gate_vec)
     {
         scale = reinterpret_cast<float*>(ws + p.gate);
         hipLaunchKernelGGL((row_gate_k<T>), dim3((n + 3) / 4), dim3(256), 0, s, static_cast<const uint16_t*>(x),
-                           static_cast<const uint16_t*>(gate_vec), n, d->H, scale);
-        const int rc = check_launch("row_gate");
-        if (rc) return rc;
+                           static_cast<const uint16_t*>(gate_vec), n, d.H, scale);
+        if ((rc = check_launch("row_gate"))) return rc;
     }
+    SkinnyArgs k = {};
+    k.T = n;
+    k.act = d.act;
+    k.scale = scale;
     GemmArgs a = {};
     a.chain = a.batch = a.splits = 1;
     a.part = reinterpret_cast<float*>(ws + p.part);
-    a.act = act_par(d->act, d->act_limit);
-    a.a[0] = d->gate; a.a[1] = d->up; a.b[0] = x; a.out[0] = h;
-    a.M = d->I; a.N = n; a.K = d->H; a.lda = a.ldb = d->H; a.ldo = d->I;
-    if (sv) { a.g = sv->g; a.u = sv->u; }
-    int rc = product<T, false, false, EPI_GU>(a, p.gu, s);
-    if (rc) return rc;
-    a.a[0] = d->down; a.a[1] = nullptr; a.b[0] = h; a.out[0] = add ? static_cast<void*>(add) : y;
-    a.M = d->H; a.K = d->I; a.lda = a.ldb = d->I; a.ldo = d->H;
+    a.act = d.act;
+    a.N = n;
     a.scale = scale;
+    char* deq = ws + p.deq;
+
+    // h = act(x Wg^T, x Wu^T)
+    if (p.skinny_gu)
+    {
+        for (int m = 0; m < 2; ++m)
+        {
+            k.w[m] = d.w[m];
+            if (d.q[0]) k.q[m] = q4_view(d.q[m]);
+        }
+        k.group = d.group();
+        k.x = static_cast<const uint16_t*>(x);
+        k.N = d.I; k.K = d.H; k.out = h; k.ldo = d.I;
+        if (sv) { k.g = static_cast<uint16_t*>(sv->g); k.u = static_cast<uint16_t*>(sv->u); }
+        if ((rc = launch_skinny(k, d.dtype, EPI_GU, s))) return rc;
+    }
+    else
+    {
+        for (int m = 0; m < 2; ++m)
+        {
+            a.a[m] = d.q[0] ? deq + (size_t)m * d.H * d.I * 2 : d.w[m];
+            if (d.q[0] && (rc = launch_q4_dequant(d.q[m], d.dtype, deq + (size_t)m * d.H * d.I * 2, s))) return rc;
+        }
+        a.b[0] = x; a.out[0] = h;
+        a.M = d.I; a.K = d.H; a.lda = a.ldb = d.H; a.ldo = d.I;
+        if (sv) { a.g = sv->g; a.u = sv->u; }
+        if ((rc = product<T, false, false, EPI_GU>(a, p.gu, s))) return rc;
+    }
+    // y = h Wd^T
+    void* out = add ? static_cast<void*>(add) : y;
+    if (p.skinny_down)
+    {
+        k.w[0] = d.w[2];
+        if (d.q[0]) k.q[0] = q4_view(d.q[2]);
+        k.group = d.q[0] ? d.q[2]->group : 0;
+        k.x = static_cast<const uint16_t*>(h);
+        k.N = d.H; k.K = d.I; k.out = out; k.ldo = d.H;
+        return launch_skinny(k, d.dtype, add ? EPI_ADD : EPI_STORE, s);
+    }
+    a.a[0] = d.q[0] ? deq : d.w[2];
+    if (d.q[0] && (rc = launch_q4_dequant(d.q[2], d.dtype, deq, s))) return rc;
+    a.a[1] = nullptr; a.b[0] = h; a.out[0] = out;
+    a.M = d.H; a.K = d.I; a.lda = a.ldb = d.I; a.ldo = d.H;
     return add ? product<T, false, false, EPI_ADD>(a, p.down, s) : product<T, false, false, EPI_STORE>(a, p.down, s);
 }
 
@@ -217,6 +300,22 @@ static int check_ffn(const bmx_ffn_desc* d, int T, const char* who)
     return BMX_OK;
 }
 
+static int check_ffn(const bmx_ffn4_desc* d, int T, const char* who)
+{
+    if (!d) return set_error(BMX_ERR_ARG, "%s: null descriptor", who);
+    for (const bmx_q4* q : {d->gate, d->up, d->down})
+        if (const int rc = check_q4(q, who)) return rc;
+    const int H = d->gate->K, I = d->gate->N;
+    if (d->up->K != H || d->up->N != I || d->down->K != I || d->down->N != H)
+        return set_error(BMX_ERR_ARG, "%s: gate and up must be [I, H], down [H, I]", who);
+    if (d->gate->group != d->up->group) return set_error(BMX_ERR_ARG, "%s: gate and up must have groups of one size", who);
+    if (!dtype_ok(d->dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", who, d->dtype);
+    if (d->act < BMX_ACT_SILU || d->act > BMX_ACT_SILU_OAI) return set_error(BMX_ERR_ARG, "%s: unknown activation %d", who, d->act);
+    if (!(d->act_limit >= 0.0f)) return set_error(BMX_ERR_ARG, "%s: act_limit must be 0 (off) or positive", who);
+    if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", who, T);
+    return BMX_OK;
+}
+
 static int check_saved(const bmx_ffn_saved* sv, const char* who)
 {
     if (!sv->g || !sv->u || !sv->h || odd16(sv->g) || odd16(sv->u) || odd16(sv->h))
@@ -231,7 +330,39 @@ static int check_ws(const void* ws, size_t have, size_t need, const char* who)
     return BMX_OK;
 }
 
-template <class T> __global__ __launch_bounds__(256) void zero16_k(u32x4* p, int64_t n)
+template <class Desc>
+static int forward_call(const char* fn, const Desc* desc, const void* x, int T, void* y, const bmx_ffn_saved* saved, void* workspace,
+                        size_t workspace_bytes, bmx_stream_t stream)
+{
+    int rc = check_ffn(desc, T, fn);
+    if (rc || T == 0) return rc;
+    if (!x || !y || odd16(x) || odd16(y)) return set_error(BMX_ERR_ARG, "%s: x or y null or not 16-byte aligned", fn);
+    if (saved && (rc = check_saved(saved, fn))) return rc;
+    const FfnIn d = ffn_in(desc);
+    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(d, T).total, fn))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    return d.dtype == BMX_DT_FP16 ? ffn_forward<f16>(d, x, T, y, nullptr, nullptr, saved, ws, s)
+                                  : ffn_forward<bf16>(d, x, T, y, nullptr, nullptr, saved, ws, s);
+}
+
+template <class Desc>
+static int add_call(const char* fn, const Desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
+                    size_t workspace_bytes, bmx_stream_t stream)
+{
+    int rc = check_ffn(desc, T, fn);
+    if (rc || T == 0) return rc;
+    if (!x || !out || odd16(x) || odd16(out)) return set_error(BMX_ERR_ARG, "%s: x or out null or not 16-byte aligned", fn);
+    if (odd16(gate_vec)) return set_error(BMX_ERR_ARG, "%s: gate_vec not 16-byte aligned", fn);
+    const FfnIn d = ffn_in(desc);
+    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(d, T).total, fn))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    return d.dtype == BMX_DT_FP16 ? ffn_forward<f16>(d, x, T, nullptr, out, gate_vec, nullptr, ws, s)
+                                  : ffn_forward<bf16>(d, x, T, nullptr, out, gate_vec, nullptr, ws, s);
+}
+
+__global__ __launch_bounds__(256) void zero16_k(u32x4* p, int64_t n)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i < n) p[i] = u32x4{0, 0, 0, 0};
@@ -245,8 +376,12 @@ extern "C" {
 
 size_t bmx_ffn_workspace(const bmx_ffn_desc* desc, int T)
 {
-    if (check_ffn(desc, T, "bmx_ffn_workspace")) return 0;
-    return ffn_plan(desc, T).total;
+    return check_ffn(desc, T, "bmx_ffn_workspace") ? 0 : ffn_plan(ffn_in(desc), T).total;
+}
+
+size_t bmx_ffn4_workspace(const bmx_ffn4_desc* desc, int T)
+{
+    return check_ffn(desc, T, "bmx_ffn4_workspace") ? 0 : ffn_plan(ffn_in(desc), T).total;
 }
 
 size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T)
@@ -258,31 +393,25 @@ size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T)
 int bmx_ffn_forward(const bmx_ffn_desc* desc, const void* x, int T, void* y, const bmx_ffn_saved* saved, void* workspace,
                     size_t workspace_bytes, bmx_stream_t stream)
 {
-    const char* fn = "bmx_ffn_forward";
-    int rc = check_ffn(desc, T, fn);
-    if (rc || T == 0) return rc;
-    if (!x || !y || odd16(x) || odd16(y)) return set_error(BMX_ERR_ARG, "%s: x or y null or not 16-byte aligned", fn);
-    if (saved && (rc = check_saved(saved, fn))) return rc;
-    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(desc, T).total, fn))) return rc;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    char* ws = static_cast<char*>(workspace);
-    return desc->dtype == BMX_DT_FP16 ? ffn_forward<f16>(desc, x, T, y, nullptr, nullptr, saved, ws, s)
-                                      : ffn_forward<bf16>(desc, x, T, y, nullptr, nullptr, saved, ws, s);
+    return forward_call("bmx_ffn_forward", desc, x, T, y, saved, workspace, workspace_bytes, stream);
+}
+
+int bmx_ffn4_forward(const bmx_ffn4_desc* desc, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
+                     bmx_stream_t stream)
+{
+    return forward_call("bmx_ffn4_forward", desc, x, T, y, nullptr, workspace, workspace_bytes, stream);
 }
 
 int bmx_ffn_add(const bmx_ffn_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
                 size_t workspace_bytes, bmx_stream_t stream)
 {
-    const char* fn = "bmx_ffn_add";
-    int rc = check_ffn(desc, T, fn);
-    if (rc || T == 0) return rc;
-    if (!x || !out || odd16(x) || odd16(out)) return set_error(BMX_ERR_ARG, "%s: x or out null or not 16-byte aligned", fn);
-    if (odd16(gate_vec)) return set_error(BMX_ERR_ARG, "%s: gate_vec not 16-byte aligned", fn);
-    if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(desc, T).total, fn))) return rc;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    char* ws = static_cast<char*>(workspace);
-    return desc->dtype == BMX_DT_FP16 ? ffn_forward<f16>(desc, x, T, nullptr, out, gate_vec, nullptr, ws, s)
-                                      : ffn_forward<bf16>(desc, x, T, nullptr, out, gate_vec, nullptr, ws, s);
+    return add_call("bmx_ffn_add", desc, x, T, gate_vec, out, workspace, workspace_bytes, stream);
+}
+
+int bmx_ffn4_add(const bmx_ffn4_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
+                 size_t workspace_bytes, bmx_stream_t stream)
+{
+    return add_call("bmx_ffn4_add", desc, x, T, gate_vec, out, workspace, workspace_bytes, stream);
 }
 
 int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_ffn_saved* saved, const void* dy, void* dx,
@@ -299,7 +428,7 @@ int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_f
         for (void* w : {dgate, dup, ddown})
             if (w)
             {
-                hipLaunchKernelGGL((zero16_k<f16>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, static_cast<u32x4*>(w), n);
+                hipLaunchKernelGGL(zero16_k, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, static_cast<u32x4*>(w), n);
                 if ((rc = check_launch(fn))) return rc;
             }
         return BMX_OK;

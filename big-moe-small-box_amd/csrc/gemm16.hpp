@@ -51,6 +51,7 @@ struct GemmArgs {
     void* out[2];
     int M, N, K;            // M: rows of A (EPI_GU: of each of its two matrices), N: rows of B
     int lda, ldb, ldo;      // elements
+    int ldp;                // EPI_PART: row of the partial sums, a multiple of 4
     int chain;              // 2: the two products are summed
     int batch;              // 2: two products side by side (grid z)
     int splits;             // of K (EPI_PART; grid z = product * splits + split)
@@ -72,9 +73,13 @@ template <class T> __device__ __forceinline__ u32x2 pack4(const f32x4 v)
 }
 
 // What becomes of four neighbouring sums of a result row, at element o of the outputs
-template <class T> __device__ __forceinline__ void store_4(const GemmArgs& p, void* out, int64_t o, const f32x4 v)
+template <class T> __device__ __forceinline__ void store_4(const GemmArgs& p, void* out, int64_t o, int m, const f32x4 v)
 {
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(out) + o) = pack4<T>(v);
+    uint16_t* q = static_cast<uint16_t*>(out) + o;
+    if (!(p.ldo & 3)) { *reinterpret_cast<u32x2*>(q) = pack4<T>(v); return; }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)                                     // rows of any length (4-bit matrices)
+        if (m + t < p.M) q[t] = to16<T>(v[t]);
 }
 
 __device__ __forceinline__ void add_4(const GemmArgs& p, int64_t o, int n, const f32x4 v)
@@ -321,10 +326,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
                 if (m >= p.M) continue;
                 const int64_t o = (int64_t)n * p.ldo + m;
                 const f32x4 v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                if (EPI == EPI_PART) *reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.M + m) = v;
+                if (EPI == EPI_PART) *reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.ldp + m) = v;
                 else if (EPI == EPI_ADD) add_4(p, o, n, v);
                 else if (EPI == EPI_DGU) dgu_4<T>(p, o, v);
-                else store_4<T>(p, p.out[prod], o, v);
+                else store_4<T>(p, p.out[prod], o, m, v);
             }
     }
 }
@@ -333,10 +338,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
 template <class T, int EPI>
 __global__ __launch_bounds__(256) void gemm_finish_k(const GemmArgs p)
 {
-    const int64_t quads = (int64_t)p.N * p.M / 4, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= quads) return;
-    const int64_t at = i * 4, plane = (int64_t)p.N * p.M;
-    const int n = (int)(at / p.M), m = (int)(at % p.M);
+    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (at >= plane) return;
+    const int n = (int)(at / p.ldp), m = (int)(at % p.ldp);
     auto sum = [&](int prod) {
         const float* q = p.part + prod * p.splits * plane + at;
         f32x4 v = ldg4f(q);
@@ -356,7 +360,7 @@ __global__ __launch_bounds__(256) void gemm_finish_k(const GemmArgs p)
     }
     else if (EPI == EPI_ADD) add_4(p, o, n, sum(0));
     else if (EPI == EPI_DGU) dgu_4<T>(p, o, sum(0));
-    else store_4<T>(p, p.out[0], o, sum(0));
+    else store_4<T>(p, p.out[0], o, m, sum(0));
 }
 
 }  // namespace bmx

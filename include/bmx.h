@@ -463,6 +463,30 @@ int bmx_host_device_ptr(void* host, uint64_t* device_addr);
 int bmx_combine(const float* y_rows, const int32_t* inv, const void* w_fp16, const int32_t* offsets, int T, int topk,
                 int H, int E, int has_shared, float* out, bmx_stream_t stream);
 
+/* ---- 4-bit matrices with group scales ----
+ * W[n][k] = scale[n][k / group] * (code[n][k] - zero[n][k / group]), codes 0 .. 15, group 32, 64 or 128, K a multiple of it,
+ * any N: the form in which many checkpoints keep linears that are not EXL3 trellis records. scale fp16 or bf16
+ * (scale_dtype), zero uint8 or NULL (8 everywhere). A bmx_q4 holds the matrix in the kernels' order: codes
+ * bmx_q4_code_bytes bytes, scale 2 and zero 1 byte for each of bmx_q4_group_count values, written by bmx_q4_pack from a
+ * checkpoint's order: codes [N][K / 2] with the even column in a byte's low half, scale and zero [N][K / group]. Device
+ * memory, 16-byte aligned. */
+enum bmx_dtype { BMX_DT_FP16 = 0, BMX_DT_BF16 = 1 };
+typedef struct bmx_q4 {
+    int32_t N, K, group, scale_dtype;
+    const void *codes, *scale, *zero;
+} bmx_q4;
+size_t bmx_q4_code_bytes(int N, int K);
+size_t bmx_q4_group_count(int N, int K, int group);
+int bmx_q4_pack(const bmx_q4* q, const void* codes, const void* scale, const void* zero, bmx_stream_t stream);
+/* out [N][K] of dtype: each weight rounded once. */
+int bmx_q4_dequant(const bmx_q4* q, int dtype, void* out, bmx_stream_t stream);
+/* y [T][N] = x [T][K] W^T, x and y of dtype, 16-byte aligned. fp32 sums, one rounding. A call of many tokens decodes the
+ * weights to dtype in the workspace first (each then rounded once: half a step of the type); a call of few multiplies x
+ * with the codes themselves, exactly. An infinite x may give NaN. */
+size_t bmx_q4_linear_workspace(const bmx_q4* q, int T);
+int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
+                  bmx_stream_t stream);
+
 /* ---- gated feed-forward block ----
  * y = act(x Wg^T, x Wu^T) Wd^T, the feed-forward block that checkpoints keep outside the routed experts' trellis records: a
  * model's leading dense layers, or a layer's shared expert in 16 bits. x, y [T, H]; gate, up [I, H]; down [H, I]; row-major,
@@ -470,7 +494,6 @@ int bmx_combine(const float* y_rows, const int32_t* inv, const void* w_fp16, con
  * (enum bmx_act; h = min(act(g), limit) * clamp(u, +-limit), or for BMX_ACT_SILU_OAI the clamps first and (u + 1);
  * act_limit 0 = off, else positive). Products accumulate in fp32; h = act(g, u) is rounded once to dtype between the two
  * products, y once at the end. NaN and infinities pass through. */
-enum bmx_dtype { BMX_DT_FP16 = 0, BMX_DT_BF16 = 1 };
 typedef struct bmx_ffn_desc {
     int32_t H, I;
     int32_t dtype;
@@ -493,6 +516,19 @@ int bmx_ffn_forward(const bmx_ffn_desc* desc, const void* x, int T, void* y, con
  * is not rounded to dtype. */
 int bmx_ffn_add(const bmx_ffn_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
                 size_t workspace_bytes, bmx_stream_t stream);
+/* The block with 4-bit weights (host pointers to three matrices; gate and up of one group size): forward only. x, y and h
+ * of dtype. */
+typedef struct bmx_ffn4_desc {
+    int32_t dtype, act;
+    float act_limit;
+    int32_t reserved;
+    const bmx_q4 *gate, *up, *down;
+} bmx_ffn4_desc;
+size_t bmx_ffn4_workspace(const bmx_ffn4_desc* desc, int T);
+int bmx_ffn4_forward(const bmx_ffn4_desc* desc, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
+                     bmx_stream_t stream);
+int bmx_ffn4_add(const bmx_ffn4_desc* desc, const void* x, int T, const void* gate_vec, float* out, void* workspace,
+                 size_t workspace_bytes, bmx_stream_t stream);
 /* Gradients from dy [T, H] and a forward pass's x and saved values: dx [T, H], dgate, dup [I, H], ddown [H, I], of dtype,
  * each NULL when it is not wanted (its products are then not computed). The gradient of h's two factors is rounded to
  * dtype before the products that use it. T = 0: the wanted weight gradients are zeroed. */

@@ -53,11 +53,24 @@ def product(a, b, da=0.0):
     return a @ b.t(), bound
 
 
-def forward(x, wg, wu, act, L):
+def q4_product(x, q, dt, da=0.0):
+    """As product for a 4-bit matrix q = (W, spread) in 64 bits. Calls of many tokens round each weight to dt first. Calls
+    of few multiply with the codes: exactly in fp16; in bf16 with 128 + code, whose sums run up to spread =
+    scale (128 + 15 + 128 + zero) per weight before the offset comes off (five more operations a group)."""
+    w, spread = q
+    y, bound = product(x, w, da)
+    bound = bound + HALF[dt] * (1 + x.shape[1] * ACC) * (x.abs() @ w.abs().t()) + 5 * ACC * (x.abs() @ w.abs().t())
+    if dt == torch.bfloat16:
+        bound = bound + (x.shape[1] + 5) * ACC * (x.abs() @ spread.t())
+    # a weight below the type's normal range is rounded to its smallest step
+    return y, bound + TINY[dt] * x.abs().sum(1, keepdim=True)
+
+
+def forward(x, wg, wu, act, L, prod=product):
     """g, u, h in 64 bits and bounds of their errors before their rounding; h's takes the activation's change over the errors
     of g and u from their four corners, twice."""
-    g, eg = product(x, wg)
-    u, eu = product(x, wu)
+    g, eg = prod(x, wg)
+    u, eu = prod(x, wu)
     h = act_h(act, g, u, L)
     ends = [(act_h(act, g + a * eg, u + b * eu, L) - h).abs() for a in (-1, 1) for b in (-1, 1)]
     # the sigmoid of z < -87.3 is below 2^-126, the smallest normal fp32 value (and exp(-z) past 88.7 is infinite, its

@@ -57,3 +57,57 @@ def test_host_tensors_are_refused():
     w = [torch.zeros(s, dtype=torch.float16) for s in ((72, 64), (72, 64), (64, 72))]
     with pytest.raises(ValueError):
         bmx.GatedFFN(*w)
+
+
+def q4(**k):
+    import bmx
+    v = dict(N=72, K=128, group=64, scale_dtype=0, codes=256, scale=256, zero=256)
+    v.update(k)
+    return bmx._lib.Q4(*(v[n] for n, _ in bmx._lib.Q4._fields_))
+
+
+@pytest.mark.parametrize("bad,text", [(dict(group=48), b"group"), (dict(group=0), b"group"), (dict(N=0), b"positive"), (dict(K=96), b"multiple"),
+                                      (dict(K=-64), b"positive"), (dict(N=1 << 21), b"2^20"), (dict(scale_dtype=3), b"scale dtype"),
+                                      (dict(codes=None), b"null"), (dict(scale=None), b"null"), (dict(codes=264), b"aligned"),
+                                      (dict(zero=8), b"aligned")])
+def test_q4_matrix_refusals(bad, text):
+    import bmx
+    L, E = bmx.lib(), bmx._lib.BMX_ERR_ARG
+    q = q4(**bad)
+    assert L.bmx_q4_pack(q, 256, 256, 256, None) == E and text in L.bmx_last_error()
+    assert L.bmx_q4_dequant(q, 0, 256, None) == E and text in L.bmx_last_error()
+    assert L.bmx_q4_linear_workspace(q, 100) == 0 and text in L.bmx_last_error()
+    assert L.bmx_q4_linear(q, 0, 256, 4, 256, 256, 1 << 30, None) == E and text in L.bmx_last_error()
+    ok = q4(N=128, K=128)
+    for three in ((q, ok, ok), (ok, q, ok), (ok, ok, q)):
+        d = bmx._lib.Ffn4Desc(0, 0, 0.0, 0, *(ctypes.pointer(m) for m in three))
+        assert L.bmx_ffn4_workspace(d, 4) == 0
+        assert L.bmx_ffn4_forward(d, 256, 4, 256, 256, 1 << 30, None) == E
+
+
+def test_q4_call_refusals():
+    import bmx
+    L, E, W = bmx.lib(), bmx._lib.BMX_ERR_ARG, bmx._lib.BMX_ERR_WORKSPACE
+    q = q4()
+    assert L.bmx_q4_code_bytes(72, 128) == 80 * 64 and L.bmx_q4_code_bytes(1, 32) == 16 * 64 and L.bmx_q4_code_bytes(0, 32) == 0
+    assert L.bmx_q4_group_count(72, 128, 64) == 80 * 2 and L.bmx_q4_group_count(1, 32, 32) == 16 * 4 and L.bmx_q4_group_count(1, 32, 31) == 0
+    assert L.bmx_q4_pack(q, None, 256, 256, None) == E and L.bmx_q4_pack(q, 256, None, 256, None) == E
+    assert L.bmx_q4_pack(q, 256, 256, None, None) == E and L.bmx_q4_pack(q4(zero=None), 256, 256, 256, None) == E
+    assert L.bmx_q4_dequant(q, 2, 256, None) == E and L.bmx_q4_dequant(q, 0, None, None) == E and L.bmx_q4_dequant(q, 0, 264, None) == E
+    lin = lambda dt=0, x=256, T=4, y=256, ws=256, n=1 << 30: L.bmx_q4_linear(q, dt, x, T, y, ws, n, None)
+    assert lin(dt=2) == E and lin(x=None) == E and lin(x=264) == E and lin(y=None) == E and lin(T=-1) == E
+    assert lin(T=(1 << 24) + 1) == E and lin(T=0, x=None, y=None, ws=None, n=0) == 0
+    need = L.bmx_q4_linear_workspace(q, 4096)
+    assert need > 0 and lin(T=4096, n=need - 1) == W and lin(T=4096, ws=None) == E and lin(T=4096, ws=264) == E
+    gu, dn = q4(N=128, K=64), q4(N=64, K=128)
+    three = lambda a, b, c: bmx._lib.Ffn4Desc(0, 0, 0.0, 0, ctypes.pointer(a), ctypes.pointer(b), ctypes.pointer(c))
+    good = three(gu, gu, dn)
+    need = L.bmx_ffn4_workspace(good, 4)
+    assert need > 0
+    for bad in (three(gu, dn, dn), three(gu, gu, gu), three(gu, q4(N=128, K=64, group=32), dn)):
+        assert L.bmx_ffn4_workspace(bad, 4) == 0
+        assert L.bmx_ffn4_forward(bad, 256, 4, 256, 256, 1 << 30, None) == E
+        assert L.bmx_ffn4_add(bad, 256, 4, None, 256, 256, 1 << 30, None) == E
+    assert L.bmx_ffn4_forward(good, 256, 4, 256, 256, need - 1, None) == W
+    assert L.bmx_ffn4_add(good, 256, 4, 258, 256, 256, need, None) == E
+    assert L.bmx_ffn4_forward(None, 256, 4, 256, 256, need, None) == E
