@@ -43,14 +43,14 @@ static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
 {
     if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.big, s);
     a.splits = tp.splits;
-    a.ldp = (a.M + 3) / 4 * 4;
+    a.ldp = (a.M + 7) / 8 * 8;
     GemmArgs g = a;
     g.batch = EPI == EPI_GU ? 2 : 1;
     if (EPI == EPI_GU) g.b[1] = g.b[0];
     int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.big, s);
     if (rc) return rc;
-    const int64_t quads = (int64_t)a.ldp / 4 * a.N;
-    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, a);
+    const int64_t pieces = (int64_t)a.ldp / 8 * a.N;
+    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a);
     return check_launch("gemm_finish");
 }
 
@@ -82,7 +82,7 @@ static int tiles_k(int K) { return (K + GK - 1) / GK; }
 size_t product_part_bytes(int N, int T, int K)
 {
     const TilePlan p = plan_product(N, T, tiles_k(K), 1, true);
-    return p.splits > 1 ? (size_t)p.splits * T * ((N + 3) / 4 * 4) * 4 : 0;
+    return p.splits > 1 ? (size_t)p.splits * T * ((N + 7) / 8 * 8) * 4 : 0;
 }
 
 int launch_product(const void* w, const void* x, int T, int N, int K, int dtype, void* y, void* part, hipStream_t s)

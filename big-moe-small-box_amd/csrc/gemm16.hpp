@@ -51,7 +51,7 @@ struct GemmArgs {
     void* out[2];
     int M, N, K;            // M: rows of A (EPI_GU: of each of its two matrices), N: rows of B
     int lda, ldb, ldo;      // elements
-    int ldp;                // EPI_PART: row of the partial sums, a multiple of 4
+    int ldp;                // EPI_PART: row of the partial sums, a multiple of 8
     int chain;              // 2: the two products are summed
     int batch;              // 2: two products side by side (grid z)
     int splits;             // of K (EPI_PART; grid z = product * splits + split)
@@ -64,68 +64,80 @@ struct GemmArgs {
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
-template <class T> __device__ __forceinline__ u32x2 pack4(const f32x4 v)
+// Eight neighbouring values of a result row: 16 bytes of 16-bit values
+struct f32x8 { float v[8]; };
+
+template <class T> __device__ __forceinline__ u32x4 pack8(const f32x8& v)
 {
-    u32x2 w;
-    w[0] = (uint32_t)to16<T>(v[0]) | ((uint32_t)to16<T>(v[1]) << 16);
-    w[1] = (uint32_t)to16<T>(v[2]) | ((uint32_t)to16<T>(v[3]) << 16);
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to16<T>(v.v[2 * i]) | (uint32_t)to16<T>(v.v[2 * i + 1]) << 16;
     return w;
 }
 
-// What becomes of four neighbouring sums of a result row, at element o of the outputs
-template <class T> __device__ __forceinline__ void store_4(const GemmArgs& p, void* out, int64_t o, int m, const f32x4 v)
+// What becomes of eight neighbouring sums of a result row (columns m .. m + 7), at element o of the outputs. Rows are
+// multiples of 8 values except in store_8 (4-bit matrices of any N), where the last ones are stored one by one.
+template <class T> __device__ __forceinline__ void store_8(const GemmArgs& p, void* out, int64_t o, int m, const f32x8& v)
 {
     uint16_t* q = static_cast<uint16_t*>(out) + o;
-    if (!(p.ldo & 3)) { *reinterpret_cast<u32x2*>(q) = pack4<T>(v); return; }
+    if (!(p.ldo & 7)) { *reinterpret_cast<u32x4*>(q) = pack8<T>(v); return; }
 #pragma unroll
-    for (int t = 0; t < 4; ++t)                                     // rows of any length (4-bit matrices)
-        if (m + t < p.M) q[t] = to16<T>(v[t]);
+    for (int t = 0; t < 8; ++t)
+        if (m + t < p.M) q[t] = to16<T>(v.v[t]);
 }
 
-__device__ __forceinline__ void add_4(const GemmArgs& p, int64_t o, int n, const f32x4 v)
+__device__ __forceinline__ void add_8(const GemmArgs& p, int64_t o, int n, const f32x8& v)
 {
     const float sc = p.scale ? p.scale[n] : 1.0f;
     f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p.out[0]) + o);
-    f32x4 c = *q;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(sc, v[t], c[t]);
-    *q = c;
+    for (int h = 0; h < 2; ++h)
+    {
+        f32x4 c = q[h];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(sc, v.v[4 * h + t], c[t]);
+        q[h] = c;
+    }
 }
 
-template <class T> __device__ __forceinline__ void gu_4(const GemmArgs& p, int64_t o, const f32x4 g, const f32x4 u)
+template <class T> __device__ __forceinline__ void gu_8(const GemmArgs& p, int64_t o, const f32x8& g, const f32x8& u)
 {
-    f32x4 h;
+    f32x8 h;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) h[t] = act_h(p.act, g[t], u[t]);
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[0]) + o) = pack4<T>(h);
+    for (int t = 0; t < 8; ++t) h.v[t] = act_h(p.act, g.v[t], u.v[t]);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(h);
     if (p.g)
     {
-        uint16_t gb[4], ub[4];
+        uint16_t gb[8], ub[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) save_gu<T>(p.act, g[t], u[t], gb[t], ub[t]);
-        u32x2 w;
-        w[0] = gb[0] | ((uint32_t)gb[1] << 16); w[1] = gb[2] | ((uint32_t)gb[3] << 16);
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.g) + o) = w;
-        w[0] = ub[0] | ((uint32_t)ub[1] << 16); w[1] = ub[2] | ((uint32_t)ub[3] << 16);
-        *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.u) + o) = w;
+        for (int t = 0; t < 8; ++t) save_gu<T>(p.act, g.v[t], u.v[t], gb[t], ub[t]);
+        u32x4 a, b;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+        {
+            a[i] = gb[2 * i] | (uint32_t)gb[2 * i + 1] << 16;
+            b[i] = ub[2 * i] | (uint32_t)ub[2 * i + 1] << 16;
+        }
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.g) + o) = a;
+        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.u) + o) = b;
     }
 }
 
-template <class T> __device__ __forceinline__ void dgu_4(const GemmArgs& p, int64_t o, const f32x4 dh)
+template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int64_t o, const f32x8& dh)
 {
-    const u32x2 gw = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.g) + o);
-    const u32x2 uw = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(p.u) + o);
-    f32x4 dg, du;
+    const u32x4 gw = ldg4(static_cast<const uint16_t*>(p.g) + o), uw = ldg4(static_cast<const uint16_t*>(p.u) + o);
+    f32x8 dg, du;
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int t = 0; t < 8; ++t)
     {
+        const int sh = (t & 1) * 16;
         float hg, hu;
-        act_grad(p.act, from16<T>((uint16_t)(gw[t >> 1] >> ((t & 1) * 16))), from16<T>((uint16_t)(uw[t >> 1] >> ((t & 1) * 16))), hg, hu);
-        dg[t] = dh[t] * hg;
-        du[t] = dh[t] * hu;
+        act_grad(p.act, from16<T>((uint16_t)(gw[t >> 1] >> sh)), from16<T>((uint16_t)(uw[t >> 1] >> sh)), hg, hu);
+        dg.v[t] = dh.v[t] * hg;
+        du.v[t] = dh.v[t] * hu;
     }
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[0]) + o) = pack4<T>(dg);
-    *reinterpret_cast<u32x2*>(static_cast<uint16_t*>(p.out[1]) + o) = pack4<T>(du);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(dg);
+    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[1]) + o) = pack8<T>(du);
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------
@@ -163,7 +175,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
     constexpr int ABYTES = BM * GK * 2, BBYTES = BN * GK * 2;
     typedef typename Elem<T>::v8 v8;
-    __shared__ __attribute__((aligned(1024))) char lds[2 * (ABYTES + BBYTES)];
+    constexpr int TILES = 2 * (ABYTES + BBYTES), TURN = WM * WN * 32 * (BM / WM + 4) * 4;
+    __shared__ __attribute__((aligned(1024))) char lds[TILES > TURN ? TILES : TURN];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -295,72 +308,96 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         }
     }
 
-    // ---- results: lane l holds column n = l % 32 and rows m = (e / 4) * 8 + (l / 32) * 4 + e % 4 of a fragment ----
-    const int ml = (lane >> 5) * 4, nl = lane & 31;
+    // ---- results ----
+    // A lane's accumulators are column n = l % 32 and rows m = (e / 4) * 8 + (l / 32) * 4 + e % 4 of a fragment: four
+    // neighbouring values of 32 different result rows. Each wave turns 32 result rows at a time over in its own part of
+    // the tiles' LDS (rows padded by 4 floats: 16 lanes at one m fall on different banks), so that what is read and written
+    // in HBM is whole 16-byte pieces of whole rows. (Straight from the accumulators, 8 bytes at a time, the gradient
+    // epilogue of 8,192 x 2,048 values cost 100 us beside a product of 120; this way TURN_US.)
+    constexpr int WROW = BM / WM, LROW = WROW + 4;                  // a wave's columns m, and an LDS row of them
+    float* turn = reinterpret_cast<float*>(lds) + wave * (32 * LROW);
+    const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
+    constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8;   // 8-value pieces of a row
+    __syncthreads();
 #pragma unroll
     for (int j = 0; j < NF; ++j)
     {
-        const int n = n0 + wn * (BN / WN) + j * 32 + nl;
-        if (n >= p.N) continue;
-        if (EPI == EPI_GU)
-        {
-#pragma unroll
-            for (int i = 0; i < MF; i += 2)
-#pragma unroll
-                for (int e = 0; e < 16; e += 4)
-                {
-                    const int m = m0 + (wm * (BM / WM) + i * 32) / 2 + e * 2 + ml;
-                    if (m >= p.M) continue;                         // M % 8 == 0: four values are in or out together
-                    const f32x4 g = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                    const f32x4 u = {acc[i + 1][j][e], acc[i + 1][j][e + 1], acc[i + 1][j][e + 2], acc[i + 1][j][e + 3]};
-                    gu_4<T>(p, (int64_t)n * p.ldo + m, g, u);
-                }
-            continue;
-        }
+        const int nb = n0 + wn * (BN / WN) + j * 32;
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4*>(turn + (lane & 31) * LROW + i * 32 + e * 2 + (lane >> 5) * 4) =
+                    f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
+        // the wave's own rows only: its LDS writes and reads are in order
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+#pragma unroll 2
+        for (int q = lane; q < 32 * PIECES; q += 64)
+        {
+            const int rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
+            if (n >= p.N || m >= p.M) continue;
+            const int64_t o = (int64_t)n * p.ldo + m;
+            auto piece = [&](int col) {
+                f32x8 v;
+                const f32x4 a = *reinterpret_cast<const f32x4*>(turn + rr * LROW + col);
+                const f32x4 b = *reinterpret_cast<const f32x4*>(turn + rr * LROW + col + 4);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) { v.v[t] = a[t]; v.v[t + 4] = b[t]; }
+                return v;
+            };
+            if (EPI == EPI_GU)
             {
-                const int m = m0 + wm * (BM / WM) + i * 32 + e * 2 + ml;
-                if (m >= p.M) continue;
-                const int64_t o = (int64_t)n * p.ldo + m;
-                const f32x4 v = {acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-                if (EPI == EPI_PART) *reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.ldp + m) = v;
-                else if (EPI == EPI_ADD) add_4(p, o, n, v);
-                else if (EPI == EPI_DGU) dgu_4<T>(p, o, v);
-                else store_4<T>(p, p.out[prod], o, m, v);
+                // gate and up rows in turn by 32
+                const int col = (c >> 5) * 64 + (c & 31);
+                gu_8<T>(p, o, piece(col), piece(col + 32));
             }
+            else if (EPI == EPI_PART)
+            {
+                const f32x8 v = piece(c);
+                f32x4* d = reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.ldp + m);
+                d[0] = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
+                d[1] = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
+            }
+            else if (EPI == EPI_ADD) add_8(p, o, n, piece(c));
+            else if (EPI == EPI_DGU) dgu_8<T>(p, o, piece(c));
+            else store_8<T>(p, p.out[prod], o, m, piece(c));
+        }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }
 }
 
-// The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Four values per thread.
+// The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Eight values per
+// thread.
 template <class T, int EPI>
 __global__ __launch_bounds__(256) void gemm_finish_k(const GemmArgs p)
 {
-    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
     if (at >= plane) return;
     const int n = (int)(at / p.ldp), m = (int)(at % p.ldp);
     auto sum = [&](int prod) {
         const float* q = p.part + prod * p.splits * plane + at;
-        f32x4 v = ldg4f(q);
-        for (int s = 1; s < p.splits; ++s)
+        f32x8 v;
+        for (int s = 0; s < p.splits; ++s)
         {
-            const f32x4 w = ldg4f(q + s * plane);
+            const f32x4 a = ldg4f(q + s * plane), b = ldg4f(q + s * plane + 4);
 #pragma unroll
-            for (int t = 0; t < 4; ++t) v[t] += w[t];
+            for (int t = 0; t < 4; ++t)
+            {
+                v.v[t] = s ? v.v[t] + a[t] : a[t];
+                v.v[t + 4] = s ? v.v[t + 4] + b[t] : b[t];
+            }
         }
         return v;
     };
     const int64_t o = (int64_t)n * p.ldo + m;
     if (EPI == EPI_GU)
     {
-        const f32x4 g = sum(0), u = sum(1);
-        gu_4<T>(p, o, g, u);
+        const f32x8 g = sum(0), u = sum(1);
+        gu_8<T>(p, o, g, u);
     }
-    else if (EPI == EPI_ADD) add_4(p, o, n, sum(0));
-    else if (EPI == EPI_DGU) dgu_4<T>(p, o, sum(0));
-    else store_4<T>(p, p.out[0], o, m, sum(0));
+    else if (EPI == EPI_ADD) add_8(p, o, n, sum(0));
+    else if (EPI == EPI_DGU) dgu_8<T>(p, o, sum(0));
+    else store_8<T>(p, p.out[0], o, m, sum(0));
 }
 
 }  // namespace bmx
