@@ -3,7 +3,7 @@ layers, a shared expert that the checkpoint keeps out of the trellis records), f
 
 The reference runs these modules as exllamav3 MLPs beside its BlockSparseMLP hooks (engine/tiers.py:703-739 wraps the routed
 experts only); here the block is a MoELayer's shared_ffn or a module of its own. Every call enqueues on torch's current
-stream of the input's device; nothing synchronises."""
+stream of the weights' device; nothing synchronises."""
 import ctypes
 
 import torch
@@ -15,35 +15,22 @@ DTYPES = {torch.float16: L.DT_FP16, torch.bfloat16: L.DT_BF16}
 
 def rows_of(x, K, dtype, device, name):
     """x [..., K] as contiguous 16-byte aligned rows [T, K] (a copy only where x is neither)."""
-    if not x.is_cuda or x.device != device:
-        raise ValueError(f"{name}: expected a tensor on {device}, got {x.device}")
-    if x.dtype != dtype:
-        raise ValueError(f"{name}: expected {dtype}, got {x.dtype}")
-    if x.dim() < 1 or x.shape[-1] != K:
-        raise ValueError(f"{name}: expected [..., {K}], got {tuple(x.shape)}")
-    if x.dim() != 2:
+    shape = x.shape
+    if x.device != device or x.dtype != dtype or not shape or shape[-1] != K:
+        raise ValueError(f"{name}: expected {dtype} [..., {K}] on {device}, got {x.dtype} {tuple(shape)} on {x.device}")
+    if len(shape) != 2:
         x = x.reshape(-1, K)
     if not x.is_contiguous():
         x = x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-class on_device:
-    """The call's device as the current one, and its current stream (entered with the stream's handle)."""
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.ctx = None
-        if torch.cuda.current_device() != self.device.index:
-            self.ctx = torch.cuda.device(self.device)
-            self.ctx.__enter__()
-        return torch.cuda.current_stream(self.device).cuda_stream
-
-    def __exit__(self, *e):
-        if self.ctx is not None:
-            self.ctx.__exit__(*e)
+def stream_here(device):
+    """The handle of the current stream of device if that is the current device, else None (the caller then enters it:
+    kernels go to the current device). The handle is read without making a Stream object: that costs 2 us, as much as a
+    decode call's other host work together."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(index) if torch.cuda.current_device() == index else None
 
 
 class GatedFFN:
@@ -123,6 +110,10 @@ class GatedFFN:
     def _forward(self, x, keep):
         """y; keep: a list that receives x's rows and the saved g, u, h."""
         r = self._rows(x)
+        s = stream_here(self.device)
+        if s is None:
+            with torch.cuda.device(self.device):
+                return self._forward(x, keep)
         T = r.shape[0]
         y = torch.empty_like(r)
         saved = None
@@ -132,20 +123,23 @@ class GatedFFN:
             saved = L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr())
         if T:
             d, lib = self.desc(r.dtype), L.lib()
-            with on_device(self.device) as s:
-                if self.quantized:
-                    ws = self._workspace(lib.bmx_ffn4_workspace(d, T))
-                    rc = lib.bmx_ffn4_forward(d, r.data_ptr(), T, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
-                else:
-                    ws = self._workspace(lib.bmx_ffn_workspace(d, T))
-                    rc = lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s)
-                L.check(rc, "GatedFFN.forward")
+            if self.quantized:
+                ws = self._workspace(lib.bmx_ffn4_workspace(d, T))
+                rc = lib.bmx_ffn4_forward(d, r.data_ptr(), T, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
+            else:
+                ws = self._workspace(lib.bmx_ffn_workspace(d, T))
+                rc = lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s)
+            L.check(rc, "GatedFFN.forward")
         return y if x.dim() == 2 else y.view(x.shape)
 
     def add_to(self, out, x, gate_vec=None):
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
         layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
         r = self._rows(x.detach())
+        s = stream_here(self.device)
+        if s is None:
+            with torch.cuda.device(self.device):
+                return self.add_to(out, x, gate_vec)
         T = r.shape[0]
         if out.dtype != torch.float32 or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 or \
                 tuple(out.shape) != (T, self.hidden_size):
@@ -156,11 +150,10 @@ class GatedFFN:
             raise ValueError(f"GatedFFN: gate_vec must be a contiguous {r.dtype} tensor of {self.hidden_size} elements")
         if T:
             d, lib = self.desc(r.dtype), L.lib()
-            with on_device(self.device) as s:
-                ws = self._workspace(lib.bmx_ffn4_workspace(d, T) if self.quantized else lib.bmx_ffn_workspace(d, T))
-                call = lib.bmx_ffn4_add if self.quantized else lib.bmx_ffn_add
-                L.check(call(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None, out.data_ptr(),
-                             ws.data_ptr(), ws.numel(), s), "GatedFFN.add_to")
+            ws = self._workspace(lib.bmx_ffn4_workspace(d, T) if self.quantized else lib.bmx_ffn_workspace(d, T))
+            call = lib.bmx_ffn4_add if self.quantized else lib.bmx_ffn_add
+            L.check(call(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None, out.data_ptr(),
+                         ws.data_ptr(), ws.numel(), s), "GatedFFN.add_to")
         return out
 
 
@@ -186,7 +179,8 @@ class _GatedFFNFunction(torch.autograd.Function):
         d, lib = L.FfnDesc(H, I, DTYPES[gate.dtype], ctx.act, ctx.act_limit, 0, gate.data_ptr(), up.data_ptr(),
                            down.data_ptr()), L.lib()
         ptr = lambda t: t.data_ptr() if t is not None else None
-        with on_device(dev) as s:
+        with torch.cuda.device(dev):            # autograd's threads have a current device of their own
+            s = torch.cuda.current_stream().cuda_stream
             need = lib.bmx_ffn_backward_workspace(d, T)
             ws = torch.empty(need, dtype=torch.uint8, device=dev)
             L.check(lib.bmx_ffn_backward(d, ptr(x), T, L.FfnSaved(ptr(g), ptr(u), ptr(h)), ptr(r), ptr(dx), ptr(dw[0]),

@@ -6,7 +6,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check, lib
-from .ffn import DTYPES, on_device, rows_of
+from .ffn import DTYPES, rows_of, stream_here
 
 
 def _stream():
@@ -60,20 +60,26 @@ def router_logits(z, weight):
 
 
 def q4_linear(x, q):
-    """y [..., N] = x W^T for a Q4Matrix q, x [..., K] fp16 or bf16 on the matrix's device; fp32 sums, one rounding."""
-    dt = DTYPES.get(x.dtype)
+    """y [..., N] = x W^T for a Q4Matrix q, x [..., K] fp16 or bf16 on the matrix's device; fp32 sums, one rounding. Enqueued
+    on the current stream of that device."""
+    dtype = x.dtype
+    dt = DTYPES.get(dtype)
     if dt is None:
-        raise ValueError(f"q4_linear: x must be fp16 or bf16, got {x.dtype}")
-    r = rows_of(x, q.K, x.dtype, q.device, "q4_linear: x")
+        raise ValueError(f"q4_linear: x must be fp16 or bf16, got {dtype}")
+    device = q.device
+    r = rows_of(x, q.K, dtype, device, "q4_linear: x")
+    s = stream_here(device)
+    if s is None:
+        with torch.cuda.device(device):
+            return q4_linear(x, q)
     T = r.shape[0]
-    y = torch.empty((T, q.N), dtype=x.dtype, device=q.device)
+    y = torch.empty((T, q.N), dtype=dtype, device=device)
     if T:
         L_ = lib()
-        with on_device(q.device) as s:
-            need = L_.bmx_q4_linear_workspace(q.struct, T)
-            ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-            check(L_.bmx_q4_linear(q.struct, dt, r.data_ptr(), T, y.data_ptr(), ws.data_ptr() if need else None, need, s),
-                  "bmx_q4_linear")
+        need = L_.bmx_q4_linear_workspace(q.struct, T)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        check(L_.bmx_q4_linear(q.struct, dt, r.data_ptr(), T, y.data_ptr(), ws.data_ptr() if need else None, need, s),
+              "bmx_q4_linear")
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (q.N,))
 
 

@@ -3,7 +3,7 @@ that a checkpoint keeps neither in 16 bits nor as EXL3 trellis records."""
 import torch
 
 from . import _lib as L
-from .ffn import DTYPES, on_device
+from .ffn import DTYPES
 
 
 class Q4Matrix:
@@ -35,7 +35,8 @@ class Q4Matrix:
         self.zero = torch.empty(n, dtype=torch.uint8, device=codes.device) if zero is not None else None
         self.struct = L.Q4(N, K, group, DTYPES[scale.dtype], self.codes.data_ptr(), self.scale.data_ptr(),
                            self.zero.data_ptr() if zero is not None else None)
-        with on_device(self.device) as s:
+        with torch.cuda.device(self.device):
+            s = torch.cuda.current_stream().cuda_stream
             L.check(lib.bmx_q4_pack(self.struct, codes.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,
                                     s), "bmx_q4_pack")
 
@@ -68,6 +69,7 @@ class Q4Matrix:
         if dtype not in DTYPES:
             raise ValueError(f"Q4Matrix.dequant: fp16 or bf16, got {dtype}")
         out = torch.empty((self.N, self.K), dtype=dtype, device=self.device)
-        with on_device(self.device) as s:
+        with torch.cuda.device(self.device):
+            s = torch.cuda.current_stream().cuda_stream
             L.check(L.lib().bmx_q4_dequant(self.struct, DTYPES[dtype], out.data_ptr(), s), "bmx_q4_dequant")
         return out

@@ -44,6 +44,7 @@ __device__ __forceinline__ float act_f(const ActPar& p, float g)
 
 __device__ __forceinline__ float act_h(const ActPar& p, float g, float u)
 {
+    if (!p.limited) return g * act_f(p, g) * (u + p.add);
     g = clamp_hi(g, p.Lg);
     return clamp_hi(g * act_f(p, g), p.La) * (clamp_both(u, p.Lu) + p.add);
 }

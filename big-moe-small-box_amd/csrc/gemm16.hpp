@@ -144,27 +144,66 @@ template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int6
 constexpr int GK = 64;      // K of a tile
 
 // LDS position of 16-byte chunk c of row r. Along K: a row is 64 values = 8 chunks; 16 rows at one chunk (a fragment read)
-// fall on 16 different 16-byte columns of the 64 banks. Across K: a row is W values; the 4 rows x 32 bytes that 16 lanes
-// read for a transposition fall on different banks, and so do those of rows 8 further (the next 16 lanes).
+// fall on 16 different 16-byte columns of the 64 banks. Across K: a row is the tile's rows; the 4 rows x 64 bytes that 32 lanes
+// read for a transposition fall on four different quarters of the banks (with 32 bytes as the unit the reads took twice the
+// cycles: 256 bytes go out at a time).
 __device__ __forceinline__ int swz_along(int r) { return (r >> 1) & 7; }
-__device__ __forceinline__ int swz_across(int r) { return ((r & 3) | ((r >> 1) & 4)) << 1; }
+__device__ __forceinline__ int swz_across(int r) { return (r & 3) << 2; }
 
-// One operand's tile of ROWS rows x GK, loaded by NT threads. ACROSS: stored [K][rows].
-template <int ROWS, int NT, bool ACROSS>
+// One operand's tiles of ROWS rows x GK, loaded by NT threads in INSTR loads of 16 bytes each. ACROSS: stored [K][rows].
+// GU: the rows are 32 of one matrix and 32 of a second in turn.
+template <int ROWS, int NT, bool ACROSS, bool GU>
 struct TileLoader {
     static constexpr int INSTR = ROWS * GK * 2 / (NT * 16);
     static constexpr int CPR = ACROSS ? ROWS / 8 : GK / 8;         // chunks of an LDS row
     static constexpr int RPI = NT / CPR;                           // LDS rows of one load of all threads
+    static_assert(RPI % (ACROSS ? 4 : 16) == 0 && (!GU || RPI == 32 || RPI == 64), "later loads' rows are swizzled as the first's, and of one matrix per wave");
+    const char *base0, *base1;      // the tile's first element, in the matrix of the even and of the odd loads
+    int64_t left;       // bytes from there to the matrix's last
+    int64_t step;       // bytes to the next tile along K
+    int rows_ld;        // bytes of a matrix row
     uint32_t voff;      // of this lane's chunk in the first load (bytes from the tile's base)
-    uint32_t step;      // from one load to the next
     int chunk;          // ... its column chunk in the matrix
-    __device__ __forceinline__ void init(int ld)
+    __device__ __forceinline__ void init(int ld, int wave)
     {
-        const int r = threadIdx.x / CPR, p = threadIdx.x % CPR;
+        const int r = GU ? (wave * 8 & 31) + (threadIdx.x & 63) / 8 : threadIdx.x / CPR, p = threadIdx.x % CPR;
         chunk = p ^ (ACROSS ? swz_across(r) : swz_along(r));
         voff = (uint32_t)r * ld * 2 + chunk * 16;
-        step = (uint32_t)RPI * ld * 2;
-        static_assert(RPI % 16 == 0 || ACROSS, "rows of later loads are swizzled as the first's");
+        rows_ld = ld * 2;
+        step = ACROSS ? (int64_t)GK * ld * 2 : GK * 2;
+    }
+    // the tile at row r0 (of the result's side) and column k0, of matrices with `rows` rows and K columns
+    __device__ __forceinline__ void seek(const void* m0, const void* m1, int r0, int k0, int rows, int K, int wave)
+    {
+        const int64_t ld = rows_ld / 2, first = ACROSS ? (int64_t)k0 * ld + r0 : (int64_t)r0 * ld + k0;
+        base0 = static_cast<const char*>(m0) + first * 2;
+        base1 = GU ? static_cast<const char*>(m1) + first * 2 : base0;
+        if (GU && RPI == 64) base0 = base1 = wave & 4 ? base1 : base0;     // one matrix for all of a wave's loads
+        left = ((ACROSS ? K : rows) * ld - first) * 2;
+    }
+    // Offsets past the range load zeros: the bytes left, at most 1 GiB (a tile spans half of that at the widest rows the
+    // entries take). tail: columns of K left; what lies past them in the last tile along K is moved out of the range.
+    __device__ __forceinline__ void load(lds_ptr to, int wave, int tail)
+    {
+        const int range = (int)(left < 0 ? 0 : left > 0x40000000 ? 0x40000000 : left);
+        uint32_t v0 = voff;
+        if (!ACROSS && tail < GK) v0 = chunk * 8 < tail ? v0 : 0x7ff00000u;
+#pragma unroll
+        for (int j = 0; j < INSTR; ++j)
+        {
+            const __amdgpu_buffer_rsrc_t r =
+                __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(j & 1 ? base1 : base0), 0, range, 0x00020000);
+            // rows of one matrix that the loads before have taken
+            const uint32_t at = (uint32_t)(GU ? (j * RPI >> 6) * 32 : j * RPI) * rows_ld;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + wave * 1024 + j * NT * 16), 16,
+                                                     v0 + at, 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ void next()
+    {
+        base0 += step;
+        base1 += step;
+        left -= step;
     }
 };
 
@@ -205,56 +244,26 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         kt_end = kt + q + (sp < r);
     }
 
-    TileLoader<BM, NT, AX> la;
-    TileLoader<BN, NT, BX> lb;
-    la.init(p.lda);
-    lb.init(p.ldb);
-
-    // Range of a tile's loads: the bytes from its first element to the matrix's last, at most 1 GiB (a tile spans half of
-    // that at the widest rows the entries take). Offsets past it load zeros; OUT is past any range.
-    constexpr uint32_t OUT = 0x7ffffff0u;
-    auto rsrc = [](const void* base, int64_t first, int64_t total) {
-        const int64_t left = (total - first) * 2;
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(static_cast<const char*>(base)) + first * 2, 0,
-                                                 (int)(left < 0 ? 0 : left > 0x40000000 ? 0x40000000 : left), 0x00020000);
+    TileLoader<BM, NT, AX, EPI == EPI_GU> la;
+    TileLoader<BN, NT, BX, false> lb;
+    la.init(p.lda, wave);
+    lb.init(p.ldb, wave);
+    int loaded = kt;                                               // the next tile to load
+    auto seek = [&](int pi, int k0) {
+        la.seek(p.a[pi], p.a[1], m0, k0, p.M, p.K, wave);
+        lb.seek(p.b[pi], nullptr, n0, k0, p.N, p.K, wave);
     };
-    auto load_tile = [&](int t, int buf) {
-        const int second = t >= nk1;                                // of a chain
-        const int pi = prod | second;
-        const int k0 = (second ? t - nk1 : t) * GK;
-        lds_ptr base = (lds_ptr)lds + buf * (ABYTES + BBYTES) + wave * 1024;
-        const int tail = p.K - k0;                                  // < GK: the last tile along K
-#pragma unroll
-        for (int j = 0; j < la.INSTR; ++j)
-        {
-            uint32_t v;
-            __amdgpu_buffer_rsrc_t r;
-            if (EPI == EPI_GU)
-            {
-                // this load's rows (8 of one wave) lie in one block of 32, of the gate or of the up matrix
-                const int row = j * la.RPI + wave * 8, blk = row >> 5;
-                const int mi = (blk >> 1) * 32 + (row & 31);        // its first row within the tile's BM / 2
-                r = rsrc(p.a[blk & 1], (int64_t)(m0 + mi) * p.lda + k0, (int64_t)p.M * p.lda);
-                v = la.voff - (uint32_t)(wave * 8) * p.lda * 2;
-            }
-            else
-            {
-                r = AX ? rsrc(p.a[pi], (int64_t)k0 * p.lda + m0, (int64_t)p.K * p.lda)
-                       : rsrc(p.a[pi], (int64_t)m0 * p.lda + k0, (int64_t)p.M * p.lda);
-                v = la.voff + j * la.step;
-            }
-            if (!AX && tail < GK) v = la.chunk * 8 < tail ? v : OUT;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(base + j * NT * 16), 16, v, 0, 0, 0);
-        }
-#pragma unroll
-        for (int j = 0; j < lb.INSTR; ++j)
-        {
-            const __amdgpu_buffer_rsrc_t r = BX ? rsrc(p.b[pi], (int64_t)k0 * p.ldb + n0, (int64_t)p.K * p.ldb)
-                                                : rsrc(p.b[pi], (int64_t)n0 * p.ldb + k0, (int64_t)p.N * p.ldb);
-            uint32_t v = lb.voff + j * lb.step;
-            if (!BX && tail < GK) v = lb.chunk * 8 < tail ? v : OUT;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(base + ABYTES + j * NT * 16), 16, v, 0, 0, 0);
-        }
+    seek(loaded >= nk1 ? 1 : prod, (loaded >= nk1 ? loaded - nk1 : loaded) * GK);
+    auto tail = [&]() { return p.K - (loaded >= nk1 ? loaded - nk1 : loaded) * GK; };
+    auto load_a = [&](int buf) {
+        if (p.chain > 1 && loaded == nk1) seek(1, 0);
+        la.load((lds_ptr)lds + buf * (ABYTES + BBYTES), wave, tail());
+    };
+    auto load_b = [&](int buf) {
+        lb.load((lds_ptr)lds + buf * (ABYTES + BBYTES) + ABYTES, wave, tail());
+        la.next();
+        lb.next();
+        ++loaded;
     };
 
     // A fragment (32 rows from row0, 16 of K from ks * 16): lane l holds row l % 32, K (l / 32) * 8 .. + 7
@@ -286,26 +295,62 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    load_tile(kt, 0);
-    for (int buf = 0; kt < kt_end; ++kt, buf ^= 1)
-    {
-        __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt 0: this wave's loads of tile kt are in LDS
-        __syncthreads();                                            // everyone's are, and the other half is read
-        if (kt + 1 < kt_end) load_tile(kt + 1, buf ^ 1);
+    // Fragments are read one step of 16 ahead of their products, across tiles too: the last step's products of a tile run
+    // while the next tile's first fragments are read, so the only wait of all waves for each other (the next tile has
+    // landed, and this one is read to the end) has products on both sides.
+    constexpr int KS = GK / 16;
+    v8 a[2][MF], b[2][NF];
+    auto read = [&](int set, int buf, int ks) {
         lds_ptr at = (lds_ptr)lds + buf * (ABYTES + BBYTES), bt = at + ABYTES;
 #pragma unroll
-        for (int ks = 0; ks < GK / 16; ++ks)
+        for (int i = 0; i < MF; ++i) a[set][i] = frag(at, wm * (BM / WM) + i * 32, ks, AX, BM);
+#pragma unroll
+        for (int j = 0; j < NF; ++j) b[set][j] = frag(bt, wn * (BN / WN) + j * 32, ks, BX, BN);
+    };
+    auto products = [&](int set) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j) acc[i][j] = Elem<T>::mfma32(a[set][i], b[set][j], acc[i][j]);
+    };
+    auto landed = [&]() {
+        __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt 0: this wave's loads are in LDS
+        lds_barrier();
+    };
+    load_a(0);
+    load_b(0);
+    landed();
+    if (kt + 1 < kt_end) { load_a(1); load_b(1); }
+    read(0, 0, 0);
+    // 256-row tiles: the loads of the tile after the next go out in two parts, behind the fragment reads and ahead of the
+    // products of the first two steps: all at once, or right behind the wait, they hold the products up (286 -> 301 us on
+    // 4,096 x 4,096 x 11,008), and later they land too late (298 us). 128-row tiles have half the products to wait behind
+    // (and a second workgroup to fill in): right behind the wait (390 -> 342 us on the same).
+    constexpr bool SPREAD = MF * NF >= 8;
+    bool fill = false;
+    for (int buf = 0; kt < kt_end; ++kt, buf ^= 1)
+    {
+#pragma unroll
+        for (int ks = 0; ks < KS - 1; ++ks)
         {
-            v8 a[MF], b[NF];
-#pragma unroll
-            for (int i = 0; i < MF; ++i) a[i] = frag(at, wm * (BM / WM) + i * 32, ks, AX, BM);
-#pragma unroll
-            for (int j = 0; j < NF; ++j) b[j] = frag(bt, wn * (BN / WN) + j * 32, ks, BX, BN);
-#pragma unroll
-            for (int i = 0; i < MF; ++i)
-#pragma unroll
-                for (int j = 0; j < NF; ++j) acc[i][j] = Elem<T>::mfma32(a[i], b[j], acc[i][j]);
+            read((ks + 1) & 1, buf, ks + 1);
+            if (SPREAD && fill)
+            {
+                if (ks == 0) load_a(buf ^ 1);
+                if (ks == 1) load_b(buf ^ 1);
+            }
+            products(ks & 1);
+            if (SPREAD) __builtin_amdgcn_sched_barrier(0);
         }
+        if (kt + 1 < kt_end)
+        {
+            landed();
+            if (!SPREAD && loaded < kt_end) { load_a(buf); load_b(buf); }
+            read(0, buf ^ 1, 0);
+        }
+        fill = loaded < kt_end;
+        products((KS - 1) & 1);
+        if (SPREAD) __builtin_amdgcn_sched_barrier(0);
     }
 
     // ---- results ----
@@ -313,7 +358,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     // neighbouring values of 32 different result rows. Each wave turns 32 result rows at a time over in its own part of
     // the tiles' LDS (rows padded by 4 floats: 16 lanes at one m fall on different banks), so that what is read and written
     // in HBM is whole 16-byte pieces of whole rows. (Straight from the accumulators, 8 bytes at a time, the gradient
-    // epilogue of 8,192 x 2,048 values cost 100 us beside a product of 120; this way TURN_US.)
+    // epilogue of 8,192 x 2,048 values cost 100 us beside a product of 120; this way about 25.)
     constexpr int WROW = BM / WM, LROW = WROW + 4;                  // a wave's columns m, and an LDS row of them
     float* turn = reinterpret_cast<float*>(lds) + wave * (32 * LROW);
     const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
