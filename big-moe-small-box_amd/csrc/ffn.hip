@@ -50,7 +50,7 @@ static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
     int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.big, s);
     if (rc) return rc;
     const int64_t pieces = (int64_t)a.ldp / 8 * a.N;
-    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a);
     return check_launch("gemm_finish");
 }
 
@@ -117,25 +117,24 @@ static FfnIn ffn_in(const bmx_ffn4_desc* d)
 
 struct FfnPlan {
     TilePlan gu, down;
-    bool skinny_gu, skinny_down;
+    bool few;                               // tokens: skinny products
     size_t h, part, gate, deq, total;       // workspace offsets
 };
 
 static FfnPlan ffn_plan(const FfnIn& d, int T)
 {
     FfnPlan p;
-    p.skinny_gu = T <= skinny_tokens_max(d.group());
-    p.skinny_down = T <= skinny_tokens_max(d.q[2] ? d.q[2]->group : 0);
+    p.few = T <= skinny_tokens_max();
     p.gu = plan_product(2 * (int64_t)d.I, T, tiles_k(d.H), 1, true);
     p.down = plan_product(d.H, T, tiles_k(d.I), 1, true);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
     p.h = take((size_t)T * d.I * 2);
     p.gate = take((size_t)T * 4);
-    const size_t pg = !p.skinny_gu && p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d.I * 4 : 0;
-    const size_t pd = !p.skinny_down && p.down.splits > 1 ? (size_t)p.down.splits * T * d.H * 4 : 0;
+    const size_t pg = p.few ? skinny_part_bytes(d.I, d.H, T, 2) : p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d.I * 4 : 0;
+    const size_t pd = p.few ? skinny_part_bytes(d.H, d.I, T, 1) : p.down.splits > 1 ? (size_t)p.down.splits * T * d.H * 4 : 0;
     p.part = take(pg > pd ? pg : pd);
-    p.deq = take(!d.q[0] ? 0 : !p.skinny_gu ? (size_t)d.H * d.I * 4 : !p.skinny_down ? (size_t)d.H * d.I * 2 : 0);
+    p.deq = take(d.q[0] && !p.few ? (size_t)d.H * d.I * 4 : 0);
     p.total = o + 256;
     return p;
 }
@@ -168,7 +167,7 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
     char* deq = ws + p.deq;
 
     // h = act(x Wg^T, x Wu^T)
-    if (p.skinny_gu)
+    if (p.few)
     {
         for (int m = 0; m < 2; ++m)
         {
@@ -179,7 +178,7 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
         k.x = static_cast<const uint16_t*>(x);
         k.N = d.I; k.K = d.H; k.out = h; k.ldo = d.I;
         if (sv) { k.g = static_cast<uint16_t*>(sv->g); k.u = static_cast<uint16_t*>(sv->u); }
-        if ((rc = launch_skinny(k, d.dtype, EPI_GU, s))) return rc;
+        if ((rc = launch_skinny(k, d.dtype, EPI_GU, a.part, s))) return rc;
     }
     else
     {
@@ -195,14 +194,14 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
     }
     // y = h Wd^T
     void* out = add ? static_cast<void*>(add) : y;
-    if (p.skinny_down)
+    if (p.few)
     {
         k.w[0] = d.w[2];
         if (d.q[0]) k.q[0] = q4_view(d.q[2]);
         k.group = d.q[0] ? d.q[2]->group : 0;
         k.x = static_cast<const uint16_t*>(h);
         k.N = d.H; k.K = d.I; k.out = out; k.ldo = d.H;
-        return launch_skinny(k, d.dtype, add ? EPI_ADD : EPI_STORE, s);
+        return launch_skinny(k, d.dtype, add ? EPI_ADD : EPI_STORE, a.part, s);
     }
     a.a[0] = d.q[0] ? deq : d.w[2];
     if (d.q[0] && (rc = launch_q4_dequant(d.q[2], d.dtype, deq, s))) return rc;

@@ -414,23 +414,36 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
 // The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Eight values per
 // thread.
 template <class T, int EPI>
-__global__ __launch_bounds__(256) void gemm_finish_k(const GemmArgs p)
+__global__ __launch_bounds__(64) void gemm_finish_k(const GemmArgs p)
 {
-    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8;
     if (at >= plane) return;
     const int n = (int)(at / p.ldp), m = (int)(at % p.ldp);
     auto sum = [&](int prod) {
         const float* q = p.part + prod * p.splits * plane + at;
         f32x8 v;
-        for (int s = 0; s < p.splits; ++s)
-        {
-            const f32x4 a = ldg4f(q + s * plane), b = ldg4f(q + s * plane + 4);
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+        for (int t = 0; t < 8; ++t) v.v[t] = 0.0f;
+        // eight splits' loads at a time: one after the other they would each wait for HBM
+        for (int s0 = 0; s0 < p.splits; s0 += 8)
+        {
+            f32x4 a[8], b[8];
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
             {
-                v.v[t] = s ? v.v[t] + a[t] : a[t];
-                v.v[t + 4] = s ? v.v[t + 4] + b[t] : b[t];
+                const float* w = q + min(s0 + s, p.splits - 1) * plane;
+                a[s] = ldg4f(w);
+                b[s] = ldg4f(w + 4);
             }
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s0 + s < p.splits)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                    {
+                        v.v[t] += a[s][t];
+                        v.v[t + 4] += b[s][t];
+                    }
         }
         return v;
     };

@@ -107,46 +107,117 @@ int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s)
 
 // ---- products of few tokens ---------------------------------------------------------------------------------------------
 
-template <class T, int NM, int TT, int G, int EPI> static int skinny_launch(const SkinnyArgs& a, hipStream_t s)
+// Tokens up to which skinny_k reads W once past x from the caches; above, slices
+static int direct_tokens() { return 16; }
+
+int skinny_tokens_max() { return SL_TT * 16; }
+
+static int padded(int n) { return (n + 7) / 8 * 8; }
+static int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
+
+size_t skinny_part_bytes(int N, int K, int T, int products)
 {
-    const dim3 grid((unsigned)((a.N + 15) / 16), (unsigned)((a.T + TT * 16 - 1) / (TT * 16)));
-    hipLaunchKernelGGL((skinny_k<T, NM, 1, TT, G, EPI>), grid, dim3(SK_W * 64), 0, s, a);
-    return check_launch("skinny");
+    return T <= direct_tokens() ? 0 : (size_t)products * slices_of(K) * T * padded(N) * 4;
 }
 
-template <class T, int NM, int G, int EPI> static int skinny_tokens(const SkinnyArgs& a, hipStream_t s)
+template <class T, int TT, int G> static int slice_launch(const SliceArgs& a, dim3 grid, hipStream_t s)
 {
-    if (a.T <= 16) return skinny_launch<T, NM, 1, G, EPI>(a, s);
-    if (a.T <= 32) return skinny_launch<T, NM, 2, G, EPI>(a, s);
-    return skinny_launch<T, NM, 4, G, EPI>(a, s);
+    hipLaunchKernelGGL((slice_k<T, TT, G>), grid, dim3(SL_W * 64), 0, s, a);
+    return check_launch("slice");
 }
 
-template <class T, int NM, int EPI> static int skinny_group(const SkinnyArgs& a, hipStream_t s)
+template <class T, int G> static int slice_tokens(const SliceArgs& a, dim3 grid, hipStream_t s)
 {
-    switch (a.group)
+    switch ((a.a.T + 15) / 16)
     {
-        case 0: return skinny_tokens<T, NM, 0, EPI>(a, s);
-        case 32: return skinny_tokens<T, NM, 32, EPI>(a, s);
-        case 64: return skinny_tokens<T, NM, 64, EPI>(a, s);
-        default: return skinny_tokens<T, NM, 128, EPI>(a, s);
+        case 1: return slice_launch<T, 1, G>(a, grid, s);
+        case 2: return slice_launch<T, 2, G>(a, grid, s);
+        case 3: return slice_launch<T, 3, G>(a, grid, s);
+        case 4: return slice_launch<T, 4, G>(a, grid, s);
+        default: return slice_launch<T, 5, G>(a, grid, s);
     }
 }
 
-int skinny_tokens_max(int group) { return 64; }
+template <class T, int EPI> static int slice_product(const SkinnyArgs& k, float* part, hipStream_t s)
+{
+    SliceArgs a;
+    a.a = k;
+    a.products = EPI == EPI_GU ? 2 : 1;
+    a.slices = slices_of(k.K);
+    a.ldp = padded(k.N);
+    a.tiles = (k.N + 15) / 16 * a.products;
+    a.part = part;
+    // up to 768 workgroups (three on a compute unit at 48 tokens), of at least a tile per wave
+    const int blocks = 768 / a.slices > 0 ? 768 / a.slices : 1;
+    a.per = ((a.tiles + blocks - 1) / blocks + SL_W - 1) / SL_W * SL_W;
+    const dim3 grid((unsigned)((a.tiles + a.per - 1) / a.per), (unsigned)a.slices);
+    int rc;
+    switch (k.group)
+    {
+        case 0: rc = slice_tokens<T, 0>(a, grid, s); break;
+        case 32: rc = slice_tokens<T, 32>(a, grid, s); break;
+        case 64: rc = slice_tokens<T, 64>(a, grid, s); break;
+        default: rc = slice_tokens<T, 128>(a, grid, s);
+    }
+    if (rc) return rc;
+    GemmArgs g = {};
+    g.M = k.N; g.N = k.T; g.ldp = a.ldp; g.splits = a.slices; g.part = part;
+    g.out[0] = k.out; g.ldo = k.ldo; g.scale = k.scale; g.act = k.act; g.g = k.g; g.u = k.u;
+    const int64_t pieces = (int64_t)a.ldp / 8 * k.T;
+    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, g);
+    return check_launch("gemm_finish");
+}
 
-int launch_skinny(const SkinnyArgs& a, int dtype, int epi, hipStream_t s)
+template <class T, int RT, int G, int EPI, bool XL> static int direct_rows(const SkinnyArgs& a, hipStream_t s)
+{
+    constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT, D = 2;
+    hipLaunchKernelGGL((skinny_k<T, RT, G, D, EPI, XL>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(SK_W * 64),
+                       XL ? (size_t)a.T * (a.K * 2 + 16) : 0, s, a);
+    return check_launch("skinny");
+}
+
+// Tiles of rows per workgroup: x is read once per workgroup, so that above 8 tokens two tiles halve what outweighs W, as long
+// as the workgroups still cover half the chip (16 tokens, us with 1 / 2 / 4 tiles: 4-bit 5120 -> 2 x 2304 13.1 / 9.0 / 11.1,
+// 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 / 11.5 / 9.7; 16-bit 2304 -> 5120 9.8 / 8.0 / 12.0, 4096 -> 2 x 2048 10.8
+// / 13.0 / 20; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5)
+template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a, hipStream_t s)
+{
+    const int tiles = (a.N + 15) / 16 * (EPI == EPI_GU ? 2 : 1);
+    if constexpr (G != 0)
+    {
+        if (a.T > 8 && tiles >= 768) return direct_rows<T, 4, G, EPI, false>(a, s);
+        if ((size_t)a.T * a.K <= 8192) return direct_rows<T, 1, G, EPI, true>(a, s);
+    }
+    if (a.T > 8 && tiles >= 288) return direct_rows<T, 2, G, EPI, false>(a, s);
+    return direct_rows<T, 1, G, EPI, false>(a, s);
+}
+
+template <class T, int EPI> static int few_tokens(const SkinnyArgs& a, float* part, hipStream_t s)
+{
+    if (a.T > direct_tokens()) return slice_product<T, EPI>(a, part, s);
+    switch (a.group)
+    {
+        case 0: return direct_launch<T, 0, EPI>(a, s);
+        case 32: return direct_launch<T, 32, EPI>(a, s);
+        case 64: return direct_launch<T, 64, EPI>(a, s);
+        default: return direct_launch<T, 128, EPI>(a, s);
+    }
+}
+
+int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s)
 {
     const bool h = dtype == BMX_DT_FP16;
-    if (epi == EPI_GU) return h ? skinny_group<f16, 2, EPI_GU>(a, s) : skinny_group<bf16, 2, EPI_GU>(a, s);
-    if (epi == EPI_ADD) return h ? skinny_group<f16, 1, EPI_ADD>(a, s) : skinny_group<bf16, 1, EPI_ADD>(a, s);
-    return h ? skinny_group<f16, 1, EPI_STORE>(a, s) : skinny_group<bf16, 1, EPI_STORE>(a, s);
+    if (epi == EPI_GU) return h ? few_tokens<f16, EPI_GU>(a, part, s) : few_tokens<bf16, EPI_GU>(a, part, s);
+    if (epi == EPI_ADD) return h ? few_tokens<f16, EPI_ADD>(a, part, s) : few_tokens<bf16, EPI_ADD>(a, part, s);
+    return h ? few_tokens<f16, EPI_STORE>(a, part, s) : few_tokens<bf16, EPI_STORE>(a, part, s);
 }
 
 // ---- y = x W^T ----------------------------------------------------------------------------------------------------------
 
 static size_t q4_linear_ws(const bmx_q4* q, int T)
 {
-    return skinny_tokens_max(q->group) >= T ? 0 : align_up((size_t)q->N * q->K * 2, 256) + product_part_bytes(q->N, T, q->K);
+    if (T <= skinny_tokens_max()) return skinny_part_bytes(q->N, q->K, T, 1);
+    return align_up((size_t)q->N * q->K * 2, 256) + product_part_bytes(q->N, T, q->K);
 }
 
 }  // namespace bmx
@@ -213,7 +284,7 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
         return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", fn);
     if (workspace_bytes < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, need);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (need)
+    if (T > skinny_tokens_max())
     {
         // many tokens: the weights once to 16 bits, then the tiled product
         if ((rc = launch_q4_dequant(q, dtype, workspace, s))) return rc;
@@ -224,7 +295,7 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
     a.x = static_cast<const uint16_t*>(x);
     a.T = T; a.N = q->N; a.K = q->K; a.group = q->group;
     a.out = y; a.ldo = q->N;
-    return launch_skinny(a, dtype, EPI_STORE, s);
+    return launch_skinny(a, dtype, EPI_STORE, static_cast<float*>(workspace), s);
 }
 
 }  // extern "C"

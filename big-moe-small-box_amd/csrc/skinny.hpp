@@ -1,7 +1,8 @@
-// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. Each wave takes 16
-// rows of W (RT tiles of 16) at every W-th 128 columns, straight from HBM to MFMA operands, so that a lane's loads are its
-// fragment and no LDS stands between; x comes through the caches in the same layout. The waves' sums are joined through LDS
-// in the waves' order (the result does not depend on timing).
+// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. A workgroup has 16 or
+// 32 rows of W (half of gate and half of up in the gated product); each of its waves takes every SK_W-th 128 columns of them straight
+// from HBM to MFMA operands, so that a lane's loads are its fragment and no LDS stands between, several steps ahead of the
+// products; x comes through the caches in the same layout. The waves' sums are joined through LDS in the waves' order (the
+// result does not depend on timing).
 //
 // v_mfma_f32_16x16x32: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 8 .. + 7; of
 // the result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3. Fewer than 16 tokens load a token again: those
@@ -40,10 +41,12 @@ struct SkinnyArgs {
 Q4View q4_view(const bmx_q4* q);
 int check_q4(const bmx_q4* q, const char* who);
 int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s);
-// skinny_k on a's weights (a.group 0: 16-bit) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU)
-int launch_skinny(const SkinnyArgs& a, int dtype, int epi, hipStream_t s);
-// the most tokens that skinny_k takes
-int skinny_tokens_max(int group);
+// A product of few tokens on a's weights (a.group 0: 16-bit) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU); part:
+// skinny_part_bytes bytes
+int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s);
+size_t skinny_part_bytes(int N, int K, int T, int products);
+// the most tokens that it takes
+int skinny_tokens_max();
 // ffn.hip: y [T][N] = x w^T with 16-bit weights on gemm16_k; part: product_part_bytes bytes
 int launch_product(const void* w, const void* x, int T, int N, int K, int dtype, void* y, void* part, hipStream_t s);
 size_t product_part_bytes(int N, int T, int K);
@@ -88,170 +91,360 @@ template <> struct Q4Dec<bf16>
     }
 };
 
-// NM: matrices (2: gate and up), RT: tiles of 16 rows a wave takes of each, TT: tiles of 16 tokens, G: group size (0: 16-bit
-// weights)
-template <class T, int NM, int RT, int TT, int G, int EPI>
+// RT: tiles of 16 rows of W (each 8 of gate and 8 of up in the gated product), G: group size (0: 16-bit weights), D: steps of
+// 128 columns in flight per wave, XL: x in LDS (dynamic, p.T rows of K values and 16 bytes): where x is small, a fragment read
+// from there costs a sixteenth of the cache lines that one from HBM asks for, which 4-bit weights notice (one token 4096 ->
+// 14336: 8.6 -> 8.0 us) and 16-bit weights do not
+template <class T, int RT, int G, int D, int EPI, bool XL>
 __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 {
     typedef typename Elem<T>::v8 v8;
-    constexpr bool Q4 = G != 0;
+    constexpr bool Q4 = G != 0, GU = EPI == EPI_GU;
     constexpr int NG = Q4 ? SK_K / G : 1, JG = 4 / NG;             // groups of a step, words of a group
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * (RT * 16), t0 = blockIdx.y * (TT * 16);
-    const int KT = (p.K + SK_K - 1) / SK_K, NT = (p.N + 15) / 16;
-
-    f32x4 acc[NM][RT][TT];
+    constexpr int ROWS = GU ? 8 : 16;                              // result columns of a tile
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int n0 = blockIdx.x * (ROWS * RT);
+    const int KT = (p.K + SK_K - 1) / SK_K;
+    // this lane's rows of W, and whose (rows past the last load it again)
+    const int mat = GU ? r >> 3 : 0;
+    const Q4View v = p.q[mat];
+    const u32x4* codes[RT];
+    int64_t sg[RT];
+    const uint16_t* w16[RT];
 #pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int t = 0; t < TT; ++t) acc[m][i][t] = f32x4{0, 0, 0, 0};
-
-    const uint16_t* xr[TT];
-#pragma unroll
-    for (int t = 0; t < TT; ++t) xr[t] = p.x + (int64_t)min(t0 + t * 16 + r, p.T - 1) * p.K + q * 8;
-
-    for (int kt = wave; kt < KT; kt += SK_W)
+    for (int i = 0; i < RT; ++i)
     {
+        const int n = min(n0 + i * ROWS + (GU ? r & 7 : r), p.N - 1);
+        codes[i] = v.codes + (int64_t)(n >> 4) * KT * 64 + q * 16 + (n & 15);
+        sg[i] = (int64_t)(n >> 4) * (KT * NG) * 16 + (n & 15);
+        w16[i] = static_cast<const uint16_t*>(p.w[mat]) + (int64_t)n * p.K + q * 8;
+    }
+    const uint16_t* xr = p.x + (int64_t)min(r, p.T - 1) * p.K + q * 8;
+    extern __shared__ __attribute__((aligned(16))) char xl[];
+    const int xrow = p.K * 2 + 16;
+
+    struct Step {
+        u32x4 w[RT][Q4 ? 1 : 4], x[XL ? 1 : 4];
+        uint16_t s[RT][NG];
+        uint8_t z[RT][NG];
+    } st[D];
+    auto load = [&](Step& b, int kt) {
         const int k0 = kt * SK_K;
-        u32x4 xv[4][TT];
-        // weights, then x; past K both are 0
-        u32x4 wv[NM][RT][Q4 ? 1 : 4];
-#pragma unroll
-        for (int m = 0; m < NM; ++m)
+        if (Q4)
+        {
 #pragma unroll
             for (int i = 0; i < RT; ++i)
             {
-                if (Q4)
-                {
-                    const int tile = min(blockIdx.x * RT + i, (unsigned)NT - 1);
-                    wv[m][i][0] = ldg4(p.q[m].codes + ((int64_t)tile * KT + kt) * 64 + lane);
-                }
-                else
-                {
-                    const uint16_t* w = static_cast<const uint16_t*>(p.w[m]) + (int64_t)min(n0 + i * 16 + r, p.N - 1) * p.K + q * 8;
+                b.w[i][0] = ldg4(codes[i] + (int64_t)kt * 64);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                    {
-                        const int k = k0 + j * 32;
-                        const bool in = k + q * 8 < p.K;
-                        wv[m][i][j] = in ? ldg4(w + k) : u32x4{0, 0, 0, 0};
-                    }
+                for (int g = 0; g < NG; ++g)
+                {
+                    b.s[i][g] = v.scale[sg[i] + (kt * NG + g) * 16];
+                    b.z[i][g] = v.zero ? v.zero[sg[i] + (kt * NG + g) * 16] : 8;
                 }
             }
-#pragma unroll
-        for (int t = 0; t < TT; ++t)
+        }
+        if (k0 + SK_K <= p.K)
+        {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
             {
-                const int k = k0 + j * 32;
-                xv[j][t] = k + q * 8 < p.K ? ldg4(xr[t] + k) : u32x4{0, 0, 0, 0};
-            }
-        if (Q4)
-        {
-            const int groups = KT * NG;
+                if (!Q4)
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi)
-            {
-                f32x4 xs[TT];                                      // the group's sums of x (bf16)
-                v8 ones;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
-#pragma unroll
-                for (int t = 0; t < TT; ++t)
-                {
-                    xs[t] = f32x4{0, 0, 0, 0};
-                    if (Q4Dec<T>::OFFSET)
-#pragma unroll
-                        for (int j = 0; j < JG; ++j)
-                            xs[t] = Elem<T>::mfma16(__builtin_bit_cast(v8, xv[gi * JG + j][t]), ones, xs[t]);
-                }
-#pragma unroll
-                for (int m = 0; m < NM; ++m)
-#pragma unroll
-                    for (int i = 0; i < RT; ++i)
-                    {
-                        const int tile = min(blockIdx.x * RT + i, (unsigned)NT - 1);
-                        const int64_t at = ((int64_t)tile * groups + kt * NG + gi) * 16 + r;
-                        const uint16_t sb = p.q[m].scale[at];
-                        const float s = p.q[m].scale_bf16 ? from16<bf16>(sb) : from16<f16>(sb);
-                        const float z = p.q[m].zero ? (float)p.q[m].zero[at] : 8.0f;
-                        Q4Dec<T> dec;
-                        dec.zero(z);
-                        f32x4 part[TT];
-#pragma unroll
-                        for (int t = 0; t < TT; ++t) part[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < JG; ++j)
-                        {
-                            const v8 w = dec(wv[m][i][0][gi * JG + j]);
-#pragma unroll
-                            for (int t = 0; t < TT; ++t)
-                                part[t] = Elem<T>::mfma16(__builtin_bit_cast(v8, xv[gi * JG + j][t]), w, part[t]);
-                        }
-#pragma unroll
-                        for (int t = 0; t < TT; ++t)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                            {
-                                const float v = Q4Dec<T>::OFFSET ? __builtin_fmaf(-128.0f - z, xs[t][e], part[t][e]) : part[t][e];
-                                acc[m][i][t][e] = __builtin_fmaf(s, v, acc[m][i][t][e]);
-                            }
-                    }
+                    for (int i = 0; i < RT; ++i) b.w[i][Q4 ? 0 : j] = ldg4(w16[i] + k0 + j * 32);
+                if (!XL) b.x[XL ? 0 : j] = ldg4(xr + k0 + j * 32);
             }
         }
         else
         {
+            // the last columns: x and 16-bit weights past K are 0
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+            {
+                const bool in = k0 + j * 32 + q * 8 < p.K;
+                if (!Q4)
+#pragma unroll
+                    for (int i = 0; i < RT; ++i) b.w[i][Q4 ? 0 : j] = in ? ldg4(w16[i] + k0 + j * 32) : u32x4{0, 0, 0, 0};
+                if (!XL) b.x[XL ? 0 : j] = in ? ldg4(xr + k0 + j * 32) : u32x4{0, 0, 0, 0};
+            }
+        }
+    };
+
+    f32x4 acc[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    auto multiply = [&](const Step& b, int kt) {
+        auto x = [&](int j) {
+            if (!XL) return __builtin_bit_cast(v8, b.x[XL ? 0 : j]);
+            const int k = kt * SK_K + j * 32 + q * 8;
+            const u32x4 v = *reinterpret_cast<const u32x4*>(xl + min(r, p.T - 1) * xrow + (k < p.K ? k : p.K) * 2);
+            return __builtin_bit_cast(v8, v);
+        };
+        if (!Q4)
+        {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int m = 0; m < NM; ++m)
+                for (int i = 0; i < RT; ++i) acc[i] = Elem<T>::mfma16(x(j), __builtin_bit_cast(v8, b.w[i][Q4 ? 0 : j]), acc[i]);
+            return;
+        }
 #pragma unroll
-                    for (int i = 0; i < RT; ++i)
+        for (int g = 0; g < NG; ++g)
+        {
+            v8 xv[JG], ones;
 #pragma unroll
-                        for (int t = 0; t < TT; ++t)
-                            acc[m][i][t] = Elem<T>::mfma16(__builtin_bit_cast(v8, xv[j][t]), __builtin_bit_cast(v8, wv[m][i][j]),
-                                                           acc[m][i][t]);
+            for (int j = 0; j < JG; ++j) xv[j] = x(g * JG + j);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ones[e] = (T)1.0f;
+            f32x4 xs = {0, 0, 0, 0};                               // the group's sums of x (bf16)
+            if (Q4Dec<T>::OFFSET)
+#pragma unroll
+                for (int j = 0; j < JG; ++j) xs = Elem<T>::mfma16(xv[j], ones, xs);
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+            {
+                const float s = v.scale_bf16 ? from16<bf16>(b.s[i][g]) : from16<f16>(b.s[i][g]), z = (float)b.z[i][g];
+                Q4Dec<T> dec;
+                dec.zero(z);
+                f32x4 part = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < JG; ++j) part = Elem<T>::mfma16(xv[j], dec(b.w[i][0][g * JG + j]), part);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    acc[i][e] = __builtin_fmaf(s, Q4Dec<T>::OFFSET ? __builtin_fmaf(-128.0f - z, xs[e], part[e]) : part[e], acc[i][e]);
+            }
+        }
+    };
+
+    int kt = wave;                                                 // the next step to multiply; D are in flight
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        if (kt + d * SK_W < KT) load(st[d], kt + d * SK_W);
+    if (XL)
+    {
+        // the rows, each with 16 bytes of zeros behind it for the columns past K
+        for (int t = 0; t < p.T; ++t)
+            for (int c = threadIdx.x; c <= p.K / 8; c += SK_W * 64)
+                *reinterpret_cast<u32x4*>(xl + t * xrow + c * 16) = c < p.K / 8 ? ldg4(p.x + (int64_t)t * p.K + c * 8) : u32x4{0, 0, 0, 0};
+        __syncthreads();
+    }
+    while (kt < KT)
+    {
+#pragma unroll
+        for (int d = 0; d < D; ++d)
+        {
+            if (kt >= KT) break;
+            multiply(st[d], kt);
+            if (kt + D * SK_W < KT) load(st[d], kt + D * SK_W);
+            kt += SK_W;
         }
     }
 
-    // join the waves: value v of a matrix = (row tile, token tile, element, lane)
-    constexpr int V = RT * TT * 256;
-    __shared__ float part[SK_W][NM * V];
+    // join the waves
+    constexpr int V = RT * 256;                                    // (row tile, element, lane)
+    __shared__ float part[SK_W][V];
 #pragma unroll
-    for (int m = 0; m < NM; ++m)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int t = 0; t < TT; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[wave][m * V + ((i * TT + t) * 4 + e) * 64 + lane] = acc[m][i][t][e];
+        for (int e = 0; e < 4; ++e) part[wave][(i * 4 + e) * 64 + lane] = acc[i][e];
     __syncthreads();
-    for (int v = threadIdx.x; v < V; v += SK_W * 64)
+    for (int i = threadIdx.x; i < V; i += SK_W * 64)
     {
-        const int l = v & 63, e = (v >> 6) & 3, t = t0 + (v >> 8) % TT * 16 + (l >> 4) * 4 + e, n = n0 + (v >> 8) / TT * 16 + (l & 15);
-        if (t >= p.T || n >= p.N) continue;
-        float s[NM];
+        const int c = i & 15, t = ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + (i >> 8) * ROWS + c;
+        if (t >= p.T || c >= ROWS || n >= p.N) continue;
+        auto sum = [&](int at) {
+            float s = part[0][at];
 #pragma unroll
-        for (int m = 0; m < NM; ++m)
-        {
-            s[m] = part[0][m * V + v];
-#pragma unroll
-            for (int w = 1; w < SK_W; ++w) s[m] += part[w][m * V + v];
-        }
+            for (int w = 1; w < SK_W; ++w) s += part[w][at];
+            return s;
+        };
+        const float s = sum(i);
         const int64_t o = (int64_t)t * p.ldo + n;
         if (EPI == EPI_GU)
         {
-            static_cast<uint16_t*>(p.out)[o] = to16<T>(act_h(p.act, s[0], s[NM - 1]));
-            if (p.g) save_gu<T>(p.act, s[0], s[NM - 1], p.g[o], p.u[o]);
+            const float u = sum(i + 8);
+            static_cast<uint16_t*>(p.out)[o] = to16<T>(act_h(p.act, s, u));
+            if (p.g) save_gu<T>(p.act, s, u, p.g[o], p.u[o]);
         }
         else if (EPI == EPI_ADD)
         {
             float* y = static_cast<float*>(p.out) + o;
-            *y = __builtin_fmaf(p.scale ? p.scale[t] : 1.0f, s[0], *y);
+            *y = __builtin_fmaf(p.scale ? p.scale[t] : 1.0f, s, *y);
         }
-        else static_cast<uint16_t*>(p.out)[o] = to16<T>(s[0]);
+        else static_cast<uint16_t*>(p.out)[o] = to16<T>(s);
+    }
+}
+
+// ---- more tokens: slices of K ---------------------------------------------------------------------------------------------
+// From some tokens on what skinny_k reads of x (16 tokens for every 16 rows of W) outgrows W. Here a workgroup keeps 512
+// columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
+// go to part (as EPI_PART), gemm_finish_k joins them.
+constexpr int SL_K = 512;           // columns of a slice
+constexpr int SL_W = 4;             // waves of a workgroup: few, so that small matrices still spread evenly
+constexpr int SL_TT = 5;            // most tiles of 16 tokens: 80 KB of x
+
+struct SliceArgs {
+    SkinnyArgs a;
+    int products, slices, ldp, tiles;   // tiles of 16 rows of all products, one after the other
+    int per;                            // tiles of a workgroup
+    float* part;
+};
+
+template <class T, int TT, int G>
+__global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
+{
+    typedef typename Elem<T>::v8 v8;
+    constexpr bool Q4 = G != 0, OFFSET = Q4 && Q4Dec<T>::OFFSET;
+    constexpr int NG = Q4 ? SK_K / G : 1, JG = 4 / NG, U = SL_K / SK_K;   // groups of a step, words of a group, steps of a tile
+    constexpr int SG = Q4 ? SL_K / G : 1;                                 // groups of a slice
+    const SkinnyArgs& p = sp.a;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
+    const int slice = blockIdx.y, k0 = slice * SL_K, KT = (p.K + SK_K - 1) / SK_K, NT = (p.N + 15) / 16;
+    const int end = min((int)(blockIdx.x + 1) * sp.per, sp.tiles);
+
+    // x: row t, 16-byte chunk c at position c ^ (t & 15): 16 tokens at one chunk (a fragment read) on different banks
+    __shared__ __attribute__((aligned(16))) char xl[TT * 16 * SL_K * 2];
+    __shared__ __attribute__((aligned(16))) float xs[OFFSET ? SG * TT * 16 : 4];   // [group][token]: sums of x (bf16)
+
+    struct Step {
+        u32x4 w[Q4 ? 1 : 4];
+        uint16_t s[NG];
+        uint8_t z[NG];
+    } st[U];
+    auto load = [&](int tile) {
+        const int m = tile >= NT ? 1 : 0, nt = tile - m * NT;
+        const Q4View v = p.q[m];
+        const int n = min(nt * 16 + r, p.N - 1);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            const int kt = k0 / SK_K + u;
+            if (kt >= KT) return;
+            Step& b = st[u];
+            if (Q4)
+            {
+                b.w[0] = ldg4(v.codes + ((int64_t)nt * KT + kt) * 64 + lane);
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                {
+                    const int64_t at = ((int64_t)nt * (KT * NG) + kt * NG + g) * 16 + r;
+                    b.s[g] = v.scale[at];
+                    b.z[g] = v.zero ? v.zero[at] : 8;
+                }
+            }
+            else
+            {
+                const uint16_t* w = static_cast<const uint16_t*>(p.w[m]) + (int64_t)n * p.K;
+                const int k = kt * SK_K + q * 8;
+                if (kt * SK_K + SK_K <= p.K)
+                {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) b.w[Q4 ? 0 : j] = ldg4(w + k + j * 32);
+                }
+                else
+                {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) b.w[Q4 ? 0 : j] = k + j * 32 < p.K ? ldg4(w + k + j * 32) : u32x4{0, 0, 0, 0};
+                }
+            }
+        }
+    };
+
+    int tile = blockIdx.x * sp.per + wave;
+    if (tile < end) load(tile);
+    // x in loads of up to 8 at a time: one after the other they would each wait for L2
+    constexpr int CH = SL_K / 8, LOADS = TT * 16 * CH / (SL_W * 64), B = LOADS % 8 ? 4 : 8;
+    static_assert(LOADS % B == 0, "whole batches");
+#pragma unroll
+    for (int l0 = 0; l0 < LOADS; l0 += B)
+    {
+        u32x4 v[B];
+#pragma unroll
+        for (int l = 0; l < B; ++l)
+        {
+            const int i = (l0 + l) * (SL_W * 64) + threadIdx.x, t = i / CH, k = k0 + i % CH * 8;
+            v[l] = t < p.T && k < p.K ? ldg4(p.x + (int64_t)t * p.K + k) : u32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int l = 0; l < B; ++l)
+        {
+            const int i = (l0 + l) * (SL_W * 64) + threadIdx.x, t = i / CH, c = i % CH;
+            *reinterpret_cast<u32x4*>(xl + t * (SL_K * 2) + ((c ^ (t & 15)) << 4)) = v[l];
+            if (OFFSET)
+            {
+                // the lanes of a group are neighbours
+                constexpr int LG = Q4 ? G / 8 : 1;
+                float sum = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += from16<T>((uint16_t)v[l][e]) + from16<T>((uint16_t)(v[l][e] >> 16));
+#pragma unroll
+                for (int o = 1; o < LG; o <<= 1) sum += __shfl_xor(sum, o);
+                if (c % LG == 0) xs[c / LG * (TT * 16) + t] = sum;
+            }
+        }
+    }
+    __syncthreads();
+
+    for (; tile < end; tile += SL_W)
+    {
+        f32x4 acc[TT];
+#pragma unroll
+        for (int t = 0; t < TT; ++t) acc[t] = f32x4{0, 0, 0, 0};
+        const int m = tile >= NT ? 1 : 0, nt = tile - m * NT;
+        const Q4View v = p.q[m];
+        auto x = [&](int u, int j, int t) {
+            const int row = t * 16 + r, c = u * (SK_K / 8) + j * 4 + q;
+            return *reinterpret_cast<const v8*>(xl + row * (SL_K * 2) + ((c ^ r) << 4));
+        };
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+        {
+            if (k0 / SK_K + u >= KT) break;
+            const Step b = st[u];
+            if (!Q4)
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) acc[t] = Elem<T>::mfma16(x(u, j, t), __builtin_bit_cast(v8, b.w[Q4 ? 0 : j]), acc[t]);
+                continue;
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
+            {
+                const float s = v.scale_bf16 ? from16<bf16>(b.s[g]) : from16<f16>(b.s[g]), z = (float)b.z[g];
+                Q4Dec<T> dec;
+                dec.zero(z);
+                f32x4 part[TT];
+#pragma unroll
+                for (int t = 0; t < TT; ++t) part[t] = f32x4{0, 0, 0, 0};
+#pragma unroll
+                for (int j = g * JG; j < (g + 1) * JG; ++j)
+                {
+                    const v8 w = dec(b.w[0][j]);
+#pragma unroll
+                    for (int t = 0; t < TT; ++t) part[t] = Elem<T>::mfma16(x(u, j, t), w, part[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < TT; ++t)
+                {
+                    f32x4 o = {0, 0, 0, 0};
+                    if (OFFSET) o = *reinterpret_cast<const f32x4*>(xs + (u * NG + g) * (TT * 16) + t * 16 + q * 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        acc[t][e] = __builtin_fmaf(s, OFFSET ? __builtin_fmaf(-128.0f - z, o[e], part[t][e]) : part[t][e], acc[t][e]);
+                }
+            }
+        }
+        if (tile + SL_W < end) load(tile + SL_W);
+        const int n = nt * 16 + r;
+        float* out = sp.part + (int64_t)(m * sp.slices + slice) * p.T * sp.ldp + n;
+        if (n < p.N)
+#pragma unroll
+            for (int t = 0; t < TT; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (t * 16 + q * 4 + e < p.T) out[(int64_t)(t * 16 + q * 4 + e) * sp.ldp] = acc[t][e];
     }
 }
 
