@@ -39,7 +39,8 @@ class GatedFFN:
     (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
 
     forward(x) -> y, x [..., H] of the weights' type. Where autograd records (x or a weight requires grad), y carries the
-    gradients of x and of the three weights; the forward pass then keeps x, g, u and h ([T, I] each, 16 bits)."""
+    gradients of x and of the three weights; the forward pass then keeps x, g and u
+    (fp32 [T, I]) and h (16 bits)."""
 
     def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
         self.quantized = not any(torch.is_tensor(w) for w in (gate, up, down))
@@ -61,6 +62,7 @@ class GatedFFN:
         self.hidden_size, self.intermediate_size = H, I
         self.device = gate.device
         self.dtype = None if self.quantized else gate.dtype      # None: the input's
+        self._descs = {}
 
     @staticmethod
     def _check_tensors(gate, up, down):
@@ -82,8 +84,12 @@ class GatedFFN:
     def desc(self, dtype=None):
         """The call descriptor for an input of dtype (default: the weights')."""
         if self.quantized:
-            ref = lambda q: ctypes.pointer(q.struct)
-            return L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up), ref(self.down))
+            d = self._descs.get(dtype)
+            if d is None:
+                ref = lambda q: ctypes.pointer(q.struct)
+                d = self._descs[dtype] = L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up),
+                                                    ref(self.down))
+            return d
         return L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0,
                          self.gate.data_ptr(), self.up.data_ptr(), self.down.data_ptr())
 
@@ -118,7 +124,8 @@ class GatedFFN:
         y = torch.empty_like(r)
         saved = None
         if keep is not None:
-            g, u, h = (torch.empty((T, self.intermediate_size), dtype=self.dtype, device=self.device) for _ in range(3))
+            g, u, h = (torch.empty((T, self.intermediate_size), dtype=dt, device=self.device)
+                       for dt in (torch.float32, torch.float32, self.dtype))
             keep.extend((r, g, u, h))
             saved = L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr())
         if T:

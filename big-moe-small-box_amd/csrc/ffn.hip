@@ -177,7 +177,7 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
         k.group = d.group();
         k.x = static_cast<const uint16_t*>(x);
         k.N = d.I; k.K = d.H; k.out = h; k.ldo = d.I;
-        if (sv) { k.g = static_cast<uint16_t*>(sv->g); k.u = static_cast<uint16_t*>(sv->u); }
+        if (sv) { k.g = sv->g; k.u = sv->u; }
         if ((rc = launch_skinny(k, d.dtype, EPI_GU, a.part, s))) return rc;
     }
     else

@@ -13,7 +13,7 @@ namespace bmx {
 
 struct ActPar {
     float c1, c3, add, Lg, La, Lu;
-    int relu2, limited;
+    int relu2, limited;              // limited: some bound is finite
 };
 
 inline ActPar act_par(int act, float limit)
@@ -59,27 +59,6 @@ __device__ __forceinline__ void act_grad(const ActPar& p, float g, float u, floa
     const bool ain = a <= p.La;
     hg = gin && ain ? (f + g * df) * (clamp_both(u, p.Lu) + p.add) : 0.0f;
     hu = uin ? clamp_hi(a, p.La) : 0.0f;
-}
-
-// g and u are kept for the backward pass in the tensors' own 16-bit type, as h is for the down product: half the bytes of
-// fp32 and the rounding every 16-bit activation of a model has. Where a clamp is near, rounding must not carry a value
-// across its border, or the whole gradient of that element would appear or vanish: such a value moves one step back to its
-// side. (Beyond a clamp only the side counts.)
-__device__ __forceinline__ uint16_t keep_side(bool inside, bool inside_rounded, uint16_t b)
-{
-    return inside == inside_rounded ? b : inside ? b - 1 : b + 1;   // sign and magnitude: towards zero, away from it
-}
-
-template <class T> __device__ __forceinline__ void save_gu(const ActPar& p, float g, float u, uint16_t& gb, uint16_t& ub)
-{
-    gb = __builtin_bit_cast(uint16_t, (T)g);
-    ub = __builtin_bit_cast(uint16_t, (T)u);
-    if (!p.limited) return;
-    const float gr = (float)__builtin_bit_cast(T, gb), ur = (float)__builtin_bit_cast(T, ub);
-    ub = keep_side(fabsf(u) <= p.Lu, fabsf(ur) <= p.Lu, ub);
-    // only one of the two bounds on the gate's side is finite; NaN is outside both before and after rounding
-    auto in = [&](float v) { const float c = clamp_hi(v, p.Lg); return v <= p.Lg && c * act_f(p, c) <= p.La; };
-    gb = keep_side(in(g), in(gr), gb);
 }
 
 }  // namespace bmx

@@ -59,7 +59,8 @@ struct GemmArgs {
     float* part;
     const float* scale;     // EPI_ADD: [N] or null
     ActPar act;
-    void *g, *u;            // EPI_GU: saved when not null; EPI_DGU: read
+    float *g, *u;           // EPI_GU: kept when not null; EPI_DGU: read. fp32: a backward pass from g and u of 16 bits is off
+                            // by as much again as its results' own rounding (both, and dg's: 1.8 times; this way 1.4)
 };
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
@@ -107,34 +108,29 @@ template <class T> __device__ __forceinline__ void gu_8(const GemmArgs& p, int64
     for (int t = 0; t < 8; ++t) h.v[t] = act_h(p.act, g.v[t], u.v[t]);
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(h);
     if (p.g)
-    {
-        uint16_t gb[8], ub[8];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) save_gu<T>(p.act, g.v[t], u.v[t], gb[t], ub[t]);
-        u32x4 a, b;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2; ++i)
         {
-            a[i] = gb[2 * i] | (uint32_t)gb[2 * i + 1] << 16;
-            b[i] = ub[2 * i] | (uint32_t)ub[2 * i + 1] << 16;
+            reinterpret_cast<f32x4*>(p.g + o)[i] = f32x4{g.v[4 * i], g.v[4 * i + 1], g.v[4 * i + 2], g.v[4 * i + 3]};
+            reinterpret_cast<f32x4*>(p.u + o)[i] = f32x4{u.v[4 * i], u.v[4 * i + 1], u.v[4 * i + 2], u.v[4 * i + 3]};
         }
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.g) + o) = a;
-        *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.u) + o) = b;
-    }
 }
 
 template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int64_t o, const f32x8& dh)
 {
-    const u32x4 gw = ldg4(static_cast<const uint16_t*>(p.g) + o), uw = ldg4(static_cast<const uint16_t*>(p.u) + o);
     f32x8 dg, du;
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int i = 0; i < 2; ++i)
     {
-        const int sh = (t & 1) * 16;
-        float hg, hu;
-        act_grad(p.act, from16<T>((uint16_t)(gw[t >> 1] >> sh)), from16<T>((uint16_t)(uw[t >> 1] >> sh)), hg, hu);
-        dg.v[t] = dh.v[t] * hg;
-        du.v[t] = dh.v[t] * hu;
+        const f32x4 g = ldg4f(p.g + o + 4 * i), u = ldg4f(p.u + o + 4 * i);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+        {
+            float hg, hu;
+            act_grad(p.act, g[t], u[t], hg, hu);
+            dg.v[4 * i + t] = dh.v[4 * i + t] * hg;
+            du.v[4 * i + t] = dh.v[4 * i + t] * hu;
+        }
     }
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(dg);
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[1]) + o) = pack8<T>(du);

@@ -34,7 +34,7 @@ struct SkinnyArgs {
     int ldo;
     const float* scale;             // EPI_ADD: [T] or null
     ActPar act;
-    uint16_t *g, *u;                // EPI_GU: saved when not null
+    float *g, *u;                   // EPI_GU: kept when not null
 };
 
 // q4.hip
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
         {
             const float u = sum(i + 8);
             static_cast<uint16_t*>(p.out)[o] = to16<T>(act_h(p.act, s, u));
-            if (p.g) save_gu<T>(p.act, s, u, p.g[o], p.u[o]);
+            if (p.g) { p.g[o] = s; p.u[o] = u; }
         }
         else if (EPI == EPI_ADD)
         {

@@ -502,9 +502,8 @@ typedef struct bmx_ffn_desc {
     int32_t reserved;
     const void *gate, *up, *down;    /* device */
 } bmx_ffn_desc;
-/* What a forward pass keeps for the backward pass: g, u, h [T, I] of dtype, device, 16-byte aligned. Values of g and u
- * beyond a clamp are kept only as being beyond it. */
-typedef struct bmx_ffn_saved { void *g, *u, *h; } bmx_ffn_saved;
+/* What a forward pass keeps for the backward pass: g, u fp32 [T, I] and h [T, I] of dtype; device, 16-byte aligned. */
+typedef struct bmx_ffn_saved { float *g, *u; void* h; } bmx_ffn_saved;
 /* Workspace bytes of the calls below for up to T tokens (0 and an error text when the descriptor is refused). */
 size_t bmx_ffn_workspace(const bmx_ffn_desc* desc, int T);
 size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T);

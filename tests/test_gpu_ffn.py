@@ -27,12 +27,9 @@ def check_forward(x, w, act, L, ffn, y, keep=None):
     g, u, h, eg, eu, eh = R.forward(x.double(), *(t.double() for t in w[:2]), act, L)
     if keep is not None:
         _, gs, us, hs = keep
-        inside = lambda v: (v.abs() <= L) if L else torch.ones_like(v, dtype=torch.bool)
-        # a step moved back at a clamp's border is at most one whole step more
-        R.check("u", torch.where(inside(u), us.double(), u), u, 3 * R.rounded(u, eu, dt))
+        R.check("g", gs, g, eg + R.TINY[torch.bfloat16])
+        R.check("u", us, u, eu + R.TINY[torch.bfloat16])
         R.check("h", hs, h, R.rounded(h, eh, dt))
-        if L == 0:
-            R.check("g", gs, g, R.rounded(g, eg, dt))
     y64, ey = R.product(h, w[2].double(), R.rounded(h, eh, dt))
     R.check("y", y, y64, R.rounded(y64, ey, dt))
     return y64, ey
@@ -114,8 +111,8 @@ def test_large_tiles(cuda, T, H, I, dt):
 
 @pytest.mark.parametrize("act,L", [(0, 0.0), (1, 2.0), (2, 0.0), (3, 2.0)])
 def test_gradients_against_autograd_and_differences(cuda, act, L):
-    """End to end in 64 bits. Norms: g, u, h, dg, du and the result are each off by at most half a step (2^-11) of
-    themselves, and the slopes carry g's and u's roundings about twice over: 16 halves are more than all together."""
+    """End to end in 64 bits. Norms: h, dg, du and the result are each off by at most half a step (2^-11) of themselves (g and
+    u are kept in fp32): 16 halves are more than all together."""
     import bmx
     x, w, dy = make(cuda, 70, 96, 136, torch.float16, seed=7)
     leaves = [t.double().requires_grad_() for t in [x] + w]
