@@ -9,31 +9,46 @@ namespace bmx {
 
 static bool dtype_ok(int d) { return d == BMX_DT_FP16 || d == BMX_DT_BF16; }
 
-struct TilePlan { int big, splits; };
+struct TilePlan { int tile, splits; };     // tile: 0 256 x 256, 1 128 x 128, 2 128 x 64 (M x N)
+constexpr int TILE_M[3] = {256, 128, 128}, TILE_N[3] = {256, 128, 64};
 
-// Tiles of a product with M x N results, `products` side by side, nk tiles of K: 256 x 256 where they fill the chip, else
-// 128 x 128, K split (partial sums joined by a second kernel) where even those leave compute units without work.
+// Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest of the three by what they
+// measured. A 256 x 256 tile has a compute unit to itself (1.45 us a K tile, 6 to begin and end); two of the others share one
+// (128 x 128: 1.0 us a K tile for the two, 0.64 alone; 128 x 64: 0.68 and 0.45; 3 to begin and end). K is split, the partial
+// sums joined by a second kernel, where that fills the chip and saves more than the second kernel (5 us) and the sums' bytes
+// (written and read at 4 TB/s) cost.
 static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split)
 {
-    auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b - 1) / b) * products; };
-    TilePlan p = {tiles(256) >= 192, 1};
-    if (p.big || !can_split) return p;
-    const int64_t t = tiles(128);
-    while (p.splits < 16 && t * p.splits * 2 <= 512 && nk / (p.splits * 2) >= 4) p.splits *= 2;
-    return p;
+    static const double alone[3] = {1.45, 0.64, 0.45}, pair[3] = {1.45, 1.0, 0.68}, ends[3] = {6.0, 3.0, 3.0};
+    TilePlan best = {0, 1};
+    double least = 1e30;
+    for (int t = 0; t < 3; ++t)
+        for (int s = 1; s <= 16; s *= 2)
+        {
+            if (s > 1 && (!can_split || nk / s < 4)) break;
+            const int64_t b = (M + TILE_M[t] - 1) / TILE_M[t] * ((N + TILE_N[t] - 1) / TILE_N[t]) * products * s;
+            const int each = (nk + s - 1) / s;
+            const int64_t per = t == 0 ? 256 : 512, full = b / per, rest = b % per;
+            double us = full * (each * pair[t] + ends[t]);
+            if (rest) us += each * (rest <= 256 ? alone[t] : pair[t]) + ends[t];
+            if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
+            if (us < least) { least = us; best = {t, s}; }
+        }
+    return best;
 }
 
 template <class T, bool AX, bool BX, int EPI>
-static int run_gemm(const GemmArgs& a, int big, hipStream_t s)
+static int run_gemm(const GemmArgs& a, int tile, hipStream_t s)
 {
     GemmArgs p = a;
     // EPI_GU: a tile's rows are half gate, half up
-    const int b = big ? 256 : 128, bm = EPI == EPI_GU ? b / 2 : b;
+    const int bm = EPI == EPI_GU ? TILE_M[tile] / 2 : TILE_M[tile];
     p.tm = (a.M + bm - 1) / bm;
-    p.tn = (a.N + b - 1) / b;
+    p.tn = (a.N + TILE_N[tile] - 1) / TILE_N[tile];
     const dim3 grid((unsigned)(p.tm * p.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * a.batch : a.batch));
-    if (big) hipLaunchKernelGGL((gemm16_k<T, 256, 256, 2, 4, AX, BX, EPI>), grid, dim3(512), 0, s, p);
-    else hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, AX, BX, EPI>), grid, dim3(256), 0, s, p);
+    if (tile == 0) hipLaunchKernelGGL((gemm16_k<T, 256, 256, 2, 4, 2, AX, BX, EPI>), grid, dim3(512), 0, s, p);
+    else if (tile == 1) hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, 2, AX, BX, EPI>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((gemm16_k<T, 128, 64, 2, 2, 3, AX, BX, EPI>), grid, dim3(256), 0, s, p);
     return check_launch("gemm16");
 }
 
@@ -41,13 +56,13 @@ static int run_gemm(const GemmArgs& a, int big, hipStream_t s)
 template <class T, bool AX, bool BX, int EPI>
 static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
 {
-    if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.big, s);
+    if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.tile, s);
     a.splits = tp.splits;
     a.ldp = (a.M + 7) / 8 * 8;
     GemmArgs g = a;
     g.batch = EPI == EPI_GU ? 2 : 1;
     if (EPI == EPI_GU) g.b[1] = g.b[0];
-    int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.big, s);
+    int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.tile, s);
     if (rc) return rc;
     const int64_t pieces = (int64_t)a.ldp / 8 * a.N;
     hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a);

@@ -116,21 +116,23 @@ template <class T> __device__ __forceinline__ void gu_8(const GemmArgs& p, int64
         }
 }
 
-template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int64_t o, const f32x8& dh)
+// g and u of eight values, loaded ahead of their use
+struct GU8 { f32x4 g[2], u[2]; };
+__device__ __forceinline__ GU8 load_gu(const GemmArgs& p, int64_t o)
+{
+    return {{ldg4f(p.g + o), ldg4f(p.g + o + 4)}, {ldg4f(p.u + o), ldg4f(p.u + o + 4)}};
+}
+
+template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int64_t o, const f32x8& dh, const GU8& s)
 {
     f32x8 dg, du;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int t = 0; t < 8; ++t)
     {
-        const f32x4 g = ldg4f(p.g + o + 4 * i), u = ldg4f(p.u + o + 4 * i);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-        {
-            float hg, hu;
-            act_grad(p.act, g[t], u[t], hg, hu);
-            dg.v[4 * i + t] = dh.v[4 * i + t] * hg;
-            du.v[4 * i + t] = dh.v[4 * i + t] * hu;
-        }
+        float hg, hu;
+        act_grad(p.act, s.g[t >> 2][t & 3], s.u[t >> 2][t & 3], hg, hu);
+        dg.v[t] = dh.v[t] * hg;
+        du.v[t] = dh.v[t] * hu;
     }
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(dg);
     *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[1]) + o) = pack8<T>(du);
@@ -144,7 +146,8 @@ constexpr int GK = 64;      // K of a tile
 // read for a transposition fall on four different quarters of the banks (with 32 bytes as the unit the reads took twice the
 // cycles: 256 bytes go out at a time).
 __device__ __forceinline__ int swz_along(int r) { return (r >> 1) & 7; }
-__device__ __forceinline__ int swz_across(int r) { return (r & 3) << 2; }
+// Rows of 64 values are half the banks: two of the four lie apart by themselves.
+template <int ROWS> __device__ __forceinline__ int swz_across(int r) { return ROWS == 64 ? (r & 2) << 1 : (r & 3) << 2; }
 
 // One operand's tiles of ROWS rows x GK, loaded by NT threads in INSTR loads of 16 bytes each. ACROSS: stored [K][rows].
 // GU: the rows are 32 of one matrix and 32 of a second in turn.
@@ -163,7 +166,7 @@ struct TileLoader {
     __device__ __forceinline__ void init(int ld, int wave)
     {
         const int r = GU ? (wave * 8 & 31) + (threadIdx.x & 63) / 8 : threadIdx.x / CPR, p = threadIdx.x % CPR;
-        chunk = p ^ (ACROSS ? swz_across(r) : swz_along(r));
+        chunk = p ^ (ACROSS ? swz_across<ROWS>(r) : swz_along(r));
         voff = (uint32_t)r * ld * 2 + chunk * 16;
         rows_ld = ld * 2;
         step = ACROSS ? (int64_t)GK * ld * 2 : GK * 2;
@@ -178,10 +181,11 @@ struct TileLoader {
         left = ((ACROSS ? K : rows) * ld - first) * 2;
     }
     // Offsets past the range load zeros: the bytes left, at most 1 GiB (a tile spans half of that at the widest rows the
-    // entries take). tail: columns of K left; what lies past them in the last tile along K is moved out of the range.
-    __device__ __forceinline__ void load(lds_ptr to, int wave, int tail)
+    // entries take); none without `on`. tail: columns of K left; what lies past them in the last tile along K is moved out
+    // of the range.
+    __device__ __forceinline__ void load(lds_ptr to, int wave, int tail, bool on)
     {
-        const int range = (int)(left < 0 ? 0 : left > 0x40000000 ? 0x40000000 : left);
+        const int range = (int)(!on || left < 0 ? 0 : left > 0x40000000 ? 0x40000000 : left);
         uint32_t v0 = voff;
         if (!ACROSS && tail < GK) v0 = chunk * 8 < tail ? v0 : 0x7ff00000u;
 #pragma unroll
@@ -203,14 +207,14 @@ struct TileLoader {
     }
 };
 
-template <class T, int BM, int BN, int WM, int WN, bool AX, bool BX, int EPI>
+template <class T, int BM, int BN, int WM, int WN, int NB, bool AX, bool BX, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
 {
     constexpr int NT = WM * WN * 64;
     constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
     constexpr int ABYTES = BM * GK * 2, BBYTES = BN * GK * 2;
     typedef typename Elem<T>::v8 v8;
-    constexpr int TILES = 2 * (ABYTES + BBYTES), TURN = WM * WN * 32 * (BM / WM + 4) * 4;
+    constexpr int TILES = NB * (ABYTES + BBYTES), TURN = WM * WN * 32 * (BM / WM + 4) * 4;
     __shared__ __attribute__((aligned(1024))) char lds[TILES > TURN ? TILES : TURN];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -253,10 +257,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     auto tail = [&]() { return p.K - (loaded >= nk1 ? loaded - nk1 : loaded) * GK; };
     auto load_a = [&](int buf) {
         if (p.chain > 1 && loaded == nk1) seek(1, 0);
-        la.load((lds_ptr)lds + buf * (ABYTES + BBYTES), wave, tail());
+        la.load((lds_ptr)lds + buf * (ABYTES + BBYTES), wave, tail(), loaded < kt_end);
     };
     auto load_b = [&](int buf) {
-        lb.load((lds_ptr)lds + buf * (ABYTES + BBYTES) + ABYTES, wave, tail());
+        lb.load((lds_ptr)lds + buf * (ABYTES + BBYTES) + ABYTES, wave, tail(), loaded < kt_end);
         la.next();
         lb.next();
         ++loaded;
@@ -276,7 +280,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         {
             const int k = ks * 16 + (lane >> 5) * 8 + i * 4 + (m >> 2);
             const s16x4 t = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(tile + k * (rows * 2) + ((c ^ swz_across(k)) << 4) + (m & 1) * 8));
+                (__attribute__((address_space(3))) s16x4*)(tile + k * (rows * 2) + ((c ^ (rows == 64 ? swz_across<64>(k) : swz_across<128>(k))) << 4) + (m & 1) * 8));
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[i * 4 + e] = t[e];
         }
@@ -309,31 +313,45 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
 #pragma unroll
             for (int j = 0; j < NF; ++j) acc[i][j] = Elem<T>::mfma32(a[set][i], b[set][j], acc[i][j]);
     };
+    // NB buffers. At the wait for tile kt + 1 the loads of the NB - 2 tiles behind it stay in flight. (Past the last tile
+    // they go on with an empty range, so that the count holds; the results wait for all of them.)
+    constexpr int BEHIND = (la.INSTR + lb.INSTR) * (NB - 2);
+    static_assert(BEHIND < 64, "vmcnt has 6 bits");
     auto landed = [&]() {
-        __builtin_amdgcn_s_waitcnt(0x0f70);                         // vmcnt 0: this wave's loads are in LDS
-        lds_barrier();
+        // this wave's loads up to the tile's are in LDS (vmcnt) and its fragment reads done (lgkmcnt 0), then everyone's. The
+        // waits are written out because a workgroup fence would wait for every load; the wavefront fences only keep the
+        // compiler from moving LDS accesses across.
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (BEHIND & 15) | (BEHIND >> 4) << 14);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
-    load_a(0);
-    load_b(0);
-    landed();
-    if (kt + 1 < kt_end) { load_a(1); load_b(1); }
-    read(0, 0, 0);
     // 256-row tiles: the loads of the tile after the next go out in two parts, behind the fragment reads and ahead of the
     // products of the first two steps: all at once, or right behind the wait, they hold the products up (286 -> 301 us on
-    // 4,096 x 4,096 x 11,008), and later they land too late (298 us). 128-row tiles have half the products to wait behind
-    // (and a second workgroup to fill in): right behind the wait (390 -> 342 us on the same).
+    // 4,096 x 4,096 x 11,008), and later they land too late (298 us). Smaller tiles have fewer products to wait behind:
+    // right behind the wait (128 rows, 390 -> 342 us on the same).
     constexpr bool SPREAD = MF * NF >= 8;
-    bool fill = false;
-    for (int buf = 0; kt < kt_end; ++kt, buf ^= 1)
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i)
     {
+        load_a(i);
+        load_b(i);
+    }
+    landed();
+    if (!SPREAD) { load_a(NB - 1); load_b(NB - 1); }
+    read(0, 0, 0);
+    int buf = 0;
+    for (; kt < kt_end; ++kt)
+    {
+        const int next = buf + 1 == NB ? 0 : buf + 1, last = buf == 0 ? NB - 1 : buf - 1;
 #pragma unroll
         for (int ks = 0; ks < KS - 1; ++ks)
         {
             read((ks + 1) & 1, buf, ks + 1);
-            if (SPREAD && fill)
+            if (SPREAD)
             {
-                if (ks == 0) load_a(buf ^ 1);
-                if (ks == 1) load_b(buf ^ 1);
+                if (ks == 0) load_a(last);
+                if (ks == 1) load_b(last);
             }
             products(ks & 1);
             if (SPREAD) __builtin_amdgcn_sched_barrier(0);
@@ -341,12 +359,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         if (kt + 1 < kt_end)
         {
             landed();
-            if (!SPREAD && loaded < kt_end) { load_a(buf); load_b(buf); }
-            read(0, buf ^ 1, 0);
+            if (!SPREAD) { load_a(buf); load_b(buf); }
+            read(0, next, 0);
         }
-        fill = loaded < kt_end;
         products((KS - 1) & 1);
         if (SPREAD) __builtin_amdgcn_sched_barrier(0);
+        buf = next;
     }
 
     // ---- results ----
@@ -359,6 +377,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     float* turn = reinterpret_cast<float*>(lds) + wave * (32 * LROW);
     const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
     constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8;   // 8-value pieces of a row
+    __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NF; ++j)
@@ -372,10 +391,22 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
                     f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
         // the wave's own rows only: its LDS writes and reads are in order
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-#pragma unroll 2
-        for (int q = lane; q < 32 * PIECES; q += 64)
+        // four pieces at a time, so that what they read from HBM (g and u) is on its way together
+        constexpr int AHEAD = 32 * PIECES / 64 < 4 ? 32 * PIECES / 64 : 4;
+        for (int q0 = lane; q0 < 32 * PIECES; q0 += 64 * AHEAD)
         {
-            const int rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
+        GU8 saved[EPI == EPI_DGU ? AHEAD : 1];
+        if (EPI == EPI_DGU)
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+            {
+                const int q = q0 + k * 64, n = nb + q / PIECES, m = wm0 + q % PIECES * 8;
+                if (n < p.N && m < p.M) saved[EPI == EPI_DGU ? k : 0] = load_gu(p, (int64_t)n * p.ldo + m);
+            }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+        {
+            const int q = q0 + k * 64, rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
             if (n >= p.N || m >= p.M) continue;
             const int64_t o = (int64_t)n * p.ldo + m;
             auto piece = [&](int col) {
@@ -400,8 +431,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
                 d[1] = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
             }
             else if (EPI == EPI_ADD) add_8(p, o, n, piece(c));
-            else if (EPI == EPI_DGU) dgu_8<T>(p, o, piece(c));
+            else if (EPI == EPI_DGU) dgu_8<T>(p, o, piece(c), saved[EPI == EPI_DGU ? k : 0]);
             else store_8<T>(p, p.out[prod], o, m, piece(c));
+        }
         }
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }
@@ -450,7 +482,11 @@ __global__ __launch_bounds__(64) void gemm_finish_k(const GemmArgs p)
         gu_8<T>(p, o, g, u);
     }
     else if (EPI == EPI_ADD) add_8(p, o, n, sum(0));
-    else if (EPI == EPI_DGU) dgu_8<T>(p, o, sum(0));
+    else if (EPI == EPI_DGU)
+    {
+        const GU8 saved = load_gu(p, o);
+        dgu_8<T>(p, o, sum(0), saved);
+    }
     else store_8<T>(p, p.out[0], o, m, sum(0));
 }
 
