@@ -9,28 +9,33 @@ namespace bmx {
 
 static bool dtype_ok(int d) { return d == BMX_DT_FP16 || d == BMX_DT_BF16; }
 
-struct TilePlan { int tile, splits; };     // tile: 0 256 x 256, 1 128 x 128, 2 128 x 64 (M x N)
-constexpr int TILE_M[3] = {256, 128, 128}, TILE_N[3] = {256, 128, 64};
+// The tiles a product can run on: results M x N, workgroups that run at once, and what was measured of each: us a K tile of
+// 64 with a workgroup on every other compute unit or fewer (alone) and with the chip full, us to begin and end.
+struct Tile { int M, N, slots; double alone, full, ends; };
+static const Tile TILES[4] = {
+    {256, 256, 256, 1.45, 1.45, 6.0},      // 8 waves, 2 buffers
+    {128, 128, 512, 0.64, 1.00, 3.0},      // 4 waves, 2 buffers, two on a compute unit
+    {128, 64, 256, 0.34, 0.38, 3.0},       // 2 groups of 4 waves, each every other K tile, 3 buffers
+    {128, 128, 256, 0.54, 0.54, 3.0},      // the same, 2 buffers
+};
+struct TilePlan { int tile, splits; };
 
-// Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest of the three by what they
-// measured. A 256 x 256 tile has a compute unit to itself (1.45 us a K tile, 6 to begin and end); two of the others share one
-// (128 x 128: 1.0 us a K tile for the two, 0.64 alone; 128 x 64: 0.68 and 0.45; 3 to begin and end). K is split, the partial
-// sums joined by a second kernel, where that fills the chip and saves more than the second kernel (5 us) and the sums' bytes
+// Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
+// the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
 // (written and read at 4 TB/s) cost.
 static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split)
 {
-    static const double alone[3] = {1.45, 0.64, 0.45}, pair[3] = {1.45, 1.0, 0.68}, ends[3] = {6.0, 3.0, 3.0};
     TilePlan best = {0, 1};
     double least = 1e30;
-    for (int t = 0; t < 3; ++t)
+    for (int t = 0; t < 4; ++t)
         for (int s = 1; s <= 16; s *= 2)
         {
             if (s > 1 && (!can_split || nk / s < 4)) break;
-            const int64_t b = (M + TILE_M[t] - 1) / TILE_M[t] * ((N + TILE_N[t] - 1) / TILE_N[t]) * products * s;
+            const Tile& c = TILES[t];
+            const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * products * s, full = b / c.slots, rest = b % c.slots;
             const int each = (nk + s - 1) / s;
-            const int64_t per = t == 0 ? 256 : 512, full = b / per, rest = b % per;
-            double us = full * (each * pair[t] + ends[t]);
-            if (rest) us += each * (rest <= 256 ? alone[t] : pair[t]) + ends[t];
+            double us = full * (each * c.full + c.ends);
+            if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
             if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
             if (us < least) { least = us; best = {t, s}; }
         }
@@ -42,13 +47,17 @@ static int run_gemm(const GemmArgs& a, int tile, hipStream_t s)
 {
     GemmArgs p = a;
     // EPI_GU: a tile's rows are half gate, half up
-    const int bm = EPI == EPI_GU ? TILE_M[tile] / 2 : TILE_M[tile];
+    const int bm = EPI == EPI_GU ? TILES[tile].M / 2 : TILES[tile].M;
     p.tm = (a.M + bm - 1) / bm;
-    p.tn = (a.N + TILE_N[tile] - 1) / TILE_N[tile];
+    p.tn = (a.N + TILES[tile].N - 1) / TILES[tile].N;
     const dim3 grid((unsigned)(p.tm * p.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * a.batch : a.batch));
-    if (tile == 0) hipLaunchKernelGGL((gemm16_k<T, 256, 256, 2, 4, 2, AX, BX, EPI>), grid, dim3(512), 0, s, p);
-    else if (tile == 1) hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, 2, AX, BX, EPI>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((gemm16_k<T, 128, 64, 2, 2, 3, AX, BX, EPI>), grid, dim3(256), 0, s, p);
+    switch (tile)
+    {
+        case 0: hipLaunchKernelGGL((gemm16_k<T, 256, 256, 2, 4, 1, 2, AX, BX, EPI>), grid, dim3(512), 0, s, p); break;
+        case 1: hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, 1, 2, AX, BX, EPI>), grid, dim3(256), 0, s, p); break;
+        case 2: hipLaunchKernelGGL((gemm16_k<T, 128, 64, 2, 2, 2, 3, AX, BX, EPI>), grid, dim3(512), 0, s, p); break;
+        default: hipLaunchKernelGGL((gemm16_k<T, 128, 128, 2, 2, 2, 2, AX, BX, EPI>), grid, dim3(512), 0, s, p);
+    }
     return check_launch("gemm16");
 }
 

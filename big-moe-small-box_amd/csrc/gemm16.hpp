@@ -149,9 +149,10 @@ __device__ __forceinline__ int swz_along(int r) { return (r >> 1) & 7; }
 // Rows of 64 values are half the banks: two of the four lie apart by themselves.
 template <int ROWS> __device__ __forceinline__ int swz_across(int r) { return ROWS == 64 ? (r & 2) << 1 : (r & 3) << 2; }
 
-// One operand's tiles of ROWS rows x GK, loaded by NT threads in INSTR loads of 16 bytes each. ACROSS: stored [K][rows].
+// One operand's tiles of ROWS rows x GK, loaded by the NT threads of a group in INSTR loads of 16 bytes each, every
+// WK-th one. ACROSS: stored [K][rows].
 // GU: the rows are 32 of one matrix and 32 of a second in turn.
-template <int ROWS, int NT, bool ACROSS, bool GU>
+template <int ROWS, int NT, int WK, bool ACROSS, bool GU>
 struct TileLoader {
     static constexpr int INSTR = ROWS * GK * 2 / (NT * 16);
     static constexpr int CPR = ACROSS ? ROWS / 8 : GK / 8;         // chunks of an LDS row
@@ -159,17 +160,17 @@ struct TileLoader {
     static_assert(RPI % (ACROSS ? 4 : 16) == 0 && (!GU || RPI == 32 || RPI == 64), "later loads' rows are swizzled as the first's, and of one matrix per wave");
     const char *base0, *base1;      // the tile's first element, in the matrix of the even and of the odd loads
     int64_t left;       // bytes from there to the matrix's last
-    int64_t step;       // bytes to the next tile along K
+    int64_t step;       // bytes to the group's next tile along K
     int rows_ld;        // bytes of a matrix row
     uint32_t voff;      // of this lane's chunk in the first load (bytes from the tile's base)
     int chunk;          // ... its column chunk in the matrix
     __device__ __forceinline__ void init(int ld, int wave)
     {
-        const int r = GU ? (wave * 8 & 31) + (threadIdx.x & 63) / 8 : threadIdx.x / CPR, p = threadIdx.x % CPR;
+        const int id = threadIdx.x % NT, r = GU ? (wave * 8 & 31) + (id & 63) / 8 : id / CPR, p = id % CPR;
         chunk = p ^ (ACROSS ? swz_across<ROWS>(r) : swz_along(r));
         voff = (uint32_t)r * ld * 2 + chunk * 16;
         rows_ld = ld * 2;
-        step = ACROSS ? (int64_t)GK * ld * 2 : GK * 2;
+        step = (ACROSS ? (int64_t)GK * ld * 2 : GK * 2) * WK;
     }
     // the tile at row r0 (of the result's side) and column k0, of matrices with `rows` rows and K columns
     __device__ __forceinline__ void seek(const void* m0, const void* m1, int r0, int k0, int rows, int K, int wave)
@@ -207,17 +208,21 @@ struct TileLoader {
     }
 };
 
-template <class T, int BM, int BN, int WM, int WN, int NB, bool AX, bool BX, int EPI>
-__global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
+// BM x BN results by WK groups of WM x WN waves, NB buffers of a K tile each. Every group has K tiles of its own (the WK-th
+// ones, loaded by itself into its own part of LDS); their sums are added at the end, in the groups' order.
+template <class T, int BM, int BN, int WM, int WN, int WK, int NB, bool AX, bool BX, int EPI>
+__global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
 {
-    constexpr int NT = WM * WN * 64;
+    constexpr int NT = WM * WN * 64;                               // threads of a group
     constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
     constexpr int ABYTES = BM * GK * 2, BBYTES = BN * GK * 2;
     typedef typename Elem<T>::v8 v8;
-    constexpr int TILES = NB * (ABYTES + BBYTES), TURN = WM * WN * 32 * (BM / WM + 4) * 4;
-    __shared__ __attribute__((aligned(1024))) char lds[TILES > TURN ? TILES : TURN];
+    constexpr int TILES = WK * NB * (ABYTES + BBYTES), TURN = WM * WN * WK * 32 * (BM / WM + 4) * 4;
+    __shared__ __attribute__((aligned(1024))) char lds_all[TILES > TURN ? TILES : TURN];
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int group = any / (WM * WN), wave = any % (WM * WN);
+    char* lds = lds_all + group * (NB * (ABYTES + BBYTES));
     const int wm = wave / WN, wn = wave % WN;
 
     // Tiles in an order that keeps an XCD (workgroups are dealt to the 8 XCDs in turn) on neighbouring tiles: each XCD takes
@@ -244,26 +249,31 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         kt_end = kt + q + (sp < r);
     }
 
-    TileLoader<BM, NT, AX, EPI == EPI_GU> la;
-    TileLoader<BN, NT, BX, false> lb;
+    TileLoader<BM, NT, WK, AX, EPI == EPI_GU> la;
+    TileLoader<BN, NT, WK, BX, false> lb;
     la.init(p.lda, wave);
     lb.init(p.ldb, wave);
-    int loaded = kt;                                               // the next tile to load
+    int loaded = kt + group;                                       // this group's next tile to load
+    bool second = loaded >= nk1;                                   // of a chain
     auto seek = [&](int pi, int k0) {
         la.seek(p.a[pi], p.a[1], m0, k0, p.M, p.K, wave);
         lb.seek(p.b[pi], nullptr, n0, k0, p.N, p.K, wave);
     };
-    seek(loaded >= nk1 ? 1 : prod, (loaded >= nk1 ? loaded - nk1 : loaded) * GK);
-    auto tail = [&]() { return p.K - (loaded >= nk1 ? loaded - nk1 : loaded) * GK; };
+    seek(second ? 1 : prod, (second ? loaded - nk1 : loaded) * GK);
+    auto tail = [&]() { return p.K - (second ? loaded - nk1 : loaded) * GK; };
     auto load_a = [&](int buf) {
-        if (p.chain > 1 && loaded == nk1) seek(1, 0);
+        if (p.chain > 1 && !second && loaded >= nk1)
+        {
+            second = true;
+            seek(1, (loaded - nk1) * GK);
+        }
         la.load((lds_ptr)lds + buf * (ABYTES + BBYTES), wave, tail(), loaded < kt_end);
     };
     auto load_b = [&](int buf) {
         lb.load((lds_ptr)lds + buf * (ABYTES + BBYTES) + ABYTES, wave, tail(), loaded < kt_end);
         la.next();
         lb.next();
-        ++loaded;
+        loaded += WK;
     };
 
     // A fragment (32 rows from row0, 16 of K from ks * 16): lane l holds row l % 32, K (l / 32) * 8 .. + 7
@@ -329,8 +339,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     // 256-row tiles: the loads of the tile after the next go out in two parts, behind the fragment reads and ahead of the
     // products of the first two steps: all at once, or right behind the wait, they hold the products up (286 -> 301 us on
     // 4,096 x 4,096 x 11,008), and later they land too late (298 us). Smaller tiles have fewer products to wait behind:
-    // right behind the wait (128 rows, 390 -> 342 us on the same).
+    // right behind the wait (128 rows, 390 -> 342 us on the same). (The branch around the last tile's loads also keeps the
+    // compiler from moving them: without it 289 -> 299 us.)
     constexpr bool SPREAD = MF * NF >= 8;
+    static_assert(!SPREAD || NB == 2, "spread loads end early: only a wait for all of them fits");
 #pragma unroll
     for (int i = 0; i < NB - 1; ++i)
     {
@@ -341,14 +353,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     if (!SPREAD) { load_a(NB - 1); load_b(NB - 1); }
     read(0, 0, 0);
     int buf = 0;
-    for (; kt < kt_end; ++kt)
+    for (; kt < kt_end; kt += WK)                                  // group 0's tile; the others' may lie past the end: zeros
     {
         const int next = buf + 1 == NB ? 0 : buf + 1, last = buf == 0 ? NB - 1 : buf - 1;
 #pragma unroll
         for (int ks = 0; ks < KS - 1; ++ks)
         {
             read((ks + 1) & 1, buf, ks + 1);
-            if (SPREAD)
+            if (SPREAD && loaded < kt_end)
             {
                 if (ks == 0) load_a(last);
                 if (ks == 1) load_b(last);
@@ -356,7 +368,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
             products(ks & 1);
             if (SPREAD) __builtin_amdgcn_sched_barrier(0);
         }
-        if (kt + 1 < kt_end)
+        if (kt + WK < kt_end)
         {
             landed();
             if (!SPREAD) { load_a(buf); load_b(buf); }
@@ -374,7 +386,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
     // in HBM is whole 16-byte pieces of whole rows. (Straight from the accumulators, 8 bytes at a time, the gradient
     // epilogue of 8,192 x 2,048 values cost 100 us beside a product of 120; this way about 25.)
     constexpr int WROW = BM / WM, LROW = WROW + 4;                  // a wave's columns m, and an LDS row of them
-    float* turn = reinterpret_cast<float*>(lds) + wave * (32 * LROW);
+    constexpr int AREA = WM * WN * 32 * LROW;                       // of a group
+    float* turn = reinterpret_cast<float*>(lds_all) + wave * (32 * LROW);
     const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
     constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8;   // 8-value pieces of a row
     __builtin_amdgcn_s_waitcnt(0x0f70);
@@ -387,13 +400,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
         for (int i = 0; i < MF; ++i)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<f32x4*>(turn + (lane & 31) * LROW + i * 32 + e * 2 + (lane >> 5) * 4) =
+                *reinterpret_cast<f32x4*>(turn + group * AREA + (lane & 31) * LROW + i * 32 + e * 2 + (lane >> 5) * 4) =
                     f32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
-        // the wave's own rows only: its LDS writes and reads are in order
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        // one group: the wave's own rows only, its LDS writes and reads are in order
+        if (WK > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         // four pieces at a time, so that what they read from HBM (g and u) is on its way together
-        constexpr int AHEAD = 32 * PIECES / 64 < 4 ? 32 * PIECES / 64 : 4;
-        for (int q0 = lane; q0 < 32 * PIECES; q0 += 64 * AHEAD)
+        constexpr int MINE = 32 * PIECES / WK, AHEAD = MINE / 64 < 4 ? MINE / 64 : 4;
+        static_assert(MINE % (64 * AHEAD) == 0, "whole steps");
+        for (int q0 = group * MINE + lane; q0 < (group + 1) * MINE; q0 += 64 * AHEAD)
         {
         GU8 saved[EPI == EPI_DGU ? AHEAD : 1];
         if (EPI == EPI_DGU)
@@ -411,10 +426,18 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
             const int64_t o = (int64_t)n * p.ldo + m;
             auto piece = [&](int col) {
                 f32x8 v;
-                const f32x4 a = *reinterpret_cast<const f32x4*>(turn + rr * LROW + col);
-                const f32x4 b = *reinterpret_cast<const f32x4*>(turn + rr * LROW + col + 4);
 #pragma unroll
-                for (int t = 0; t < 4; ++t) { v.v[t] = a[t]; v.v[t + 4] = b[t]; }
+                for (int w = 0; w < WK; ++w)
+                {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(turn + w * AREA + rr * LROW + col);
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(turn + w * AREA + rr * LROW + col + 4);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                    {
+                        v.v[t] = w ? v.v[t] + a[t] : a[t];
+                        v.v[t + 4] = w ? v.v[t + 4] + b[t] : b[t];
+                    }
+                }
                 return v;
             };
             if (EPI == EPI_GU)
@@ -435,7 +458,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm16_k(const GemmArgs p)
             else store_8<T>(p, p.out[prod], o, m, piece(c));
         }
         }
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        if (WK > 1) __syncthreads();
+        else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }
 }
 

@@ -360,3 +360,10 @@ def test_refusals(cuda):
         u.mul_(2.0)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(y, g, dy)
+
+
+# every tile shape and split count that the planner chooses: few and many rows against long and short K
+@pytest.mark.parametrize("T,H,I", [(100, 2048, 64), (100, 64, 2048), (517, 768, 512), (700, 1032, 1160), (300, 4104, 520),
+                                   (1100, 1544, 776), (90, 4096, 4096)])
+def test_tile_plans(cuda, T, H, I):
+    backward_check(cuda, T, H, I, torch.float16, 0, 0.0)
