@@ -13,7 +13,7 @@ static bool dtype_ok(int d) { return d == BMX_DT_FP16 || d == BMX_DT_BF16; }
 // 64 with a workgroup on every other compute unit or fewer (alone) and with the chip full, us to begin and end.
 struct Tile { int M, N, slots; double alone, full, ends; };
 static const Tile TILES[4] = {
-    {256, 256, 256, 1.45, 1.45, 6.0},      // 8 waves, 2 buffers
+    {256, 256, 256, 1.60, 1.60, 6.0},      // 8 waves, 2 buffers
     {128, 128, 512, 0.64, 1.00, 3.0},      // 4 waves, 2 buffers, two on a compute unit
     {128, 64, 256, 0.34, 0.38, 3.0},       // 2 groups of 4 waves, each every other K tile, 3 buffers
     {128, 128, 256, 0.54, 0.54, 3.0},      // the same, 2 buffers
@@ -23,7 +23,7 @@ struct TilePlan { int tile, splits; };
 // Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
 // the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
 // (written and read at 4 TB/s) cost.
-static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split)
+static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool across = false)
 {
     TilePlan best = {0, 1};
     double least = 1e30;
@@ -34,8 +34,10 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
             const Tile& c = TILES[t];
             const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * products * s, full = b / c.slots, rest = b % c.slots;
             const int each = (nk + s - 1) / s;
+            // with a side across K, and the gradients' epilogue behind half of those, about a fourth more
             double us = full * (each * c.full + c.ends);
             if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
+            if (across) us *= 1.25;
             if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
             if (us < least) { least = us; best = {t, s}; }
         }
@@ -73,7 +75,7 @@ static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
     if (EPI == EPI_GU) g.b[1] = g.b[0];
     int rc = run_gemm<T, AX, BX, EPI_PART>(g, tp.tile, s);
     if (rc) return rc;
-    const int64_t pieces = (int64_t)a.ldp / 8 * a.N;
+    const int64_t pieces = (int64_t)a.ldp / 4 * a.N;
     hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a);
     return check_launch("gemm_finish");
 }
@@ -242,8 +244,8 @@ struct FfnBackPlan {
 static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
 {
     FfnBackPlan p;
-    p.dh = plan_product(d->I, T, tiles_k(d->H), 1, true);
-    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true);
+    p.dh = plan_product(d->I, T, tiles_k(d->H), 1, true, true);
+    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true, true);
     p.dd = plan_product(d->I, d->H, tiles_k(T), 1, false);
     p.dw = plan_product(d->H, d->I, tiles_k(T), 2, false);
     size_t o = 0;

@@ -65,77 +65,86 @@ struct GemmArgs {
 
 typedef __attribute__((address_space(3))) char* lds_ptr;
 
-// Eight neighbouring values of a result row: 16 bytes of 16-bit values
-struct f32x8 { float v[8]; };
+// W (4 or 8) neighbouring values of a result row: 8 or 16 bytes of 16-bit values
+template <int W> struct Vals { float v[W]; };
 
-template <class T> __device__ __forceinline__ u32x4 pack8(const f32x8& v)
+template <class T, int W> __device__ __forceinline__ void store16(uint16_t* q, const Vals<W>& v)
 {
-    u32x4 w;
+    uint32_t w[W / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to16<T>(v.v[2 * i]) | (uint32_t)to16<T>(v.v[2 * i + 1]) << 16;
-    return w;
+    for (int i = 0; i < W / 2; ++i) w[i] = (uint32_t)to16<T>(v.v[2 * i]) | (uint32_t)to16<T>(v.v[2 * i + 1]) << 16;
+    if constexpr (W == 8) *reinterpret_cast<u32x4*>(q) = u32x4{w[0], w[1], w[2], w[3]};
+    else *reinterpret_cast<u32x2*>(q) = u32x2{w[0], w[1]};
+}
+template <int W> __device__ __forceinline__ void store32(float* q, const Vals<W>& v)
+{
+#pragma unroll
+    for (int i = 0; i < W; i += 4) *reinterpret_cast<f32x4*>(q + i) = f32x4{v.v[i], v.v[i + 1], v.v[i + 2], v.v[i + 3]};
+}
+template <int W> __device__ __forceinline__ Vals<W> load32(const float* q)
+{
+    Vals<W> v;
+#pragma unroll
+    for (int i = 0; i < W; i += 4)
+    {
+        const f32x4 a = ldg4f(q + i);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) v.v[i + t] = a[t];
+    }
+    return v;
 }
 
-// What becomes of eight neighbouring sums of a result row (columns m .. m + 7), at element o of the outputs. Rows are
-// multiples of 8 values except in store_8 (4-bit matrices of any N), where the last ones are stored one by one.
-template <class T> __device__ __forceinline__ void store_8(const GemmArgs& p, void* out, int64_t o, int m, const f32x8& v)
+// What becomes of W neighbouring sums of a result row (columns m .. m + W - 1), at element o of the outputs. Rows are
+// multiples of 8 values except in put (4-bit matrices of any N), where the last ones are stored one by one.
+template <class T, int W> __device__ __forceinline__ void put(const GemmArgs& p, void* out, int64_t o, int m, const Vals<W>& v)
 {
     uint16_t* q = static_cast<uint16_t*>(out) + o;
-    if (!(p.ldo & 7)) { *reinterpret_cast<u32x4*>(q) = pack8<T>(v); return; }
+    if (!(p.ldo & 7)) { store16<T>(q, v); return; }
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int t = 0; t < W; ++t)
         if (m + t < p.M) q[t] = to16<T>(v.v[t]);
 }
 
-__device__ __forceinline__ void add_8(const GemmArgs& p, int64_t o, int n, const f32x8& v)
+template <int W> __device__ __forceinline__ void put_add(const GemmArgs& p, int64_t o, int n, const Vals<W>& v)
 {
     const float sc = p.scale ? p.scale[n] : 1.0f;
-    f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p.out[0]) + o);
+    float* q = static_cast<float*>(p.out[0]) + o;
+    Vals<W> c = load32<W>(q);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int t = 0; t < W; ++t) c.v[t] = __builtin_fmaf(sc, v.v[t], c.v[t]);
+    store32(q, c);
+}
+
+template <class T, int W> __device__ __forceinline__ void put_gu(const GemmArgs& p, int64_t o, const Vals<W>& g, const Vals<W>& u)
+{
+    Vals<W> h;
+#pragma unroll
+    for (int t = 0; t < W; ++t) h.v[t] = act_h(p.act, g.v[t], u.v[t]);
+    store16<T>(static_cast<uint16_t*>(p.out[0]) + o, h);
+    if (p.g)
     {
-        f32x4 c = q[h];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) c[t] = __builtin_fmaf(sc, v.v[4 * h + t], c[t]);
-        q[h] = c;
+        store32(p.g + o, g);
+        store32(p.u + o, u);
     }
 }
 
-template <class T> __device__ __forceinline__ void gu_8(const GemmArgs& p, int64_t o, const f32x8& g, const f32x8& u)
-{
-    f32x8 h;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) h.v[t] = act_h(p.act, g.v[t], u.v[t]);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(h);
-    if (p.g)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-        {
-            reinterpret_cast<f32x4*>(p.g + o)[i] = f32x4{g.v[4 * i], g.v[4 * i + 1], g.v[4 * i + 2], g.v[4 * i + 3]};
-            reinterpret_cast<f32x4*>(p.u + o)[i] = f32x4{u.v[4 * i], u.v[4 * i + 1], u.v[4 * i + 2], u.v[4 * i + 3]};
-        }
-}
+// g and u, loaded ahead of their use
+template <int W> struct GU { Vals<W> g, u; };
+template <int W> __device__ __forceinline__ GU<W> load_gu(const GemmArgs& p, int64_t o) { return {load32<W>(p.g + o), load32<W>(p.u + o)}; }
 
-// g and u of eight values, loaded ahead of their use
-struct GU8 { f32x4 g[2], u[2]; };
-__device__ __forceinline__ GU8 load_gu(const GemmArgs& p, int64_t o)
+template <class T, int W> __device__ __forceinline__ void put_dgu(const GemmArgs& p, int64_t o, const Vals<W>& dh, const GU<W>& s)
 {
-    return {{ldg4f(p.g + o), ldg4f(p.g + o + 4)}, {ldg4f(p.u + o), ldg4f(p.u + o + 4)}};
-}
-
-template <class T> __device__ __forceinline__ void dgu_8(const GemmArgs& p, int64_t o, const f32x8& dh, const GU8& s)
-{
-    f32x8 dg, du;
+    Vals<W> dg, du;
 #pragma unroll
-    for (int t = 0; t < 8; ++t)
+    for (int t = 0; t < W; ++t)
     {
         float hg, hu;
-        act_grad(p.act, s.g[t >> 2][t & 3], s.u[t >> 2][t & 3], hg, hu);
+        act_grad(p.act, s.g.v[t], s.u.v[t], hg, hu);
         dg.v[t] = dh.v[t] * hg;
         du.v[t] = dh.v[t] * hu;
     }
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[0]) + o) = pack8<T>(dg);
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p.out[1]) + o) = pack8<T>(du);
+    store16<T>(static_cast<uint16_t*>(p.out[0]) + o, dg);
+    store16<T>(static_cast<uint16_t*>(p.out[1]) + o, du);
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------
@@ -410,13 +419,13 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         static_assert(MINE % (64 * AHEAD) == 0, "whole steps");
         for (int q0 = group * MINE + lane; q0 < (group + 1) * MINE; q0 += 64 * AHEAD)
         {
-        GU8 saved[EPI == EPI_DGU ? AHEAD : 1];
+        GU<8> saved[EPI == EPI_DGU ? AHEAD : 1];
         if (EPI == EPI_DGU)
 #pragma unroll
             for (int k = 0; k < AHEAD; ++k)
             {
                 const int q = q0 + k * 64, n = nb + q / PIECES, m = wm0 + q % PIECES * 8;
-                if (n < p.N && m < p.M) saved[EPI == EPI_DGU ? k : 0] = load_gu(p, (int64_t)n * p.ldo + m);
+                if (n < p.N && m < p.M) saved[EPI == EPI_DGU ? k : 0] = load_gu<8>(p, (int64_t)n * p.ldo + m);
             }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
@@ -425,7 +434,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
             if (n >= p.N || m >= p.M) continue;
             const int64_t o = (int64_t)n * p.ldo + m;
             auto piece = [&](int col) {
-                f32x8 v;
+                Vals<8> v;
 #pragma unroll
                 for (int w = 0; w < WK; ++w)
                 {
@@ -444,18 +453,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
             {
                 // gate and up rows in turn by 32
                 const int col = (c >> 5) * 64 + (c & 31);
-                gu_8<T>(p, o, piece(col), piece(col + 32));
+                put_gu<T>(p, o, piece(col), piece(col + 32));
             }
-            else if (EPI == EPI_PART)
-            {
-                const f32x8 v = piece(c);
-                f32x4* d = reinterpret_cast<f32x4*>(p.part + ((int64_t)z * p.N + n) * p.ldp + m);
-                d[0] = f32x4{v.v[0], v.v[1], v.v[2], v.v[3]};
-                d[1] = f32x4{v.v[4], v.v[5], v.v[6], v.v[7]};
-            }
-            else if (EPI == EPI_ADD) add_8(p, o, n, piece(c));
-            else if (EPI == EPI_DGU) dgu_8<T>(p, o, piece(c), saved[EPI == EPI_DGU ? k : 0]);
-            else store_8<T>(p, p.out[prod], o, m, piece(c));
+            else if (EPI == EPI_PART) store32(p.part + ((int64_t)z * p.N + n) * p.ldp + m, piece(c));
+            else if (EPI == EPI_ADD) put_add(p, o, n, piece(c));
+            else if (EPI == EPI_DGU) put_dgu<T>(p, o, piece(c), saved[EPI == EPI_DGU ? k : 0]);
+            else put<T>(p, p.out[prod], o, m, piece(c));
         }
         }
         if (WK > 1) __syncthreads();
@@ -463,55 +466,43 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     }
 }
 
-// The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Eight values per
-// thread.
+// The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Four values per thread
+// and up to 16 splits' loads at a time: the kernel is a few waves, each load round of which waits for HBM once.
 template <class T, int EPI>
 __global__ __launch_bounds__(64) void gemm_finish_k(const GemmArgs p)
 {
-    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 8;
+    constexpr int W = 4, PRODS = EPI == EPI_GU ? 2 : 1, B = 16 / PRODS;
+    const int64_t plane = (int64_t)p.N * p.ldp, at = ((int64_t)blockIdx.x * 64 + threadIdx.x) * W;
     if (at >= plane) return;
     const int n = (int)(at / p.ldp), m = (int)(at % p.ldp);
-    auto sum = [&](int prod) {
-        const float* q = p.part + prod * p.splits * plane + at;
-        f32x8 v;
+    const int64_t o = (int64_t)n * p.ldo + m;
+    GU<W> saved;
+    if (EPI == EPI_DGU) saved = load_gu<W>(p, o);
+    Vals<W> sum[PRODS];
 #pragma unroll
-        for (int t = 0; t < 8; ++t) v.v[t] = 0.0f;
-        // eight splits' loads at a time: one after the other they would each wait for HBM
-        for (int s0 = 0; s0 < p.splits; s0 += 8)
-        {
-            f32x4 a[8], b[8];
+    for (int k = 0; k < PRODS; ++k)
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
-            {
-                const float* w = q + min(s0 + s, p.splits - 1) * plane;
-                a[s] = ldg4f(w);
-                b[s] = ldg4f(w + 4);
-            }
+        for (int t = 0; t < W; ++t) sum[k].v[t] = 0.0f;
+    for (int s0 = 0; s0 < p.splits; s0 += B)
+    {
+        Vals<W> part[PRODS][B];
 #pragma unroll
-            for (int s = 0; s < 8; ++s)
+        for (int s = 0; s < B; ++s)
+#pragma unroll
+            for (int k = 0; k < PRODS; ++k)
+                if (s0 + s < p.splits) part[k][s] = load32<W>(p.part + (k * p.splits + s0 + s) * plane + at);
+#pragma unroll
+        for (int s = 0; s < B; ++s)
+#pragma unroll
+            for (int k = 0; k < PRODS; ++k)
                 if (s0 + s < p.splits)
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                    {
-                        v.v[t] += a[s][t];
-                        v.v[t + 4] += b[s][t];
-                    }
-        }
-        return v;
-    };
-    const int64_t o = (int64_t)n * p.ldo + m;
-    if (EPI == EPI_GU)
-    {
-        const f32x8 g = sum(0), u = sum(1);
-        gu_8<T>(p, o, g, u);
+                    for (int t = 0; t < W; ++t) sum[k].v[t] += part[k][s].v[t];
     }
-    else if (EPI == EPI_ADD) add_8(p, o, n, sum(0));
-    else if (EPI == EPI_DGU)
-    {
-        const GU8 saved = load_gu(p, o);
-        dgu_8<T>(p, o, sum(0), saved);
-    }
-    else store_8<T>(p, p.out[0], o, m, sum(0));
+    if (EPI == EPI_GU) put_gu<T>(p, o, sum[0], sum[PRODS - 1]);
+    else if (EPI == EPI_ADD) put_add(p, o, n, sum[0]);
+    else if (EPI == EPI_DGU) put_dgu<T>(p, o, sum[0], saved);
+    else put<T>(p, p.out[0], o, m, sum[0]);
 }
 
 }  // namespace bmx

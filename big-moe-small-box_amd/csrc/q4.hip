@@ -122,7 +122,7 @@ size_t skinny_part_bytes(int N, int K, int T, int products)
 
 template <class T, int TT, int G> static int slice_launch(const SliceArgs& a, dim3 grid, hipStream_t s)
 {
-    hipLaunchKernelGGL((slice_k<T, TT, G>), grid, dim3(SL_W * 64), 0, s, a);
+    hipLaunchKernelGGL((slice_k<T, TT, G>), grid, dim3(SL_W<TT> * 64), 0, s, a);
     return check_launch("slice");
 }
 
@@ -147,9 +147,10 @@ template <class T, int EPI> static int slice_product(const SkinnyArgs& k, float*
     a.ldp = padded(k.N);
     a.tiles = (k.N + 15) / 16 * a.products;
     a.part = part;
-    // up to 768 workgroups (three on a compute unit at 48 tokens), of at least a tile per wave
-    const int blocks = 768 / a.slices > 0 ? 768 / a.slices : 1;
-    a.per = ((a.tiles + blocks - 1) / blocks + SL_W - 1) / SL_W * SL_W;
+    // up to 768 workgroups of 4 waves or 512 of 8 (what the compute units hold at 48 and 64 tokens), of at least a tile per wave
+    const int waves = k.T <= 48 ? SL_W<3> : SL_W<4>, most = k.T <= 48 ? 768 : 512;
+    const int blocks = most / a.slices > 0 ? most / a.slices : 1;
+    a.per = ((a.tiles + blocks - 1) / blocks + waves - 1) / waves * waves;
     const dim3 grid((unsigned)((a.tiles + a.per - 1) / a.per), (unsigned)a.slices);
     int rc;
     switch (k.group)
@@ -163,7 +164,7 @@ template <class T, int EPI> static int slice_product(const SkinnyArgs& k, float*
     GemmArgs g = {};
     g.M = k.N; g.N = k.T; g.ldp = a.ldp; g.splits = a.slices; g.part = part;
     g.out[0] = k.out; g.ldo = k.ldo; g.scale = k.scale; g.act = k.act; g.g = k.g; g.u = k.u;
-    const int64_t pieces = (int64_t)a.ldp / 8 * k.T;
+    const int64_t pieces = (int64_t)a.ldp / 4 * k.T;
     hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, g);
     return check_launch("gemm_finish");
 }

@@ -100,7 +100,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 {
     typedef typename Elem<T>::v8 v8;
     constexpr bool Q4 = G != 0, GU = EPI == EPI_GU;
-    constexpr int NG = Q4 ? SK_K / G : 1, JG = 4 / NG;             // groups of a step, words of a group
+    constexpr int NG = Q4 ? SK_K / (G ? G : 1) : 1, JG = 4 / NG;             // groups of a step, words of a group
     constexpr int ROWS = GU ? 8 : 16;                              // result columns of a tile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * (ROWS * RT);
@@ -280,7 +280,8 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 // columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
 // go to part (as EPI_PART), gemm_finish_k joins them.
 constexpr int SL_K = 512;           // columns of a slice
-constexpr int SL_W = 4;             // waves of a workgroup: few, so that small matrices still spread evenly
+// waves of a workgroup: few, so that small matrices still spread evenly; more where x leaves room for one or two workgroups
+template <int TT> constexpr int SL_W = TT <= 3 ? 4 : 8;
 constexpr int SL_TT = 5;            // most tiles of 16 tokens: 80 KB of x
 
 struct SliceArgs {
@@ -291,12 +292,12 @@ struct SliceArgs {
 };
 
 template <class T, int TT, int G>
-__global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
+__global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
 {
     typedef typename Elem<T>::v8 v8;
     constexpr bool Q4 = G != 0, OFFSET = Q4 && Q4Dec<T>::OFFSET;
-    constexpr int NG = Q4 ? SK_K / G : 1, JG = 4 / NG, U = SL_K / SK_K;   // groups of a step, words of a group, steps of a tile
-    constexpr int SG = Q4 ? SL_K / G : 1;                                 // groups of a slice
+    constexpr int NG = Q4 ? SK_K / (G ? G : 1) : 1, JG = 4 / NG, U = SL_K / SK_K;   // groups of a step, words of a group, steps of a tile
+    constexpr int SG = Q4 ? SL_K / (G ? G : 1) : 1;                                 // groups of a slice
     const SkinnyArgs& p = sp.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const int slice = blockIdx.y, k0 = slice * SL_K, KT = (p.K + SK_K - 1) / SK_K, NT = (p.N + 15) / 16;
@@ -353,7 +354,7 @@ __global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
     int tile = blockIdx.x * sp.per + wave;
     if (tile < end) load(tile);
     // x in loads of up to 8 at a time: one after the other they would each wait for L2
-    constexpr int CH = SL_K / 8, LOADS = TT * 16 * CH / (SL_W * 64), B = LOADS % 8 ? 4 : 8;
+    constexpr int CH = SL_K / 8, LOADS = TT * 16 * CH / (SL_W<TT> * 64), B = LOADS % 8 == 0 ? 8 : LOADS % 5 == 0 ? 5 : 4;
     static_assert(LOADS % B == 0, "whole batches");
 #pragma unroll
     for (int l0 = 0; l0 < LOADS; l0 += B)
@@ -362,13 +363,13 @@ __global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
 #pragma unroll
         for (int l = 0; l < B; ++l)
         {
-            const int i = (l0 + l) * (SL_W * 64) + threadIdx.x, t = i / CH, k = k0 + i % CH * 8;
+            const int i = (l0 + l) * (SL_W<TT> * 64) + threadIdx.x, t = i / CH, k = k0 + i % CH * 8;
             v[l] = t < p.T && k < p.K ? ldg4(p.x + (int64_t)t * p.K + k) : u32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int l = 0; l < B; ++l)
         {
-            const int i = (l0 + l) * (SL_W * 64) + threadIdx.x, t = i / CH, c = i % CH;
+            const int i = (l0 + l) * (SL_W<TT> * 64) + threadIdx.x, t = i / CH, c = i % CH;
             *reinterpret_cast<u32x4*>(xl + t * (SL_K * 2) + ((c ^ (t & 15)) << 4)) = v[l];
             if (OFFSET)
             {
@@ -385,7 +386,7 @@ __global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
     }
     __syncthreads();
 
-    for (; tile < end; tile += SL_W)
+    for (; tile < end; tile += SL_W<TT>)
     {
         f32x4 acc[TT];
 #pragma unroll
@@ -436,7 +437,7 @@ __global__ __launch_bounds__(SL_W * 64) void slice_k(const SliceArgs sp)
                 }
             }
         }
-        if (tile + SL_W < end) load(tile + SL_W);
+        if (tile + SL_W<TT> < end) load(tile + SL_W<TT>);
         const int n = nt * 16 + r;
         float* out = sp.part + (int64_t)(m * sp.slices + slice) * p.T * sp.ldp + n;
         if (n < p.N)
