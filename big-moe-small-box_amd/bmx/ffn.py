@@ -25,12 +25,15 @@ def rows_of(x, K, dtype, device, name):
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+
+
 def stream_here(device):
     """The handle of the current stream of device if that is the current device, else None (the caller then enters it:
     kernels go to the current device). The handle is read without making a Stream object: that costs 2 us, as much as a
     decode call's other host work together."""
     index = device.index
-    return torch._C._cuda_getCurrentRawStream(index) if torch.cuda.current_device() == index else None
+    return _raw_stream(index) if _current_device() == index else None
 
 
 class GatedFFN:

@@ -66,6 +66,8 @@ def q4_linear(x, q):
     dt = DTYPES.get(dtype)
     if dt is None:
         raise ValueError(f"q4_linear: x must be fp16 or bf16, got {dtype}")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise ValueError("q4_linear: 4-bit weights have no gradients (detach x, or torch.no_grad())")
     device = q.device
     r = rows_of(x, q.K, dtype, device, "q4_linear: x")
     s = stream_here(device)
@@ -73,7 +75,7 @@ def q4_linear(x, q):
         with torch.cuda.device(device):
             return q4_linear(x, q)
     T = r.shape[0]
-    y = torch.empty((T, q.N), dtype=dtype, device=device)
+    y = r.new_empty((T, q.N))
     if T:
         L_ = lib()
         need = L_.bmx_q4_linear_workspace(q.struct, T)

@@ -18,15 +18,14 @@ static const Tile TILES[4] = {
     {128, 64, 256, 0.34, 0.38, 3.0},       // 2 groups of 4 waves, each every other K tile, 3 buffers
     {128, 128, 256, 0.54, 0.54, 3.0},      // the same, 2 buffers
 };
-struct TilePlan { int tile, splits; };
+struct TilePlan { int tile, splits; double us; };
 
 // Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
 // the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
 // (written and read at 4 TB/s) cost.
 static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool across = false)
 {
-    TilePlan best = {0, 1};
-    double least = 1e30;
+    TilePlan best = {0, 1, 1e30};
     for (int t = 0; t < 4; ++t)
         for (int s = 1; s <= 16; s *= 2)
         {
@@ -39,7 +38,7 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
             if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
             if (across) us *= 1.25;
             if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
-            if (us < least) { least = us; best = {t, s}; }
+            if (us < best.us) best = {t, s, us};
         }
     return best;
 }
@@ -105,21 +104,24 @@ __global__ __launch_bounds__(256) void row_gate_k(const uint16_t* __restrict__ x
 
 static int tiles_k(int K) { return (K + GK - 1) / GK; }
 
-size_t product_part_bytes(int N, int T, int K)
+// EPI_GU is one product of twice the rows, but two where K is split
+static TilePlan plan_for(int N, int T, int K, int products) { return plan_product((int64_t)N * products, T, tiles_k(K), 1, true); }
+
+double product_us(int N, int T, int K, int products) { return plan_for(N, T, K, products).us; }
+
+size_t product_part_bytes(int N, int T, int K, int products)
 {
-    const TilePlan p = plan_product(N, T, tiles_k(K), 1, true);
-    return p.splits > 1 ? (size_t)p.splits * T * ((N + 7) / 8 * 8) * 4 : 0;
+    const TilePlan p = plan_for(N, T, K, products);
+    return p.splits > 1 ? (size_t)p.splits * products * T * ((N + 7) / 8 * 8) * 4 : 0;
 }
 
-int launch_product(const void* w, const void* x, int T, int N, int K, int dtype, void* y, void* part, hipStream_t s)
+int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s)
 {
-    GemmArgs a = {};
-    a.chain = a.batch = a.splits = 1;
-    a.part = static_cast<float*>(part);
-    a.a[0] = w; a.b[0] = x; a.out[0] = y;
-    a.M = N; a.N = T; a.K = K; a.lda = a.ldb = K; a.ldo = N;
-    const TilePlan p = plan_product(N, T, tiles_k(K), 1, true);
-    return dtype == BMX_DT_FP16 ? product<f16, false, false, EPI_STORE>(a, p, s) : product<bf16, false, false, EPI_STORE>(a, p, s);
+    const TilePlan p = plan_for(g.M, g.N, g.K, epi == EPI_GU ? 2 : 1);
+    const bool h = dtype == BMX_DT_FP16;
+    if (epi == EPI_GU) return h ? product<f16, false, false, EPI_GU>(g, p, s) : product<bf16, false, false, EPI_GU>(g, p, s);
+    if (epi == EPI_ADD) return h ? product<f16, false, false, EPI_ADD>(g, p, s) : product<bf16, false, false, EPI_ADD>(g, p, s);
+    return h ? product<f16, false, false, EPI_STORE>(g, p, s) : product<bf16, false, false, EPI_STORE>(g, p, s);
 }
 
 // A forward pass's weights: 16-bit, or q[3] (4-bit)
@@ -128,7 +130,7 @@ struct FfnIn {
     ActPar act;
     const void* w[3];
     const bmx_q4* q[3];
-    int group() const { return q[0] ? q[0]->group : 0; }
+    int group(int m) const { return q[0] ? q[m]->group : 0; }
 };
 
 static FfnIn ffn_in(const bmx_ffn_desc* d)
@@ -141,28 +143,47 @@ static FfnIn ffn_in(const bmx_ffn4_desc* d)
     return {d->gate->K, d->gate->N, d->dtype, act_par(d->act, d->act_limit), {nullptr, nullptr, nullptr}, {d->gate, d->up, d->down}};
 }
 
-struct FfnPlan {
-    TilePlan gu, down;
-    bool few;                               // tokens: skinny products
-    size_t h, part, gate, deq, total;       // workspace offsets
-};
+struct FfnPlan { size_t h, gate, part, total; };       // workspace offsets; part: what the larger of the products needs
+
+static size_t product_bytes(const FfnIn& d, int N, int K, int T, int products, int group)
+{
+    if (T <= skinny_tokens_max()) return skinny_part_bytes(N, K, T, products);
+    return group ? q4_many_bytes(N, K, T, products, group) : product_part_bytes(N, T, K, products);
+}
 
 static FfnPlan ffn_plan(const FfnIn& d, int T)
 {
     FfnPlan p;
-    p.few = T <= skinny_tokens_max();
-    p.gu = plan_product(2 * (int64_t)d.I, T, tiles_k(d.H), 1, true);
-    p.down = plan_product(d.H, T, tiles_k(d.I), 1, true);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
     p.h = take((size_t)T * d.I * 2);
     p.gate = take((size_t)T * 4);
-    const size_t pg = p.few ? skinny_part_bytes(d.I, d.H, T, 2) : p.gu.splits > 1 ? (size_t)p.gu.splits * 2 * T * d.I * 4 : 0;
-    const size_t pd = p.few ? skinny_part_bytes(d.H, d.I, T, 1) : p.down.splits > 1 ? (size_t)p.down.splits * T * d.H * 4 : 0;
-    p.part = take(pg > pd ? pg : pd);
-    p.deq = take(d.q[0] && !p.few ? (size_t)d.H * d.I * 4 : 0);
+    const size_t gu = product_bytes(d, d.I, d.H, T, 2, d.group(0)), down = product_bytes(d, d.H, d.I, T, 1, d.group(2));
+    p.part = take(gu > down ? gu : down);
     p.total = o + 256;
     return p;
+}
+
+// One of the block's products on the kernel for its tokens and weights. first: 0 gate and up (EPI_GU), 2 down
+static int block_product(const FfnIn& d, const SkinnyArgs& base, int first, int epi, char* part, hipStream_t s)
+{
+    SkinnyArgs k = base;
+    const int n = epi == EPI_GU ? 2 : 1;
+    for (int m = 0; m < n; ++m)
+    {
+        k.w[m] = d.w[first + m];
+        if (d.q[0]) k.q[m] = q4_view(d.q[first + m]);
+    }
+    k.group = d.group(first);
+    if (k.T <= skinny_tokens_max()) return launch_skinny(k, d.dtype, epi, reinterpret_cast<float*>(part), s);
+    if (k.group) return launch_q4_many(k, d.q + first, d.dtype, epi, part, s);
+    GemmArgs a = {};
+    a.chain = a.batch = a.splits = 1;
+    a.part = reinterpret_cast<float*>(part);
+    a.act = k.act; a.scale = k.scale; a.g = k.g; a.u = k.u;
+    a.a[0] = k.w[0]; a.a[1] = k.w[1]; a.b[0] = k.x; a.out[0] = k.out;
+    a.M = k.N; a.N = k.T; a.K = k.K; a.lda = a.ldb = k.K; a.ldo = k.ldo;
+    return launch_product(a, d.dtype, epi, s);
 }
 
 template <class T>
@@ -171,69 +192,27 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
 {
     const FfnPlan p = ffn_plan(d, n);
     void* h = sv ? sv->h : ws + p.h;
-    float* scale = nullptr;
-    int rc = BMX_OK;
-    if (gate_vec)
-    {
-        scale = reinterpret_cast<float*>(ws + p.gate);
-        hipLaunchKernelGGL((row_gate_k<T>), dim3((n + 3) / 4), dim3(256), 0, s, static_cast<const uint16_t*>(x),
-                           static_cast<const uint16_t*>(gate_vec), n, d.H, scale);
-        if ((rc = check_launch("row_gate"))) return rc;
-    }
     SkinnyArgs k = {};
     k.T = n;
     k.act = d.act;
-    k.scale = scale;
-    GemmArgs a = {};
-    a.chain = a.batch = a.splits = 1;
-    a.part = reinterpret_cast<float*>(ws + p.part);
-    a.act = d.act;
-    a.N = n;
-    a.scale = scale;
-    char* deq = ws + p.deq;
-
     // h = act(x Wg^T, x Wu^T)
-    if (p.few)
+    k.x = static_cast<const uint16_t*>(x);
+    k.N = k.ldo = d.I; k.K = d.H; k.out = h;
+    if (sv) { k.g = sv->g; k.u = sv->u; }
+    int rc = block_product(d, k, 0, EPI_GU, ws + p.part, s);
+    if (rc) return rc;
+    if (gate_vec)
     {
-        for (int m = 0; m < 2; ++m)
-        {
-            k.w[m] = d.w[m];
-            if (d.q[0]) k.q[m] = q4_view(d.q[m]);
-        }
-        k.group = d.group();
-        k.x = static_cast<const uint16_t*>(x);
-        k.N = d.I; k.K = d.H; k.out = h; k.ldo = d.I;
-        if (sv) { k.g = sv->g; k.u = sv->u; }
-        if ((rc = launch_skinny(k, d.dtype, EPI_GU, a.part, s))) return rc;
-    }
-    else
-    {
-        for (int m = 0; m < 2; ++m)
-        {
-            a.a[m] = d.q[0] ? deq + (size_t)m * d.H * d.I * 2 : d.w[m];
-            if (d.q[0] && (rc = launch_q4_dequant(d.q[m], d.dtype, deq + (size_t)m * d.H * d.I * 2, s))) return rc;
-        }
-        a.b[0] = x; a.out[0] = h;
-        a.M = d.I; a.K = d.H; a.lda = a.ldb = d.H; a.ldo = d.I;
-        if (sv) { a.g = sv->g; a.u = sv->u; }
-        if ((rc = product<T, false, false, EPI_GU>(a, p.gu, s))) return rc;
+        float* scale = reinterpret_cast<float*>(ws + p.gate);
+        hipLaunchKernelGGL((row_gate_k<T>), dim3((n + 3) / 4), dim3(256), 0, s, static_cast<const uint16_t*>(x),
+                           static_cast<const uint16_t*>(gate_vec), n, d.H, scale);
+        if ((rc = check_launch("row_gate"))) return rc;
+        k.scale = scale;
     }
     // y = h Wd^T
-    void* out = add ? static_cast<void*>(add) : y;
-    if (p.few)
-    {
-        k.w[0] = d.w[2];
-        if (d.q[0]) k.q[0] = q4_view(d.q[2]);
-        k.group = d.q[0] ? d.q[2]->group : 0;
-        k.x = static_cast<const uint16_t*>(h);
-        k.N = d.H; k.K = d.I; k.out = out; k.ldo = d.H;
-        return launch_skinny(k, d.dtype, add ? EPI_ADD : EPI_STORE, a.part, s);
-    }
-    a.a[0] = d.q[0] ? deq : d.w[2];
-    if (d.q[0] && (rc = launch_q4_dequant(d.q[2], d.dtype, deq, s))) return rc;
-    a.a[1] = nullptr; a.b[0] = h; a.out[0] = out;
-    a.M = d.H; a.K = d.I; a.lda = a.ldb = d.I; a.ldo = d.H;
-    return add ? product<T, false, false, EPI_ADD>(a, p.down, s) : product<T, false, false, EPI_STORE>(a, p.down, s);
+    k.x = static_cast<const uint16_t*>(h);
+    k.N = k.ldo = d.H; k.K = d.I; k.out = add ? static_cast<void*>(add) : y;
+    return block_product(d, k, 2, add ? EPI_ADD : EPI_STORE, ws + p.part, s);
 }
 
 struct FfnBackPlan {

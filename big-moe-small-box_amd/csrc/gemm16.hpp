@@ -217,6 +217,62 @@ struct TileLoader {
     }
 };
 
+// 32 result rows from nb, turned over in LDS: turn [32][WROW + 4] of a wave, one of each of WK groups WM * WN * 32 rows apart,
+// whose sums belong together. The columns are those of the result from wm0 (EPI_GU: gate and up in turn by 32).
+template <class T, int EPI, int WROW, int WK>
+__device__ __forceinline__ void store_turned(const GemmArgs& p, const float* turn, int area, int lane, int group, int nb, int wm0, int z,
+                                             int prod)
+{
+    constexpr int LROW = WROW + 4, PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8;   // 8-value pieces of a row
+    // four pieces at a time, so that what they read from HBM (g and u) is on its way together
+    constexpr int MINE = 32 * PIECES / WK, AHEAD = MINE / 64 < 4 ? MINE / 64 : 4;
+    static_assert(MINE % (64 * AHEAD) == 0, "whole steps");
+    for (int q0 = group * MINE + lane; q0 < (group + 1) * MINE; q0 += 64 * AHEAD)
+    {
+        GU<8> saved[EPI == EPI_DGU ? AHEAD : 1];
+        if (EPI == EPI_DGU)
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k)
+            {
+                const int q = q0 + k * 64, n = nb + q / PIECES, m = wm0 + q % PIECES * 8;
+                if (n < p.N && m < p.M) saved[EPI == EPI_DGU ? k : 0] = load_gu<8>(p, (int64_t)n * p.ldo + m);
+            }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+        {
+            const int q = q0 + k * 64, rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
+            if (n >= p.N || m >= p.M) continue;
+            const int64_t o = (int64_t)n * p.ldo + m;
+            auto piece = [&](int col) {
+                Vals<8> v;
+#pragma unroll
+                for (int w = 0; w < WK; ++w)
+                {
+                    const f32x4 a = *reinterpret_cast<const f32x4*>(turn + w * area + rr * LROW + col);
+                    const f32x4 b = *reinterpret_cast<const f32x4*>(turn + w * area + rr * LROW + col + 4);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                    {
+                        v.v[t] = w ? v.v[t] + a[t] : a[t];
+                        v.v[t + 4] = w ? v.v[t + 4] + b[t] : b[t];
+                    }
+                }
+                return v;
+            };
+            if (EPI == EPI_GU)
+            {
+                // gate and up rows in turn by 32
+                const int col = (c >> 5) * 64 + (c & 31);
+                put_gu<T>(p, o, piece(col), piece(col + 32));
+            }
+            else if (EPI == EPI_PART) store32(p.part + ((int64_t)z * p.N + n) * p.ldp + m, piece(c));
+            else if (EPI == EPI_ADD) put_add(p, o, n, piece(c));
+            else if (EPI == EPI_DGU) put_dgu<T>(p, o, piece(c), saved[EPI == EPI_DGU ? k : 0]);
+            else put<T>(p, p.out[prod], o, m, piece(c));
+        }
+    }
+}
+
 // BM x BN results by WK groups of WM x WN waves, NB buffers of a K tile each. Every group has K tiles of its own (the WK-th
 // ones, loaded by itself into its own part of LDS); their sums are added at the end, in the groups' order.
 template <class T, int BM, int BN, int WM, int WN, int WK, int NB, bool AX, bool BX, int EPI>
@@ -398,7 +454,6 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     constexpr int AREA = WM * WN * 32 * LROW;                       // of a group
     float* turn = reinterpret_cast<float*>(lds_all) + wave * (32 * LROW);
     const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
-    constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8;   // 8-value pieces of a row
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
 #pragma unroll
@@ -414,53 +469,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         // one group: the wave's own rows only, its LDS writes and reads are in order
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        // four pieces at a time, so that what they read from HBM (g and u) is on its way together
-        constexpr int MINE = 32 * PIECES / WK, AHEAD = MINE / 64 < 4 ? MINE / 64 : 4;
-        static_assert(MINE % (64 * AHEAD) == 0, "whole steps");
-        for (int q0 = group * MINE + lane; q0 < (group + 1) * MINE; q0 += 64 * AHEAD)
-        {
-        GU<8> saved[EPI == EPI_DGU ? AHEAD : 1];
-        if (EPI == EPI_DGU)
-#pragma unroll
-            for (int k = 0; k < AHEAD; ++k)
-            {
-                const int q = q0 + k * 64, n = nb + q / PIECES, m = wm0 + q % PIECES * 8;
-                if (n < p.N && m < p.M) saved[EPI == EPI_DGU ? k : 0] = load_gu<8>(p, (int64_t)n * p.ldo + m);
-            }
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-        {
-            const int q = q0 + k * 64, rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
-            if (n >= p.N || m >= p.M) continue;
-            const int64_t o = (int64_t)n * p.ldo + m;
-            auto piece = [&](int col) {
-                Vals<8> v;
-#pragma unroll
-                for (int w = 0; w < WK; ++w)
-                {
-                    const f32x4 a = *reinterpret_cast<const f32x4*>(turn + w * AREA + rr * LROW + col);
-                    const f32x4 b = *reinterpret_cast<const f32x4*>(turn + w * AREA + rr * LROW + col + 4);
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                    {
-                        v.v[t] = w ? v.v[t] + a[t] : a[t];
-                        v.v[t + 4] = w ? v.v[t + 4] + b[t] : b[t];
-                    }
-                }
-                return v;
-            };
-            if (EPI == EPI_GU)
-            {
-                // gate and up rows in turn by 32
-                const int col = (c >> 5) * 64 + (c & 31);
-                put_gu<T>(p, o, piece(col), piece(col + 32));
-            }
-            else if (EPI == EPI_PART) store32(p.part + ((int64_t)z * p.N + n) * p.ldp + m, piece(c));
-            else if (EPI == EPI_ADD) put_add(p, o, n, piece(c));
-            else if (EPI == EPI_DGU) put_dgu<T>(p, o, piece(c), saved[EPI == EPI_DGU ? k : 0]);
-            else put<T>(p, p.out[prod], o, m, piece(c));
-        }
-        }
+        store_turned<T, EPI, WROW, WK>(p, turn, AREA, lane, group, nb, wm0, z, prod);
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }

@@ -1,5 +1,5 @@
 // 4-bit matrices with group scales: packing into fragment order, decoding to 16 bits, and products of few tokens (skinny_k).
-#include "skinny.hpp"
+#include "q4_gemm.hpp"
 
 namespace bmx {
 
@@ -213,12 +213,115 @@ int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStrea
     return h ? few_tokens<f16, EPI_STORE>(a, part, s) : few_tokens<bf16, EPI_STORE>(a, part, s);
 }
 
+// ---- products of many tokens ----------------------------------------------------------------------------------------------
+
+// What was measured of gemm_q4_k: us a step of 128 columns with a workgroup on every other compute unit or fewer, and with
+// two on each; of decoding a matrix first: bytes at 4.8 TB/s and a launch
+struct Q4Plan { bool direct; int splits; double us; };
+
+static Q4Plan q4_plan(int N, int K, int T, int products, int group)
+{
+    const int KT = (K + SK_K - 1) / SK_K;
+    const int64_t tiles = (int64_t)((N + QG_N - 1) / QG_N) * ((T + QG_T - 1) / QG_T) * products;
+    const double more = group == 128 ? 1.0 : group == 64 ? 1.15 : 1.4;
+    Q4Plan best = {true, 1, 1e30};
+    for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); s *= 2)
+    {
+        const int64_t b = tiles * s, full = b / 512, rest = b % 512;
+        const int each = (KT + s - 1) / s;
+        double us = full * (each * 2.0 * more + 3.0);
+        if (rest) us += each * (rest <= 256 ? 1.3 : 2.0) * more + 3.0;
+        if (s > 1) us += 5.0 + (double)N * T * products * s * 8.0 / 4e6;
+        if (us < best.us) best = {true, s, us};
+    }
+    const double first = products * ((double)N * K * 2.5 / 4.8e6 + 2.0) + product_us(N, T, K, products);
+    if (first < best.us) best = {false, 1, first};
+    return best;
+}
+
+static size_t group_sums_bytes(int K, int T, int group) { return align_up((size_t)(ceil_to(K, SK_K) / group) * ceil_to(T, QG_T) * 4, 256); }
+
+// part and sums of a direct product; the decoded matrices and the tiled product's partial sums of the other
+size_t q4_many_bytes(int N, int K, int T, int products, int group)
+{
+    const Q4Plan p = q4_plan(N, K, T, products, group);
+    if (!p.direct) return align_up((size_t)products * N * K * 2, 256) + product_part_bytes(N, T, K, products);
+    return group_sums_bytes(K, T, group) + (p.splits > 1 ? (size_t)products * p.splits * T * padded(N) * 4 : 0);
+}
+
+template <class T, int G, int EPI> static int gemm_q4_launch(Q4GemmArgs a, int splits, hipStream_t s)
+{
+    constexpr int PRODS = EPI == EPI_GU ? 2 : 1;
+    if (Q4Dec<T>::OFFSET)
+    {
+        const int64_t n = (int64_t)a.g.N * (ceil_to(a.g.K, SK_K) / 8);
+        hipLaunchKernelGGL((group_sums_k<T, G>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a.x, a.g.N, a.g.K,
+                           const_cast<float*>(a.xs), a.xs_ld);
+        const int rc = check_launch("group_sums");
+        if (rc) return rc;
+    }
+    a.g.tn = (a.g.N + QG_T - 1) / QG_T;
+    a.g.splits = splits;
+    if (splits == 1)
+    {
+        const int rows = EPI == EPI_GU ? QG_N / 2 : QG_N;
+        a.g.tm = (a.g.M + rows - 1) / rows;
+        hipLaunchKernelGGL((gemm_q4_k<T, G, EPI>), dim3((unsigned)(a.g.tm * a.g.tn)), dim3(256), 0, s, a);
+        return check_launch("gemm_q4");
+    }
+    a.g.tm = (a.g.M + QG_N - 1) / QG_N;
+    hipLaunchKernelGGL((gemm_q4_k<T, G, EPI_PART>), dim3((unsigned)(a.g.tm * a.g.tn), 1, (unsigned)(splits * PRODS)), dim3(256), 0, s, a);
+    const int rc = check_launch("gemm_q4");
+    if (rc) return rc;
+    const int64_t pieces = (int64_t)a.g.ldp / 4 * a.g.N;
+    hipLaunchKernelGGL((gemm_finish_k<T, EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a.g);
+    return check_launch("gemm_finish");
+}
+
+template <class T, int EPI> static int q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, char* ws, hipStream_t s)
+{
+    constexpr int PRODS = EPI == EPI_GU ? 2 : 1;
+    const Q4Plan plan = q4_plan(k.N, k.K, k.T, PRODS, k.group);
+    Q4GemmArgs a = {};
+    a.g.chain = a.g.batch = a.g.splits = 1;
+    a.g.M = k.N; a.g.N = k.T; a.g.K = k.K; a.g.ldo = k.ldo; a.g.ldp = padded(k.N);
+    a.g.out[0] = k.out; a.g.scale = k.scale; a.g.act = k.act;
+    if (!plan.direct)
+    {
+        const size_t one = (size_t)k.N * k.K * 2;
+        for (int m = 0; m < PRODS; ++m)
+            if (const int rc = launch_q4_dequant(q[m], dtype, ws + m * one, s)) return rc;
+        a.g.a[0] = ws; a.g.a[1] = ws + one; a.g.b[0] = k.x;
+        a.g.lda = a.g.ldb = k.K;
+        a.g.part = reinterpret_cast<float*>(ws + align_up(PRODS * one, 256));
+        return launch_product(a.g, dtype, EPI, s);
+    }
+    a.q[0] = k.q[0]; a.q[1] = k.q[1];
+    a.x = k.x;
+    a.xs = reinterpret_cast<float*>(ws);
+    a.xs_ld = (int)ceil_to(k.T, QG_T);
+    a.g.part = reinterpret_cast<float*>(ws + group_sums_bytes(k.K, k.T, k.group));
+    switch (k.group)
+    {
+        case 32: return gemm_q4_launch<T, 32, EPI>(a, plan.splits, s);
+        case 64: return gemm_q4_launch<T, 64, EPI>(a, plan.splits, s);
+        default: return gemm_q4_launch<T, 128, EPI>(a, plan.splits, s);
+    }
+}
+
+int launch_q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, int epi, char* ws, hipStream_t s)
+{
+    const bool h = dtype == BMX_DT_FP16;
+    if (epi == EPI_GU) return h ? q4_many<f16, EPI_GU>(k, q, dtype, ws, s) : q4_many<bf16, EPI_GU>(k, q, dtype, ws, s);
+    if (epi == EPI_ADD) return h ? q4_many<f16, EPI_ADD>(k, q, dtype, ws, s) : q4_many<bf16, EPI_ADD>(k, q, dtype, ws, s);
+    return h ? q4_many<f16, EPI_STORE>(k, q, dtype, ws, s) : q4_many<bf16, EPI_STORE>(k, q, dtype, ws, s);
+}
+
 // ---- y = x W^T ----------------------------------------------------------------------------------------------------------
 
 static size_t q4_linear_ws(const bmx_q4* q, int T)
 {
-    if (T <= skinny_tokens_max()) return skinny_part_bytes(q->N, q->K, T, 1);
-    return align_up((size_t)q->N * q->K * 2, 256) + product_part_bytes(q->N, T, q->K);
+    return T <= skinny_tokens_max() ? skinny_part_bytes(q->N, q->K, T, 1) : q4_many_bytes(q->N, q->K, T, 1, q->group);
 }
 
 }  // namespace bmx
@@ -285,17 +388,12 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
         return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", fn);
     if (workspace_bytes < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, need);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (T > skinny_tokens_max())
-    {
-        // many tokens: the weights once to 16 bits, then the tiled product
-        if ((rc = launch_q4_dequant(q, dtype, workspace, s))) return rc;
-        return launch_product(workspace, x, T, q->N, q->K, dtype, y, static_cast<char*>(workspace) + align_up((size_t)q->N * q->K * 2, 256), s);
-    }
     SkinnyArgs a = {};
     a.q[0] = q4_view(q);
     a.x = static_cast<const uint16_t*>(x);
     a.T = T; a.N = q->N; a.K = q->K; a.group = q->group;
     a.out = y; a.ldo = q->N;
+    if (T > skinny_tokens_max()) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
     return launch_skinny(a, dtype, EPI_STORE, static_cast<float*>(workspace), s);
 }
 

@@ -47,9 +47,14 @@ int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStrea
 size_t skinny_part_bytes(int N, int K, int T, int products);
 // the most tokens that it takes
 int skinny_tokens_max();
-// ffn.hip: y [T][N] = x w^T with 16-bit weights on gemm16_k; part: product_part_bytes bytes
-int launch_product(const void* w, const void* x, int T, int N, int K, int dtype, void* y, void* part, hipStream_t s);
-size_t product_part_bytes(int N, int T, int K);
+// A product of more tokens on 4-bit weights q[0] (and q[1]: EPI_GU); ws: q4_many_bytes bytes
+int launch_q4_many(const SkinnyArgs& a, const bmx_q4* const* q, int dtype, int epi, char* ws, hipStream_t s);
+size_t q4_many_bytes(int N, int K, int T, int products, int group);
+// ffn.hip: a product of 16-bit weights on gemm16_k (EPI_STORE, EPI_ADD, EPI_GU with two matrices); g.part:
+// product_part_bytes bytes; about how long it takes
+int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s);
+size_t product_part_bytes(int N, int T, int K, int products);
+double product_us(int N, int T, int K, int products);
 
 // One decoded word: 8 weights. fp16: 1024 + c is 0x6400 | c, 1024 + 16 c is 0x6400 | c << 4; subtracting the offset and the
 // zero point is exact. bf16 has no packed arithmetic here: 128 + c is 0x4300 | c, and the 128 + z comes off the sum, as

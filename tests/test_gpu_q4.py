@@ -59,7 +59,7 @@ def test_linear(cuda, T, G, dt):
         R.check(f"y {N} {K}", y, y64, R.rounded(y64, e, DT[dt]))
 
 
-@pytest.mark.parametrize("T,K,N", [(1, 2048, 14336), (8, 5120, 2304), (3, 11008, 4096), (64, 4096, 1536), (600, 512, 3016)])
+@pytest.mark.parametrize("T,K,N", [(1, 2048, 14336), (520, 4096, 520), (1100, 1024, 4096), (4200, 256, 1032), (8, 5120, 2304), (3, 11008, 4096), (64, 4096, 1536), (600, 512, 3016)])
 def test_linear_of_model_sizes(cuda, T, K, N):
     import bmx
     given, q64 = codes(cuda, N, K, 128, "mid", torch.float16)
@@ -71,7 +71,7 @@ def test_linear_of_model_sizes(cuda, T, K, N):
 
 @pytest.mark.parametrize("dt", sorted(DT))
 @pytest.mark.parametrize("T,H,I,G", [(1, 128, 256, 128), (2, 192, 64, 64), (5, 96, 160, 32), (16, 512, 384, 128), (17, 320, 448, 64),
-                                     (33, 256, 96, 32), (64, 128, 128, 64), (65, 384, 640, 128), (200, 192, 320, 64),
+                                     (33, 256, 96, 32), (64, 128, 128, 64), (65, 384, 640, 128), (81, 160, 96, 32), (200, 192, 320, 64),
                                      (520, 2048, 768, 128)])
 def test_gated_block(cuda, T, H, I, G, dt):
     import bmx
@@ -113,6 +113,8 @@ def test_mixed_groups_and_layouts(cuda):
     leaf = x.clone().requires_grad_()
     with pytest.raises(ValueError):
         ffn.forward(leaf)
+    with pytest.raises(ValueError):
+        bmx.ops.q4_linear(leaf, ffn.gate)
     with torch.no_grad():
         assert torch.equal(ffn.forward(leaf), ffn.forward(x))
 
