@@ -223,14 +223,14 @@ static Q4Plan q4_plan(int N, int K, int T, int products, int group)
 {
     const int KT = (K + SK_K - 1) / SK_K;
     const int64_t tiles = (int64_t)((N + QG_N - 1) / QG_N) * ((T + QG_T - 1) / QG_T) * products;
-    const double more = group == 128 ? 1.0 : group == 64 ? 1.15 : 1.4;
+    const double more = group == 128 ? 1.0 : group == 64 ? 1.08 : 1.35;
     Q4Plan best = {true, 1, 1e30};
     for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); s *= 2)
     {
         const int64_t b = tiles * s, full = b / 512, rest = b % 512;
         const int each = (KT + s - 1) / s;
-        double us = full * (each * 2.0 * more + 3.0);
-        if (rest) us += each * (rest <= 256 ? 1.3 : 2.0) * more + 3.0;
+        double us = full * (each * 2.3 * more + 3.0);
+        if (rest) us += each * (rest <= 256 ? 1.37 : 2.3) * more + 3.0;
         if (s > 1) us += 5.0 + (double)N * T * products * s * 8.0 / 4e6;
         if (us < best.us) best = {true, s, us};
     }

@@ -2,8 +2,9 @@
 // codes stay codes until they are operands: a step's 8 KB of them lie in LDS beside 32 KB of x, a lane reads its 32 rows' 64
 // codes of 128 columns with two loads and decodes eight at a time for one matrix instruction (skinny.hpp, Q4Dec). Scales and
 // zero points go onto each group's sums, so the weights are never rounded. Against decoding the matrix to 16 bits first (the
-// bytes written and read again: 4096 -> 11008 23 us beside a product of 62 for 517 tokens) this wins until the tokens are so
-// many that the larger tiles of gemm16_k pay for it (q4_plan).
+// bytes written and read again: 4096 -> 11008 23 us beside a product of 65 for 517 tokens) this wins, 78 us, until the tokens
+// are so many that the larger tiles of gemm16_k pay for it (q4_plan; 4,096 tokens 442 against 370 us). A wave's step is 32
+// matrix instructions (1,024 cycles, 1,280 with the bf16 correction) and about 240 others.
 //
 // v_mfma_f32_32x32x16: A = 32 tokens, B = 32 rows of W; the result's column is the row of W, its rows the tokens.
 #pragma once
@@ -101,8 +102,11 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_k(const Q4GemmArgs qp)
         }
         ++loaded;
     };
-    // scales and zero points of this lane's rows, a step ahead
-    struct Scales { uint16_t s[NW][NG]; uint8_t z[NW][NG]; } sc, sn;
+    // Scales and zero points of this lane's rows of W, and (bf16) the sums of x of its tokens, a step ahead. The 128 + zero
+    // that bf16 codes carry too much come off as one more product over the groups, sums of x times -scale (128 + zero), on
+    // the fp32 matrix instruction of two columns: lanes 0 .. 31 hold the even group of a pair, 32 .. 63 the odd (or nothing).
+    constexpr int NP = (NG + 1) / 2;
+    struct Scales { uint16_t s[NW][NG]; uint8_t z[NW][NG]; float xs[MT][NP]; } sc, sn;
     auto load_scales = [&](Scales& v, int at) {
 #pragma unroll
         for (int i = 0; i < NW; ++i)
@@ -119,6 +123,16 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_k(const Q4GemmArgs qp)
                 v.z[i][g] = zp ? zp[o] : 8;
             }
         }
+        if (OFFSET)
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < NP; ++q)
+                {
+                    const int g = q * 2 + (NG > 1 ? h : 0);
+                    const float xs = qp.xs[(int64_t)(at * NG + g) * qp.xs_ld + t0 + wm * 64 + m * 32 + (lane & 31)];
+                    v.xs[m][q] = NG == 1 && h ? 0.0f : xs;
+                }
     };
     const bool sbf[2] = {(GATED ? qp.q[0] : qp.q[prod]).scale_bf16 != 0, (GATED ? qp.q[1] : qp.q[prod]).scale_bf16 != 0};
 
@@ -152,6 +166,17 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_k(const Q4GemmArgs qp)
             for (int o = 0; o < 2; ++o)
                 code[i][o] = *(__attribute__((address_space(3))) u32x4*)(at + 2 * XB + ((wn * 2 + i) * 2 + half) * 1024 +
                                                                          ((o * 2 + h) * 16 + r) * 16);
+        // x fragments one product ahead
+        v8 x[2][MT];
+        auto read = [&](int kk) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+            {
+                const int row = wm * 64 + m * 32 + (lane & 31), c = (kk & 3) * 2 + h;
+                x[kk & 1][m] = *(__attribute__((address_space(3))) v8*)(at + (kk >> 2) * XB + row * (GK * 2) + ((c ^ swz_along(row)) << 4));
+            }
+        };
+        read(0);
 #pragma unroll
         for (int g = 0; g < NG; ++g)
         {
@@ -168,41 +193,38 @@ __global__ __launch_bounds__(256, 2) void gemm_q4_k(const Q4GemmArgs qp)
 #pragma unroll
             for (int kk = g * (G / 16); kk < (g + 1) * (G / 16); ++kk)
             {
-                v8 x[MT], w[NW];
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-                {
-                    const int row = wm * 64 + m * 32 + (lane & 31), c = (kk & 3) * 2 + h;
-                    x[m] = *(__attribute__((address_space(3))) v8*)(at + (kk >> 2) * XB + row * (GK * 2) + ((c ^ swz_along(row)) << 4));
-                }
+                v8 w[NW];
+                if (kk < 7) read(kk + 1);
 #pragma unroll
                 for (int i = 0; i < NW; ++i) w[i] = dec[i](code[i][kk & 1][kk >> 1]);
 #pragma unroll
                 for (int m = 0; m < MT; ++m)
 #pragma unroll
-                    for (int i = 0; i < NW; ++i) part[m][i] = Elem<T>::mfma32(x[m], w[i], part[m][i]);
+                    for (int i = 0; i < NW; ++i) part[m][i] = Elem<T>::mfma32(x[kk & 1][m], w[i], part[m][i]);
+            }
+            float s[NW], off[NW];
+#pragma unroll
+            for (int i = 0; i < NW; ++i)
+            {
+                s[i] = sbf[i] ? from16<bf16>(sc.s[i][g]) : from16<f16>(sc.s[i][g]);
+                off[i] = s[i] * (-128.0f - (float)sc.z[i][g]);
+                if (NG > 1 && (g & 1))
+                {
+                    const float even = (sbf[i] ? from16<bf16>(sc.s[i][g & ~1]) : from16<f16>(sc.s[i][g & ~1])) *
+                                       (-128.0f - (float)sc.z[i][g & ~1]);
+                    off[i] = h ? off[i] : even;
+                }
             }
 #pragma unroll
             for (int m = 0; m < MT; ++m)
-            {
-                f32x4 xs[4];
-                if (OFFSET)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        xs[e] = ldg4f(qp.xs + (int64_t)(kt * NG + g) * qp.xs_ld + t0 + wm * 64 + m * 32 + e * 8 + h * 4);
 #pragma unroll
                 for (int i = 0; i < NW; ++i)
                 {
-                    const float s = sbf[i] ? from16<bf16>(sc.s[i][g]) : from16<f16>(sc.s[i][g]);
-                    const float off = OFFSET ? -128.0f - (float)sc.z[i][g] : 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                    {
-                        const float v = OFFSET ? __builtin_fmaf(off, xs[e >> 2][e & 3], part[m][i][e]) : part[m][i][e];
-                        acc[m][i][e] = __builtin_fmaf(s, v, acc[m][i][e]);
-                    }
+                    for (int e = 0; e < 16; ++e) acc[m][i][e] = __builtin_fmaf(s[i], part[m][i][e], acc[m][i][e]);
+                    if (OFFSET && (NG == 1 || (g & 1)))
+                        acc[m][i] = __builtin_amdgcn_mfma_f32_32x32x2f32(sc.xs[m][g / 2], off[i], acc[m][i], 0, 0, 0);
                 }
-            }
         }
         sc = sn;
     }

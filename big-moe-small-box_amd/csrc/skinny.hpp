@@ -56,6 +56,16 @@ int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s);
 size_t product_part_bytes(int N, int T, int K, int products);
 double product_us(int N, int T, int K, int products);
 
+// (v & mask) | magic in one v_and_or_b32, which takes one scalar register and no literals: the constants are put into
+// registers, or the compiler would make two instructions of two literals. (The instruction itself is the compiler's: a matrix
+// instruction may read its result only two wait states later, which it would not know of one in inline asm.)
+__device__ __forceinline__ uint32_t and_or(uint32_t v, uint32_t mask, uint32_t magic)
+{
+    asm("" : "+s"(mask));
+    asm("" : "+v"(magic));
+    return (v & mask) | magic;
+}
+
 // One decoded word: 8 weights. fp16: 1024 + c is 0x6400 | c, 1024 + 16 c is 0x6400 | c << 4; subtracting the offset and the
 // zero point is exact. bf16 has no packed arithmetic here: 128 + c is 0x4300 | c, and the 128 + z comes off the sum, as
 // (128 + z) times the group's sum of x.
@@ -76,9 +86,9 @@ template <> struct Q4Dec<f16>
 #pragma unroll
         for (int h = 0; h < 2; ++h, v >>= 8)
         {
-            r[2 * h] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, (v & 0x000f000fu) | 0x64006400u) + c0);
+            r[2 * h] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2, and_or(v, 0x000f000fu, 0x64006400u)) + c0);
             r[2 * h + 1] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(
-                __builtin_bit_cast(f16x2, (v & 0x00f000f0u) | 0x64006400u), s, c1));
+                __builtin_bit_cast(f16x2, and_or(v, 0x00f000f0u, 0x64006400u)), s, c1));
         }
         return __builtin_bit_cast(f16x8, u32x4{r[0], r[1], r[2], r[3]});
     }
@@ -91,7 +101,7 @@ template <> struct Q4Dec<bf16>
     {
         u32x4 r;
 #pragma unroll
-        for (int p = 0; p < 4; ++p, v >>= 4) r[p] = (v & 0x000f000fu) | 0x43004300u;
+        for (int p = 0; p < 4; ++p, v >>= 4) r[p] = and_or(v, 0x000f000fu, 0x43004300u);
         return __builtin_bit_cast(bf16x8, r);
     }
 };
