@@ -147,7 +147,7 @@ struct FfnPlan { size_t h, gate, part, total; };       // workspace offsets; par
 
 static size_t product_bytes(const FfnIn& d, int N, int K, int T, int products, int group)
 {
-    if (T <= skinny_tokens_max()) return skinny_part_bytes(N, K, T, products);
+    if (T <= skinny_tokens_max(group)) return skinny_part_bytes(N, K, T, products);
     return group ? q4_many_bytes(N, K, T, products, group) : product_part_bytes(N, T, K, products);
 }
 
@@ -175,7 +175,7 @@ static int block_product(const FfnIn& d, const SkinnyArgs& base, int first, int 
         if (d.q[0]) k.q[m] = q4_view(d.q[first + m]);
     }
     k.group = d.group(first);
-    if (k.T <= skinny_tokens_max()) return launch_skinny(k, d.dtype, epi, reinterpret_cast<float*>(part), s);
+    if (k.T <= skinny_tokens_max(k.group)) return launch_skinny(k, d.dtype, epi, reinterpret_cast<float*>(part), s);
     if (k.group) return launch_q4_many(k, d.q + first, d.dtype, epi, part, s);
     GemmArgs a = {};
     a.chain = a.batch = a.splits = 1;

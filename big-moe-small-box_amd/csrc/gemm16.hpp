@@ -291,14 +291,15 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     const int wm = wave / WN, wn = wave % WN;
 
     // Tiles in an order that keeps an XCD (workgroups are dealt to the 8 XCDs in turn) on neighbouring tiles: each XCD takes
-    // one contiguous run, and a run walks N within groups of 8 tiles of M, so that its L2 holds the rows it shares
+    // one contiguous run, and a run walks N within groups of 8 or 4 tiles of M, so that its L2 holds the rows it shares
+    // (without the first, products across K take a sixth longer)
     const int nwg = p.tm * p.tn;
     int id = blockIdx.x;
     {
         const int q = nwg / 8, r = nwg % 8, x = id & 7;
         id = x * q + (x < r ? x : r) + (id >> 3);
     }
-    constexpr int GRP = 8;
+    constexpr int GRP = AX ? 4 : 8;                                 // (A across K: 4; 2 x 2,048 x 4,096 x 8,192 251 -> 240 us)
     const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
     const int tm = g0 + (id % per) % gn, tn = (id % per) / gn;
     const int m0 = EPI == EPI_GU ? tm * (BM / 2) : tm * BM, n0 = tn * BN;

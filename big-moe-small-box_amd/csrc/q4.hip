@@ -110,7 +110,9 @@ int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s)
 // Tokens up to which skinny_k reads W once past x from the caches; above, slices
 static int direct_tokens() { return 16; }
 
-int skinny_tokens_max() { return SL_TT * 16; }
+// 16-bit weights: gemm16_k from 17 tokens on (33 tokens through a 5120 x 2304 block 25.9 us, by slices 29.0; 4096 x 11008 65
+// and 88). 4-bit weights: slices up to 80 (33 tokens 4096 -> 4096 10.4 us, by gemm_q4_k 12.4; 80 tokens 14.8 and 16.3)
+int skinny_tokens_max(int group) { return group ? SL_TT * 16 : direct_tokens(); }
 
 static int padded(int n) { return (n + 7) / 8 * 8; }
 static int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
@@ -155,7 +157,6 @@ template <class T, int EPI> static int slice_product(const SkinnyArgs& k, float*
     int rc;
     switch (k.group)
     {
-        case 0: rc = slice_tokens<T, 0>(a, grid, s); break;
         case 32: rc = slice_tokens<T, 32>(a, grid, s); break;
         case 64: rc = slice_tokens<T, 64>(a, grid, s); break;
         default: rc = slice_tokens<T, 128>(a, grid, s);
@@ -177,20 +178,32 @@ template <class T, int RT, int G, int EPI, bool XL> static int direct_rows(const
     return check_launch("skinny");
 }
 
-// Tiles of rows per workgroup: x is read once per workgroup, so that above 8 tokens two tiles halve what outweighs W, as long
-// as the workgroups still cover half the chip (16 tokens, us with 1 / 2 / 4 tiles: 4-bit 5120 -> 2 x 2304 13.1 / 9.0 / 11.1,
-// 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 / 11.5 / 9.7; 16-bit 2304 -> 5120 9.8 / 8.0 / 12.0, 4096 -> 2 x 2048 10.8
-// / 13.0 / 20; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5)
+// Tiles of rows per workgroup (1, 2 or 4). x is read once per workgroup, so more tiles save what x costs beside a tile of W
+// (about 0.2 of a 4-bit tile a token, 0.05 of a 16-bit one); but the compute unit with the most workgroups is the last to end,
+// so their number goes up in whole rounds of the 256 units. Against measurements (us with 1 / 2 / 4 tiles): 16 tokens, 4-bit
+// 5120 -> 2 x 2304 13.1 / 9.0 / 11.1, 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 / 11.5 / 9.7, 16-bit 2304 -> 5120 9.8 /
+// 8.0 / 12.0, 4096 -> 2 x 2048 10.8 / 13.0; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5; 4 tokens 4096 -> 11008 9.4 / 11.8.
+static int row_tiles(int tiles, int T, bool q4)
+{
+    int best = 1;
+    double least = 1e30;
+    for (int rt = 1; rt <= (q4 ? 4 : 2); rt *= 2)
+    {
+        const double us = ((tiles + rt - 1) / rt + 255) / 256 * (rt + T * (q4 ? 0.2 : 0.05));
+        if (us < least) { least = us; best = rt; }
+    }
+    return best;
+}
+
 template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a, hipStream_t s)
 {
-    const int tiles = (a.N + 15) / 16 * (EPI == EPI_GU ? 2 : 1);
+    const int rt = row_tiles((a.N + 15) / 16 * (EPI == EPI_GU ? 2 : 1), a.T, G != 0);
     if constexpr (G != 0)
     {
-        if (a.T > 8 && tiles >= 768) return direct_rows<T, 4, G, EPI, false>(a, s);
-        if ((size_t)a.T * a.K <= 8192) return direct_rows<T, 1, G, EPI, true>(a, s);
+        if (a.T == 1 && a.K <= 8192) return direct_rows<T, 1, G, EPI, true>(a, s);
+        if (rt == 4) return direct_rows<T, 4, G, EPI, false>(a, s);
     }
-    if (a.T > 8 && tiles >= 288) return direct_rows<T, 2, G, EPI, false>(a, s);
-    return direct_rows<T, 1, G, EPI, false>(a, s);
+    return rt == 2 ? direct_rows<T, 2, G, EPI, false>(a, s) : direct_rows<T, 1, G, EPI, false>(a, s);
 }
 
 template <class T, int EPI> static int few_tokens(const SkinnyArgs& a, float* part, hipStream_t s)
@@ -321,7 +334,7 @@ int launch_q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, int e
 
 static size_t q4_linear_ws(const bmx_q4* q, int T)
 {
-    return T <= skinny_tokens_max() ? skinny_part_bytes(q->N, q->K, T, 1) : q4_many_bytes(q->N, q->K, T, 1, q->group);
+    return T <= skinny_tokens_max(q->group) ? skinny_part_bytes(q->N, q->K, T, 1) : q4_many_bytes(q->N, q->K, T, 1, q->group);
 }
 
 }  // namespace bmx
@@ -393,7 +406,7 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
     a.x = static_cast<const uint16_t*>(x);
     a.T = T; a.N = q->N; a.K = q->K; a.group = q->group;
     a.out = y; a.ldo = q->N;
-    if (T > skinny_tokens_max()) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
+    if (T > skinny_tokens_max(q->group)) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
     return launch_skinny(a, dtype, EPI_STORE, static_cast<float*>(workspace), s);
 }
 

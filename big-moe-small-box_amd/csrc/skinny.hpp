@@ -41,12 +41,12 @@ struct SkinnyArgs {
 Q4View q4_view(const bmx_q4* q);
 int check_q4(const bmx_q4* q, const char* who);
 int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s);
-// A product of few tokens on a's weights (a.group 0: 16-bit) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU); part:
+// A product of few tokens on a's weights (a.group 0: 16-bit, up to 16 tokens) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU); part:
 // skinny_part_bytes bytes
 int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s);
 size_t skinny_part_bytes(int N, int K, int T, int products);
 // the most tokens that it takes
-int skinny_tokens_max();
+int skinny_tokens_max(int group);
 // A product of more tokens on 4-bit weights q[0] (and q[1]: EPI_GU); ws: q4_many_bytes bytes
 int launch_q4_many(const SkinnyArgs& a, const bmx_q4* const* q, int dtype, int epi, char* ws, hipStream_t s);
 size_t q4_many_bytes(int N, int K, int T, int products, int group);
@@ -290,7 +290,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
     }
 }
 
-// ---- more tokens: slices of K ---------------------------------------------------------------------------------------------
+// ---- 4-bit weights, more tokens: slices of K ---------------------------------------------------------------------------------------------
 // From some tokens on what skinny_k reads of x (16 tokens for every 16 rows of W) outgrows W. Here a workgroup keeps 512
 // columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
 // go to part (as EPI_PART), gemm_finish_k joins them.
@@ -310,9 +310,9 @@ template <class T, int TT, int G>
 __global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
 {
     typedef typename Elem<T>::v8 v8;
-    constexpr bool Q4 = G != 0, OFFSET = Q4 && Q4Dec<T>::OFFSET;
-    constexpr int NG = Q4 ? SK_K / (G ? G : 1) : 1, JG = 4 / NG, U = SL_K / SK_K;   // groups of a step, words of a group, steps of a tile
-    constexpr int SG = Q4 ? SL_K / (G ? G : 1) : 1;                                 // groups of a slice
+    constexpr bool OFFSET = Q4Dec<T>::OFFSET;
+    constexpr int NG = SK_K / G, JG = 4 / NG, U = SL_K / SK_K;     // groups of a step, words of a group, steps of a tile
+    constexpr int SG = SL_K / G;                                   // groups of a slice
     const SkinnyArgs& p = sp.a;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const int slice = blockIdx.y, k0 = slice * SL_K, KT = (p.K + SK_K - 1) / SK_K, NT = (p.N + 15) / 16;
@@ -323,45 +323,26 @@ __global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
     __shared__ __attribute__((aligned(16))) float xs[OFFSET ? SG * TT * 16 : 4];   // [group][token]: sums of x (bf16)
 
     struct Step {
-        u32x4 w[Q4 ? 1 : 4];
+        u32x4 w;
         uint16_t s[NG];
         uint8_t z[NG];
     } st[U];
     auto load = [&](int tile) {
         const int m = tile >= NT ? 1 : 0, nt = tile - m * NT;
         const Q4View v = p.q[m];
-        const int n = min(nt * 16 + r, p.N - 1);
 #pragma unroll
         for (int u = 0; u < U; ++u)
         {
             const int kt = k0 / SK_K + u;
             if (kt >= KT) return;
             Step& b = st[u];
-            if (Q4)
+            b.w = ldg4(v.codes + ((int64_t)nt * KT + kt) * 64 + lane);
+#pragma unroll
+            for (int g = 0; g < NG; ++g)
             {
-                b.w[0] = ldg4(v.codes + ((int64_t)nt * KT + kt) * 64 + lane);
-#pragma unroll
-                for (int g = 0; g < NG; ++g)
-                {
-                    const int64_t at = ((int64_t)nt * (KT * NG) + kt * NG + g) * 16 + r;
-                    b.s[g] = v.scale[at];
-                    b.z[g] = v.zero ? v.zero[at] : 8;
-                }
-            }
-            else
-            {
-                const uint16_t* w = static_cast<const uint16_t*>(p.w[m]) + (int64_t)n * p.K;
-                const int k = kt * SK_K + q * 8;
-                if (kt * SK_K + SK_K <= p.K)
-                {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b.w[Q4 ? 0 : j] = ldg4(w + k + j * 32);
-                }
-                else
-                {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) b.w[Q4 ? 0 : j] = k + j * 32 < p.K ? ldg4(w + k + j * 32) : u32x4{0, 0, 0, 0};
-                }
+                const int64_t at = ((int64_t)nt * (KT * NG) + kt * NG + g) * 16 + r;
+                b.s[g] = v.scale[at];
+                b.z[g] = v.zero ? v.zero[at] : 8;
             }
         }
     };
@@ -389,7 +370,7 @@ __global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
             if (OFFSET)
             {
                 // the lanes of a group are neighbours
-                constexpr int LG = Q4 ? G / 8 : 1;
+                constexpr int LG = G / 8;
                 float sum = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum += from16<T>((uint16_t)v[l][e]) + from16<T>((uint16_t)(v[l][e] >> 16));
@@ -417,14 +398,6 @@ __global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
         {
             if (k0 / SK_K + u >= KT) break;
             const Step b = st[u];
-            if (!Q4)
-            {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int t = 0; t < TT; ++t) acc[t] = Elem<T>::mfma16(x(u, j, t), __builtin_bit_cast(v8, b.w[Q4 ? 0 : j]), acc[t]);
-                continue;
-            }
 #pragma unroll
             for (int g = 0; g < NG; ++g)
             {
@@ -437,7 +410,7 @@ __global__ __launch_bounds__(SL_W<TT> * 64) void slice_k(const SliceArgs sp)
 #pragma unroll
                 for (int j = g * JG; j < (g + 1) * JG; ++j)
                 {
-                    const v8 w = dec(b.w[0][j]);
+                    const v8 w = dec(b.w[j]);
 #pragma unroll
                     for (int t = 0; t < TT; ++t) part[t] = Elem<T>::mfma16(x(u, j, t), w, part[t]);
                 }
