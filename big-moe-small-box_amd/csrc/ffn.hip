@@ -27,7 +27,7 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
 {
     TilePlan best = {0, 1, 1e30};
     for (int t = 0; t < 4; ++t)
-        for (int s = 1; s <= 16; s *= 2)
+        for (int s = 1; s <= 16; ++s)
         {
             if (s > 1 && (!can_split || nk / s < 4)) break;
             const Tile& c = TILES[t];

@@ -172,7 +172,8 @@ template <class T, int EPI> static int slice_product(const SkinnyArgs& k, float*
 
 template <class T, int RT, int G, int EPI, bool XL> static int direct_rows(const SkinnyArgs& a, hipStream_t s)
 {
-    constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT, D = 2;
+    constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT;
+    constexpr int D = RT == 4 && G == 32 ? 1 : 2;                  // (two steps of four tiles and 16 groups spill)
     hipLaunchKernelGGL((skinny_k<T, RT, G, D, EPI, XL>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(SK_W * 64),
                        XL ? (size_t)a.T * (a.K * 2 + 16) : 0, s, a);
     return check_launch("skinny");
@@ -238,7 +239,7 @@ static Q4Plan q4_plan(int N, int K, int T, int products, int group)
     const int64_t tiles = (int64_t)((N + QG_N - 1) / QG_N) * ((T + QG_T - 1) / QG_T) * products;
     const double more = group == 128 ? 1.0 : group == 64 ? 1.08 : 1.35;
     Q4Plan best = {true, 1, 1e30};
-    for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); s *= 2)
+    for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); ++s)
     {
         const int64_t b = tiles * s, full = b / 512, rest = b % 512;
         const int each = (KT + s - 1) / s;
