@@ -18,14 +18,15 @@ static const Tile TILES[4] = {
     {128, 64, 256, 0.34, 0.38, 3.0},       // 2 groups of 4 waves, each every other K tile, 3 buffers
     {128, 128, 256, 0.54, 0.54, 3.0},      // the same, 2 buffers
 };
-struct TilePlan { int tile, splits; double us; };
+struct TilePlan { int tile, splits; int64_t head; double us; };   // head: rows of M that go first, on 256 x 256 tiles
 
 // Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
 // the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
 // (written and read at 4 TB/s) cost.
 static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool across = false)
 {
-    TilePlan best = {0, 1, 1e30};
+    TilePlan best = {0, 1, 0, 1e30};
+    if (M <= 0 || N <= 0) return {0, 1, 0, 0.0};                   // no tokens
     for (int t = 0; t < 4; ++t)
         for (int s = 1; s <= 16; ++s)
         {
@@ -38,8 +39,17 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
             if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
             if (across) us *= 1.25;
             if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
-            if (us < best.us) best = {t, s, us};
+            if (us < best.us) best = {t, s, 0, us};
         }
+    // Large tiles for as many rows of M as fill whole rounds of the chip, the rest on the tiles that suit it: a last round of
+    // a few large tiles would cost as much as a full one (4,096 tokens through 2 x 11,008 rows, 5.4 rounds: 665 us, in two parts 630)
+    const int64_t tn = (N + 255) / 256, rounds = (M + 255) / 256 * tn / 256, head = rounds * 256 / tn * 256;
+    if (products == 1 && head > 0 && head < M)
+    {
+        const TilePlan tail = plan_product(M - head, N, nk, 1, false, across);
+        const double us = rounds * (nk * TILES[0].full + TILES[0].ends) * (across ? 1.25 : 1.0) + tail.us + 2.0;
+        if (tail.head == 0 && us < best.us) best = {tail.tile, 1, head, us};
+    }
     return best;
 }
 
@@ -62,10 +72,26 @@ static int run_gemm(const GemmArgs& a, int tile, hipStream_t s)
     return check_launch("gemm16");
 }
 
-// One product, split or not; EPI: what becomes of the sums
+// One product, split or in two parts or not; EPI: what becomes of the sums
 template <class T, bool AX, bool BX, int EPI>
 static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
 {
+    if (tp.head)
+    {
+        const int rows = (int)(EPI == EPI_GU ? tp.head / 2 : tp.head);
+        GemmArgs h = a;
+        h.M = rows;
+        const int rc = run_gemm<T, AX, BX, EPI>(h, 0, s);
+        if (rc) return rc;
+        for (int i = 0; i < 2; ++i)
+        {
+            if (a.a[i]) a.a[i] = static_cast<const char*>(a.a[i]) + (AX ? (int64_t)rows : (int64_t)rows * a.lda) * 2;
+            if (a.out[i]) a.out[i] = static_cast<char*>(a.out[i]) + (int64_t)rows * (EPI == EPI_ADD ? 4 : 2);
+        }
+        if (a.g) { a.g += rows; a.u += rows; }
+        a.M -= rows;
+        return run_gemm<T, AX, BX, EPI>(a, tp.tile, s);
+    }
     if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.tile, s);
     a.splits = tp.splits;
     a.ldp = (a.M + 7) / 8 * 8;

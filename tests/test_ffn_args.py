@@ -111,3 +111,22 @@ def test_q4_call_refusals():
     assert L.bmx_ffn4_forward(good, 256, 4, 256, 256, need - 1, None) == W
     assert L.bmx_ffn4_add(good, 256, 4, 258, 256, 256, need, None) == E
     assert L.bmx_ffn4_forward(None, 256, 4, 256, 256, need, None) == E
+
+
+def test_workspaces_of_any_token_count():
+    """The workspace queries plan on the host: no tokens and the most of them among the counts, each at least its largest part,
+    never less for more tokens of one path."""
+    import bmx
+    L = bmx.lib()
+    for H, I in ((8, 8), (64, 72), (4096, 2048), (4096, 11008), (1 << 20, 8), (8, 1 << 20)):
+        d = desc(H=H, I=I)
+        for T in (0, 1, 16, 17, 80, 81, 517, 4096, 100000, 1 << 24):
+            assert L.bmx_ffn_workspace(d, T) >= T * I * 2 and L.bmx_ffn_backward_workspace(d, T) >= 2 * T * I * 2
+    for N, K, G in ((1, 32, 32), (77, 4096, 128), (11008, 4096, 64), (1 << 20, 128, 128)):
+        q = q4(N=N, K=K, group=G)
+        for T in (0, 1, 16, 17, 80, 81, 517, 4096, 1 << 24):
+            assert L.bmx_q4_linear_workspace(q, T) < 1 << 45
+    gu, dn = q4(N=128, K=64), q4(N=64, K=128)
+    d = bmx._lib.Ffn4Desc(0, 0, 0.0, 0, ctypes.pointer(gu), ctypes.pointer(gu), ctypes.pointer(dn))
+    for T in (0, 1, 16, 17, 80, 81, 517, 1 << 24):
+        assert L.bmx_ffn4_workspace(d, T) >= T * 128 * 2

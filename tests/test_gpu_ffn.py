@@ -364,6 +364,6 @@ def test_refusals(cuda):
 
 # every tile shape and split count that the planner chooses: few and many rows against long and short K
 @pytest.mark.parametrize("T,H,I", [(100, 2048, 64), (100, 64, 2048), (517, 768, 512), (700, 1032, 1160), (300, 4104, 520),
-                                   (1100, 1544, 776), (90, 4096, 4096)])
+                                   (1100, 1544, 776), (90, 4096, 4096), (2050, 1024, 3848), (2050, 7696, 512)])
 def test_tile_plans(cuda, T, H, I):
     backward_check(cuda, T, H, I, torch.float16, 0, 0.0)
