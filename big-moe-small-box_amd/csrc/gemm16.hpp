@@ -327,16 +327,16 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     };
     seek(second ? 1 : prod, (second ? loaded - nk1 : loaded) * GK);
     auto tail = [&]() { return p.K - (second ? loaded - nk1 : loaded) * GK; };
-    auto load_a = [&](int buf) {
+    auto load_a = [&](lds_ptr to) {
         if (p.chain > 1 && !second && loaded >= nk1)
         {
             second = true;
             seek(1, (loaded - nk1) * GK);
         }
-        la.load((lds_ptr)lds + buf * (ABYTES + BBYTES), wave, tail(), loaded < kt_end);
+        la.load(to, wave, tail(), loaded < kt_end);
     };
-    auto load_b = [&](int buf) {
-        lb.load((lds_ptr)lds + buf * (ABYTES + BBYTES) + ABYTES, wave, tail(), loaded < kt_end);
+    auto load_b = [&](lds_ptr to) {
+        lb.load(to + ABYTES, wave, tail(), loaded < kt_end);
         la.next();
         lb.next();
         loaded += WK;
@@ -371,17 +371,13 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
 
-    // Fragments are read one step of 16 ahead of their products, across tiles too: the last step's products of a tile run
-    // while the next tile's first fragments are read, so the only wait of all waves for each other (the next tile has
-    // landed, and this one is read to the end) has products on both sides.
     constexpr int KS = GK / 16;
     v8 a[2][MF], b[2][NF];
-    auto read = [&](int set, int buf, int ks) {
-        lds_ptr at = (lds_ptr)lds + buf * (ABYTES + BBYTES), bt = at + ABYTES;
+    auto read = [&](int set, lds_ptr at, int ks) {
 #pragma unroll
         for (int i = 0; i < MF; ++i) a[set][i] = frag(at, wm * (BM / WM) + i * 32, ks, AX, BM);
 #pragma unroll
-        for (int j = 0; j < NF; ++j) b[set][j] = frag(bt, wn * (BN / WN) + j * 32, ks, BX, BN);
+        for (int j = 0; j < NF; ++j) b[set][j] = frag(at + ABYTES, wn * (BN / WN) + j * 32, ks, BX, BN);
     };
     auto products = [&](int set) {
 #pragma unroll
@@ -409,41 +405,50 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     // compiler from moving them: without it 289 -> 299 us.)
     constexpr bool SPREAD = MF * NF >= 8;
     static_assert(!SPREAD || NB == 2, "spread loads end early: only a wait for all of them fits");
-#pragma unroll
-    for (int i = 0; i < NB - 1; ++i)
-    {
-        load_a(i);
-        load_b(i);
-    }
-    landed();
-    if (!SPREAD) { load_a(NB - 1); load_b(NB - 1); }
-    read(0, 0, 0);
-    int buf = 0;
-    for (; kt < kt_end; kt += WK)                                  // group 0's tile; the others' may lie past the end: zeros
-    {
-        const int next = buf + 1 == NB ? 0 : buf + 1, last = buf == 0 ? NB - 1 : buf - 1;
+    // One tile: its products, but for the last step's, behind the last step's of the tile before. Fragments are read one step
+    // of 16 ahead of their products, across tiles too, so that the only wait of all waves for each other (this tile has
+    // landed, and the one before is read to the end) has products on both sides.
+    // The loads that go out meanwhile fill the buffer of the tile before: `to` is not `at`, and the compiler has to know it.
+    // Without __restrict__ it holds every transposing read back until all loads out have landed, those just sent too (2 x 2,048 x 4,096 x 8,192, both operands across K: 246 us, this way 208).
+    auto tile = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
+        if (!SPREAD) { load_a(to); load_b(to); }
+        read(0, at, 0);
+        products((KS - 1) & 1);
+        if (SPREAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KS - 1; ++ks)
         {
-            read((ks + 1) & 1, buf, ks + 1);
+            read((ks + 1) & 1, at, ks + 1);
             if (SPREAD && loaded < kt_end)
             {
-                if (ks == 0) load_a(last);
-                if (ks == 1) load_b(last);
+                if (ks == 0) load_a(to);
+                if (ks == 1) load_b(to);
             }
             products(ks & 1);
             if (SPREAD) __builtin_amdgcn_sched_barrier(0);
         }
-        if (kt + WK < kt_end)
-        {
-            landed();
-            if (!SPREAD) { load_a(buf); load_b(buf); }
-            read(0, next, 0);
-        }
-        products((KS - 1) & 1);
-        if (SPREAD) __builtin_amdgcn_sched_barrier(0);
-        buf = next;
+    };
+    constexpr int BUF = ABYTES + BBYTES;
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i)
+    {
+        load_a((lds_ptr)lds + i * BUF);
+        load_b((lds_ptr)lds + i * BUF);
     }
+    // the first tile follows products with zeros
+#pragma unroll
+    for (int i = 0; i < MF; ++i) a[(KS - 1) & 1][i] = v8{};
+#pragma unroll
+    for (int j = 0; j < NF; ++j) b[(KS - 1) & 1][j] = v8{};
+    int buf = 0, before = NB - 1;
+    for (; kt < kt_end; kt += WK)                                  // group 0's tile; the others' may lie past the end: zeros
+    {
+        landed();
+        tile((lds_ptr)lds + buf * BUF, (lds_ptr)lds + before * BUF);
+        before = buf;
+        buf = buf + 1 == NB ? 0 : buf + 1;
+    }
+    products((KS - 1) & 1);
 
     // ---- results ----
     // A lane's accumulators are column n = l % 32 and rows m = (e / 4) * 8 + (l / 32) * 4 + e % 4 of a fragment: four
