@@ -23,7 +23,7 @@ struct TilePlan { int tile, splits; int64_t head; double us; };   // head: rows 
 // Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
 // the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
 // (written and read at 4 TB/s) cost.
-static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool across = false)
+static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool grads = false)
 {
     TilePlan best = {0, 1, 0, 1e30};
     if (M <= 0 || N <= 0) return {0, 1, 0, 0.0};                   // no tokens
@@ -34,10 +34,10 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
             const Tile& c = TILES[t];
             const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * products * s, full = b / c.slots, rest = b % c.slots;
             const int each = (nk + s - 1) / s;
-            // with a side across K, and the gradients' epilogue behind half of those, about a fourth more
+            // the gradients' epilogue reads and writes 12 bytes a result: about a fourth more
             double us = full * (each * c.full + c.ends);
             if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
-            if (across) us *= 1.25;
+            if (grads) us *= 1.25;
             if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
             if (us < best.us) best = {t, s, 0, us};
         }
@@ -46,8 +46,8 @@ static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool ca
     const int64_t tn = (N + 255) / 256, rounds = (M + 255) / 256 * tn / 256, head = rounds * 256 / tn * 256;
     if (products == 1 && head > 0 && head < M)
     {
-        const TilePlan tail = plan_product(M - head, N, nk, 1, false, across);
-        const double us = rounds * (nk * TILES[0].full + TILES[0].ends) * (across ? 1.25 : 1.0) + tail.us + 2.0;
+        const TilePlan tail = plan_product(M - head, N, nk, 1, false, grads);
+        const double us = rounds * (nk * TILES[0].full + TILES[0].ends) * (grads ? 1.25 : 1.0) + tail.us + 2.0;
         if (tail.head == 0 && us < best.us) best = {tail.tile, 1, head, us};
     }
     return best;
@@ -250,7 +250,7 @@ static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
 {
     FfnBackPlan p;
     p.dh = plan_product(d->I, T, tiles_k(d->H), 1, true, true);
-    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true, true);
+    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true);
     p.dd = plan_product(d->I, d->H, tiles_k(T), 1, false);
     p.dw = plan_product(d->H, d->I, tiles_k(T), 2, false);
     size_t o = 0;
