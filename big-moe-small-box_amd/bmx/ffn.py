@@ -181,18 +181,18 @@ class _GatedFFNFunction(torch.autograd.Function):
     def backward(ctx, dy):
         gate, up, down, x, g, u, h = ctx.saved_tensors
         I, H = gate.shape
-        want = ctx.needs_input_grad
         T, dev = x.shape[0], x.device
+        s = stream_here(dev)
+        if s is None:                           # autograd's threads have a current device of their own
+            with torch.cuda.device(dev):
+                return _GatedFFNFunction.backward(ctx, dy)
         r = rows_of(dy, H, gate.dtype, dev, "GatedFFN: the gradient of y")
-        dx = torch.empty_like(x) if want[0] else None
-        dw = [torch.empty_like(w) if n else None for w, n in zip((gate, up, down), want[1:4])]
+        dx, dg, du, dd = [torch.empty_like(t) if n else None for t, n in zip((x, gate, up, down), ctx.needs_input_grad)]
         d, lib = L.FfnDesc(H, I, DTYPES[gate.dtype], ctx.act, ctx.act_limit, 0, gate.data_ptr(), up.data_ptr(),
                            down.data_ptr()), L.lib()
-        ptr = lambda t: t.data_ptr() if t is not None else None
-        with torch.cuda.device(dev):            # autograd's threads have a current device of their own
-            s = torch.cuda.current_stream().cuda_stream
-            need = lib.bmx_ffn_backward_workspace(d, T)
-            ws = torch.empty(need, dtype=torch.uint8, device=dev)
-            L.check(lib.bmx_ffn_backward(d, ptr(x), T, L.FfnSaved(ptr(g), ptr(u), ptr(h)), ptr(r), ptr(dx), ptr(dw[0]),
-                                         ptr(dw[1]), ptr(dw[2]), ptr(ws), need, s), "bmx_ffn_backward")
-        return dx.view(dy.shape) if dx is not None else None, dw[0], dw[1], dw[2], None
+        ptr = lambda t: None if t is None else t.data_ptr()
+        need = lib.bmx_ffn_backward_workspace(d, T)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        L.check(lib.bmx_ffn_backward(d, x.data_ptr(), T, L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr()), r.data_ptr(),
+                                     ptr(dx), ptr(dg), ptr(du), ptr(dd), ws.data_ptr(), need, s), "bmx_ffn_backward")
+        return None if dx is None else dx.view(dy.shape), dg, du, dd, None
