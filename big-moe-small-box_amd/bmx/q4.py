@@ -46,15 +46,18 @@ class Q4Matrix:
         (symmetric: zero point 8, the largest magnitude at code 0 or 15)."""
         if w.dim() != 2 or w.dtype not in DTYPES or not w.is_cuda or group not in (32, 64, 128) or w.shape[1] % group:
             raise ValueError("Q4Matrix.quantize: w must be an fp16 or bf16 device tensor [N, K], K a multiple of the group")
+        if not w.numel():
+            raise ValueError("Q4Matrix.quantize: w has no elements")
+        w = w.detach().contiguous()
         v = w.float().view(w.shape[0], -1, group)
         if symmetric:
             scale, zero = v.abs().amax(2) / 7.5, None
         else:
             lo, hi = v.amin(2).clamp(max=0.0), v.amax(2).clamp(min=0.0)
             scale = (hi - lo) / 15.0
-        # the stored scale decides the codes; an empty range keeps scale 1 (every code the zero point)
-        tiny = torch.finfo(w.dtype).smallest_normal
-        scale = torch.where(scale < tiny, torch.ones_like(scale), scale).to(w.dtype)
+        # the stored scale decides the codes; one that is stored as 0 becomes 1 (every code the zero point)
+        scale = scale.to(w.dtype)
+        scale = torch.where(scale == 0, torch.ones_like(scale), scale)
         s = scale.float()
         if symmetric:
             z = torch.full_like(s, 8.0)

@@ -243,3 +243,23 @@ def test_refusals(cuda):
         bmx.GatedFFN(q, other, down)
     with pytest.raises(ValueError):
         bmx.GatedFFN(q, q, rand(cuda, 256, 48, dt=torch.float16, seed=1))
+
+
+def test_quantize_of_views_leaves_and_small_groups(cuda):
+    """A transposed view and a leaf give the plain tensor's matrix; a group whose scale is below fp16's normal range keeps its
+    values within that scale's own steps; no elements are refused."""
+    import bmx
+    w = rand(cuda, 64, 96, dt=torch.float16, seed=2)
+    want = bmx.Q4Matrix.quantize(w, 32).dequant()
+    assert torch.equal(bmx.Q4Matrix.quantize(w.t().contiguous().t(), 32).dequant(), want)
+    assert torch.equal(bmx.Q4Matrix.quantize(w.clone().requires_grad_(), 32).dequant(), want)
+    small = (w.float() * 2.0 ** -13).half()
+    got = bmx.Q4Matrix.quantize(small, 32).dequant().double()
+    v = small.double().view(64, 3, 32)
+    span = (v.amax(2).clamp(min=0) - v.amin(2).clamp(max=0)) / 15
+    # half a step, the zero point's half step, and the scale's own rounding, half of 2^-24, over up to 15 codes and in each
+    # half step
+    bound = span + 16 * 2.0 ** -25
+    assert bool(((got - small.double()).view(64, 3, 32).abs().amax(2) <= bound).all())
+    with pytest.raises(ValueError):
+        bmx.Q4Matrix.quantize(w[:0], 32)
