@@ -42,8 +42,10 @@ class GatedFFN:
     (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
 
     forward(x) -> y, x [..., H] of the weights' type. Where autograd records (x or a weight requires grad), y carries the
-    gradients of x and of the three weights; the forward pass then keeps x, g and u
-    (fp32 [T, I]) and h (16 bits)."""
+    gradients of x and of the three weights; the forward pass then keeps x, g and u (fp32 [T, I]) and h (16 bits). Passes
+    with gradients may be captured into a graph through torch.autograd.grad; with backward(), which accumulates into the
+    leaves, only while no eager result of the same leaves is alive (torch's accumulation belongs to the stream that the
+    leaf was first used on)."""
 
     def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
         self.quantized = not any(torch.is_tensor(w) for w in (gate, up, down))

@@ -299,7 +299,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         const int q = nwg / 8, r = nwg % 8, x = id & 7;
         id = x * q + (x < r ? x : r) + (id >> 3);
     }
-    constexpr int GRP = AX ? 4 : 8;                                 // (A across K: 4; 2 x 2,048 x 4,096 x 8,192 251 -> 240 us)
+    constexpr int GRP = AX ? 4 : 8;                                 // (A across K: dh of 8,192 x 2,048 168 us with 8, 156)
     const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
     const int tm = g0 + (id % per) % gn, tn = (id % per) / gn;
     const int m0 = EPI == EPI_GU ? tm * (BM / 2) : tm * BM, n0 = tn * BN;
@@ -412,7 +412,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     // of 16 ahead of their products, across tiles too, so that the only wait of all waves for each other (this tile has
     // landed, and the one before is read to the end) has products on both sides.
     // The loads that go out meanwhile fill the buffer of the tile before: `to` is not `at`, and the compiler has to know it.
-    // Without __restrict__ it holds every transposing read back until all loads out have landed, those just sent too (2 x 2,048 x 4,096 x 8,192, both operands across K: 246 us, this way 208).
+    // Without __restrict__ it holds every transposing read back until all loads out have landed, those just sent too
+    // (2 x 2,048 x 4,096 x 8,192, both operands across K: 246 us, this way 208).
     auto tile = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
         if (!SPREAD) { load_a(to); load_b(to); }
         read(0, at, 0);

@@ -1,8 +1,8 @@
-// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. A workgroup has 16 or
-// 32 rows of W (half of gate and half of up in the gated product); each of its waves takes every SK_W-th 128 columns of them straight
-// from HBM to MFMA operands, so that a lane's loads are its fragment and no LDS stands between, several steps ahead of the
-// products; x comes through the caches in the same layout. The waves' sums are joined through LDS in the waves' order (the
-// result does not depend on timing).
+// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. A workgroup has 16,
+// 32 or 64 rows of W (half of gate and half of up in the gated product); each of its waves takes every SK_W-th 128 columns of
+// them straight from HBM to MFMA operands, so that a lane's loads are its fragment and no LDS stands between, several steps
+// ahead of the products; x comes through the caches in the same layout. The waves' sums are joined through LDS in the waves'
+// order (the result does not depend on timing).
 //
 // v_mfma_f32_16x16x32: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 8 .. + 7; of
 // the result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3. Fewer than 16 tokens load a token again: those
@@ -41,8 +41,8 @@ struct SkinnyArgs {
 Q4View q4_view(const bmx_q4* q);
 int check_q4(const bmx_q4* q, const char* who);
 int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s);
-// A product of few tokens on a's weights (a.group 0: 16-bit, up to 16 tokens) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU); part:
-// skinny_part_bytes bytes
+// A product of few tokens on a's weights (a.group 0: 16-bit, up to 16 tokens) with one matrix (EPI_STORE, EPI_ADD) or two
+// (EPI_GU); part: skinny_part_bytes bytes
 int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s);
 size_t skinny_part_bytes(int N, int K, int T, int products);
 // the most tokens that it takes

@@ -480,9 +480,10 @@ size_t bmx_q4_group_count(int N, int K, int group);
 int bmx_q4_pack(const bmx_q4* q, const void* codes, const void* scale, const void* zero, bmx_stream_t stream);
 /* out [N][K] of dtype: each weight rounded once. */
 int bmx_q4_dequant(const bmx_q4* q, int dtype, void* out, bmx_stream_t stream);
-/* y [T][N] = x [T][K] W^T, x and y of dtype, 16-byte aligned. fp32 sums, one rounding. A call of many tokens decodes the
- * weights to dtype in the workspace first (each then rounded once: half a step of the type); a call of few multiplies x
- * with the codes themselves, exactly. An infinite x may give NaN. */
+/* y [T][N] = x [T][K] W^T, x and y of dtype, 16-byte aligned, y apart from x. fp32 sums, one rounding; x is multiplied with
+ * the codes themselves, exactly, but where so many tokens come that decoding the weights to dtype first is faster (each
+ * then rounded once: half a step of the type). An infinite bf16 x may give NaN. The workspace is that of a call of T tokens;
+ * a call of fewer may need more. */
 size_t bmx_q4_linear_workspace(const bmx_q4* q, int T);
 int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
                   bmx_stream_t stream);
@@ -504,7 +505,8 @@ typedef struct bmx_ffn_desc {
 } bmx_ffn_desc;
 /* What a forward pass keeps for the backward pass: g, u fp32 [T, I] and h [T, I] of dtype; device, 16-byte aligned. */
 typedef struct bmx_ffn_saved { float *g, *u; void* h; } bmx_ffn_saved;
-/* Workspace bytes of the calls below for up to T tokens (0 and an error text when the descriptor is refused). */
+/* Workspace bytes of a call of T tokens (0 and an error text when the descriptor is refused). A call of fewer tokens may need
+ * more: long sums of few rows are split. Outputs overlap neither inputs nor the workspace, in all calls below. */
 size_t bmx_ffn_workspace(const bmx_ffn_desc* desc, int T);
 size_t bmx_ffn_backward_workspace(const bmx_ffn_desc* desc, int T);
 /* y [T, H]; saved NULL: nothing kept. */

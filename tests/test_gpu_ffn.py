@@ -367,3 +367,30 @@ def test_refusals(cuda):
                                    (1100, 1544, 776), (90, 4096, 4096), (2050, 1024, 3848), (2050, 7696, 512)])
 def test_tile_plans(cuda, T, H, I):
     backward_check(cuda, T, H, I, torch.float16, 0, 0.0)
+
+
+@pytest.mark.parametrize("T,H,I", [(4100, 4104, 1032), (4100, 1032, 5200)])
+def test_products_in_two_parts(cuda, T, H, I):
+    """Whole rounds of large tiles and the rest on smaller ones: y and dx by rows of H, then h, dg and du by rows of I; the
+    added form's sums are those that y rounds."""
+    import bmx
+    backward_check(cuda, T, H, I, torch.bfloat16, 0, 0.0)
+    x, w, _ = make(cuda, T, H, I, torch.bfloat16)
+    ffn = bmx.GatedFFN(*w)
+    out = ffn.add_to(torch.zeros((T, H), device=cuda), x)
+    assert torch.equal(out.to(x.dtype), ffn.forward(x))
+
+
+def test_one_tensor_as_gate_and_up(cuda):
+    """Its gradient is the sum of the two."""
+    import bmx
+    x, w, dy = make(cuda, 40, 72, 136, torch.float16)
+    for t in w:
+        t.requires_grad_()
+    one, = torch.autograd.grad(bmx.GatedFFN(w[0], w[0], w[2]).forward(x), [w[0]], dy)
+    other = w[0].detach().clone().requires_grad_()
+    a, b = torch.autograd.grad(bmx.GatedFFN(w[0], other, w[2]).forward(x), [w[0], other], dy)
+    assert torch.equal(one, a + b)
+    both = bmx.GatedFFN(w[0], w[0], w[2]).forward(x)
+    both.backward(dy)
+    assert torch.equal(w[0].grad, one)
