@@ -379,11 +379,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
 #pragma unroll
         for (int j = 0; j < NF; ++j) b[set][j] = frag(at + ABYTES, wn * (BN / WN) + j * 32, ks, BX, BN);
     };
-    auto products = [&](int set) {
+    auto products = [&](int set, int from, int to) {
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
-            for (int j = 0; j < NF; ++j) acc[i][j] = Elem<T>::mfma32(a[set][i], b[set][j], acc[i][j]);
+            for (int j = 0; j < NF; ++j)
+                if (i >= from && i < to) acc[i][j] = Elem<T>::mfma32(a[set][i], b[set][j], acc[i][j]);
     };
     // NB buffers. At the wait for tile kt + 1 the loads of the NB - 2 tiles behind it stay in flight. (Past the last tile
     // they go on with an empty range, so that the count holds; the results wait for all of them.)
@@ -398,11 +399,12 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
-    // 256-row tiles: the loads of the tile after the next go out in two parts, behind the fragment reads and ahead of the
-    // products of the first two steps: all at once, or right behind the wait, they hold the products up (286 -> 301 us on
-    // 4,096 x 4,096 x 11,008), and later they land too late (298 us). Smaller tiles have fewer products to wait behind:
-    // right behind the wait (128 rows, 390 -> 342 us on the same). (The branch around the last tile's loads also keeps the
-    // compiler from moving them: without it 289 -> 299 us.)
+    // 256-row tiles: the loads of the next tile go out in two parts, ahead of the products of the first two steps: all at once,
+    // or right behind the wait, they hold the products up (286 -> 301 us on 4,096 x 4,096 x 11,008), later they land too late
+    // (298 us), and dealt out one by one between the products they stall each of them (274 -> 317 us). The next step's
+    // fragments are read between the two halves of a step's products (282 -> 274 us; gate and up of 2,048 x 8,192 x 4,096 222 ->
+    // 217). Smaller tiles have fewer products to wait behind: loads right behind the wait (128 rows, 390 -> 342 us on the
+    // same). (The branch around the last tile's loads also keeps the compiler from moving them: without it 289 -> 299 us.)
     constexpr bool SPREAD = MF * NF >= 8;
     // the compiler keeps to this order of reads and products, but where a step is only two products (128 x 64; 4,096 -> 4,096
     // for 128 tokens on 128 x 128 50 -> 44 us, dx of 517 x 2,048 on 128 x 64 12.4 -> 11.8 without)
@@ -417,18 +419,23 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     auto tile = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
         if (!SPREAD) { load_a(to); load_b(to); }
         read(0, at, 0);
-        products((KS - 1) & 1);
+        products((KS - 1) & 1, 0, MF);
         if (IN_STEPS) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int ks = 0; ks < KS - 1; ++ks)
         {
-            read((ks + 1) & 1, at, ks + 1);
-            if (SPREAD && loaded < kt_end)
+            if (SPREAD)
             {
-                if (ks == 0) load_a(to);
-                if (ks == 1) load_b(to);
+                if (loaded < kt_end)
+                {
+                    if (ks == 0) load_a(to);
+                    if (ks == 1) load_b(to);
+                }
+                products(ks & 1, 0, MF / 2);
+                __builtin_amdgcn_sched_barrier(0);
             }
-            products(ks & 1);
+            read((ks + 1) & 1, at, ks + 1);
+            products(ks & 1, SPREAD ? MF / 2 : 0, MF);
             if (IN_STEPS) __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -452,7 +459,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         before = buf;
         buf = buf + 1 == NB ? 0 : buf + 1;
     }
-    products((KS - 1) & 1);
+    products((KS - 1) & 1, 0, MF);
 
     // ---- results ----
     // A lane's accumulators are column n = l % 32 and rows m = (e / 4) * 8 + (l / 32) * 4 + e % 4 of a fragment: four
