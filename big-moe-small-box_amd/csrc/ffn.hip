@@ -1,6 +1,8 @@
 // Gated feed-forward block: forward and the form that adds to a layer's output (16-bit and 4-bit weights), gradients (16-bit).
-// The products are skinny_k's for few tokens and gemm16_k's for many (4-bit weights then decoded to 16 bits first); this file
-// plans tiles and splits, lays out the workspace and checks arguments.
+// The products are skinny_k's for few tokens and gemm16_k's for many (4-bit weights: slice_k's and gemm_q4_k's between); this
+// file plans tiles and splits, lays out the workspace and checks arguments.
+#include <algorithm>
+
 #include "skinny.hpp"
 
 namespace bmx {
@@ -243,8 +245,22 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
 
 struct FfnBackPlan {
     TilePlan dh, dx, dd, dw;
+    bool two;               // dh and down's gradient in one launch, when both are wanted
     size_t dg, du, part, total;
 };
+
+// Whether down's gradient (tiles of `a` steps of K) and dh (of `b`) end sooner in one grid: the former's tiles, one a compute
+// unit, start first; dh's take the other units, then all
+static bool two_at_once(const bmx_ffn_desc* d, int T, const FfnBackPlan& p)
+{
+    auto over = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
+    const int64_t units = TILES[0].slots, it = over(d->I, 256), na = it * over(d->H, 256), nb = it * over(T, 256);
+    const int64_t a = tiles_k(T), b = tiles_k(d->H);
+    if (p.dh.tile != 0 || p.dh.head || p.dh.splits > 1 || na >= units) return false;
+    const int64_t beside = (units - na) * (a / b), left = nb > beside ? nb - beside : 0;
+    const int64_t steps = left ? (a > a / b * b ? a : a / b * b) + over(left, units) * b : std::max(a, over(nb, units - na) * b);
+    return steps * TILES[0].full + TILES[0].ends * 2 < p.dh.us + p.dd.us;
+}
 
 static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
 {
@@ -253,6 +269,7 @@ static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
     p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true);
     p.dd = plan_product(d->I, d->H, tiles_k(T), 1, false);
     p.dw = plan_product(d->H, d->I, tiles_k(T), 2, false);
+    p.two = two_at_once(d, T, p);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
     p.dg = take((size_t)T * d->I * 2);
@@ -275,13 +292,26 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
     z.part = reinterpret_cast<float*>(ws + p.part);
     z.act = act_par(d->act, d->act_limit);
     int rc = BMX_OK;
-    if (dx || dgate || dup)
+    GemmArgs h = z;                                                // dh = dy Wd, then dg, du
+    h.a[0] = d->down; h.b[0] = dy; h.out[0] = ws + p.dg; h.out[1] = ws + p.du;
+    h.g = sv->g; h.u = sv->u;
+    h.M = I; h.N = n; h.K = H; h.lda = I; h.ldb = H; h.ldo = I;
+    GemmArgs w = z;                                                // dWd = dy^T h
+    w.a[0] = sv->h; w.b[0] = dy; w.out[0] = ddown;
+    w.M = I; w.N = H; w.K = n; w.lda = I; w.ldb = H; w.ldo = I;
+    const bool need_dh = dx || dgate || dup;
+    if (need_dh && ddown && p.two)
     {
-        GemmArgs a = z;                                            // dh = dy Wd, then dg, du
-        a.a[0] = d->down; a.b[0] = dy; a.out[0] = ws + p.dg; a.out[1] = ws + p.du;
-        a.g = sv->g; a.u = sv->u;
-        a.M = I; a.N = n; a.K = H; a.lda = I; a.ldb = H; a.ldo = I;
-        rc = product<T, true, false, EPI_DGU>(a, p.dh, s);
+        h.tm = w.tm = (I + 255) / 256;
+        h.tn = (n + 255) / 256;
+        w.tn = (H + 255) / 256;
+        hipLaunchKernelGGL((gemm16_two_k<T>), dim3((unsigned)(w.tm * w.tn + h.tm * h.tn)), dim3(512), 0, s, w, h);
+        rc = check_launch("gemm16_two");
+    }
+    else
+    {
+        if (need_dh) rc = product<T, true, false, EPI_DGU>(h, p.dh, s);
+        if (!rc && ddown) rc = product<T, true, true, EPI_STORE>(w, p.dd, s);
     }
     if (!rc && dx)
     {
@@ -290,13 +320,6 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
         a.chain = 2;
         a.M = H; a.N = n; a.K = I; a.lda = H; a.ldb = I; a.ldo = H;
         rc = product<T, true, false, EPI_STORE>(a, p.dx, s);
-    }
-    if (!rc && ddown)
-    {
-        GemmArgs a = z;                                            // dWd = dy^T h
-        a.a[0] = sv->h; a.b[0] = dy; a.out[0] = ddown;
-        a.M = I; a.N = H; a.K = n; a.lda = I; a.ldb = H; a.ldo = I;
-        rc = product<T, true, true, EPI_STORE>(a, p.dd, s);
     }
     if (!rc && (dgate || dup))
     {

@@ -275,15 +275,20 @@ __device__ __forceinline__ void store_turned(const GemmArgs& p, const float* tur
 
 // BM x BN results by WK groups of WM x WN waves, NB buffers of a K tile each. Every group has K tiles of its own (the WK-th
 // ones, loaded by itself into its own part of LDS); their sums are added at the end, in the groups' order.
+template <int BM, int BN, int WM, int WN, int WK, int NB> constexpr int gemm16_lds()
+{
+    constexpr int TILES = WK * NB * (BM + BN) * GK * 2, TURN = WM * WN * WK * 32 * (BM / WM + 4) * 4;
+    return TILES > TURN ? TILES : TURN;
+}
+
+// tile `block` (of p.tm * p.tn) of product or split z; lds_all: gemm16_lds bytes
 template <class T, int BM, int BN, int WM, int WN, int WK, int NB, bool AX, bool BX, int EPI>
-__global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
+__device__ __forceinline__ void gemm16_tile(const GemmArgs& p, char* lds_all, int block, int z)
 {
     constexpr int NT = WM * WN * 64;                               // threads of a group
     constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
     constexpr int ABYTES = BM * GK * 2, BBYTES = BN * GK * 2;
     typedef typename Elem<T>::v8 v8;
-    constexpr int TILES = WK * NB * (ABYTES + BBYTES), TURN = WM * WN * WK * 32 * (BM / WM + 4) * 4;
-    __shared__ __attribute__((aligned(1024))) char lds_all[TILES > TURN ? TILES : TURN];
 
     const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int group = any / (WM * WN), wave = any % (WM * WN);
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     // one contiguous run, and a run walks N within groups of 8 or 4 tiles of M, so that its L2 holds the rows it shares
     // (without the first, products across K take a sixth longer)
     const int nwg = p.tm * p.tn;
-    int id = blockIdx.x;
+    int id = block;
     {
         const int q = nwg / 8, r = nwg % 8, x = id & 7;
         id = x * q + (x < r ? x : r) + (id >> 3);
@@ -303,8 +308,6 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
     const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
     const int tm = g0 + (id % per) % gn, tn = (id % per) / gn;
     const int m0 = EPI == EPI_GU ? tm * (BM / 2) : tm * BM, n0 = tn * BN;
-    const int z = blockIdx.z;
-
     const int nk1 = (p.K + GK - 1) / GK;                           // K tiles of one product
     int kt = 0, kt_end = nk1 * p.chain;
     const int prod = EPI == EPI_PART ? z / p.splits : z;           // which of the products side by side
@@ -490,6 +493,26 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     }
+}
+
+template <class T, int BM, int BN, int WM, int WN, int WK, int NB, bool AX, bool BX, int EPI>
+__global__ __launch_bounds__(WM * WN * WK * 64) void gemm16_k(const GemmArgs p)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[gemm16_lds<BM, BN, WM, WN, WK, NB>()];
+    gemm16_tile<T, BM, BN, WM, WN, WK, NB, AX, BX, EPI>(p, lds, blockIdx.x, blockIdx.z);
+}
+
+// Two independent products of a backward pass in one grid of 256 x 256 tiles: down's gradient (long sums over the tokens),
+// then dh with the activation's gradient behind it. Neither fills the chip in whole rounds by itself, and one's products run
+// beside the other's epilogue, which by itself waits for HBM (8,192 tokens' forward and backward of 4096 x 2048 1,104 us,
+// in a launch each 1,129).
+template <class T>
+__global__ __launch_bounds__(512) void gemm16_two_k(const GemmArgs dd, const GemmArgs dh)
+{
+    __shared__ __attribute__((aligned(1024))) char lds[gemm16_lds<256, 256, 2, 4, 1, 2>()];
+    const int first = dd.tm * dd.tn;
+    if ((int)blockIdx.x < first) gemm16_tile<T, 256, 256, 2, 4, 1, 2, true, true, EPI_STORE>(dd, lds, blockIdx.x, 0);
+    else gemm16_tile<T, 256, 256, 2, 4, 1, 2, true, false, EPI_DGU>(dh, lds, blockIdx.x - first, 0);
 }
 
 // The sums over the splits of a product (EPI_PART), in the splits' order, and what EPI does with them. Four values per thread

@@ -394,3 +394,20 @@ def test_one_tensor_as_gate_and_up(cuda):
     both = bmx.GatedFFN(w[0], w[0], w[2]).forward(x)
     both.backward(dy)
     assert torch.equal(w[0].grad, one)
+
+
+@pytest.mark.parametrize("dt", sorted(DT))
+@pytest.mark.parametrize("T,H,I", [(2050, 1032, 4104), (3100, 2056, 2568)])
+def test_down_gradient_beside_dh(cuda, T, H, I, dt):
+    """Sizes at which down's gradient and dh share a launch; each wanted alone is the same sums in the same order."""
+    import bmx
+    backward_check(cuda, T, H, I, DT[dt], 1, 0.0)
+    x, w, dy = make(cuda, T, H, I, DT[dt])
+    for t in [x] + w:
+        t.requires_grad_()
+    y = bmx.GatedFFN(*w).forward(x)
+    all_of = torch.autograd.grad(y, [x] + w, dy, retain_graph=True)
+    some = [torch.autograd.grad(bmx.GatedFFN(*w[:2], w[2].detach()).forward(x), [x] + w[:2], dy),
+            torch.autograd.grad(bmx.GatedFFN(w[0].detach(), w[1].detach(), w[2]).forward(x.detach()), [w[2]], dy)]
+    for got, want in zip(some[0] + some[1], all_of):
+        assert torch.equal(got, want)
