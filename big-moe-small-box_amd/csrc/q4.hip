@@ -107,19 +107,57 @@ int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s)
 
 // ---- products of few tokens ---------------------------------------------------------------------------------------------
 
-// Tokens up to which skinny_k reads W once past x from the caches; above, slices
-static int direct_tokens() { return 16; }
+// skinny_k: tiles of 16 rows per workgroup (1, 2 or, in 4 bits, 4), and how long it takes. x is read once per workgroup, so more
+// tiles save what x costs beside a tile of W (about 0.2 of a 4-bit tile a token, 0.05 of a 16-bit one); but the compute unit
+// with the most workgroups is the last to end, so time goes up in whole rounds of the 256 units. Tiles against measurements
+// (us with 1 / 2 / 4): 16 tokens, 4-bit 5120 -> 2 x 2304 13.1 / 9.0 / 11.1, 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 /
+// 11.5 / 9.7, 16-bit 2304 -> 5120 9.8 / 8.0 / 12.0, 4096 -> 2 x 2048 10.8 / 13.0; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5; 4 tokens
+// 4096 -> 11008 9.4 / 11.8. Time, planned and measured: 4-bit 4096 -> 4096 32 / 64 / 80 tokens 7.9 / 10.0 / 17.5, 7.6 / 9.6 / 16.5;
+// 4096 -> 14336 48 tokens 25.0, 25.9; 16-bit block of 4096 x 2048 17 / 33 tokens 22 / 37, 22 / 38.
+struct DirectPlan { int rt; double us; };
 
-// 16-bit weights: gemm16_k from 17 tokens on (33 tokens through a 5120 x 2304 block 25.9 us, by slices 29.0; 4096 x 11008 65
-// and 88). 4-bit weights: slices up to 80 (33 tokens 4096 -> 4096 10.4 us, by gemm_q4_k 12.4; 80 tokens 14.8 and 16.3)
-int skinny_tokens_max(int group) { return group ? SL_TT * 16 : direct_tokens(); }
+static DirectPlan direct_plan(int N, int K, int T, int products, bool q4)
+{
+    const int64_t tiles = (int64_t)(N + 15) / 16 * products, tt = (T + 15) / 16;
+    const double x = (T < 16 ? T : 16) * (q4 ? 0.2 : 0.05), us = (K > 1024 ? K / 1024.0 : 1.0) * (q4 ? 0.26 : 1.0);
+    DirectPlan best = {1, 1e30};
+    for (int rt = 1; rt <= (q4 ? 4 : 2); rt *= 2)
+    {
+        const double t = 2.5 + (((tiles + rt - 1) / rt * tt + 255) / 256) * (rt + x) * us;
+        if (t < best.us) best = {rt, t};
+    }
+    return best;
+}
+
+// slice_k and the joining kernel, fp16 and bf16 alike (us, planned and measured in both): 768 x 2048 32 tokens 6.5, 6.0 and 7.5;
+// 4096 x 4096 48 tokens 13, 12.5 and 14.8; 14336 x 4096 64 tokens 31, 26 and 28
+static double slices_us(int N, int K, int T, int products)
+{
+    return 1.08 * (4.3 + 0.05 * T + (double)N * K * products / 1e6 * (0.13 + 0.0039 * T));
+}
+
+static double q4_many_us(int N, int K, int T, int products, int group);
+
+// Up to 16 tokens skinny_k: W once. Beyond, it reads W once more for every 16 tokens (from L2), against slices, which join their
+// sums in a second launch, up to SL_TT tiles of tokens, and the tiled products: whichever is planned sooner. Both sides in us:
+// 4-bit 768 x 2048 80 tokens 4.5 / 9.0 by slices, 2560 -> 2304 48 tokens 6.4 / 8.8, 4096 -> 11008 80 tokens bf16 30 / 33, 4096 -> 14336
+// 64 tokens 32 / 28; 16-bit block of 2048 x 768 33 tokens 12.5 / 15.9 by gemm16_k, 5120 x 2304 44 / 29.
+ProductPath product_path(int N, int K, int T, int products, int group)
+{
+    if (T <= 16) return FEW_DIRECT;
+    const double us = T <= 1024 ? direct_plan(N, K, T, products, group != 0).us : 1e30;
+    if (!group) return us < product_us(N, T, K, products) ? FEW_DIRECT : MANY;
+    if (T <= SL_TT * 16) return us < slices_us(N, K, T, products) ? FEW_DIRECT : FEW_SLICES;
+    // (beyond 80 tokens the plan is a tenth short: 160 tokens 2304 -> 5120 19, 23.5; by gemm_q4_k 20.3)
+    return us * 1.15 < q4_many_us(N, K, T, products, group) ? FEW_DIRECT : MANY;
+}
 
 static int padded(int n) { return (n + 7) / 8 * 8; }
 static int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
 
-size_t skinny_part_bytes(int N, int K, int T, int products)
+size_t skinny_part_bytes(int N, int K, int T, int products, int group)
 {
-    return T <= direct_tokens() ? 0 : (size_t)products * slices_of(K) * T * padded(N) * 4;
+    return product_path(N, K, T, products, group) == FEW_SLICES ? (size_t)products * slices_of(K) * T * padded(N) * 4 : 0;
 }
 
 template <class T, int TT, int G> static int slice_launch(const SliceArgs& a, dim3 grid, hipStream_t s)
@@ -174,31 +212,15 @@ template <class T, int RT, int G, int EPI, bool XL> static int direct_rows(const
 {
     constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT;
     constexpr int D = RT == 4 && G == 32 ? 1 : 2;                  // (two steps of four tiles and 16 groups spill)
-    hipLaunchKernelGGL((skinny_k<T, RT, G, D, EPI, XL>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(SK_W * 64),
+    const int64_t rows = (a.N + ROWS - 1) / ROWS, blocks = a.T <= 16 ? rows : (rows + 7) / 8 * 8 * ((a.T + 15) / 16);
+    hipLaunchKernelGGL((skinny_k<T, RT, G, D, EPI, XL>), dim3((unsigned)blocks), dim3(SK_W * 64),
                        XL ? (size_t)a.T * (a.K * 2 + 16) : 0, s, a);
     return check_launch("skinny");
 }
 
-// Tiles of rows per workgroup (1, 2 or 4). x is read once per workgroup, so more tiles save what x costs beside a tile of W
-// (about 0.2 of a 4-bit tile a token, 0.05 of a 16-bit one); but the compute unit with the most workgroups is the last to end,
-// so their number goes up in whole rounds of the 256 units. Against measurements (us with 1 / 2 / 4 tiles): 16 tokens, 4-bit
-// 5120 -> 2 x 2304 13.1 / 9.0 / 11.1, 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 / 11.5 / 9.7, 16-bit 2304 -> 5120 9.8 /
-// 8.0 / 12.0, 4096 -> 2 x 2048 10.8 / 13.0; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5; 4 tokens 4096 -> 11008 9.4 / 11.8.
-static int row_tiles(int tiles, int T, bool q4)
-{
-    int best = 1;
-    double least = 1e30;
-    for (int rt = 1; rt <= (q4 ? 4 : 2); rt *= 2)
-    {
-        const double us = ((tiles + rt - 1) / rt + 255) / 256 * (rt + T * (q4 ? 0.2 : 0.05));
-        if (us < least) { least = us; best = rt; }
-    }
-    return best;
-}
-
 template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a, hipStream_t s)
 {
-    const int rt = row_tiles((a.N + 15) / 16 * (EPI == EPI_GU ? 2 : 1), a.T, G != 0);
+    const int rt = direct_plan(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, G != 0).rt;
     if constexpr (G != 0)
     {
         if (a.T == 1 && a.K <= 8192) return direct_rows<T, 1, G, EPI, true>(a, s);
@@ -209,7 +231,7 @@ template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a,
 
 template <class T, int EPI> static int few_tokens(const SkinnyArgs& a, float* part, hipStream_t s)
 {
-    if (a.T > direct_tokens()) return slice_product<T, EPI>(a, part, s);
+    if (a.T > 16 && product_path(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, a.group) == FEW_SLICES) return slice_product<T, EPI>(a, part, s);
     switch (a.group)
     {
         case 0: return direct_launch<T, 0, EPI>(a, s);
@@ -252,6 +274,8 @@ static Q4Plan q4_plan(int N, int K, int T, int products, int group)
     if (first < best.us) best = {false, 1, first};
     return best;
 }
+
+static double q4_many_us(int N, int K, int T, int products, int group) { return q4_plan(N, K, T, products, group).us; }
 
 static size_t group_sums_bytes(int K, int T, int group) { return align_up((size_t)(ceil_to(K, SK_K) / group) * ceil_to(T, QG_T) * 4, 256); }
 
@@ -335,7 +359,8 @@ int launch_q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, int e
 
 static size_t q4_linear_ws(const bmx_q4* q, int T)
 {
-    return T <= skinny_tokens_max(q->group) ? skinny_part_bytes(q->N, q->K, T, 1) : q4_many_bytes(q->N, q->K, T, 1, q->group);
+    return product_path(q->N, q->K, T, 1, q->group) == MANY ? q4_many_bytes(q->N, q->K, T, 1, q->group)
+                                                            : skinny_part_bytes(q->N, q->K, T, 1, q->group);
 }
 
 }  // namespace bmx
@@ -407,7 +432,7 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
     a.x = static_cast<const uint16_t*>(x);
     a.T = T; a.N = q->N; a.K = q->K; a.group = q->group;
     a.out = y; a.ldo = q->N;
-    if (T > skinny_tokens_max(q->group)) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
+    if (product_path(q->N, q->K, T, 1, q->group) == MANY) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
     return launch_skinny(a, dtype, EPI_STORE, static_cast<float*>(workspace), s);
 }
 

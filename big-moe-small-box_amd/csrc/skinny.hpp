@@ -1,8 +1,8 @@
-// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. A workgroup has 16,
-// 32 or 64 rows of W (half of gate and half of up in the gated product); each of its waves takes every SK_W-th 128 columns of
-// them straight from HBM to MFMA operands, so that a lane's loads are its fragment and no LDS stands between, several steps
-// ahead of the products; x comes through the caches in the same layout. The waves' sums are joined through LDS in the waves'
-// order (the result does not depend on timing).
+// Products of few tokens with a weight matrix: y[t][n] = sum_k x[t][k] W[n][k], bound by the bytes of W. A workgroup has 16
+// tokens and 16, 32 or 64 rows of W (half of gate and half of up in the gated product); each of its waves takes every
+// SK_W-th 128 columns of them straight from HBM to MFMA operands, so that a lane's loads are its fragment and no LDS stands
+// between, several steps ahead of the products; x comes through the caches in the same layout. The waves' sums are joined
+// through LDS in the waves' order (the result does not depend on timing).
 //
 // v_mfma_f32_16x16x32: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 8 .. + 7; of
 // the result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3. Fewer than 16 tokens load a token again: those
@@ -41,12 +41,13 @@ struct SkinnyArgs {
 Q4View q4_view(const bmx_q4* q);
 int check_q4(const bmx_q4* q, const char* who);
 int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s);
-// A product of few tokens on a's weights (a.group 0: 16-bit, up to 16 tokens) with one matrix (EPI_STORE, EPI_ADD) or two
-// (EPI_GU); part: skinny_part_bytes bytes
+// Which kernel a product of T tokens with an N x K matrix (or two, side by side) runs on: skinny_k, slice_k or one for many tokens
+enum ProductPath { FEW_DIRECT, FEW_SLICES, MANY };
+ProductPath product_path(int N, int K, int T, int products, int group);
+// A product on skinny_k or slice_k, on a's weights (a.group 0: 16-bit) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU);
+// part: skinny_part_bytes bytes
 int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s);
-size_t skinny_part_bytes(int N, int K, int T, int products);
-// the most tokens that it takes
-int skinny_tokens_max(int group);
+size_t skinny_part_bytes(int N, int K, int T, int products, int group);
 // A product of more tokens on 4-bit weights q[0] (and q[1]: EPI_GU); ws: q4_many_bytes bytes
 int launch_q4_many(const SkinnyArgs& a, const bmx_q4* const* q, int dtype, int epi, char* ws, hipStream_t s);
 size_t q4_many_bytes(int N, int K, int T, int products, int group);
@@ -118,7 +119,17 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
     constexpr int NG = Q4 ? SK_K / (G ? G : 1) : 1, JG = 4 / NG;             // groups of a step, words of a group
     constexpr int ROWS = GU ? 8 : 16;                              // result columns of a tile
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    const int n0 = blockIdx.x * (ROWS * RT);
+    // 16 tokens a workgroup; those of one block of rows follow one another on one XCD (workgroups are dealt to the 8 in turn), so
+    // that all but the first find W in its L2
+    int row = blockIdx.x, t0 = 0;
+    if (p.T > 16)
+    {
+        const int tt = (p.T + 15) >> 4, rest = row >> 3;
+        t0 = rest % tt * 16;
+        row = rest / tt * 8 + (row & 7);
+    }
+    const int n0 = row * (ROWS * RT);
+    if (n0 >= p.N) return;
     const int KT = (p.K + SK_K - 1) / SK_K;
     // this lane's rows of W, and whose (rows past the last load it again)
     const int mat = GU ? r >> 3 : 0;
@@ -134,7 +145,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
         sg[i] = (int64_t)(n >> 4) * (KT * NG) * 16 + (n & 15);
         w16[i] = static_cast<const uint16_t*>(p.w[mat]) + (int64_t)n * p.K + q * 8;
     }
-    const uint16_t* xr = p.x + (int64_t)min(r, p.T - 1) * p.K + q * 8;
+    const uint16_t* xr = p.x + (int64_t)min(t0 + r, p.T - 1) * p.K + q * 8;
     extern __shared__ __attribute__((aligned(16))) char xl[];
     const int xrow = p.K * 2 + 16;
 
@@ -265,7 +276,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
     __syncthreads();
     for (int i = threadIdx.x; i < V; i += SK_W * 64)
     {
-        const int c = i & 15, t = ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + (i >> 8) * ROWS + c;
+        const int c = i & 15, t = t0 + ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + (i >> 8) * ROWS + c;
         if (t >= p.T || c >= ROWS || n >= p.N) continue;
         auto sum = [&](int at) {
             float s = part[0][at];
@@ -291,7 +302,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 }
 
 // ---- 4-bit weights, more tokens: slices of K ---------------------------------------------------------------------------------------------
-// From some tokens on what skinny_k reads of x (16 tokens for every 16 rows of W) outgrows W. Here a workgroup keeps 512
+// skinny_k decodes W again for every 16 tokens. Here a workgroup keeps 512
 // columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
 // go to part (as EPI_PART), gemm_finish_k joins them.
 constexpr int SL_K = 512;           // columns of a slice
