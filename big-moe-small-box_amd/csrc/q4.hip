@@ -1,4 +1,6 @@
 // 4-bit matrices with group scales: packing into fragment order, decoding to 16 bits, and products of few tokens (skinny_k).
+#include <algorithm>
+
 #include "q4_gemm.hpp"
 
 namespace bmx {
@@ -147,9 +149,11 @@ ProductPath product_path(int N, int K, int T, int products, int group)
     if (T <= 16) return FEW_DIRECT;
     const double us = T <= 1024 ? direct_plan(N, K, T, products, group != 0).us : 1e30;
     if (!group) return us < product_us(N, T, K, products) ? FEW_DIRECT : MANY;
-    if (T <= SL_TT * 16) return us < slices_us(N, K, T, products) ? FEW_DIRECT : FEW_SLICES;
+    // the others' two or three launches keep the host of a call outside a graph about 11 us, the one 7
+    const double least = 10.0;
+    if (T <= SL_TT * 16) return us < std::max(slices_us(N, K, T, products), least) ? FEW_DIRECT : FEW_SLICES;
     // (beyond 80 tokens the plan is a tenth short: 160 tokens 2304 -> 5120 19, 23.5; by gemm_q4_k 20.3)
-    return us * 1.15 < q4_many_us(N, K, T, products, group) ? FEW_DIRECT : MANY;
+    return us * 1.15 < std::max(q4_many_us(N, K, T, products, group), least) ? FEW_DIRECT : MANY;
 }
 
 static int padded(int n) { return (n + 7) / 8 * 8; }
