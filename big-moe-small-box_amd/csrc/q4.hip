@@ -174,7 +174,6 @@ template <class T, int G> static int slice_tokens(const SliceArgs& a, dim3 grid,
 {
     switch ((a.a.T + 15) / 16)
     {
-        case 1: return slice_launch<T, 1, G>(a, grid, s);
         case 2: return slice_launch<T, 2, G>(a, grid, s);
         case 3: return slice_launch<T, 3, G>(a, grid, s);
         case 4: return slice_launch<T, 4, G>(a, grid, s);

@@ -411,3 +411,14 @@ def test_down_gradient_beside_dh(cuda, T, H, I, dt):
             torch.autograd.grad(bmx.GatedFFN(w[0].detach(), w[1].detach(), w[2]).forward(x.detach()), [w[2]], dy)]
     for got, want in zip(some[0] + some[1], all_of):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("T,H,I", [(100, 520, 4096), (90, 4096, 2048), (300, 1032, 2056), (700, 520, 264), (20, 5120, 2304), (40, 776, 264)])
+def test_added_form_is_y_before_its_rounding(cuda, T, H, I):
+    """Products with K split and not, and the kernel of few tokens: added to zeros and rounded, the sums are y."""
+    import bmx
+    x, w, _ = make(cuda, T, H, I, torch.bfloat16)
+    ffn = bmx.GatedFFN(*w)
+    y = ffn.forward(x)
+    assert torch.equal(ffn.add_to(torch.zeros((T, H), device=cuda), x).to(x.dtype), y)
+    check_forward(x, w, 0, 0.0, ffn, y)

@@ -263,3 +263,25 @@ def test_quantize_of_views_leaves_and_small_groups(cuda):
     assert bool(((got - small.double()).view(64, 3, 32).abs().amax(2) <= bound).all())
     with pytest.raises(ValueError):
         bmx.Q4Matrix.quantize(w[:0], 32)
+
+
+# larger matrices, whose products leave the kernel of few tokens: slices of 2 to 5 tiles of tokens, then tiles with K split and not
+@pytest.mark.parametrize("T,K,N,G", [(20, 3264, 8232, 64), (30, 3200, 8232, 32), (33, 3232, 6152, 32), (40, 3200, 6150, 128),
+                                     (50, 3328, 4120, 128), (64, 3200, 4120, 64), (77, 4128, 4100, 32), (77, 4096, 4120, 64),
+                                     (80, 4096, 4120, 128), (81, 4128, 3080, 32), (128, 4096, 2056, 128), (129, 4160, 2056, 64),
+                                     (300, 4096, 1000, 64), (200, 256, 4120, 32), (100, 320, 8232, 64), (130, 256, 6152, 128)])
+def test_linear_of_larger_matrices(cuda, T, K, N, G):
+    import bmx
+    for dt in DT.values():
+        given, q64 = codes(cuda, N, K, G, "any" if T % 2 else "none", dt, seed=T)
+        x = rand(cuda, T, K, dt=dt, seed=T)
+        y64, e = R.q4_product(x.double(), q64, dt)
+        R.check("y", bmx.ops.q4_linear(x, bmx.Q4Matrix(*given, group=G)), y64, R.rounded(y64, e, dt))
+
+
+@pytest.mark.parametrize("dt", sorted(DT))
+@pytest.mark.parametrize("T,H,I,G", [(40, 4096, 4096, 64), (50, 4096, 2560, 32), (70, 4096, 4096, 128), (77, 4096, 4096, 32),
+                                     (77, 4096, 2048, 64), (100, 512, 4096, 64), (100, 2560, 4096, 32), (150, 2048, 4096, 128),
+                                     (150, 4096, 4096, 32), (300, 1024, 4096, 64), (300, 4096, 1024, 128), (300, 4096, 512, 128)])
+def test_gated_block_of_larger_matrices(cuda, T, H, I, G, dt):
+    test_gated_block(cuda, T, H, I, G, dt)
