@@ -11,50 +11,6 @@ namespace bmx {
 
 static bool dtype_ok(int d) { return d == BMX_DT_FP16 || d == BMX_DT_BF16; }
 
-// The tiles a product can run on: results M x N, workgroups that run at once, and what was measured of each: us a K tile of
-// 64 with a workgroup on every other compute unit or fewer (alone) and with the chip full, us to begin and end.
-struct Tile { int M, N, slots; double alone, full, ends; };
-static const Tile TILES[4] = {
-    {256, 256, 256, 1.60, 1.60, 6.0},      // 8 waves, 2 buffers
-    {128, 128, 512, 0.64, 1.00, 3.0},      // 4 waves, 2 buffers, two on a compute unit
-    {128, 64, 256, 0.34, 0.38, 3.0},       // 2 groups of 4 waves, each every other K tile, 3 buffers
-    {128, 128, 256, 0.54, 0.54, 3.0},      // the same, 2 buffers
-};
-struct TilePlan { int tile, splits; int64_t head; double us; };   // head: rows of M that go first, on 256 x 256 tiles
-
-// Tiles of a product with M x N results, `products` side by side, nk tiles of K: the cheapest by those times. K is split,
-// the partial sums joined by a second kernel, where that saves more than the second kernel (5 us) and the sums' bytes
-// (written and read at 4 TB/s) cost.
-static TilePlan plan_product(int64_t M, int64_t N, int nk, int products, bool can_split, bool grads = false)
-{
-    TilePlan best = {0, 1, 0, 1e30};
-    if (M <= 0 || N <= 0) return {0, 1, 0, 0.0};                   // no tokens
-    for (int t = 0; t < 4; ++t)
-        for (int s = 1; s <= 16; ++s)
-        {
-            if (s > 1 && (!can_split || nk / s < 4)) break;
-            const Tile& c = TILES[t];
-            const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * products * s, full = b / c.slots, rest = b % c.slots;
-            const int each = (nk + s - 1) / s;
-            // the gradients' epilogue reads and writes 12 bytes a result: about a fourth more
-            double us = full * (each * c.full + c.ends);
-            if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
-            if (grads) us *= 1.25;
-            if (s > 1) us += 5.0 + (double)M * N * products * s * 8.0 / 4e6;
-            if (us < best.us) best = {t, s, 0, us};
-        }
-    // Large tiles for as many rows of M as fill whole rounds of the chip, the rest on the tiles that suit it: a last round of
-    // a few large tiles would cost as much as a full one (4,096 tokens through 2 x 11,008 rows, 5.4 rounds: 665 us, in two parts 630)
-    const int64_t tn = (N + 255) / 256, rounds = (M + 255) / 256 * tn / 256, head = rounds * 256 / tn * 256;
-    if (products == 1 && head > 0 && head < M)
-    {
-        const TilePlan tail = plan_product(M - head, N, nk, 1, false, grads);
-        const double us = rounds * (nk * TILES[0].full + TILES[0].ends) * (grads ? 1.25 : 1.0) + tail.us + 2.0;
-        if (tail.head == 0 && us < best.us) best = {tail.tile, 1, head, us};
-    }
-    return best;
-}
-
 template <class T, bool AX, bool BX, int EPI>
 static int run_gemm(const GemmArgs& a, int tile, hipStream_t s)
 {
@@ -78,23 +34,22 @@ static int run_gemm(const GemmArgs& a, int tile, hipStream_t s)
 template <class T, bool AX, bool BX, int EPI>
 static int product(GemmArgs a, const TilePlan& tp, hipStream_t s)
 {
-    if (tp.head)
+    if (tp.splits == 1)
     {
-        const int rows = (int)(EPI == EPI_GU ? tp.head / 2 : tp.head);
-        GemmArgs h = a;
-        h.M = rows;
-        const int rc = run_gemm<T, AX, BX, EPI>(h, 0, s);
-        if (rc) return rc;
-        for (int i = 0; i < 2; ++i)
+        ProductPart part[2];
+        const int n = product_parts(tp, a.M, EPI == EPI_GU ? 2 : 1, part);
+        for (int i = 0; i < n; ++i)
         {
-            if (a.a[i]) a.a[i] = static_cast<const char*>(a.a[i]) + (AX ? (int64_t)rows : (int64_t)rows * a.lda) * 2;
-            if (a.out[i]) a.out[i] = static_cast<char*>(a.out[i]) + (int64_t)rows * (EPI == EPI_ADD ? 4 : 2);
+            GemmArgs g = a;
+            g.from = part[i].from;
+            g.M = part[i].rows;
+            for (void*& o : g.out)
+                if (o) o = static_cast<char*>(o) + (int64_t)g.from * (EPI == EPI_ADD ? 4 : 2);
+            if (g.g) { g.g += g.from; g.u += g.from; }
+            if (const int rc = run_gemm<T, AX, BX, EPI>(g, part[i].tile, s)) return rc;
         }
-        if (a.g) { a.g += rows; a.u += rows; }
-        a.M -= rows;
-        return run_gemm<T, AX, BX, EPI>(a, tp.tile, s);
+        return BMX_OK;
     }
-    if (tp.splits == 1) return run_gemm<T, AX, BX, EPI>(a, tp.tile, s);
     a.splits = tp.splits;
     a.ldp = (a.M + 7) / 8 * 8;
     GemmArgs g = a;
@@ -128,19 +83,6 @@ __global__ __launch_bounds__(256) void row_gate_k(const uint16_t* __restrict__ x
 #pragma unroll
     for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o);
     if (lane == 0) out[t] = sigmoid_fixed(sum);
-}
-
-static int tiles_k(int K) { return (K + GK - 1) / GK; }
-
-// EPI_GU is one product of twice the rows, but two where K is split
-static TilePlan plan_for(int N, int T, int K, int products) { return plan_product((int64_t)N * products, T, tiles_k(K), 1, true); }
-
-double product_us(int N, int T, int K, int products) { return plan_for(N, T, K, products).us; }
-
-size_t product_part_bytes(int N, int T, int K, int products)
-{
-    const TilePlan p = plan_for(N, T, K, products);
-    return p.splits > 1 ? (size_t)p.splits * products * T * ((N + 7) / 8 * 8) * 4 : 0;
 }
 
 int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s)
@@ -244,38 +186,20 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
 }
 
 struct FfnBackPlan {
-    TilePlan dh, dx, dd, dw;
-    bool two;               // dh and down's gradient in one launch, when both are wanted
+    BackTiles t;
     size_t dg, du, part, total;
 };
-
-// Whether down's gradient (tiles of `a` steps of K) and dh (of `b`) end sooner in one grid: the former's tiles, one a compute
-// unit, start first; dh's take the other units, then all
-static bool two_at_once(const bmx_ffn_desc* d, int T, const FfnBackPlan& p)
-{
-    auto over = [](int64_t n, int64_t by) { return (n + by - 1) / by; };
-    const int64_t units = TILES[0].slots, it = over(d->I, 256), na = it * over(d->H, 256), nb = it * over(T, 256);
-    const int64_t a = tiles_k(T), b = tiles_k(d->H);
-    if (p.dh.tile != 0 || p.dh.head || p.dh.splits > 1 || na >= units) return false;
-    const int64_t beside = (units - na) * (a / b), left = nb > beside ? nb - beside : 0;
-    const int64_t steps = left ? (a > a / b * b ? a : a / b * b) + over(left, units) * b : std::max(a, over(nb, units - na) * b);
-    return steps * TILES[0].full + TILES[0].ends * 2 < p.dh.us + p.dd.us;
-}
 
 static FfnBackPlan ffn_back_plan(const bmx_ffn_desc* d, int T)
 {
     FfnBackPlan p;
-    p.dh = plan_product(d->I, T, tiles_k(d->H), 1, true, true);
-    p.dx = plan_product(d->H, T, 2 * tiles_k(d->I), 1, true);
-    p.dd = plan_product(d->I, d->H, tiles_k(T), 1, false);
-    p.dw = plan_product(d->H, d->I, tiles_k(T), 2, false);
-    p.two = two_at_once(d, T, p);
+    p.t = back_tiles(d->H, d->I, T);
     size_t o = 0;
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
     p.dg = take((size_t)T * d->I * 2);
     p.du = take((size_t)T * d->I * 2);
-    const size_t ph = p.dh.splits > 1 ? (size_t)p.dh.splits * T * d->I * 4 : 0;
-    const size_t px = p.dx.splits > 1 ? (size_t)p.dx.splits * T * d->H * 4 : 0;
+    const size_t ph = p.t.dh.splits > 1 ? (size_t)p.t.dh.splits * T * d->I * 4 : 0;
+    const size_t px = p.t.dx.splits > 1 ? (size_t)p.t.dx.splits * T * d->H * 4 : 0;
     p.part = take(ph > px ? ph : px);
     p.total = o + 256;
     return p;
@@ -300,7 +224,7 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
     w.a[0] = sv->h; w.b[0] = dy; w.out[0] = ddown;
     w.M = I; w.N = H; w.K = n; w.lda = I; w.ldb = H; w.ldo = I;
     const bool need_dh = dx || dgate || dup;
-    if (need_dh && ddown && p.two)
+    if (need_dh && ddown && p.t.two)
     {
         h.tm = w.tm = (I + 255) / 256;
         h.tn = (n + 255) / 256;
@@ -310,8 +234,8 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
     }
     else
     {
-        if (need_dh) rc = product<T, true, false, EPI_DGU>(h, p.dh, s);
-        if (!rc && ddown) rc = product<T, true, true, EPI_STORE>(w, p.dd, s);
+        if (need_dh) rc = product<T, true, false, EPI_DGU>(h, p.t.dh, s);
+        if (!rc && ddown) rc = product<T, true, true, EPI_STORE>(w, p.t.dd, s);
     }
     if (!rc && dx)
     {
@@ -319,7 +243,7 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
         a.a[0] = d->gate; a.a[1] = d->up; a.b[0] = ws + p.dg; a.b[1] = ws + p.du; a.out[0] = dx;
         a.chain = 2;
         a.M = H; a.N = n; a.K = I; a.lda = H; a.ldb = I; a.ldo = H;
-        rc = product<T, true, false, EPI_STORE>(a, p.dx, s);
+        rc = product<T, true, false, EPI_STORE>(a, p.t.dx, s);
     }
     if (!rc && (dgate || dup))
     {
@@ -329,7 +253,7 @@ static int ffn_backward(const bmx_ffn_desc* d, const void* x, int n, const bmx_f
         a.b[0] = dgate ? ws + p.dg : ws + p.du; a.out[0] = dgate ? dgate : dup;
         a.b[1] = ws + p.du; a.out[1] = dup;
         a.M = H; a.N = I; a.K = n; a.lda = H; a.ldb = I; a.ldo = H;
-        rc = product<T, true, true, EPI_STORE>(a, p.dw, s);
+        rc = product<T, true, true, EPI_STORE>(a, p.t.dw, s);
     }
     return rc;
 }

@@ -10,6 +10,7 @@
 #pragma once
 #include "ffn_act.hpp"
 #include "bmx_internal.hpp"
+#include "product_plan.hpp"
 
 typedef __bf16 bf16;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -50,6 +51,7 @@ struct GemmArgs {
     const void* b[2];
     void* out[2];
     int M, N, K;            // M: rows of A (EPI_GU: of each of its two matrices), N: rows of B
+    int from;               // A's first row: the rows before are another launch's; out, g and u start at it
     int lda, ldb, ldo;      // elements
     int ldp;                // EPI_PART: row of the partial sums, a multiple of 8
     int chain;              // 2: the two products are summed
@@ -148,8 +150,6 @@ template <class T, int W> __device__ __forceinline__ void put_dgu(const GemmArgs
 }
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------
-constexpr int GK = 64;      // K of a tile
-
 // LDS position of 16-byte chunk c of row r. Along K: a row is 64 values = 8 chunks; 16 rows at one chunk (a fragment read)
 // fall on 16 different 16-byte columns of the 64 banks. Across K: a row is the tile's rows; the 4 rows x 64 bytes that 32 lanes
 // read for a transposition fall on four different quarters of the banks (with 32 bytes as the unit the reads took twice the
@@ -184,11 +184,11 @@ struct TileLoader {
     // the tile at row r0 (of the result's side) and column k0, of matrices with `rows` rows and K columns
     __device__ __forceinline__ void seek(const void* m0, const void* m1, int r0, int k0, int rows, int K, int wave)
     {
-        const int64_t ld = rows_ld / 2, first = ACROSS ? (int64_t)k0 * ld + r0 : (int64_t)r0 * ld + k0;
-        base0 = static_cast<const char*>(m0) + first * 2;
-        base1 = GU ? static_cast<const char*>(m1) + first * 2 : base0;
+        const OperandSpan at = operand_span(ACROSS, rows_ld / 2, rows, K, r0, k0);
+        base0 = static_cast<const char*>(m0) + at.first;
+        base1 = GU ? static_cast<const char*>(m1) + at.first : base0;
         if (GU && RPI == 64) base0 = base1 = wave & 4 ? base1 : base0;     // one matrix for all of a wave's loads
-        left = ((ACROSS ? K : rows) * ld - first) * 2;
+        left = at.left;
     }
     // Offsets past the range load zeros: the bytes left, at most 1 GiB (a tile spans half of that at the widest rows the
     // entries take); none without `on`. tail: columns of K left; what lies past them in the last tile along K is moved out
@@ -325,7 +325,7 @@ __device__ __forceinline__ void gemm16_tile(const GemmArgs& p, char* lds_all, in
     int loaded = kt + group;                                       // this group's next tile to load
     bool second = loaded >= nk1;                                   // of a chain
     auto seek = [&](int pi, int k0) {
-        la.seek(p.a[pi], p.a[1], m0, k0, p.M, p.K, wave);
+        la.seek(p.a[pi], p.a[1], p.from + m0, k0, p.from + p.M, p.K, wave);
         lb.seek(p.b[pi], nullptr, n0, k0, p.N, p.K, wave);
     };
     seek(second ? 1 : prod, (second ? loaded - nk1 : loaded) * GK);

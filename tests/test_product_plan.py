@@ -1,0 +1,55 @@
+"""The planner of the tiled products on the CPU: its own header, built with g++ (tests/native/product_plan.cpp)."""
+import ctypes
+import os
+import shutil
+import subprocess
+
+import pytest
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+CSRC = os.path.join(os.path.dirname(HERE), "big-moe-small-box_amd", "csrc")
+
+
+@pytest.fixture(scope="module")
+def plan(tmp_path_factory):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not found")
+    out = str(tmp_path_factory.mktemp("plan") / "product_plan.so")
+    b = subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-shared", "-fPIC", "-I", CSRC, "-o", out,
+                        os.path.join(HERE, "native", "product_plan.cpp")], capture_output=True, text=True, timeout=300)
+    assert b.returncode == 0, b.stderr[-4000:]
+    lib = ctypes.CDLL(out)
+    lib.plan_past_the_end.restype = ctypes.c_int64
+    return lib
+
+
+# (H, I, T, products in two parts with A stored across K and a ragged last tile)
+TWO_PARTS = [(2880, 2880, 8192, (2, 3)), (2048, 10944, 8192, (2, 4)), (2048, 10944, 16384, (4,)), (4104, 1032, 4100, (3,)), (1032, 5200, 4100, (2,))]
+
+
+def past(plan, H, I, T, which, moved=0):
+    parts = ctypes.c_int()
+    return plan.plan_past_the_end(H, I, T, which, moved, ctypes.byref(parts)), parts.value
+
+
+@pytest.mark.parametrize("H,I,T,which", TWO_PARTS)
+def test_second_parts_end_where_the_matrix_ends(plan, H, I, T, which):
+    """A launch's loads are cut off at the end of the matrix that they read, whichever rows of it the launch takes. (Counted from
+    a pointer moved to the second part's rows, a matrix stored across K would end as many values too late.)"""
+    for w in which:
+        got, parts = past(plan, H, I, T, w)
+        assert parts == 2 and got == 0, (w, got, parts)
+        assert past(plan, H, I, T, w, moved=1)[0] > 0
+
+
+def test_no_product_reads_past_its_operands(plan):
+    two = 0
+    for H, I in ((8, 8), (72, 264), (520, 4096), (768, 2048), (2048, 768), (2048, 10944), (2880, 2880), (4096, 2048), (4096, 11008),
+                 (5120, 2304), (1032, 5200)):
+        for T in (1, 17, 33, 130, 517, 1100, 2050, 4100, 8192):
+            for w in range(6):
+                got, parts = past(plan, H, I, T, w)
+                assert got == 0, (H, I, T, w, got)
+                two += parts == 2
+    assert two > 20
