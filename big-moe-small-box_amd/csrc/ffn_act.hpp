@@ -5,7 +5,8 @@
 //   h = min(a, La) (clamp(u, -Lu, Lu) + add)
 // silu c1 = 1; gelu (tanh form, 1 + tanh t = 2 sigmoid(2 t)) c1 = 2 sqrt(2 / pi), c3 = 0.044715 c1; silu_oai c1 = 1.702,
 // add = 1. silu_oai clamps g before the activation, the others clamp a after it; no clamp is a clamp at infinity.
-// A NaN stays one through the clamps; a gradient passes at a clamp's border itself and is zero beyond it.
+// A NaN stays one through the clamps; a gradient passes at a clamp's border itself and is zero beyond it. A NaN is beyond none:
+// the comparisons ask what is outside, so that a NaN's gradient is one too, not a clean zero that no check for overflow sees.
 #pragma once
 #include "bmx_common.hpp"
 
@@ -52,13 +53,12 @@ __device__ __forceinline__ float act_h(const ActPar& p, float g, float u)
 // dh/dg and dh/du at (g, u): a' = f + g f', f' = s (1 - s) (c1 + 3 c3 g^2), or the step for the squared relu
 __device__ __forceinline__ void act_grad(const ActPar& p, float g, float u, float& hg, float& hu)
 {
-    const bool gin = g <= p.Lg, uin = fabsf(u) <= p.Lu;
+    const bool gout = g > p.Lg, uout = fabsf(u) > p.Lu;
     g = clamp_hi(g, p.Lg);
     const float f = act_f(p, g), a = g * f;
     const float df = p.relu2 ? (g > 0.0f ? 1.0f : 0.0f) : f * (1.0f - f) * (p.c1 + 3.0f * p.c3 * fminf(g * g, 1e30f));
-    const bool ain = a <= p.La;
-    hg = gin && ain ? (f + g * df) * (clamp_both(u, p.Lu) + p.add) : 0.0f;
-    hu = uin ? clamp_hi(a, p.La) : 0.0f;
+    hg = gout || a > p.La ? 0.0f : (f + g * df) * (clamp_both(u, p.Lu) + p.add);
+    hu = uout ? 0.0f : clamp_hi(a, p.La);
 }
 
 }  // namespace bmx

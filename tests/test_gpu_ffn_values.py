@@ -1,0 +1,88 @@
+"""GatedFFN where values are not finite: what NaN and infinite activations give, in the result and in the gradients."""
+import pytest
+import torch
+
+import ffn_ref as R
+
+pytestmark = pytest.mark.gpu
+
+
+def tensors(cuda, T, H, I, dt=torch.bfloat16, seed=1):
+    g = torch.Generator(device=cuda)
+    g.manual_seed(seed)
+    n = lambda *s: torch.randn(s, device=cuda, generator=g)
+    return n(T, H).to(dt), [(n(a, b) / b ** 0.5).to(dt) for a, b in ((I, H), (I, H), (H, I))], n(T, H).to(dt)
+
+
+def gradients(ffn, x, g, u, h, dy):
+    """dx, dgate, dup, ddown of bmx_ffn_backward from the saved values given."""
+    import bmx
+    lib, d, T = bmx.lib(), ffn.desc(), x.shape[0]
+    ws = torch.empty(lib.bmx_ffn_backward_workspace(d, T), dtype=torch.uint8, device=x.device)
+    out = [torch.empty_like(t) for t in (x, ffn.gate, ffn.up, ffn.down)]
+    bmx._lib.check(lib.bmx_ffn_backward(d, x.data_ptr(), T, bmx._lib.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr()),
+                                        dy.data_ptr(), *(o.data_ptr() for o in out), ws.data_ptr(), ws.numel(),
+                                        torch.cuda.current_stream().cuda_stream))
+    return out
+
+
+# the gradient epilogue behind whole sums, behind sums over splits of K, and in the launch shared with down's gradient
+@pytest.mark.parametrize("T,H,I", [(5, 64, 72), (517, 2048, 768), (2050, 1032, 4104)])
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("L", [0.0, 2.0])
+def test_gradients_of_nan_activations(cuda, T, H, I, act, L):
+    """g = NaN: both slopes are NaN. u = NaN: dh/dg is NaN, dh/du does not depend on u. Everything else keeps its bits."""
+    import bmx
+    x, w, dy = tensors(cuda, T, H, I)
+    ffn = bmx.GatedFFN(*w, act=act, act_limit=L)
+    keep = []
+    ffn._forward(x, keep)
+    _, g, u, h = keep
+    t, j = T // 2, I // 3
+    g[t, j] = u[t, j] = 0.5                      # inside every limit
+    dx, dg, du, dd = gradients(ffn, x, g, u, h, dy)
+    assert all(bool(v.isfinite().all()) for v in (dx, dg, du, dd))
+    rows, units = torch.arange(T, device=cuda) != t, torch.arange(I, device=cuda) != j
+    for bad in ("g", "u"):
+        gb, ub = g.clone(), u.clone()
+        (gb if bad == "g" else ub)[t, j] = float("nan")
+        dxb, dgb, dub, ddb = gradients(ffn, x, gb, ub, h, dy)
+        assert bool(dxb[t].isnan().all()) and torch.equal(dxb[rows], dx[rows])
+        assert bool(dgb[j].isnan().all()) and torch.equal(dgb[units], dg[units])
+        assert torch.equal(dub[units], du[units])
+        assert bool(dub[j].isnan().all()) if bad == "g" else torch.equal(dub[j], du[j])
+        assert torch.equal(ddb, dd)
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("L", [0.0, 2.0])
+def test_nan_in_x_reaches_its_gradients(cuda, act, L):
+    """A NaN in x, or in a row of a weight, is in every gradient that depends on it. (Where a clamp holds a, dh/dg is 0 whatever u
+    is: those tokens' dx does not depend on up's row.)"""
+    import bmx
+    nan = float("nan")
+    for T in (3, 90):
+        x, w, dy = tensors(cuda, T, 136, 200)
+        for bad in ("x", "gate", "up"):
+            leaves = [v.clone() for v in [x] + w]
+            if bad == "x":
+                leaves[0][T // 2, 5] = nan
+            else:
+                leaves[1 if bad == "gate" else 2][7, 3] = nan
+            for v in leaves:
+                v.requires_grad_()
+            y = bmx.GatedFFN(*leaves[1:], act=act, act_limit=L).forward(leaves[0])
+            dx, dg, du, dd = torch.autograd.grad(y, leaves, dy)
+            if bad == "x":
+                assert bool(y[T // 2].isnan().all()) and bool(dx[T // 2].isnan().all())
+                assert all(bool(v.isnan().all()) for v in (dg, du, dd))
+            else:
+                inside = torch.ones(T, dtype=torch.bool, device=cuda)
+                if bad == "up" and L:
+                    g = x.double() @ w[0][7].double()
+                    inside = (g if act == 3 else R.act_a(act, g)) < 0.99 * L
+                    assert bool(inside.any())
+                assert bool(y.isnan().all()) and bool(dx[inside].isnan().all())
+                assert bool(dg[7].isnan().all()) and bool(dd[:, 7].isnan().all())
+                assert bool(du[7].isnan().all()) if bad == "gate" else bool(du.isfinite().all())
+                assert bool(dg[8:].isfinite().all()) and bool(du[8:].isfinite().all())
