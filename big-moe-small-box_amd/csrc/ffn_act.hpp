@@ -1,7 +1,8 @@
 // Gated activations of the feed-forward block: h = act(g, u), and dh/dg, dh/du. The functions are act_gate's (bmx_common.hpp),
 // in fp32 with the hardware exp2 and reciprocal (about 1 ulp each), and in one form without branches, so that an epilogue
 // over a hundred values per lane stays short:
-//   a = g' f(g'),  g' = min(g, Lg),  f = sigmoid(g' (c1 + c3 g'^2)), or max(g', 0) for the squared relu
+//   a = g' f(g'),  g' = min(g, Lg),  f = sigmoid(g' (c1 + c3 g'^2));  a = f f, f = max(g', 0) for the squared relu (g' f would
+//   be NaN at minus infinity)
 //   h = min(a, La) (clamp(u, -Lu, Lu) + add)
 // silu c1 = 1; gelu (tanh form, 1 + tanh t = 2 sigmoid(2 t)) c1 = 2 sqrt(2 / pi), c3 = 0.044715 c1; silu_oai c1 = 1.702,
 // add = 1. silu_oai clamps g before the activation, the others clamp a after it; no clamp is a clamp at infinity.
@@ -43,21 +44,23 @@ __device__ __forceinline__ float act_f(const ActPar& p, float g)
     return p.relu2 ? (g < 0.0f ? 0.0f : g) : s;
 }
 
+__device__ __forceinline__ float act_a(const ActPar& p, float g, float f) { return (p.relu2 ? f : g) * f; }
+
 __device__ __forceinline__ float act_h(const ActPar& p, float g, float u)
 {
-    if (!p.limited) return g * act_f(p, g) * (u + p.add);
+    if (!p.limited) return act_a(p, g, act_f(p, g)) * (u + p.add);
     g = clamp_hi(g, p.Lg);
-    return clamp_hi(g * act_f(p, g), p.La) * (clamp_both(u, p.Lu) + p.add);
+    return clamp_hi(act_a(p, g, act_f(p, g)), p.La) * (clamp_both(u, p.Lu) + p.add);
 }
 
-// dh/dg and dh/du at (g, u): a' = f + g f', f' = s (1 - s) (c1 + 3 c3 g^2), or the step for the squared relu
+// dh/dg and dh/du at (g, u): a' = f + g f', f' = s (1 - s) (c1 + 3 c3 g^2); 2 f for the squared relu
 __device__ __forceinline__ void act_grad(const ActPar& p, float g, float u, float& hg, float& hu)
 {
     const bool gout = g > p.Lg, uout = fabsf(u) > p.Lu;
     g = clamp_hi(g, p.Lg);
-    const float f = act_f(p, g), a = g * f;
-    const float df = p.relu2 ? (g > 0.0f ? 1.0f : 0.0f) : f * (1.0f - f) * (p.c1 + 3.0f * p.c3 * fminf(g * g, 1e30f));
-    hg = gout || a > p.La ? 0.0f : (f + g * df) * (clamp_both(u, p.Lu) + p.add);
+    const float f = act_f(p, g), a = act_a(p, g, f);
+    const float da = p.relu2 ? f + f : f + g * (f * (1.0f - f) * (p.c1 + 3.0f * p.c3 * fminf(g * g, 1e30f)));
+    hg = gout || a > p.La ? 0.0f : da * (clamp_both(u, p.Lu) + p.add);
     hu = uout ? 0.0f : clamp_hi(a, p.La);
 }
 

@@ -86,3 +86,29 @@ def test_nan_in_x_reaches_its_gradients(cuda, act, L):
                 assert bool(dg[7].isnan().all()) and bool(dd[:, 7].isnan().all())
                 assert bool(du[7].isnan().all()) if bad == "gate" else bool(du.isfinite().all())
                 assert bool(dg[8:].isfinite().all()) and bool(du[8:].isfinite().all())
+
+
+@pytest.mark.parametrize("T", [3, 20, 90, 600])
+def test_squared_relu_of_minus_infinity(cuda, T):
+    """relu(g)^2 is 0 at g = -inf as at every other g below zero, with slopes of 0."""
+    import bmx
+    x, w, dy = tensors(cuda, T, 136, 200)
+    x[:, 5] = 1.0
+    for L in (0.0, 2.0):
+        low = [v.clone() for v in w]
+        low[0][7] = 0.0
+        low[0][7, 5] = -1.0
+        want = bmx.GatedFFN(*low, act=bmx.ACT_RELU2, act_limit=L).forward(x)
+        low[0][7, 5] = float("-inf")
+        ffn = bmx.GatedFFN(*low, act=bmx.ACT_RELU2, act_limit=L)
+        assert torch.equal(ffn.forward(x), want) and bool(want.isfinite().all())
+        keep = []
+        ffn._forward(x, keep)
+        _, g, u, h = keep
+        assert bool((g[:, 7] == float("-inf")).all()) and bool((h[:, 7] == 0).all())
+        # the slopes, with weights that are finite
+        ffn = bmx.GatedFFN(*w, act=bmx.ACT_RELU2, act_limit=L)
+        got = gradients(ffn, x, g, u, h, dy)
+        g[:, 7] = -1.0
+        for a, b in zip(got, gradients(ffn, x, g, u, h, dy)):
+            assert bool(b.isfinite().all()) and torch.equal(a, b)
