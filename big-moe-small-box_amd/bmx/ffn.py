@@ -48,8 +48,15 @@ class GatedFFN:
     leaf was first used on)."""
 
     def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
-        self.quantized = not any(torch.is_tensor(w) for w in (gate, up, down))
-        if self.quantized:
+        self.gate, self.up, self.down = gate, up, down
+        self.act, self.act_limit = act, act_limit
+        self._check()
+
+    def _check(self):
+        """The weights and options as they are now, and what follows from them."""
+        gate, up, down = weights = self.gate, self.up, self.down
+        quantized = not any(torch.is_tensor(w) for w in weights)
+        if quantized:
             I, H = gate.N, gate.K
             for name, q, shape in (("gate", gate, (I, H)), ("up", up, (I, H)), ("down", down, (H, I))):
                 if (q.N, q.K) != shape or q.device != gate.device:
@@ -58,16 +65,31 @@ class GatedFFN:
                 raise ValueError(f"GatedFFN: gate and up must have groups of one size, got {gate.group} and {up.group}")
         else:
             I, H = self._check_tensors(gate, up, down)
-        if act not in (L.ACT_SILU, L.ACT_GELU, L.ACT_RELU2, L.ACT_SILU_OAI):
-            raise ValueError(f"GatedFFN: unknown activation {act}")
-        if not act_limit >= 0.0:
-            raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {act_limit}")
-        self.gate, self.up, self.down = gate, up, down
-        self.act, self.act_limit = act, float(act_limit)
+        if self.act not in (L.ACT_SILU, L.ACT_GELU, L.ACT_RELU2, L.ACT_SILU_OAI):
+            raise ValueError(f"GatedFFN: unknown activation {self.act}")
+        if not self.act_limit >= 0.0:
+            raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {self.act_limit}")
+        self.act_limit = float(self.act_limit)
+        self.quantized = quantized
         self.hidden_size, self.intermediate_size = H, I
         self.device = gate.device
-        self.dtype = None if self.quantized else gate.dtype      # None: the input's
+        self.dtype = None if quantized else gate.dtype      # None: the input's
+        self._checked = (*weights, self.act, self.act_limit)
+        self._shapes = None if quantized else (gate.shape, down.shape)
         self._descs = {}
+
+    def _current(self):
+        """Checks again what was replaced since: an attribute, or (16 bits) what a weight tensor holds (Parameter.data). A call
+        hands the kernels addresses, so one with unchecked sizes would read past them."""
+        g, u, d, act, limit = self._checked
+        same = g is self.gate and u is self.up and d is self.down and act == self.act and limit == self.act_limit
+        if same and not self.quantized:
+            (gs, ds), dt, dev = self._shapes, self.dtype, self.device
+            same = (g.shape == gs and u.shape == gs and d.shape == ds and g.dtype is dt and u.dtype is dt and d.dtype is dt and
+                    g.is_contiguous() and u.is_contiguous() and d.is_contiguous() and
+                    g.device == dev and u.device == dev and d.device == dev)
+        if not same:
+            self._check()
 
     @staticmethod
     def _check_tensors(gate, up, down):
@@ -88,6 +110,10 @@ class GatedFFN:
 
     def desc(self, dtype=None):
         """The call descriptor for an input of dtype (default: the weights')."""
+        self._current()
+        return self._desc(dtype)
+
+    def _desc(self, dtype):
         if self.quantized:
             d = self._descs.get(dtype)
             if d is None:
@@ -109,6 +135,7 @@ class GatedFFN:
         return torch.empty(need, dtype=torch.uint8, device=self.device)
 
     def forward(self, x):
+        self._current()
         if not self.quantized and torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or
                                                                self.up.requires_grad or self.down.requires_grad):
             return _GatedFFNFunction.apply(x, self.gate, self.up, self.down, self)
@@ -119,7 +146,7 @@ class GatedFFN:
     __call__ = forward
 
     def _forward(self, x, keep):
-        """y; keep: a list that receives x's rows and the saved g, u, h."""
+        """y; keep: a list that receives x's rows and the saved g, u, h. Behind _current()."""
         r = self._rows(x)
         s = stream_here(self.device)
         if s is None:
@@ -134,7 +161,7 @@ class GatedFFN:
             keep.extend((r, g, u, h))
             saved = L.FfnSaved(g.data_ptr(), u.data_ptr(), h.data_ptr())
         if T:
-            d, lib = self.desc(r.dtype), L.lib()
+            d, lib = self._desc(r.dtype), L.lib()
             if self.quantized:
                 ws = self._workspace(lib.bmx_ffn4_workspace(d, T))
                 rc = lib.bmx_ffn4_forward(d, r.data_ptr(), T, y.data_ptr(), ws.data_ptr(), ws.numel(), s)
@@ -147,6 +174,7 @@ class GatedFFN:
     def add_to(self, out, x, gate_vec=None):
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
         layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
+        self._current()
         r = self._rows(x.detach())
         s = stream_here(self.device)
         if s is None:
@@ -161,7 +189,7 @@ class GatedFFN:
                                      gate_vec.data_ptr() % 16):
             raise ValueError(f"GatedFFN: gate_vec must be a contiguous {r.dtype} tensor of {self.hidden_size} elements")
         if T:
-            d, lib = self.desc(r.dtype), L.lib()
+            d, lib = self._desc(r.dtype), L.lib()
             ws = self._workspace(lib.bmx_ffn4_workspace(d, T) if self.quantized else lib.bmx_ffn_workspace(d, T))
             call = lib.bmx_ffn4_add if self.quantized else lib.bmx_ffn_add
             L.check(call(d, r.data_ptr(), T, gate_vec.data_ptr() if gate_vec is not None else None, out.data_ptr(),
@@ -184,6 +212,9 @@ class _GatedFFNFunction(torch.autograd.Function):
         gate, up, down, x, g, u, h = ctx.saved_tensors
         I, H = gate.shape
         T, dev = x.shape[0], x.device
+        if up.shape != gate.shape or down.shape != (H, I) or g.shape != (T, I) or x.shape[1] != H or \
+                any(w.dtype != h.dtype or w.device != dev or not w.is_contiguous() for w in (gate, up, down)):
+            raise RuntimeError("GatedFFN: a weight was replaced between the forward and the backward pass")
         s = stream_here(dev)
         if s is None:                           # autograd's threads have a current device of their own
             with torch.cuda.device(dev):

@@ -11,7 +11,11 @@ class Q4Matrix:
 
     codes: uint8 [N, K / 2], the even column in a byte's low half; scale: fp16 or bf16 [N, K / group]; zero: uint8
     [N, K / group] or None (8 everywhere); group 32, 64 or 128, K a multiple of it. Contiguous device tensors of one device,
-    copied into the kernels' order here (the given ones are not kept)."""
+    copied into the kernels' order here (the given ones are not kept). Read-only: the kernels get the sizes and addresses that
+    it was made with."""
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"Q4Matrix: {name} is read-only")
 
     def __init__(self, codes, scale, zero=None, group=128):
         if group not in (32, 64, 128):
@@ -27,14 +31,15 @@ class Q4Matrix:
         if zero is not None and (zero.dtype != torch.uint8 or tuple(zero.shape) != shape or zero.device != codes.device or
                                  not zero.is_contiguous()):
             raise ValueError(f"Q4Matrix: zero must be a contiguous uint8 tensor {list(shape)} on {codes.device}")
-        self.N, self.K, self.group, self.device = N, K, group, codes.device
-        lib = L.lib()
+        lib, device = L.lib(), codes.device
         n = lib.bmx_q4_group_count(N, K, group)
-        self.codes = torch.empty(lib.bmx_q4_code_bytes(N, K), dtype=torch.uint8, device=codes.device)
-        self.scale = torch.empty(n, dtype=scale.dtype, device=codes.device)
-        self.zero = torch.empty(n, dtype=torch.uint8, device=codes.device) if zero is not None else None
-        self.struct = L.Q4(N, K, group, DTYPES[scale.dtype], self.codes.data_ptr(), self.scale.data_ptr(),
-                           self.zero.data_ptr() if zero is not None else None)
+        own = dict(N=N, K=K, group=group, device=device,
+                   codes=torch.empty(lib.bmx_q4_code_bytes(N, K), dtype=torch.uint8, device=device),
+                   scale=torch.empty(n, dtype=scale.dtype, device=device),
+                   zero=torch.empty(n, dtype=torch.uint8, device=device) if zero is not None else None)
+        own["struct"] = L.Q4(N, K, group, DTYPES[scale.dtype], own["codes"].data_ptr(), own["scale"].data_ptr(),
+                             own["zero"].data_ptr() if zero is not None else None)
+        self.__dict__.update(own)
         with torch.cuda.device(self.device):
             s = torch.cuda.current_stream().cuda_stream
             L.check(lib.bmx_q4_pack(self.struct, codes.data_ptr(), scale.data_ptr(), zero.data_ptr() if zero is not None else None,

@@ -130,3 +130,42 @@ def test_workspaces_of_any_token_count():
     d = bmx._lib.Ffn4Desc(0, 0, 0.0, 0, ctypes.pointer(gu), ctypes.pointer(gu), ctypes.pointer(dn))
     for T in (0, 1, 16, 17, 80, 81, 517, 1 << 24):
         assert L.bmx_ffn4_workspace(d, T) >= T * 128 * 2
+
+
+def matrix(N, K, group=64):
+    """What GatedFFN takes of a Q4Matrix, without a device."""
+    import types
+    return types.SimpleNamespace(N=N, K=K, group=group, device=torch.device("cpu"), struct=q4(N=N, K=K, group=group, codes=256 * N))
+
+
+def test_replaced_4_bit_matrices_reach_the_next_call():
+    """The descriptor is that of the matrices and options as they are, checked as the constructor checks them."""
+    import bmx
+    gate, up, down = matrix(128, 64), matrix(128, 64), matrix(64, 128)
+    ffn = bmx.GatedFFN(gate, up, down)
+    at = lambda p: ctypes.addressof(p.contents)
+    d = ffn.desc(torch.float16)
+    assert at(d.gate) == ctypes.addressof(gate.struct) and ffn.desc(torch.float16) is d
+    other = matrix(128, 64)
+    ffn.gate = other
+    d = ffn.desc(torch.float16)
+    assert at(d.gate) == ctypes.addressof(other.struct) and at(d.up) == ctypes.addressof(up.struct)
+    ffn.act, ffn.act_limit = bmx.ACT_GELU, 2.0
+    d = ffn.desc(torch.bfloat16)
+    assert (d.act, d.act_limit) == (bmx.ACT_GELU, 2.0)
+    for bad in (matrix(192, 64), matrix(128, 128), matrix(128, 64, group=32), torch.zeros(128, 64)):
+        ffn.gate = bad
+        for _ in range(2):
+            with pytest.raises(ValueError):
+                ffn.desc(torch.float16)
+        with pytest.raises(ValueError):
+            ffn.forward(torch.zeros((1, 64), dtype=torch.float16))
+        with pytest.raises(ValueError):
+            ffn.add_to(torch.zeros((1, 64)), torch.zeros((1, 64), dtype=torch.float16))
+    ffn.gate, ffn.act = gate, 7
+    with pytest.raises(ValueError):
+        ffn.desc(torch.float16)
+    # all three, of other sizes
+    ffn.gate, ffn.up, ffn.down, ffn.act = matrix(192, 128), matrix(192, 128), matrix(128, 192), bmx.ACT_SILU
+    ffn.desc(torch.float16)
+    assert (ffn.hidden_size, ffn.intermediate_size) == (128, 192)

@@ -112,3 +112,39 @@ def test_squared_relu_of_minus_infinity(cuda, T):
         g[:, 7] = -1.0
         for a, b in zip(got, gradients(ffn, x, g, u, h, dy)):
             assert bool(b.isfinite().all()) and torch.equal(a, b)
+
+
+def test_replaced_weights(cuda):
+    """Weights replaced between calls are the next call's, of whatever form; tensors that do not fit are refused before the
+    kernels get their addresses, in the backward pass too. A 4-bit matrix is read-only."""
+    import bmx
+    x, w, dy = tensors(cuda, 5, 64, 72, torch.float16)
+    _, w2, _ = tensors(cuda, 5, 64, 72, torch.float16, seed=2)
+    ffn = bmx.GatedFFN(*(t.clone() for t in w))
+    ffn.gate = w2[0]
+    assert torch.equal(ffn.forward(x), bmx.GatedFFN(w2[0], *w[1:]).forward(x))
+    ffn.up.data = w2[1]
+    assert torch.equal(ffn.forward(x), bmx.GatedFFN(*w2[:2], w[2]).forward(x))
+    out = torch.zeros((5, 64), device=cuda)
+    for bad in (w[0].t(), w[0][:64].contiguous(), w[0].bfloat16(), w[0].cpu(), w[0].view(-1)[1:].clone()):
+        ffn.up = bad
+        with pytest.raises(ValueError):
+            ffn.forward(x)
+        with pytest.raises(ValueError):
+            ffn.add_to(out, x)
+    ffn.up = torch.nn.Parameter(w[1].clone())
+    y = ffn.forward(x)
+    ffn.up.data = w[1][:64].clone()
+    with pytest.raises((ValueError, RuntimeError)):
+        torch.autograd.grad(y, ffn.up, dy)
+    with pytest.raises(ValueError):
+        ffn.forward(x)
+    q = [bmx.Q4Matrix.quantize(torch.randn(n, k, device=cuda).half(), 64) for n, k in ((128, 64), (128, 64), (64, 128), (128, 64))]
+    ffn = bmx.GatedFFN(*q[:3])
+    ffn.forward(x)
+    ffn.gate = q[3]
+    assert torch.equal(ffn.forward(x), bmx.GatedFFN(q[3], q[1], q[2]).forward(x))
+    with pytest.raises(AttributeError):
+        q[0].codes = q[3].codes
+    with pytest.raises(AttributeError):
+        q[0].N = 64
