@@ -7,6 +7,7 @@ stream of the weights' device; nothing synchronises."""
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -34,6 +35,20 @@ def stream_here(device):
     decode call's other host work together."""
     index = device.index
     return _raw_stream(index) if _current_device() == index else None
+
+
+# where a program is followed by its torch operations, one of these says so (asked before eager_only: 0.15 us of a call)
+_tracing, _modes = torch._C._is_tracing, torch._C._len_torch_dispatch_stack
+
+
+def eager_only(who, *tensors):
+    """Refuses what follows a program by its torch operations: the kernels are called by address, so forward-mode
+    derivatives would come out as none, and a traced program would hold the result's allocation and nothing that fills it.
+    (torch.compile runs the calls between its graphs; other tracers have no addresses to give.)"""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{who}: no forward-mode derivatives")
+    if _tracing() or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{who}: cannot be traced")
 
 
 class GatedFFN:
@@ -108,6 +123,9 @@ class GatedFFN:
             raise ValueError(f"GatedFFN: H ({H}) and I ({I}) must be positive multiples of 8")
         return I, H
 
+    def _tensors(self):
+        return () if self.quantized else (self.gate, self.up, self.down)
+
     def desc(self, dtype=None):
         """The call descriptor for an input of dtype (default: the weights')."""
         self._current()
@@ -136,6 +154,8 @@ class GatedFFN:
 
     def forward(self, x):
         self._current()
+        if forward_ad._current_level >= 0 or _tracing() or _modes():
+            eager_only("GatedFFN", x, *self._tensors())
         if not self.quantized and torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or
                                                                self.up.requires_grad or self.down.requires_grad):
             return _GatedFFNFunction.apply(x, self.gate, self.up, self.down, self)
@@ -175,6 +195,8 @@ class GatedFFN:
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
         layer's shared expert. y is not rounded to 16 bits; no gradients. Returns out."""
         self._current()
+        if forward_ad._current_level >= 0 or _tracing() or _modes():
+            eager_only("GatedFFN", x, out, gate_vec, *self._tensors())
         r = self._rows(x.detach())
         s = stream_here(self.device)
         if s is None:

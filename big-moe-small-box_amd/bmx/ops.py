@@ -6,7 +6,7 @@ import torch
 
 from . import _lib as L
 from ._lib import check, lib
-from .ffn import DTYPES, rows_of, stream_here
+from .ffn import DTYPES, _modes, _tracing, eager_only, forward_ad, rows_of, stream_here
 
 
 def _stream():
@@ -68,6 +68,8 @@ def q4_linear(x, q):
         raise ValueError(f"q4_linear: x must be fp16 or bf16, got {dtype}")
     if x.requires_grad and torch.is_grad_enabled():
         raise ValueError("q4_linear: 4-bit weights have no gradients (detach x, or torch.no_grad())")
+    if forward_ad._current_level >= 0 or _tracing() or _modes():
+        eager_only("q4_linear", x)
     device = q.device
     r = rows_of(x, q.K, dtype, device, "q4_linear: x")
     s = stream_here(device)

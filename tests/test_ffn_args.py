@@ -169,3 +169,29 @@ def test_replaced_4_bit_matrices_reach_the_next_call():
     ffn.gate, ffn.up, ffn.down, ffn.act = matrix(192, 128), matrix(192, 128), matrix(128, 192), bmx.ACT_SILU
     ffn.desc(torch.float16)
     assert (ffn.hidden_size, ffn.intermediate_size) == (128, 192)
+
+
+def test_forward_mode_and_tracing_are_refused():
+    """Neither would see more than the output's allocation."""
+    import torch.autograd.forward_ad as fw
+    from torch.fx.experimental.proxy_tensor import make_fx
+    import bmx
+    ffn = bmx.GatedFFN(matrix(128, 64), matrix(128, 64), matrix(64, 128))
+    x, out = torch.zeros((3, 64), dtype=torch.float16), torch.zeros((3, 64))
+    calls = (lambda v: ffn.forward(v), lambda v: ffn.add_to(out, v), lambda v: bmx.ops.q4_linear(v, ffn.gate))
+    with fw.dual_level():
+        d = fw.make_dual(x, torch.ones_like(x))
+        for f in calls:
+            with pytest.raises(ValueError, match="forward-mode"):
+                f(d)
+        with pytest.raises(ValueError, match="forward-mode"):
+            ffn.add_to(fw.make_dual(out, torch.ones_like(out)), x)
+        with pytest.raises(ValueError, match="forward-mode"):
+            ffn.add_to(out, x, fw.make_dual(x[0], torch.ones_like(x[0])))
+    for f in calls:
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))
+        with pytest.raises(RuntimeError, match="traced"):
+            make_fx(f)(x)
+        with pytest.raises(RuntimeError, match="traced"):
+            torch.jit.trace(f, (x,), check_trace=False)

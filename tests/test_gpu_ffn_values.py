@@ -148,3 +148,25 @@ def test_replaced_weights(cuda):
         q[0].codes = q[3].codes
     with pytest.raises(AttributeError):
         q[0].N = 64
+
+
+def test_forward_mode_is_refused_and_compiled_programs_call_the_kernels(cuda):
+    import torch.autograd.forward_ad as fw
+    import bmx
+    x, w, _ = tensors(cuda, 5, 64, 72, torch.float16)
+    ffn, q = bmx.GatedFFN(*w), bmx.Q4Matrix.quantize(w[0], 64)
+    with fw.dual_level():
+        for f in (ffn.forward, lambda v: bmx.ops.q4_linear(v, q)):
+            with pytest.raises(ValueError):
+                f(fw.make_dual(x, torch.ones_like(x)))
+            assert f(x).shape[0] == 5                # no tangent: an ordinary call
+        dual = bmx.GatedFFN(w[0], fw.make_dual(w[1], torch.ones_like(w[1])), w[2])
+        with pytest.raises(ValueError):
+            dual.forward(x)
+        with pytest.raises(ValueError):
+            dual.add_to(torch.zeros((5, 64), device=cuda), x)
+    program = torch.compile(lambda v: (ffn.forward(v * 2), bmx.ops.q4_linear(v * 2, q)), backend="eager")
+    for k in range(3):
+        v = x + k
+        for a, b in zip(program(v), (ffn.forward(v * 2), bmx.ops.q4_linear(v * 2, q))):
+            assert torch.equal(a, b)
