@@ -195,3 +195,14 @@ def test_forward_mode_and_tracing_are_refused():
             make_fx(f)(x)
         with pytest.raises(RuntimeError, match="traced"):
             torch.jit.trace(f, (x,), check_trace=False)
+
+
+def test_the_added_form_has_no_gradients():
+    """Where autograd records it is refused, as the 4-bit block's forward pass: a leaf would train on nothing."""
+    import bmx
+    ffn = bmx.GatedFFN(matrix(128, 64), matrix(128, 64), matrix(64, 128))
+    x, out, vec = torch.zeros((3, 64), dtype=torch.float16), torch.zeros((3, 64)), torch.zeros(64, dtype=torch.float16)
+    leaf = lambda t: t.clone().requires_grad_()
+    for a in ((leaf(out), x, vec), (out, leaf(x), vec), (out, x, leaf(vec)), (out, leaf(x), None)):
+        with pytest.raises(ValueError, match="no gradients"):
+            ffn.add_to(*a)

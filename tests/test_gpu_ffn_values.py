@@ -170,3 +170,26 @@ def test_forward_mode_is_refused_and_compiled_programs_call_the_kernels(cuda):
         v = x + k
         for a, b in zip(program(v), (ffn.forward(v * 2), bmx.ops.q4_linear(v * 2, q))):
             assert torch.equal(a, b)
+
+
+def test_the_added_form_has_no_gradients(cuda):
+    """Nor has a layer that uses it: a block whose weights require grad is refused there unless autograd is off, and x is
+    detached by whoever wants the layer's output alone."""
+    import bmx
+    x, w, _ = tensors(cuda, 5, 256, 72, torch.float16)
+    plain = bmx.GatedFFN(*w)
+    ffn = bmx.GatedFFN(*(torch.nn.Parameter(t.clone()) for t in w))
+    tab = bmx.ExpertTable.random(256, 128, 16, (bmx.TF_K3,) * 3, seed=2, device=cuda)
+    lg = torch.randn((5, 16), device=cuda).half()
+    want = bmx.MoELayer(tab, 4, shared_ffn=plain).forward(x, lg)
+    layer = bmx.MoELayer(tab, 4, shared_ffn=ffn)
+    with pytest.raises(ValueError, match="no gradients"):
+        layer.forward(x, lg)
+    with torch.no_grad():
+        assert torch.equal(layer.forward(x, lg), want)
+    for t in (ffn.gate, ffn.up, ffn.down):
+        t.requires_grad_(False)
+    assert torch.equal(layer.forward(x, lg), want)
+    ffn.down.requires_grad_()
+    with pytest.raises(ValueError, match="no gradients"):
+        ffn.add_to(torch.zeros((5, 256), device=cuda), x)
