@@ -173,7 +173,8 @@ class GatedFFN:
             with torch.cuda.device(self.device):
                 return self._forward(x, keep)
         T = r.shape[0]
-        y = torch.empty_like(r)
+        # of x's shape from the start: a view made in here could not be changed in place where autograd records
+        y = torch.empty(x.shape, dtype=r.dtype, device=self.device)
         saved = None
         if keep is not None:
             g, u, h = (torch.empty((T, self.intermediate_size), dtype=dt, device=self.device)
@@ -189,7 +190,7 @@ class GatedFFN:
                 ws = self._workspace(lib.bmx_ffn_workspace(d, T))
                 rc = lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s)
             L.check(rc, "GatedFFN.forward")
-        return y if x.dim() == 2 else y.view(x.shape)
+        return y
 
     def add_to(self, out, x, gate_vec=None):
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a

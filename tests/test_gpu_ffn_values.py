@@ -193,3 +193,22 @@ def test_the_added_form_has_no_gradients(cuda):
     ffn.down.requires_grad_()
     with pytest.raises(ValueError, match="no gradients"):
         ffn.add_to(torch.zeros((5, 256), device=cuda), x)
+
+
+@pytest.mark.parametrize("shape", [(6,), (6, 64), (2, 3, 64), (64,)])
+def test_the_result_may_be_changed_in_place(cuda, shape):
+    """As any tensor that autograd records, whatever the leading dimensions: a residual added to y, then its gradients."""
+    import bmx
+    shape = shape if shape[-1] == 64 else (*shape, 64)
+    _, w, _ = tensors(cuda, 5, 64, 72, torch.float16)
+    x = torch.randn(shape, device=cuda).half().requires_grad_()
+    w = [t.requires_grad_() for t in w]
+    ffn, dy = bmx.GatedFFN(*w), torch.randn(shape, device=cuda).half()
+    y = ffn.forward(x)
+    want = torch.autograd.grad(y + x, [x] + w, dy)
+    y = ffn.forward(x)
+    before = y.detach().clone()
+    y += x
+    assert y.shape == x.shape and torch.equal(y, before + x)
+    for a, b in zip(torch.autograd.grad(y, [x] + w, dy), want):
+        assert torch.equal(a, b)
