@@ -192,15 +192,20 @@ class GatedFFN:
             L.check(rc, "GatedFFN.forward")
         return y
 
+    def check_added(self, x, out, gate_vec):
+        """What add_to refuses of x, out, gate_vec (None: not there) and the weights, but for shapes and types."""
+        self._current()
+        given = (x, out, gate_vec, *self._tensors())
+        if forward_ad._current_level >= 0 or _tracing() or _modes():
+            eager_only("GatedFFN", *given)
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+            raise ValueError("GatedFFN: the added form has no gradients (torch.no_grad(), or out + forward(x))")
+
     def add_to(self, out, x, gate_vec=None):
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
         layer's shared expert. y is not rounded to 16 bits. No gradients: refused where autograd records and x, gate_vec, out or a
         weight requires grad (torch.no_grad(), or forward()). Returns out."""
-        self._current()
-        if forward_ad._current_level >= 0 or _tracing() or _modes():
-            eager_only("GatedFFN", x, out, gate_vec, *self._tensors())
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, out, gate_vec, *self._tensors())):
-            raise ValueError("GatedFFN: the added form has no gradients (torch.no_grad(), or out + forward(x))")
+        self.check_added(x, out, gate_vec)
         r = self._rows(x)
         s = stream_here(self.device)
         if s is None:

@@ -27,6 +27,8 @@ class MoELayer:
     sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 or 4-bit weights as the layer's shared expert, for
     tables without one (shared_gate then scales its output); slots / li: an ExpertSlots table and this layer's index in it."""
 
+    shared_ffn = shared_ffn_gate = None
+
     def __init__(self, table, topk, first=0, score=L.SCORE_SIGMOID, bias=None, n_group=1, topk_group=1, renorm=True,
                  scale=1.0, act=L.ACT_SILU, gated=True, act_limit=0.0, router_weight=None, slots=None, li=0,
                  shared_gate=None, shared_ffn=None):
@@ -36,11 +38,11 @@ class MoELayer:
             if shared_ffn.hidden_size != table.H or shared_ffn.dtype not in (None, torch.float16) or \
                     shared_ffn.device != table.device:
                 raise ValueError(f"shared_ffn: expected fp16 or 4-bit weights of H = {table.H} on {table.device}")
-        self.shared_ffn, self.shared_ffn_gate = shared_ffn, None
+        self.shared_ffn = shared_ffn
         if shared_ffn is not None and shared_gate is not None:
-            if (shared_gate.dtype != torch.float16 or shared_gate.numel() != table.H or not shared_gate.is_cuda or
-                    not shared_gate.is_contiguous()):
-                raise ValueError("shared_gate must be a contiguous fp16 device tensor of H elements")
+            if (shared_gate.dtype != torch.float16 or shared_gate.numel() != table.H or shared_gate.device != table.device or
+                    not shared_gate.is_contiguous() or shared_gate.data_ptr() % 16):
+                raise ValueError("shared_gate must be a contiguous, 16-byte aligned fp16 tensor of H elements on the table's device")
             self.shared_ffn_gate, shared_gate = shared_gate, None
         self.table = table
         self.num_experts_per_tok = topk
@@ -138,7 +140,13 @@ class MoELayer:
         """out += the shared_ffn's output on the rows x, when there is one."""
         return out if self.shared_ffn is None else self.shared_ffn.add_to(out, x, self.shared_ffn_gate)
 
+    def _check_shared(self, z):
+        """What the shared_ffn refuses is refused before the layer's work: no step is taken that is not carried out."""
+        if self.shared_ffn is not None:
+            self.shared_ffn.check_added(z, None, self.shared_ffn_gate)
+
     def run_bszN(self, z, sel, rw, path=L.PATH_AUTO):
+        self._check_shared(z)
         x = z.view(-1, self.hidden_size)
         if x.dtype != torch.float16 or not x.is_contiguous():
             x = x.half().contiguous()
@@ -277,6 +285,7 @@ class MoELayer:
         return fhs
 
     def forward(self, z, logits=None, path=L.PATH_AUTO):
+        self._check_shared(z)
         if (logits is not None or self.router_weight is not None) and self.slots is None:
             # the whole call in one library entry (router + dispatch fused at decode sizes; the router projection of z
             # first when no logits are given)

@@ -212,3 +212,26 @@ def test_the_result_may_be_changed_in_place(cuda, shape):
     assert y.shape == x.shape and torch.equal(y, before + x)
     for a, b in zip(torch.autograd.grad(y, [x] + w, dy), want):
         assert torch.equal(a, b)
+
+
+def test_a_layer_refuses_before_its_work(cuda):
+    """A gate vector that the block cannot take is refused with the layer, a weight that requires grad before a step is taken
+    on the slot table."""
+    import bmx
+    x, w, _ = tensors(cuda, 5, 256, 72, torch.float16)
+    tab = bmx.ExpertTable.random(256, 128, 16, (bmx.TF_K3,) * 3, seed=2, device=cuda)
+    ffn, odd = bmx.GatedFFN(*w), torch.zeros(257, dtype=torch.float16, device=cuda)[1:]
+    for vec in (odd, odd.clone().cpu(), odd.float(), odd[:128]):
+        with pytest.raises(ValueError):
+            bmx.MoELayer(tab, 4, shared_ffn=ffn, shared_gate=vec)
+    slots = bmx.ExpertSlots([tab], 8, maxj=4)
+    layer = bmx.MoELayer(tab, 4, shared_ffn=ffn, slots=slots)
+    lg = torch.randn((1, 16), device=cuda).half()
+    steps = list(slots.seq)
+    ffn.up.requires_grad_()
+    for f in (lambda: layer.forward(x[:1], lg), lambda: layer.run_bszN(x[:1], torch.zeros((1, 4), dtype=torch.int64, device=cuda), x[:1, :4])):
+        with pytest.raises(ValueError, match="no gradients"):
+            f()
+    assert list(slots.seq) == steps and layer.out_bszn is None
+    with torch.no_grad():
+        layer.forward(x[:1], lg)
