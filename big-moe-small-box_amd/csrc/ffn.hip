@@ -101,6 +101,8 @@ struct FfnIn {
     const void* w[3];
     const bmx_q4* q[3];
     int group(int m) const { return q[0] ? q[m]->group : 0; }
+    // of the product whose first matrix is m
+    bool keep(int m) const { return q[0] && (q4_keep(q[m], dtype) || (m == 0 && q4_keep(q[1], dtype))); }
 };
 
 static FfnIn ffn_in(const bmx_ffn_desc* d)
@@ -115,12 +117,6 @@ static FfnIn ffn_in(const bmx_ffn4_desc* d)
 
 struct FfnPlan { size_t h, gate, part, total; };       // workspace offsets; part: what the larger of the products needs
 
-static size_t product_bytes(int N, int K, int T, int products, int group)
-{
-    if (product_path(N, K, T, products, group) != MANY) return skinny_part_bytes(N, K, T, products, group);
-    return group ? q4_many_bytes(N, K, T, products, group) : product_part_bytes(N, T, K, products);
-}
-
 static FfnPlan ffn_plan(const FfnIn& d, int T)
 {
     FfnPlan p;
@@ -128,7 +124,8 @@ static FfnPlan ffn_plan(const FfnIn& d, int T)
     auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
     p.h = take((size_t)T * d.I * 2);
     p.gate = take((size_t)T * 4);
-    const size_t gu = product_bytes(d.I, d.H, T, 2, d.group(0)), down = product_bytes(d.H, d.I, T, 1, d.group(2));
+    const size_t gu = product_bytes(d.I, d.H, T, 2, d.group(0), d.keep(0)),
+                 down = product_bytes(d.H, d.I, T, 1, d.group(2), d.keep(2));
     p.part = take(gu > down ? gu : down);
     p.total = o + 256;
     return p;
@@ -145,7 +142,8 @@ static int block_product(const FfnIn& d, const SkinnyArgs& base, int first, int 
         if (d.q[0]) k.q[m] = q4_view(d.q[first + m]);
     }
     k.group = d.group(first);
-    if (product_path(k.N, k.K, k.T, n, k.group) != MANY) return launch_skinny(k, d.dtype, epi, reinterpret_cast<float*>(part), s);
+    k.keep = d.keep(first);
+    if (product_path(k.N, k.K, k.T, n, k.group, k.keep) != MANY) return launch_skinny(k, d.dtype, epi, reinterpret_cast<float*>(part), s);
     if (k.group) return launch_q4_many(k, d.q + first, d.dtype, epi, part, s);
     GemmArgs a = {};
     a.chain = a.batch = a.splits = 1;

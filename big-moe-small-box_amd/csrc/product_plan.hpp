@@ -1,5 +1,5 @@
-// Plans of the tiled products (gemm16.hpp): tiles, splits of K, parts of a product, and where an operand's tile ends. Plain host
-// C++ without HIP: the library's calls and the CPU tests run the same arithmetic.
+// Plans of the products: which kernel, tiles, splits of K, parts of a product, workspaces, and where an operand's tile ends. Plain
+// host C++ without HIP: the library's calls and the CPU tests run the same arithmetic.
 #pragma once
 #include <algorithm>
 #include <cstddef>
@@ -7,7 +7,13 @@
 
 namespace bmx {
 
-constexpr int GK = 64;      // K of a tile
+constexpr int GK = 64;      // K of a tile (gemm16_k)
+constexpr int SK_K = 128;   // columns of a step on 4-bit weights, and of skinny_k
+constexpr int SL_K = 512;   // columns of a slice (slice_k)
+constexpr int SL_TT = 5;    // slice_k's most tiles of 16 tokens: 80 KB of x
+constexpr int QG_T = 128, QG_N = 128;      // tokens and rows of W of a workgroup (gemm_q4_k)
+
+constexpr int64_t round_up(int64_t v, int64_t a) { return (v + a - 1) / a * a; }
 
 // The tiles a product can run on: results M x N, workgroups that run at once, and what was measured of each: us a K tile of
 // 64 with a workgroup on every other compute unit or fewer (alone) and with the chip full, us to begin and end.
@@ -120,6 +126,120 @@ inline BackTiles back_tiles(int H, int I, int T)
     p.dw = plan_product(H, I, tiles_k(T), 2, false);
     p.two = two_at_once(H, I, T, p);
     return p;
+}
+
+// ---- few tokens, and 4-bit weights --------------------------------------------------------------------------------------
+
+// Which kernel a product of T tokens with an N x K matrix (or two, side by side) runs on: skinny_k, slice_k or one for many tokens
+enum ProductPath { FEW_DIRECT, FEW_SLICES, MANY };
+
+// skinny_k: tiles of 16 rows per workgroup (1, 2 or, in 4 bits, 4), and how long it takes. x is read once per workgroup, so more
+// tiles save what x costs beside a tile of W (about 0.2 of a 4-bit tile a token, 0.05 of a 16-bit one); but the compute unit
+// with the most workgroups is the last to end, so time goes up in whole rounds of the 256 units. Tiles against measurements
+// (us with 1 / 2 / 4): 16 tokens, 4-bit 5120 -> 2 x 2304 13.1 / 9.0 / 11.1, 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 /
+// 11.5 / 9.7, 16-bit 2304 -> 5120 9.8 / 8.0 / 12.0, 4096 -> 2 x 2048 10.8 / 13.0; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5; 4 tokens
+// 4096 -> 11008 9.4 / 11.8. Time, planned and measured: 4-bit 4096 -> 4096 32 / 64 / 80 tokens 7.9 / 10.0 / 17.5, 7.6 / 9.6 / 16.5;
+// 4096 -> 14336 48 tokens 25.0, 25.9; 16-bit block of 4096 x 2048 17 / 33 tokens 22 / 37, 22 / 38.
+struct DirectPlan { int rt; double us; };
+
+inline DirectPlan direct_plan(int N, int K, int T, int products, bool q4)
+{
+    const int64_t tiles = (int64_t)(N + 15) / 16 * products, tt = (T + 15) / 16;
+    const double x = (T < 16 ? T : 16) * (q4 ? 0.2 : 0.05), us = (K > 1024 ? K / 1024.0 : 1.0) * (q4 ? 0.26 : 1.0);
+    DirectPlan best = {1, 1e30};
+    for (int rt = 1; rt <= (q4 ? 4 : 2); rt *= 2)
+    {
+        const double t = 2.5 + (((tiles + rt - 1) / rt * tt + 255) / 256) * (rt + x) * us;
+        if (t < best.us) best = {rt, t};
+    }
+    return best;
+}
+
+// slice_k and the joining kernel, fp16 and bf16 alike (us, planned and measured in both): 768 x 2048 32 tokens 6.5, 6.0 and 7.5;
+// 4096 x 4096 48 tokens 13, 12.5 and 14.8; 14336 x 4096 64 tokens 31, 26 and 28
+inline double slices_us(int N, int K, int T, int products)
+{
+    return 1.08 * (4.3 + 0.05 * T + (double)N * K * products / 1e6 * (0.13 + 0.0039 * T));
+}
+
+// 4-bit weights of the products of many tokens: codes multiplied as they are (gemm_q4_k), the weights never rounded, or each
+// decoded and rounded to 16 bits first, for gemm16_k's larger tiles. By tokens alone, so that of one matrix a call of more tokens
+// never keeps more digits than one of fewer: to 1,024 as they are, with groups of 32, whose scales cost gemm_q4_k the most, to
+// 256. us as they are / decoded first (bf16 x): groups of 128, 4096 -> 4096 400 tokens 41 / 37, 1,024 61 / 51, 1,100 67 / 61, 2,048
+// 75 / 75, 4,096 155 / 116; 4096 -> 11008 517 71 / 80, 1,024 121 / 110, 4,096 437 / 317; 5120 -> 2304 517 35 / 39, 1,024 48 / 57, 2,048
+// 82 / 71; 32, 4096 -> 4096 200 34 / 35, 300 37 / 38, 400 47 / 39, 1,024 72 / 51; 4096 -> 11008 200 72 / 59, 300 85 / 70.
+constexpr int q4_whole_most(int group) { return group == 32 ? 256 : 1024; }
+
+inline double q4_many_us(int N, int K, int T, int products, int group, bool keep);
+
+// Up to 16 tokens skinny_k: W once. Beyond, it reads W once more for every 16 tokens (from L2), against slices, which join their
+// sums in a second launch, up to SL_TT tiles of tokens, and the tiled products: whichever is planned sooner. Both sides in us:
+// 4-bit 768 x 2048 80 tokens 4.5 / 9.0 by slices, 2560 -> 2304 48 tokens 6.4 / 8.8, 4096 -> 11008 80 tokens bf16 30 / 33, 4096 -> 14336
+// 64 tokens 32 / 28; 16-bit block of 2048 x 768 33 tokens 12.5 / 15.9 by gemm16_k, 5120 x 2304 44 / 29.
+// keep: weights that 16 bits of x's type may not hold are not decoded first.
+inline ProductPath product_path(int N, int K, int T, int products, int group, bool keep)
+{
+    if (T <= 16) return FEW_DIRECT;
+    const double us = T <= 1024 ? direct_plan(N, K, T, products, group != 0).us : 1e30;
+    if (!group) return us < product_us(N, T, K, products) ? FEW_DIRECT : MANY;
+    // the others' two or three launches keep the host of a call outside a graph about 11 us, the one 7
+    const double least = 10.0;
+    if (T <= SL_TT * 16) return us < std::max(slices_us(N, K, T, products), least) ? FEW_DIRECT : FEW_SLICES;
+    // (beyond 80 tokens the plan is a tenth short: 160 tokens 2304 -> 5120 19, 23.5; by gemm_q4_k 20.3). Where the other side
+    // rounds the weights, its time is that of the fewest tokens for which it does: one count at which it takes over.
+    const int at = keep ? T : std::min(T, q4_whole_most(group) + 1);
+    return us * 1.15 < std::max(q4_many_us(N, K, at, products, group, keep), least) ? FEW_DIRECT : MANY;
+}
+
+inline int padded(int n) { return (n + 7) / 8 * 8; }
+inline int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
+
+inline size_t skinny_part_bytes(int N, int K, int T, int products, int group)
+{
+    return product_path(N, K, T, products, group, false) == FEW_SLICES ? (size_t)products * slices_of(K) * T * padded(N) * 4 : 0;
+}
+
+// What was measured of gemm_q4_k: us a step of 128 columns with a workgroup on every other compute unit or fewer, and with
+// two on each; of decoding a matrix first: bytes at 4.8 TB/s and a launch
+struct Q4Plan { bool direct; int splits; double us; };
+
+inline Q4Plan q4_plan(int N, int K, int T, int products, int group, bool keep)
+{
+    if (!keep && T > q4_whole_most(group))
+        return {false, 1, products * ((double)N * K * 2.5 / 4.8e6 + 2.0) + product_us(N, T, K, products)};
+    const int KT = (K + SK_K - 1) / SK_K;
+    const int64_t tiles = (int64_t)((N + QG_N - 1) / QG_N) * ((T + QG_T - 1) / QG_T) * products;
+    const double more = group == 128 ? 1.0 : group == 64 ? 1.08 : 1.35;
+    Q4Plan best = {true, 1, 1e30};
+    for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); ++s)
+    {
+        const int64_t b = tiles * s, full = b / 512, rest = b % 512;
+        const int each = (KT + s - 1) / s;
+        double us = full * (each * 2.3 * more + 3.0);
+        if (rest) us += each * (rest <= 256 ? 1.37 : 2.3) * more + 3.0;
+        if (s > 1) us += 5.0 + (double)N * T * products * s * 8.0 / 4e6;
+        if (us < best.us) best = {true, s, us};
+    }
+    return best;
+}
+
+inline double q4_many_us(int N, int K, int T, int products, int group, bool keep) { return q4_plan(N, K, T, products, group, keep).us; }
+
+inline size_t group_sums_bytes(int K, int T, int group) { return round_up((size_t)(round_up(K, SK_K) / group) * round_up(T, QG_T) * 4, 256); }
+
+// part and sums of a direct product; the decoded matrices and the tiled product's partial sums of the other
+inline size_t q4_many_bytes(int N, int K, int T, int products, int group, bool keep)
+{
+    const Q4Plan p = q4_plan(N, K, T, products, group, keep);
+    if (!p.direct) return round_up((size_t)products * N * K * 2, 256) + product_part_bytes(N, T, K, products);
+    return group_sums_bytes(K, T, group) + (p.splits > 1 ? (size_t)products * p.splits * T * padded(N) * 4 : 0);
+}
+
+// Workspace of a product
+inline size_t product_bytes(int N, int K, int T, int products, int group, bool keep)
+{
+    if (product_path(N, K, T, products, group, keep) != MANY) return skinny_part_bytes(N, K, T, products, group);
+    return group ? q4_many_bytes(N, K, T, products, group, keep) : product_part_bytes(N, T, K, products);
 }
 
 }  // namespace bmx

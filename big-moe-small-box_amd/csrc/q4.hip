@@ -1,4 +1,5 @@
-// 4-bit matrices with group scales: packing into fragment order, decoding to 16 bits, and products of few tokens (skinny_k).
+// 4-bit matrices with group scales: packing into fragment order, decoding to 16 bits, and the launches of their products (skinny_k,
+// slice_k, gemm_q4_k, gemm16_k behind a decoding); skinny_k also for 16-bit weights.
 #include <algorithm>
 
 #include "q4_gemm.hpp"
@@ -109,61 +110,6 @@ int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s)
 
 // ---- products of few tokens ---------------------------------------------------------------------------------------------
 
-// skinny_k: tiles of 16 rows per workgroup (1, 2 or, in 4 bits, 4), and how long it takes. x is read once per workgroup, so more
-// tiles save what x costs beside a tile of W (about 0.2 of a 4-bit tile a token, 0.05 of a 16-bit one); but the compute unit
-// with the most workgroups is the last to end, so time goes up in whole rounds of the 256 units. Tiles against measurements
-// (us with 1 / 2 / 4): 16 tokens, 4-bit 5120 -> 2 x 2304 13.1 / 9.0 / 11.1, 2304 -> 5120 6.7 / 5.0 / 5.9, 4096 -> 14336 17.8 /
-// 11.5 / 9.7, 16-bit 2304 -> 5120 9.8 / 8.0 / 12.0, 4096 -> 2 x 2048 10.8 / 13.0; 8 tokens 5120 -> 2304 5.6 / 6.3 / 9.5; 4 tokens
-// 4096 -> 11008 9.4 / 11.8. Time, planned and measured: 4-bit 4096 -> 4096 32 / 64 / 80 tokens 7.9 / 10.0 / 17.5, 7.6 / 9.6 / 16.5;
-// 4096 -> 14336 48 tokens 25.0, 25.9; 16-bit block of 4096 x 2048 17 / 33 tokens 22 / 37, 22 / 38.
-struct DirectPlan { int rt; double us; };
-
-static DirectPlan direct_plan(int N, int K, int T, int products, bool q4)
-{
-    const int64_t tiles = (int64_t)(N + 15) / 16 * products, tt = (T + 15) / 16;
-    const double x = (T < 16 ? T : 16) * (q4 ? 0.2 : 0.05), us = (K > 1024 ? K / 1024.0 : 1.0) * (q4 ? 0.26 : 1.0);
-    DirectPlan best = {1, 1e30};
-    for (int rt = 1; rt <= (q4 ? 4 : 2); rt *= 2)
-    {
-        const double t = 2.5 + (((tiles + rt - 1) / rt * tt + 255) / 256) * (rt + x) * us;
-        if (t < best.us) best = {rt, t};
-    }
-    return best;
-}
-
-// slice_k and the joining kernel, fp16 and bf16 alike (us, planned and measured in both): 768 x 2048 32 tokens 6.5, 6.0 and 7.5;
-// 4096 x 4096 48 tokens 13, 12.5 and 14.8; 14336 x 4096 64 tokens 31, 26 and 28
-static double slices_us(int N, int K, int T, int products)
-{
-    return 1.08 * (4.3 + 0.05 * T + (double)N * K * products / 1e6 * (0.13 + 0.0039 * T));
-}
-
-static double q4_many_us(int N, int K, int T, int products, int group);
-
-// Up to 16 tokens skinny_k: W once. Beyond, it reads W once more for every 16 tokens (from L2), against slices, which join their
-// sums in a second launch, up to SL_TT tiles of tokens, and the tiled products: whichever is planned sooner. Both sides in us:
-// 4-bit 768 x 2048 80 tokens 4.5 / 9.0 by slices, 2560 -> 2304 48 tokens 6.4 / 8.8, 4096 -> 11008 80 tokens bf16 30 / 33, 4096 -> 14336
-// 64 tokens 32 / 28; 16-bit block of 2048 x 768 33 tokens 12.5 / 15.9 by gemm16_k, 5120 x 2304 44 / 29.
-ProductPath product_path(int N, int K, int T, int products, int group)
-{
-    if (T <= 16) return FEW_DIRECT;
-    const double us = T <= 1024 ? direct_plan(N, K, T, products, group != 0).us : 1e30;
-    if (!group) return us < product_us(N, T, K, products) ? FEW_DIRECT : MANY;
-    // the others' two or three launches keep the host of a call outside a graph about 11 us, the one 7
-    const double least = 10.0;
-    if (T <= SL_TT * 16) return us < std::max(slices_us(N, K, T, products), least) ? FEW_DIRECT : FEW_SLICES;
-    // (beyond 80 tokens the plan is a tenth short: 160 tokens 2304 -> 5120 19, 23.5; by gemm_q4_k 20.3)
-    return us * 1.15 < std::max(q4_many_us(N, K, T, products, group), least) ? FEW_DIRECT : MANY;
-}
-
-static int padded(int n) { return (n + 7) / 8 * 8; }
-static int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
-
-size_t skinny_part_bytes(int N, int K, int T, int products, int group)
-{
-    return product_path(N, K, T, products, group) == FEW_SLICES ? (size_t)products * slices_of(K) * T * padded(N) * 4 : 0;
-}
-
 template <class T, int TT, int G> static int slice_launch(const SliceArgs& a, dim3 grid, hipStream_t s)
 {
     hipLaunchKernelGGL((slice_k<T, TT, G>), grid, dim3(SL_W<TT> * 64), 0, s, a);
@@ -234,7 +180,7 @@ template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a,
 
 template <class T, int EPI> static int few_tokens(const SkinnyArgs& a, float* part, hipStream_t s)
 {
-    if (a.T > 16 && product_path(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, a.group) == FEW_SLICES) return slice_product<T, EPI>(a, part, s);
+    if (a.T > 16 && product_path(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, a.group, a.keep) == FEW_SLICES) return slice_product<T, EPI>(a, part, s);
     switch (a.group)
     {
         case 0: return direct_launch<T, 0, EPI>(a, s);
@@ -253,42 +199,6 @@ int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStrea
 }
 
 // ---- products of many tokens ----------------------------------------------------------------------------------------------
-
-// What was measured of gemm_q4_k: us a step of 128 columns with a workgroup on every other compute unit or fewer, and with
-// two on each; of decoding a matrix first: bytes at 4.8 TB/s and a launch
-struct Q4Plan { bool direct; int splits; double us; };
-
-static Q4Plan q4_plan(int N, int K, int T, int products, int group)
-{
-    const int KT = (K + SK_K - 1) / SK_K;
-    const int64_t tiles = (int64_t)((N + QG_N - 1) / QG_N) * ((T + QG_T - 1) / QG_T) * products;
-    const double more = group == 128 ? 1.0 : group == 64 ? 1.08 : 1.35;
-    Q4Plan best = {true, 1, 1e30};
-    for (int s = 1; s <= 16 && (s == 1 || KT / s >= 2); ++s)
-    {
-        const int64_t b = tiles * s, full = b / 512, rest = b % 512;
-        const int each = (KT + s - 1) / s;
-        double us = full * (each * 2.3 * more + 3.0);
-        if (rest) us += each * (rest <= 256 ? 1.37 : 2.3) * more + 3.0;
-        if (s > 1) us += 5.0 + (double)N * T * products * s * 8.0 / 4e6;
-        if (us < best.us) best = {true, s, us};
-    }
-    const double first = products * ((double)N * K * 2.5 / 4.8e6 + 2.0) + product_us(N, T, K, products);
-    if (first < best.us) best = {false, 1, first};
-    return best;
-}
-
-static double q4_many_us(int N, int K, int T, int products, int group) { return q4_plan(N, K, T, products, group).us; }
-
-static size_t group_sums_bytes(int K, int T, int group) { return align_up((size_t)(ceil_to(K, SK_K) / group) * ceil_to(T, QG_T) * 4, 256); }
-
-// part and sums of a direct product; the decoded matrices and the tiled product's partial sums of the other
-size_t q4_many_bytes(int N, int K, int T, int products, int group)
-{
-    const Q4Plan p = q4_plan(N, K, T, products, group);
-    if (!p.direct) return align_up((size_t)products * N * K * 2, 256) + product_part_bytes(N, T, K, products);
-    return group_sums_bytes(K, T, group) + (p.splits > 1 ? (size_t)products * p.splits * T * padded(N) * 4 : 0);
-}
 
 template <class T, int G, int EPI> static int gemm_q4_launch(Q4GemmArgs a, int splits, hipStream_t s)
 {
@@ -322,7 +232,7 @@ template <class T, int G, int EPI> static int gemm_q4_launch(Q4GemmArgs a, int s
 template <class T, int EPI> static int q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, char* ws, hipStream_t s)
 {
     constexpr int PRODS = EPI == EPI_GU ? 2 : 1;
-    const Q4Plan plan = q4_plan(k.N, k.K, k.T, PRODS, k.group);
+    const Q4Plan plan = q4_plan(k.N, k.K, k.T, PRODS, k.group, k.keep);
     Q4GemmArgs a = {};
     a.g.chain = a.g.batch = a.g.splits = 1;
     a.g.M = k.N; a.g.N = k.T; a.g.K = k.K; a.g.ldo = k.ldo; a.g.ldp = padded(k.N);
@@ -360,11 +270,7 @@ int launch_q4_many(const SkinnyArgs& k, const bmx_q4* const* q, int dtype, int e
 
 // ---- y = x W^T ----------------------------------------------------------------------------------------------------------
 
-static size_t q4_linear_ws(const bmx_q4* q, int T)
-{
-    return product_path(q->N, q->K, T, 1, q->group) == MANY ? q4_many_bytes(q->N, q->K, T, 1, q->group)
-                                                            : skinny_part_bytes(q->N, q->K, T, 1, q->group);
-}
+static size_t q4_linear_ws(const bmx_q4* q, int T, bool keep) { return product_bytes(q->N, q->K, T, 1, q->group, keep); }
 
 }  // namespace bmx
 
@@ -411,7 +317,8 @@ int bmx_q4_dequant(const bmx_q4* q, int dtype, void* out, bmx_stream_t stream)
 size_t bmx_q4_linear_workspace(const bmx_q4* q, int T)
 {
     if (check_q4(q, "bmx_q4_linear_workspace") || T < 0 || T > (1 << 24)) return 0;
-    return q4_linear_ws(q, T);
+    // of either type of x
+    return std::max(q4_linear_ws(q, T, q4_keep(q, BMX_DT_FP16)), q4_linear_ws(q, T, q4_keep(q, BMX_DT_BF16)));
 }
 
 int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
@@ -425,7 +332,8 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
     if (T == 0) return BMX_OK;
     if (!x || !y || reinterpret_cast<uintptr_t>(x) % 16 || reinterpret_cast<uintptr_t>(y) % 16)
         return set_error(BMX_ERR_ARG, "%s: x or y null or not 16-byte aligned", fn);
-    const size_t need = q4_linear_ws(q, T);
+    const bool keep = q4_keep(q, dtype);
+    const size_t need = q4_linear_ws(q, T, keep);
     if (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16))
         return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", fn);
     if (workspace_bytes < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, need);
@@ -433,9 +341,9 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
     SkinnyArgs a = {};
     a.q[0] = q4_view(q);
     a.x = static_cast<const uint16_t*>(x);
-    a.T = T; a.N = q->N; a.K = q->K; a.group = q->group;
+    a.T = T; a.N = q->N; a.K = q->K; a.group = q->group; a.keep = keep;
     a.out = y; a.ldo = q->N;
-    if (product_path(q->N, q->K, T, 1, q->group) == MANY) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
+    if (product_path(q->N, q->K, T, 1, q->group, keep) == MANY) return launch_q4_many(a, &q, dtype, EPI_STORE, static_cast<char*>(workspace), s);
     return launch_skinny(a, dtype, EPI_STORE, static_cast<float*>(workspace), s);
 }
 

@@ -2,8 +2,8 @@
 // codes stay codes until they are operands: a step's 8 KB of them lie in LDS beside 32 KB of x, a lane reads its 32 rows' 64
 // codes of 128 columns with two loads and decodes eight at a time for one matrix instruction (skinny.hpp, Q4Dec). Scales and
 // zero points go onto each group's sums, so the weights are never rounded. Against decoding the matrix to 16 bits first (the
-// bytes written and read again: 4096 -> 11008 23 us beside a product of 65 for 517 tokens) this wins, 78 us, until the tokens
-// are so many that the larger tiles of gemm16_k pay for it (q4_plan; 4,096 tokens 442 against 370 us). A wave's step is 32
+// bytes written and read again: 4096 -> 11008 23 us beside a product of 57 for 517 tokens, 80) this wins, 71 us, until the tokens
+// are so many that the larger tiles of gemm16_k pay for it (q4_whole_most; 4,096 tokens 437 against 317 us). A wave's step is 32
 // matrix instructions (1,024 cycles, 1,280 with the bf16 correction) and about 240 others.
 //
 // v_mfma_f32_32x32x16: A = 32 tokens, B = 32 rows of W; the result's column is the row of W, its rows the tokens.
@@ -19,8 +19,6 @@ struct Q4GemmArgs {
     const float* xs;        // bf16: [groups][padded tokens] sums of x over each group
     int xs_ld;
 };
-
-constexpr int QG_T = 128, QG_N = 128;      // tokens and rows of W of a workgroup
 
 // xs[g][t] = sum of x[t] over group g, 0 for the groups between K and its next multiple of 128; 8 values a lane, the G / 8
 // lanes of a group are neighbours

@@ -13,7 +13,6 @@
 namespace bmx {
 
 constexpr int SK_W = 8;             // waves of a workgroup
-constexpr int SK_K = 128;           // columns of a wave's step
 
 // 4-bit weights in fragment order (bmx_q4): per tile of 16 rows x 128 columns, lane l's 32 codes are 16 bytes: word j holds
 // row l % 16, columns j * 32 + (l / 16) * 8 + e, code e = 2 p in bits 4 p, e = 2 p + 1 in bits 4 p + 16, so that a mask
@@ -30,6 +29,7 @@ struct SkinnyArgs {
     Q4View q[2];
     const uint16_t* x;
     int T, N, K, group;
+    bool keep;                      // 4-bit weights are not to be rounded to 16 bits (q4_keep)
     void* out;
     int ldo;
     const float* scale;             // EPI_ADD: [T] or null
@@ -40,22 +40,17 @@ struct SkinnyArgs {
 // q4.hip
 Q4View q4_view(const bmx_q4* q);
 int check_q4(const bmx_q4* q, const char* who);
+// Whether fp16 may not hold the weights: bf16 scales reach past both ends of its range
+inline bool q4_keep(const bmx_q4* q, int dtype) { return dtype == BMX_DT_FP16 && q->scale_dtype == BMX_DT_BF16; }
 int launch_q4_dequant(const bmx_q4* q, int dtype, void* out, hipStream_t s);
-// Which kernel a product of T tokens with an N x K matrix (or two, side by side) runs on: skinny_k, slice_k or one for many tokens
-enum ProductPath { FEW_DIRECT, FEW_SLICES, MANY };
-ProductPath product_path(int N, int K, int T, int products, int group);
 // A product on skinny_k or slice_k, on a's weights (a.group 0: 16-bit) with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU);
 // part: skinny_part_bytes bytes
 int launch_skinny(const SkinnyArgs& a, int dtype, int epi, float* part, hipStream_t s);
-size_t skinny_part_bytes(int N, int K, int T, int products, int group);
 // A product of more tokens on 4-bit weights q[0] (and q[1]: EPI_GU); ws: q4_many_bytes bytes
 int launch_q4_many(const SkinnyArgs& a, const bmx_q4* const* q, int dtype, int epi, char* ws, hipStream_t s);
-size_t q4_many_bytes(int N, int K, int T, int products, int group);
 // ffn.hip: a product of 16-bit weights on gemm16_k (EPI_STORE, EPI_ADD, EPI_GU with two matrices); g.part:
-// product_part_bytes bytes; about how long it takes
+// product_part_bytes bytes
 int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s);
-size_t product_part_bytes(int N, int T, int K, int products);
-double product_us(int N, int T, int K, int products);
 
 // (v & mask) | magic in one v_and_or_b32, which takes one scalar register and no literals: the constants are put into
 // registers, or the compiler would make two instructions of two literals. (The instruction itself is the compiler's: a matrix
@@ -305,10 +300,8 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 // skinny_k decodes W again for every 16 tokens. Here a workgroup keeps 512
 // columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
 // go to part (as EPI_PART), gemm_finish_k joins them.
-constexpr int SL_K = 512;           // columns of a slice
 // waves of a workgroup: few, so that small matrices still spread evenly; more where x leaves room for one or two workgroups
 template <int TT> constexpr int SL_W = TT <= 3 ? 4 : 8;
-constexpr int SL_TT = 5;            // most tiles of 16 tokens: 80 KB of x
 
 struct SliceArgs {
     SkinnyArgs a;

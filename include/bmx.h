@@ -480,10 +480,11 @@ size_t bmx_q4_group_count(int N, int K, int group);
 int bmx_q4_pack(const bmx_q4* q, const void* codes, const void* scale, const void* zero, bmx_stream_t stream);
 /* out [N][K] of dtype: each weight rounded once. */
 int bmx_q4_dequant(const bmx_q4* q, int dtype, void* out, bmx_stream_t stream);
-/* y [T][N] = x [T][K] W^T, x and y of dtype, 16-byte aligned, y apart from x. fp32 sums, one rounding; x is multiplied with
- * the codes themselves, exactly, but where so many tokens come that decoding the weights to dtype first is faster (each
- * then rounded once: half a step of the type). An infinite bf16 x may give NaN. The workspace is that of a call of T tokens;
- * a call of fewer may need more. */
+/* y [T][N] = x [T][K] W^T, x and y of dtype, 16-byte aligned, y apart from x. fp32 sums, one rounding. To 1,024 tokens (256 with
+ * groups of 32) x is multiplied with the codes themselves, exactly; more tokens may have the weights decoded to dtype first, each
+ * then rounded once, half a step of the type (fp16: a weight past 65,504 becomes infinite), but never for fp16 x with bf16
+ * scales, whose range fp16 does not hold. bf16 x whose products with up to 143, summed over a group, leave fp32's range (infinite
+ * ones, or past 1e34) may give NaN. The workspace is that of a call of T tokens; a call of fewer may need more. */
 size_t bmx_q4_linear_workspace(const bmx_q4* q, int T);
 int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, void* workspace, size_t workspace_bytes,
                   bmx_stream_t stream);

@@ -57,4 +57,10 @@ int64_t plan_past_the_end(int H, int I, int T, int which, int moved, int* parts)
     }
 }
 
+// Whether a 4-bit product decodes and rounds the weights first
+int plan_rounds(int N, int K, int T, int products, int group, int keep)
+{
+    return product_path(N, K, T, products, group, keep) == MANY && !q4_plan(N, K, T, products, group, keep).direct;
+}
+
 }  // extern "C"

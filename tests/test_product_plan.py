@@ -53,3 +53,17 @@ def test_no_product_reads_past_its_operands(plan):
                 assert got == 0, (H, I, T, w, got)
                 two += parts == 2
     assert two > 20
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("N,K", [(139, 5888), (768, 2048), (1536, 4096), (4096, 4096), (11008, 4096), (4096, 11008), (2304, 5120), (5120, 2304)])
+def test_more_tokens_never_keep_more_digits_of_a_4_bit_matrix(plan, N, K, group):
+    """Weights are rounded to 16 bits from one count of tokens on, the documented one at the least, and never where 16 bits may
+    not hold them."""
+    K = K // group * group
+    for products in (1, 2):
+        counts = list(range(1, 2100)) + [2304, 3000, 4096, 4097, 5392, 8192, 1 << 16, 1 << 20]
+        rounds = [plan.plan_rounds(N, K, T, products, group, 0) for T in counts]
+        assert rounds == sorted(rounds) and rounds[-1] == 1
+        assert not any(rounds[:256 if group == 32 else 1024])
+        assert not any(plan.plan_rounds(N, K, T, products, group, 1) for T in counts[::37])
