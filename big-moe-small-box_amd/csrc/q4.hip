@@ -8,24 +8,29 @@ namespace bmx {
 
 // ---- packing and decoding -----------------------------------------------------------------------------------------------
 
-// Checkpoint codes [N][K / 2] (the even column in a byte's low half) -> fragment order; one word (8 codes) per thread
+// Packing: a thread takes every PACK_BLOCKS * 256-th value, since a launch has to stay below 2^32 threads and a matrix of 2^20 rows
+// has more words
+constexpr int PACK_BLOCKS = 1 << 20;
+
+// Checkpoint codes [N][K / 2] (the even column in a byte's low half) -> fragment order; one word (8 codes) at a time
 __global__ __launch_bounds__(256) void q4_pack_codes_k(const uint8_t* __restrict__ in, int N, int K, uint32_t* __restrict__ out,
                                                        int64_t words)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= words) return;
     const int KT = (K + SK_K - 1) / SK_K;
-    const int j = (int)(i & 3), lane = (int)(i >> 2) & 63;
-    const int64_t tile = i >> 8;
-    const int n = (int)(tile / KT) * 16 + (lane & 15), k = (int)(tile % KT) * SK_K + j * 32 + (lane >> 4) * 8;
-    uint32_t w = 0;
-    if (n < N && k < K)
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < words; i += (int64_t)gridDim.x * 256)
     {
-        const uint8_t* b = in + (int64_t)n * (K / 2) + k / 2;
+        const int j = (int)(i & 3), lane = (int)(i >> 2) & 63;
+        const int64_t tile = i >> 8;
+        const int n = (int)(tile / KT) * 16 + (lane & 15), k = (int)(tile % KT) * SK_K + j * 32 + (lane >> 4) * 8;
+        uint32_t w = 0;
+        if (n < N && k < K)
+        {
+            const uint8_t* b = in + (int64_t)n * (K / 2) + k / 2;
 #pragma unroll
-        for (int p = 0; p < 4; ++p) w |= (uint32_t)(b[p] & 15) << (4 * p) | (uint32_t)(b[p] >> 4) << (4 * p + 16);
+            for (int p = 0; p < 4; ++p) w |= (uint32_t)(b[p] & 15) << (4 * p) | (uint32_t)(b[p] >> 4) << (4 * p + 16);
+        }
+        out[i] = w;
     }
-    out[i] = w;
 }
 
 // Scales and zero points [N][K / group] -> [tile of 16 rows][group][16]; outside the matrix scale 0
@@ -33,13 +38,14 @@ __global__ __launch_bounds__(256) void q4_pack_scales_k(const uint16_t* __restri
                                                         int groups, int padded, uint16_t* __restrict__ so, uint8_t* __restrict__ zo,
                                                         int64_t n)
 {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= n) return;
-    const int64_t row = i / 16 / padded * 16 + (i & 15);
-    const int g = (int)(i / 16 % padded);
-    const bool in = row < N && g < groups;
-    so[i] = in ? scale[row * groups + g] : 0;
-    if (zo) zo[i] = in ? zero[row * groups + g] : 0;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+    {
+        const int64_t row = i / 16 / padded * 16 + (i & 15);
+        const int g = (int)(i / 16 % padded);
+        const bool in = row < N && g < groups;
+        so[i] = in ? scale[row * groups + g] : 0;
+        if (zo) zo[i] = in ? zero[row * groups + g] : 0;
+    }
 }
 
 // w = scale (code - zero), exact in fp32 (5 and 11 bits), rounded once to 16 bits; one lane's 32 codes per thread
@@ -296,10 +302,11 @@ int bmx_q4_pack(const bmx_q4* q, const void* codes, const void* scale, const voi
     if (!codes || !scale || !zero != !q->zero) return set_error(BMX_ERR_ARG, "%s: null pointer, or zero points on one side only", fn);
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int64_t words = (int64_t)bmx_q4_code_bytes(q->N, q->K) / 4, n = (int64_t)bmx_q4_group_count(q->N, q->K, q->group);
-    hipLaunchKernelGGL(q4_pack_codes_k, dim3((unsigned)((words + 255) / 256)), dim3(256), 0, s, static_cast<const uint8_t*>(codes),
+    const auto blocks = [](int64_t v) { return dim3((unsigned)std::min<int64_t>((v + 255) / 256, PACK_BLOCKS)); };
+    hipLaunchKernelGGL(q4_pack_codes_k, blocks(words), dim3(256), 0, s, static_cast<const uint8_t*>(codes),
                        q->N, q->K, static_cast<uint32_t*>(const_cast<void*>(q->codes)), words);
     if ((rc = check_launch(fn))) return rc;
-    hipLaunchKernelGGL(q4_pack_scales_k, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, static_cast<const uint16_t*>(scale),
+    hipLaunchKernelGGL(q4_pack_scales_k, blocks(n), dim3(256), 0, s, static_cast<const uint16_t*>(scale),
                        static_cast<const uint8_t*>(zero), q->N, q->K / q->group, (int)(ceil_to(q->K, SK_K) / q->group),
                        static_cast<uint16_t*>(const_cast<void*>(q->scale)), static_cast<uint8_t*>(const_cast<void*>(q->zero)), n);
     return check_launch(fn);

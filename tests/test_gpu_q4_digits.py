@@ -64,3 +64,30 @@ def test_scales_outside_the_range_of_fp16(cuda, T, low):
         # 512 products 2^-23 each of themselves at the most, the activation's dozen operations 2^-23 each: 2^-9 is twice as much
         assert bool(y.isfinite().all())
         assert float((y.double() - y64).norm()) <= 2.0 ** -9 * float(y64.norm())
+
+
+def test_a_matrix_of_more_than_2_32_words(cuda):
+    """2^20 rows of 32,896 columns, 17 GB of codes: packed whole, and products of few and many tokens that reach every row."""
+    import bmx
+    N, K, G = 1 << 20, 257 * 128, 128
+    g = torch.Generator(device=cuda)
+    g.manual_seed(1)
+    row = torch.randint(0, 256, (1009, K // 2), device=cuda, generator=g, dtype=torch.uint8)     # rows repeat every 1,009
+    codes = torch.empty((N, K // 2), dtype=torch.uint8, device=cuda)
+    for n in range(0, N, 1009):
+        codes[n:n + 1009] = row[:min(1009, N - n)]
+    scale = torch.empty((N, K // G), dtype=torch.float16, device=cuda)
+    scale[:] = (1.0 + torch.arange(N, device=cuda) % 7)[:, None].half()                          # and scales every 7
+    q = bmx.Q4Matrix(codes, scale, None, G)
+    del codes, scale
+    x = torch.zeros((100, K), device=cuda)
+    at = torch.randint(0, K, (100, 4), device=cuda, generator=g)
+    x.scatter_(1, at, 1.0)
+    x = x.half()
+    c = torch.stack((row & 15, row >> 4), 2).view(1009, K).double() - 8.0
+    part = x.double() @ c.t()                                                                     # whole numbers: exact
+    rows = torch.arange(N, device=cuda)
+    for T in (1, 3, 20, 100):
+        y = bmx.ops.q4_linear(x[:T], q)
+        for t in range(T):
+            assert torch.equal(y[t].double(), part[t][rows % 1009] * (1 + rows % 7))
