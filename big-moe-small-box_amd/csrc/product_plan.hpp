@@ -155,6 +155,15 @@ inline DirectPlan direct_plan(int N, int K, int T, int products, bool q4)
     return best;
 }
 
+// The form that runs: tiles of rows, x in LDS (one token on 4-bit weights of up to 8,192 columns, 16 KB)
+struct FewForm { int rt; bool xl; };
+
+inline FewForm few_form(int N, int K, int T, int products, int group)
+{
+    if (group && T == 1 && K <= 8192) return {1, true};
+    return {direct_plan(N, K, T, products, group != 0).rt, false};
+}
+
 // slice_k and the joining kernel, fp16 and bf16 alike (us, planned and measured in both): 768 x 2048 32 tokens 6.5, 6.0 and 7.5;
 // 4096 x 4096 48 tokens 13, 12.5 and 14.8; 14336 x 4096 64 tokens 31, 26 and 28
 inline double slices_us(int N, int K, int T, int products)

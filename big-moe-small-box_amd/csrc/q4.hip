@@ -175,13 +175,13 @@ template <class T, int RT, int G, int EPI, bool XL> static int direct_rows(const
 
 template <class T, int G, int EPI> static int direct_launch(const SkinnyArgs& a, hipStream_t s)
 {
-    const int rt = direct_plan(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, G != 0).rt;
+    const FewForm f = few_form(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, G);
     if constexpr (G != 0)
     {
-        if (a.T == 1 && a.K <= 8192) return direct_rows<T, 1, G, EPI, true>(a, s);
-        if (rt == 4) return direct_rows<T, 4, G, EPI, false>(a, s);
+        if (f.xl) return direct_rows<T, 1, G, EPI, true>(a, s);
+        if (f.rt == 4) return direct_rows<T, 4, G, EPI, false>(a, s);
     }
-    return rt == 2 ? direct_rows<T, 2, G, EPI, false>(a, s) : direct_rows<T, 1, G, EPI, false>(a, s);
+    return f.rt == 2 ? direct_rows<T, 2, G, EPI, false>(a, s) : direct_rows<T, 1, G, EPI, false>(a, s);
 }
 
 template <class T, int EPI> static int few_tokens(const SkinnyArgs& a, float* part, hipStream_t s)

@@ -1,4 +1,7 @@
 // The planner and the operand spans of the tiled products (csrc/product_plan.hpp), built with g++ for the CPU tests.
+#include <cstdio>
+#include <string>
+
 #include "product_plan.hpp"
 
 using namespace bmx;
@@ -34,9 +37,52 @@ int64_t past_the_end(const TilePlan& p, int M, int mats, int K, int ld, bool acr
     return next == M ? worst : INT64_MAX;
 }
 
+// ---- the kernel instances that a call launches, as text, one a line ----
+std::string number(const char* name, int v) { return std::string(" ") + name + std::to_string(v); }
+
+// A product on gemm16_k; how: which operands lie across K, what becomes of the sums
+std::string tiled(const TilePlan& p, const std::string& how, const std::string& epi)
+{
+    if (p.splits > 1) return "gemm16" + number("tile", p.tile) + " " + how + " part\nfinish " + epi + "\n";
+    if (p.head) return "gemm16 tile0 " + how + " " + epi + " head\ngemm16" + number("tile", p.tile) + " " + how + " " + epi + " rest\n";
+    return "gemm16" + number("tile", p.tile) + " " + how + " " + epi + "\n";
+}
+
+std::string product_names(int N, int K, int T, int products, int group, bool keep, const std::string& epi)
+{
+    const ProductPath path = product_path(N, K, T, products, group, keep);
+    if (path == FEW_DIRECT)
+    {
+        const FewForm f = few_form(N, K, T, products, group);
+        return "skinny" + number("rt", f.rt) + number("g", group) + " " + epi + (f.xl ? " xl" : T > 16 ? " tiles" : "") + "\n";
+    }
+    if (path == FEW_SLICES) return "slice" + number("tt", (T + 15) / 16) + number("g", group) + "\nfinish " + epi + "\n";
+    if (!group) return tiled(plan_for(N, T, K, products), "along", epi);
+    const Q4Plan p = q4_plan(N, K, T, products, group, keep);
+    if (!p.direct) return tiled(plan_for(N, T, K, products), "along", epi) + "dequant\n";
+    if (p.splits > 1) return "gemm_q4" + number("g", group) + " part\nfinish " + epi + "\n";
+    return "gemm_q4" + number("g", group) + " " + epi + "\n";
+}
+
 }  // namespace
 
 extern "C" {
+
+// op: 0 a 4-bit product (H -> I, group), 1 / 2 a block with 16-bit (group 0) or 4-bit weights, 2 its added form, 3 the gradients
+int plan_names(int op, int T, int H, int I, int group, char* out, int size)
+{
+    std::string s;
+    if (op == 0) s = product_names(I, H, T, 1, group, false, "store");
+    else if (op < 3) s = product_names(I, H, T, 2, group, false, "gu") + product_names(H, I, T, 1, group, false, op == 2 ? "add" : "store");
+    else
+    {
+        const BackTiles b = back_tiles(H, I, T);
+        if (b.two) s += "gemm16_two\n";
+        // (down's gradient alone, or without it, has a launch of its own either way)
+        s += tiled(b.dh, "across", "dgu") + tiled(b.dd, "both", "store") + tiled(b.dx, "across", "store") + tiled(b.dw, "both", "store");
+    }
+    return snprintf(out, size, "%s", s.c_str()) < size;
+}
 
 // The products of a block's passes: 0 gate and up, 1 down, 2 dh, 3 dx, 4 down's gradient, 5 gate's and up's. Returns the bytes
 // past A's end; parts: of how many launches (0: K split)

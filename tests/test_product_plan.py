@@ -67,3 +67,38 @@ def test_more_tokens_never_keep_more_digits_of_a_4_bit_matrix(plan, N, K, group)
         assert rounds == sorted(rounds) and rounds[-1] == 1
         assert not any(rounds[:256 if group == 32 else 1024])
         assert not any(plan.plan_rounds(N, K, T, products, group, 1) for T in counts[::37])
+
+
+def names(plan, op, T, H, I, group=0):
+    buf = ctypes.create_string_buffer(4096)
+    assert plan.plan_names(op, T, H, I, group, buf, len(buf))
+    return set(buf.value.decode().split("\n")) - {""}
+
+
+def test_every_kernel_instance_is_compared_with_sharp_bounds(plan):
+    """The sizes of ffn_sizes.py, at which test_gpu_sharp.py compares every result in both types, reach each kernel instance that
+    calls of any size are planned on: skinny_k by row tiles, group, epilogue and form, slice_k, gemm_q4_k, gemm16_k by tile, operands
+    and epilogue, whole, split, as head and as rest."""
+    import math
+    import random
+    import ffn_sizes as Z
+    reached = set()
+    for T, K, N, G in Z.LINEAR:
+        reached |= names(plan, 0, T, K, N, G)
+    for T, H, I, G in Z.BLOCK4:
+        reached |= names(plan, 1, T, H, I, G) | names(plan, 2, T, H, I, G)
+    for T, H, I in Z.BLOCK16:
+        reached |= names(plan, 1, T, H, I) | names(plan, 2, T, H, I) | names(plan, 3, T, H, I)
+    rng = random.Random(3)
+    log = lambda lo, hi: int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+    launched = set()
+    for _ in range(40000):
+        T = rng.choice((log(1, 16), log(17, 80), log(81, 1100), log(1100, 16384)))
+        op = rng.choice((0, 1, 2, 3, 4, 5))
+        if op in (0, 4, 5):
+            G = rng.choice((32, 64, 128))
+            launched |= names(plan, op % 3, T, G * log(1, 12288 // G), log(1, 16384) if op == 0 else G * log(1, 16384 // G), G)
+        else:
+            launched |= names(plan, op, T, 8 * log(1, 1100), 8 * log(1, 1376))
+    assert len(launched) > 150
+    assert not launched - reached, sorted(launched - reached)
