@@ -1,6 +1,6 @@
 """The feed-forward block and the 4-bit matrices at the sizes of ffn_sizes.py, every value against 64 bits with bounds that an output
 of zeros, a lost step of K or an exchanged row does not keep (sharp_ref.py, test_sharp_ref.py): each step from what the kernels kept
-of the one before."""
+of the one before. And two calls at once, on streams and in graphs, of products whose partial sums lie in workspaces."""
 import pytest
 import torch
 
@@ -111,3 +111,67 @@ def weight_gradient(d, v, ed, dt):
     """d^T v over the tokens, and its bound."""
     y, e = S.product(d.t().contiguous(), v.t().contiguous(), ed.t().contiguous() if torch.is_tensor(ed) else 0.0)
     return y, S.rounded(y, e, dt)
+
+
+def twice(calls, inputs):
+    """Every call on two streams at once and in two graphs, replayed with new inputs between eager calls: the eager bits."""
+    want = [c() for c in calls]
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        for st in streams:
+            with torch.cuda.stream(st):
+                outs.append([c() for c in calls])
+    for st in streams:
+        torch.cuda.current_stream().wait_stream(st)
+    for o in outs:
+        for a, b in zip(o, want):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
+    torch.cuda.synchronize()
+    graphs, caught = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for gr in graphs:
+        with torch.cuda.graph(gr):
+            caught.append([c() for c in calls])
+    for k in range(4):
+        with torch.no_grad():
+            for i, t in enumerate(inputs):
+                t.copy_(normal(t.device, 100 * k + i, *t.shape))
+        for gr in graphs:
+            gr.replay()
+        torch.cuda.synchronize()
+        eager = [c() for c in calls]
+        for one in caught:
+            for a, b in zip(one, eager):
+                assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dt", sorted(DT))
+def test_4_bit_products_in_parts_at_once(cuda, dt):
+    """Slices, K split with and without group sums, decoded weights: each with a workspace."""
+    import bmx
+    for T, K, N, G in ((39, 7360, 73, 32), (77, 4096, 4096, 32), (300, 4096, 1000, 64), (1100, 1024, 520, 128)):
+        q = bmx.Q4Matrix(*S.symmetric_codes(cuda, N, K, G, True, torch.float16, seed=1)[0], group=G)
+        x = normal(cuda, 1, T, K).to(DT[dt])
+        twice([lambda: (bmx.ops.q4_linear(x, q),)], [x])
+    for T, H, I, G in ((50, 4096, 2560, 32), (150, 4096, 1024, 32)):
+        mats = [bmx.Q4Matrix(*S.symmetric_codes(cuda, n, k, G, True, torch.float16, seed=1)[0], group=G) for n, k in ((I, H), (I, H), (H, I))]
+        ffn, x = bmx.GatedFFN(*mats), normal(cuda, 1, T, H).to(DT[dt])
+        twice([lambda: (ffn.forward(x),), lambda: (ffn.add_to(torch.zeros((T, H), device=cuda), x),)], [x])
+
+
+@pytest.mark.parametrize("T,H,I", [(33, 5120, 2304), (517, 2048, 768), (2050, 1032, 4104)])
+def test_16_bit_products_in_parts_at_once(cuda, T, H, I):
+    """K split in the forward and the backward pass, and down's gradient beside dh."""
+    import bmx
+    x, dy = normal(cuda, 1, T, H).half(), normal(cuda, 2, T, H).half()
+    w = [(normal(cuda, s, a, b) / b ** 0.5).half() for s, (a, b) in enumerate(((I, H), (I, H), (H, I)))]
+    plain = bmx.GatedFFN(*w)
+    leaves = [t.clone().requires_grad_() for t in [x] + w]
+    ffn = bmx.GatedFFN(*leaves[1:])
+
+    def step():
+        y = ffn.forward(leaves[0])
+        return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+
+    twice([step, lambda: (plain.forward(x),), lambda: (plain.add_to(torch.zeros((T, H), device=cuda), x),)], [x, leaves[0], dy])
