@@ -91,3 +91,30 @@ def test_a_matrix_of_more_than_2_32_words(cuda):
         y = bmx.ops.q4_linear(x[:T], q)
         for t in range(T):
             assert torch.equal(y[t].double(), part[t][rows % 1009] * (1 + rows % 7))
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("dt", sorted(DT))
+def test_quantized_weights_are_within_half_a_step(cuda, G, symmetric, dt):
+    """s the group's step, |s - step| <= half a rounding of it. A value whose code is in range is off by at most s / 2, whatever the
+    zero point (a whole number). At the ends, up to 15 steps from the zero point's end (7.5 symmetric), the zero point's rounding or the
+    missing half code takes up to s / 2 and the scale's rounding up to 15 of its own; then the decoded weight is rounded. Codes that
+    are cut instead of rounded are off by up to a step."""
+    import bmx
+    dt = DT[dt]
+    half = torch.finfo(dt).eps / 2
+    w = torch.randn((200, 4 * G), device=cuda, generator=torch.Generator(device=cuda).manual_seed(G)).to(dt)
+    w[0], w[1], w[2], w[3] = 0, 0.5, w[2].abs(), -w[3].abs()
+    w[4, :G] *= 64.0
+    v = w.double().view(200, 4, G)
+    lo, hi = v.amin(2).clamp(max=0), v.amax(2).clamp(min=0)
+    step = v.abs().amax(2) / 7.5 if symmetric else (hi - lo) / 15
+    bound = step * (0.5 * (1 + half) + 15 * half + 2.0 ** -19) + half * v.abs().amax(2)
+    q = bmx.Q4Matrix.quantize(w, G, symmetric)
+    err = (q.dequant(dt).double().view(200, 4, G) - v).abs().amax(2)
+    assert bool((err <= bound).all()), float((err / bound).nan_to_num().max())
+    s = step.clamp(min=1e-9)[..., None]
+    z = 8.0 if symmetric else (-lo[..., None] / s).round()
+    cut = ((v / s + z).floor().clamp(0, 15) - z) * s
+    assert bool(((cut - v).abs().amax(2) > bound)[5:].any())
