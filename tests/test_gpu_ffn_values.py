@@ -235,3 +235,36 @@ def test_a_layer_refuses_before_its_work(cuda):
     assert list(slots.seq) == steps and layer.out_bszn is None
     with torch.no_grad():
         layer.forward(x[:1], lg)
+
+
+def test_saved_values_elsewhere(cuda):
+    """Recomputed (checkpoint), kept in host memory, used twice (retain_graph), accumulated into .grad: the plain gradients' bits."""
+    import torch.utils.checkpoint as C
+    import bmx
+    x, w, dy = tensors(cuda, 90, 136, 264, torch.float16)
+    leaves = [t.requires_grad_() for t in [x] + w]
+    ffn = bmx.GatedFFN(*w)
+    want = torch.autograd.grad(ffn.forward(x), leaves, dy)
+    same = lambda got: all(torch.equal(a, b) for a, b in zip(got, want))
+    for reentrant in (False, True):
+        y = C.checkpoint(ffn.forward, x, use_reentrant=reentrant)
+        y.backward(dy)
+        assert same([t.grad for t in leaves])
+        for t in leaves:
+            t.grad = None
+    with torch.autograd.graph.save_on_cpu():
+        y = ffn.forward(x)
+    assert same(torch.autograd.grad(y, leaves, dy))
+    y = ffn.forward(x)
+    assert same(torch.autograd.grad(y, leaves, dy, retain_graph=True)) and same(torch.autograd.grad(y, leaves, dy))
+    # two blocks on the same weights, one behind the other
+    z = bmx.GatedFFN(*w).forward(ffn.forward(x))
+    a = torch.autograd.grad(z, w, dy)
+    mid = ffn.forward(x)
+    parts = torch.autograd.grad(ffn.forward(mid.detach().requires_grad_()), w, dy)
+    m = mid.detach().requires_grad_()
+    dm, = torch.autograd.grad(ffn.forward(m), m, dy)
+    for got, p, q in zip(a, parts, torch.autograd.grad(mid, w, dm)):
+        assert torch.equal(got, p + q)
+    with torch.inference_mode():
+        assert torch.equal(ffn.forward(x), mid)
