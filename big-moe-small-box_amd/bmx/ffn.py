@@ -90,19 +90,21 @@ class GatedFFN:
         self.device = gate.device
         self.dtype = None if quantized else gate.dtype      # None: the input's
         self._checked = (*weights, self.act, self.act_limit)
-        self._shapes = None if quantized else (gate.shape, down.shape)
+        if not quantized:
+            self._at = tuple(w.data_ptr() for w in weights), gate.shape, down.shape
         self._descs = {}
 
     def _current(self):
         """Checks again what was replaced since: an attribute, or (16 bits) what a weight tensor holds (Parameter.data). A call
-        hands the kernels addresses, so one with unchecked sizes would read past them."""
+        hands the kernels addresses, so one with unchecked sizes would read past them. (A weight on another device lies at another
+        address.)"""
         g, u, d, act, limit = self._checked
         same = g is self.gate and u is self.up and d is self.down and act == self.act and limit == self.act_limit
         if same and not self.quantized:
-            (gs, ds), dt, dev = self._shapes, self.dtype, self.device
-            same = (g.shape == gs and u.shape == gs and d.shape == ds and g.dtype is dt and u.dtype is dt and d.dtype is dt and
+            (at, gs, ds), dt = self._at, self.dtype
+            same = ((g.data_ptr(), u.data_ptr(), d.data_ptr()) == at and g.shape == gs and u.shape == gs and d.shape == ds and
                     g.is_contiguous() and u.is_contiguous() and d.is_contiguous() and
-                    g.device == dev and u.device == dev and d.device == dev)
+                    g.dtype is dt and u.dtype is dt and d.dtype is dt)
         if not same:
             self._check()
 
@@ -132,15 +134,16 @@ class GatedFFN:
         return self._desc(dtype)
 
     def _desc(self, dtype):
-        if self.quantized:
-            d = self._descs.get(dtype)
-            if d is None:
+        """Of the weights as _current() has left them, kept for the next call."""
+        d = self._descs.get(dtype)
+        if d is None:
+            if self.quantized:
                 ref = lambda q: ctypes.pointer(q.struct)
-                d = self._descs[dtype] = L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up),
-                                                    ref(self.down))
-            return d
-        return L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0,
-                         self.gate.data_ptr(), self.up.data_ptr(), self.down.data_ptr())
+                d = L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up), ref(self.down))
+            else:
+                d = L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0, *self._at[0])
+            self._descs[dtype] = d
+        return d
 
     def _rows(self, x):
         if self.quantized and x.dtype not in DTYPES:
@@ -174,7 +177,7 @@ class GatedFFN:
                 return self._forward(x, keep)
         T = r.shape[0]
         # of x's shape from the start: a view made in here could not be changed in place where autograd records
-        y = torch.empty(x.shape, dtype=r.dtype, device=self.device)
+        y = torch.empty_like(r) if r is x else x.new_empty(x.shape)
         saved = None
         if keep is not None:
             g, u, h = (torch.empty((T, self.intermediate_size), dtype=dt, device=self.device)
@@ -189,7 +192,8 @@ class GatedFFN:
             else:
                 ws = self._workspace(lib.bmx_ffn_workspace(d, T))
                 rc = lib.bmx_ffn_forward(d, r.data_ptr(), T, y.data_ptr(), saved, ws.data_ptr(), ws.numel(), s)
-            L.check(rc, "GatedFFN.forward")
+            if rc:
+                L.check(rc, "GatedFFN.forward")
         return y
 
     def check_added(self, x, out, gate_vec):

@@ -82,8 +82,9 @@ def q4_linear(x, q):
         L_ = lib()
         need = L_.bmx_q4_linear_workspace(q.struct, T)
         ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        check(L_.bmx_q4_linear(q.struct, dt, r.data_ptr(), T, y.data_ptr(), ws.data_ptr() if need else None, need, s),
-              "bmx_q4_linear")
+        rc = L_.bmx_q4_linear(q.struct, dt, r.data_ptr(), T, y.data_ptr(), ws.data_ptr() if need else None, need, s)
+        if rc:
+            check(rc, "bmx_q4_linear")
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (q.N,))
 
 
