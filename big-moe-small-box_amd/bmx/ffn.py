@@ -108,6 +108,10 @@ class GatedFFN:
         if not same:
             self._check()
 
+    def __getstate__(self):
+        """Without the calls' descriptors, which hold addresses: a copy has weights of its own."""
+        return {**self.__dict__, "_descs": {}}
+
     @staticmethod
     def _check_tensors(gate, up, down):
         if not all(torch.is_tensor(w) for w in (gate, up, down)):

@@ -25,7 +25,8 @@ class MoELayer:
     (routed_scaling_factor); activation, gated, act_limit; router_weight: fp16 [E, H] gate weight (checkpoint layout),
     used when no logits are given; shared_gate: fp16 [H] gate vector of the shared expert (its output scaled by
     sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 or 4-bit weights as the layer's shared expert, for
-    tables without one (shared_gate then scales its output); slots / li: an ExpertSlots table and this layer's index in it."""
+    tables without one (shared_gate then scales its output; no gradients: GatedFFN.add_to); slots / li: an
+    ExpertSlots table and this layer's index in it."""
 
     shared_ffn = shared_ffn_gate = None
 

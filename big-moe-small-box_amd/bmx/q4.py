@@ -15,7 +15,9 @@ class Q4Matrix:
     it was made with."""
 
     def __setattr__(self, name, value):
-        raise AttributeError(f"Q4Matrix: {name} is read-only")
+        if name in ("N", "K", "group", "device", "codes", "scale", "zero", "struct"):
+            raise AttributeError(f"Q4Matrix: {name} is read-only")
+        super().__setattr__(name, value)
 
     def __init__(self, codes, scale, zero=None, group=128):
         if group not in (32, 64, 128):

@@ -268,3 +268,21 @@ def test_saved_values_elsewhere(cuda):
         assert torch.equal(got, p + q)
     with torch.inference_mode():
         assert torch.equal(ffn.forward(x), mid)
+
+
+def test_copies(cuda):
+    """A copied block has weights of its own, also one that has been called; a 4-bit matrix takes attributes of the user's."""
+    import copy
+    import bmx
+    x, w, _ = tensors(cuda, 5, 64, 72, torch.float16)
+    ffn = bmx.GatedFFN(*w)
+    want = ffn.forward(x)
+    other = copy.deepcopy(ffn)
+    assert torch.equal(other.forward(x), want) and other.gate.data_ptr() != ffn.gate.data_ptr()
+    with torch.no_grad():
+        ffn.down.zero_()
+    assert torch.equal(other.forward(x), want) and not bool(ffn.forward(x).any())
+    q = bmx.Q4Matrix.quantize(w[0], 64)
+    q.name = "gate_proj"
+    q.name = "up_proj"
+    assert q.name == "up_proj"
