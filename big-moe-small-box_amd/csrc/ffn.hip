@@ -1,6 +1,6 @@
 // Gated feed-forward block: forward and the form that adds to a layer's output (16-bit and 4-bit weights), gradients (16-bit).
-// The products are skinny_k's for few tokens and gemm16_k's for many (4-bit weights: slice_k's and gemm_q4_k's between); this
-// file plans tiles and splits, lays out the workspace and checks arguments.
+// The products are skinny_k's for few tokens and gemm16_k's for many (4-bit weights: slice_k's and gemm_q4_k's between), planned
+// in product_plan.hpp; this file launches gemm16_k, lays out the workspace and checks arguments.
 #include <algorithm>
 
 #include "skinny.hpp"

@@ -191,7 +191,9 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
     if (T <= 16) return FEW_DIRECT;
     const double us = T <= 1024 ? direct_plan(N, K, T, products, group != 0).us : 1e30;
     if (!group) return us < product_us(N, T, K, products) ? FEW_DIRECT : MANY;
-    // the others' two or three launches keep the host of a call outside a graph about 11 us, the one 7
+    // The others' two or three launches keep the host of a call outside a graph about 11 us, the one 7. A graph has no such host, but
+    // its nodes' own ends: us a call / in a graph, this way and by their times alone, 4-bit 512 -> 2553 226 tokens 7.4 / 7.5, 9.8 / 9.9;
+    // 4416 -> 750 30 tokens 7.0 / 7.0, 10.8 / 6.9; 256 -> 4342 149 tokens 7.1 / 6.9, 8.5 / 7.7; 5888 -> 139 23 tokens 7.9 / 7.8, 10.9 / 6.1.
     const double least = 10.0;
     if (T <= SL_TT * 16) return us < std::max(slices_us(N, K, T, products), least) ? FEW_DIRECT : FEW_SLICES;
     // (beyond 80 tokens the plan is a tenth short: 160 tokens 2304 -> 5120 19, 23.5; by gemm_q4_k 20.3). Where the other side

@@ -284,7 +284,7 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
         if (EPI == EPI_GU)
         {
             const float u = sum(i + 8);
-            static_cast<uint16_t*>(p.out)[o] = to16<T>(act_h(p.act, s, u));
+            static_cast<uint16_t*>(p.out)[o] = to16<T>(act_h(p.act, s, u));            // (16 bits: put_gu)
             if (p.g) { p.g[o] = s; p.u[o] = u; }
         }
         else if (EPI == EPI_ADD)
@@ -297,9 +297,8 @@ __global__ __launch_bounds__(SK_W * 64) void skinny_k(const SkinnyArgs p)
 }
 
 // ---- 4-bit weights, more tokens: slices of K ---------------------------------------------------------------------------------------------
-// skinny_k decodes W again for every 16 tokens. Here a workgroup keeps 512
-// columns of x in LDS and streams rows of W past them, a tile of 16 rows x 512 columns per wave at a time; every slice's sums
-// go to part (as EPI_PART), gemm_finish_k joins them.
+// skinny_k decodes W again for every 16 tokens. Here a workgroup keeps 512 columns of x in LDS and streams rows of W past them, a
+// tile of 16 rows x 512 columns per wave at a time; every slice's sums go to part (as EPI_PART), gemm_finish_k joins them.
 // waves of a workgroup: few, so that small matrices still spread evenly; more where x leaves room for one or two workgroups
 template <int TT> constexpr int SL_W = TT <= 3 ? 4 : 8;
 

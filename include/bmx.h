@@ -495,7 +495,8 @@ int bmx_q4_linear(const bmx_q4* q, int dtype, const void* x, int T, void* y, voi
  * contiguous, all of type dtype, 16-byte aligned; H and I multiples of 8; any T >= 0. act, act_limit as the routed experts'
  * (enum bmx_act; h = min(act(g), limit) * clamp(u, +-limit), or for BMX_ACT_SILU_OAI the clamps first and (u + 1);
  * act_limit 0 = off, else positive). Products accumulate in fp32; h = act(g, u) is rounded once to dtype between the two
- * products, y once at the end. NaN and infinities pass through. */
+ * products (in fp16 an h past 65,504 is infinite), y once at the end. NaN and infinities pass through, and a NaN's gradient is
+ * one. */
 typedef struct bmx_ffn_desc {
     int32_t H, I;
     int32_t dtype;
