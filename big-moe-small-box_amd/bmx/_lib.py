@@ -15,7 +15,7 @@ STAGE_GATE_UP, STAGE_ACT, STAGE_DOWN, STAGE_COMBINE, STAGE_DOWN_OUT, STAGE_PREP 
 STAGE_GATE_UP_RESIDENT, STAGE_GATE_UP_STAGED = 6, 7
 STAGE_ROUTE = 8
 STAGE_DOWN_RESIDENT, STAGE_DOWN_STAGED = 9, 10
-DT_FP16, DT_BF16 = 0, 1
+DT_FP16, DT_BF16, DT_FP32 = 0, 1, 2
 LANE_VRAM, LANE_ADMIT, LANE_HOME, LANE_CPU = 0, 1, 2, 3
 PLAN_MAXP, PLAN_MAXT = 64, 8
 
@@ -74,6 +74,20 @@ class Q4(ctypes.Structure):
 class Ffn4Desc(ctypes.Structure):
     _fields_ = [("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("act_limit", ctypes.c_float), ("reserved", ctypes.c_int32),
                 ("gate", ctypes.POINTER(Q4)), ("up", ctypes.POINTER(Q4)), ("down", ctypes.POINTER(Q4))]
+
+
+class Q8(ctypes.Structure):
+    _fields_ = [("N", ctypes.c_int32), ("K", ctypes.c_int32), ("ld", ctypes.c_int64), ("codes", _P), ("scale", _P)]
+
+
+class Ffn8Desc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("act", ctypes.c_int32), ("act_limit", ctypes.c_float), ("reserved", ctypes.c_int32),
+                ("gate", ctypes.POINTER(Q8)), ("up", ctypes.POINTER(Q8)), ("down", ctypes.POINTER(Q8))]
+
+
+class NormDesc(ctypes.Structure):
+    _fields_ = [("H", ctypes.c_int32), ("dtype", ctypes.c_int32), ("x_dtype", ctypes.c_int32), ("residual_dtype", ctypes.c_int32),
+                ("weight_dtype", ctypes.c_int32), ("eps", ctypes.c_float), ("weight", _P)]
 
 
 class FfnSaved(ctypes.Structure):
@@ -154,6 +168,16 @@ SIGNATURES = {
     "bmx_ffn_forward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, ctypes.POINTER(FfnSaved), _P, _SZ, _P]),
     "bmx_ffn_add": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, _P, _P, _SZ, _P]),
     "bmx_ffn_backward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, ctypes.POINTER(FfnSaved), _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "bmx_q8_quantize": (_I, [_P, _I, ctypes.POINTER(Q8), _P]),
+    "bmx_q8_dequant": (_I, [ctypes.POINTER(Q8), _I, _P, _P]),
+    "bmx_q8_linear_workspace": (_SZ, [ctypes.POINTER(Q8), _I]),
+    "bmx_q8_linear": (_I, [ctypes.POINTER(Q8), _I, _P, ctypes.POINTER(Q8), _I, _P, _P, _SZ, _P]),
+    "bmx_ffn8_workspace": (_SZ, [ctypes.POINTER(Ffn8Desc), _I]),
+    "bmx_ffn8_forward": (_I, [ctypes.POINTER(Ffn8Desc), _P, ctypes.POINTER(Q8), _I, _P, _P, _SZ, _P]),
+    "bmx_ffn8_add": (_I, [ctypes.POINTER(Ffn8Desc), _P, ctypes.POINTER(Q8), _I, _P, _P, _P, _SZ, _P]),
+    "bmx_rms_norm": (_I, [ctypes.POINTER(NormDesc), _P, _P, _I, _P, _P, ctypes.POINTER(Q8), _P]),
+    "bmx_rms_norm_backward_workspace": (_SZ, [ctypes.POINTER(NormDesc), _I]),
+    "bmx_rms_norm_backward": (_I, [ctypes.POINTER(NormDesc), _P, _I, _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "bmx_host_device_ptr": (_I, [_P, ctypes.POINTER(ctypes.c_uint64)]),
 }
 

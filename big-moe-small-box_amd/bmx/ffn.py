@@ -52,11 +52,12 @@ def eager_only(who, *tensors):
 
 
 class GatedFFN:
-    """gate, up [I, H] and down [H, I]: contiguous fp16 or bf16 device tensors of one type (H, I multiples of 8), or three
-    Q4Matrix (gate and up of one group size; x may then be fp16 or bf16, and there are no gradients); act: ACT_SILU, ACT_GELU
-    (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit: the activation's clamp (0: none), both as MoELayer's.
+    """gate, up [I, H] and down [H, I]: contiguous fp16 or bf16 device tensors of one type (H, I multiples of 8), three Q4Matrix
+    (gate and up of one group size), or three Q8Matrix (H, I multiples of 8; x and act(g, u) are quantized per token); with 4 or 8
+    bits x may be fp16 or bf16, and there are no gradients. act: ACT_SILU, ACT_GELU (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit:
+    the activation's clamp (0: none), both as MoELayer's.
 
-    forward(x) -> y, x [..., H] of the weights' type. Where autograd records (x or a weight requires grad), y carries the
+    forward(x) -> y, x [..., H] of the weights' type (8-bit weights: or Rows8, as RMSNorm.rows8 gives them). Where autograd records (x or a weight requires grad), y carries the
     gradients of x and of the three weights; the forward pass then keeps x, g and u (fp32 [T, I]) and h (16 bits). Passes
     with gradients may be captured into a graph through torch.autograd.grad; with backward(), which accumulates into the
     leaves, only while no eager result of the same leaves is alive (torch's accumulation belongs to the stream that the
@@ -71,12 +72,19 @@ class GatedFFN:
         """The weights and options as they are now, and what follows from them."""
         gate, up, down = weights = self.gate, self.up, self.down
         quantized = not any(torch.is_tensor(w) for w in weights)
+        bits = 16
         if quantized:
+            from .q8 import Q8Matrix
+            bits = 8 if isinstance(gate, Q8Matrix) else 4
+            if any(isinstance(w, Q8Matrix) != (bits == 8) for w in weights):
+                raise ValueError("GatedFFN: three tensors, three Q4Matrix or three Q8Matrix")
             I, H = gate.N, gate.K
             for name, q, shape in (("gate", gate, (I, H)), ("up", up, (I, H)), ("down", down, (H, I))):
                 if (q.N, q.K) != shape or q.device != gate.device:
                     raise ValueError(f"GatedFFN: {name} must be {list(shape)} on {gate.device}, got {[q.N, q.K]} on {q.device}")
-            if gate.group != up.group:
+            if bits == 8 and (H % 8 or I % 8):
+                raise ValueError(f"GatedFFN: H ({H}) and I ({I}) must be multiples of 8")
+            if bits == 4 and gate.group != up.group:
                 raise ValueError(f"GatedFFN: gate and up must have groups of one size, got {gate.group} and {up.group}")
         else:
             I, H = self._check_tensors(gate, up, down)
@@ -85,7 +93,7 @@ class GatedFFN:
         if not self.act_limit >= 0.0:
             raise ValueError(f"GatedFFN: act_limit must be 0 (off) or positive, got {self.act_limit}")
         self.act_limit = float(self.act_limit)
-        self.quantized = quantized
+        self.quantized, self.bits = quantized, bits
         self.hidden_size, self.intermediate_size = H, I
         self.device = gate.device
         self.dtype = None if quantized else gate.dtype      # None: the input's
@@ -143,7 +151,8 @@ class GatedFFN:
         if d is None:
             if self.quantized:
                 ref = lambda q: ctypes.pointer(q.struct)
-                d = L.Ffn4Desc(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up), ref(self.down))
+                kind = L.Ffn8Desc if self.bits == 8 else L.Ffn4Desc
+                d = kind(DTYPES[dtype], self.act, self.act_limit, 0, ref(self.gate), ref(self.up), ref(self.down))
             else:
                 d = L.FfnDesc(self.hidden_size, self.intermediate_size, DTYPES[self.dtype], self.act, self.act_limit, 0, *self._at[0])
             self._descs[dtype] = d
@@ -161,6 +170,8 @@ class GatedFFN:
 
     def forward(self, x):
         self._current()
+        if self.bits == 8:
+            return self._forward8(x)
         if forward_ad._current_level >= 0 or _tracing() or _modes():
             eager_only("GatedFFN", x, *self._tensors())
         if not self.quantized and torch.is_grad_enabled() and (x.requires_grad or self.gate.requires_grad or
@@ -200,6 +211,38 @@ class GatedFFN:
                 L.check(rc, "GatedFFN.forward")
         return y
 
+    def _input8(self, x):
+        """x's rows and Rows8 (one of them None), checked, with 8-bit weights."""
+        if torch.is_tensor(x):
+            if forward_ad._current_level >= 0 or _tracing() or _modes():
+                eager_only("GatedFFN", x)
+            if x.requires_grad and torch.is_grad_enabled():
+                raise ValueError("GatedFFN: 8-bit weights have no gradients (detach x, or torch.no_grad())")
+            return self._rows(x), None
+        from .q8 import Rows8
+        if not isinstance(x, Rows8) or x.K != self.hidden_size or x.device != self.device:
+            raise ValueError(f"GatedFFN: x must be a tensor or Rows8 of {self.hidden_size} codes on {self.device}")
+        if _tracing() or _modes():
+            eager_only("GatedFFN")
+        return None, x
+
+    def _forward8(self, x):
+        r, rows = self._input8(x)
+        s = stream_here(self.device)
+        if s is None:
+            with torch.cuda.device(self.device):
+                return self._forward8(x)
+        y = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        T = rows.N if r is None else r.shape[0]
+        if T:
+            d, lib = self._desc(x.dtype), L.lib()
+            ws = self._workspace(lib.bmx_ffn8_workspace(d, T))
+            rc = lib.bmx_ffn8_forward(d, None if r is None else r.data_ptr(), None if rows is None else rows.struct, T, y.data_ptr(),
+                                      ws.data_ptr(), ws.numel(), s)
+            if rc:
+                L.check(rc, "GatedFFN.forward")
+        return y
+
     def check_added(self, x, out, gate_vec):
         """What add_to refuses of x, out, gate_vec (None: not there) and the weights, but for shapes and types."""
         self._current()
@@ -209,16 +252,21 @@ class GatedFFN:
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
             raise ValueError("GatedFFN: the added form has no gradients (torch.no_grad(), or out + forward(x))")
 
-    def add_to(self, out, x, gate_vec=None):
+    def check_rows(self, rows, T):
+        if self.bits != 8 or rows.N != T or rows.K != self.hidden_size or rows.device != self.device:
+            raise ValueError(f"GatedFFN: rows must be {T} of {self.hidden_size} codes on {self.device}, for 8-bit weights")
+
+    def add_to(self, out, x, gate_vec=None, rows=None):
         """out [T, H] (fp32, contiguous) += y, or sigmoid(x . gate_vec) * y with gate_vec [H] of x's type: the block as a
         layer's shared expert. y is not rounded to 16 bits. No gradients: refused where autograd records and x, gate_vec, out or a
-        weight requires grad (torch.no_grad(), or forward()). Returns out."""
+        weight requires grad (torch.no_grad(), or forward()). rows: x's Rows8, with 8-bit weights, if they are there already
+        (RMSNorm.both). Returns out."""
         self.check_added(x, out, gate_vec)
         r = self._rows(x)
         s = stream_here(self.device)
         if s is None:
             with torch.cuda.device(self.device):
-                return self.add_to(out, x, gate_vec)
+                return self.add_to(out, x, gate_vec, rows)
         T = r.shape[0]
         if out.dtype != torch.float32 or out.device != self.device or not out.is_contiguous() or out.data_ptr() % 16 or \
                 tuple(out.shape) != (T, self.hidden_size):
@@ -227,7 +275,15 @@ class GatedFFN:
                                      gate_vec.numel() != self.hidden_size or not gate_vec.is_contiguous() or
                                      gate_vec.data_ptr() % 16):
             raise ValueError(f"GatedFFN: gate_vec must be a contiguous {r.dtype} tensor of {self.hidden_size} elements")
-        if T:
+        if rows is not None:
+            self.check_rows(rows, T)
+        if T and self.bits == 8:
+            d, lib = self._desc(r.dtype), L.lib()
+            ws = self._workspace(lib.bmx_ffn8_workspace(d, T))
+            L.check(lib.bmx_ffn8_add(d, r.data_ptr(), None if rows is None else rows.struct, T,
+                                     gate_vec.data_ptr() if gate_vec is not None else None, out.data_ptr(), ws.data_ptr(), ws.numel(), s),
+                    "GatedFFN.add_to")
+        elif T:
             d, lib = self._desc(r.dtype), L.lib()
             ws = self._workspace(lib.bmx_ffn4_workspace(d, T) if self.quantized else lib.bmx_ffn_workspace(d, T))
             call = lib.bmx_ffn4_add if self.quantized else lib.bmx_ffn_add

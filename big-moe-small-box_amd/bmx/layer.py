@@ -24,21 +24,24 @@ class MoELayer:
     score (SCORE_SOFTMAX / SCORE_SIGMOID / SCORE_SQRTSP), selection bias fp32 [E], group limit, renorm, scale
     (routed_scaling_factor); activation, gated, act_limit; router_weight: fp16 [E, H] gate weight (checkpoint layout),
     used when no logits are given; shared_gate: fp16 [H] gate vector of the shared expert (its output scaled by
-    sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16 or 4-bit weights as the layer's shared expert, for
-    tables without one (shared_gate then scales its output; no gradients: GatedFFN.add_to); slots / li: an
-    ExpertSlots table and this layer's index in it."""
+    sigmoid(x . shared_gate)) or None; shared_ffn: a GatedFFN of fp16, 4-bit or 8-bit weights as the layer's shared expert,
+    for tables without one (shared_gate then scales its output; no gradients: GatedFFN.add_to); norm: the RMSNorm that stands
+    before the layer in the stream (block); slots / li: an ExpertSlots table and this layer's index in it."""
 
-    shared_ffn = shared_ffn_gate = None
+    shared_ffn = shared_ffn_gate = norm = None
 
     def __init__(self, table, topk, first=0, score=L.SCORE_SIGMOID, bias=None, n_group=1, topk_group=1, renorm=True,
                  scale=1.0, act=L.ACT_SILU, gated=True, act_limit=0.0, router_weight=None, slots=None, li=0,
-                 shared_gate=None, shared_ffn=None):
+                 shared_gate=None, shared_ffn=None, norm=None):
         if shared_ffn is not None:
             if table.has_shared:
                 raise ValueError("shared_ffn: the table already has a shared expert")
             if shared_ffn.hidden_size != table.H or shared_ffn.dtype not in (None, torch.float16) or \
                     shared_ffn.device != table.device:
-                raise ValueError(f"shared_ffn: expected fp16 or 4-bit weights of H = {table.H} on {table.device}")
+                raise ValueError(f"shared_ffn: expected fp16, 4-bit or 8-bit weights of H = {table.H} on {table.device}")
+        if norm is not None:
+            self._check_norm(norm, table)
+        self.norm = norm
         self.shared_ffn = shared_ffn
         if shared_ffn is not None and shared_gate is not None:
             if (shared_gate.dtype != torch.float16 or shared_gate.numel() != table.H or shared_gate.device != table.device or
@@ -68,6 +71,11 @@ class MoELayer:
                                    router_weight.data_ptr() if router_weight is not None else None)
         self._ws = None
         self.out_bszn = None
+
+    @staticmethod
+    def _check_norm(norm, table):
+        if norm.hidden_size != table.H or norm._out != torch.float16 or norm.device != table.device:
+            raise ValueError(f"norm: expected an RMSNorm into fp16 of H = {table.H} on {table.device}")
 
     # ---- router ----
     def router_logits(self, z):
@@ -137,17 +145,22 @@ class MoELayer:
         return self._ws
 
     # ---- experts + combine ----
-    def _add_shared(self, out, x):
-        """out += the shared_ffn's output on the rows x, when there is one."""
-        return out if self.shared_ffn is None else self.shared_ffn.add_to(out, x, self.shared_ffn_gate)
+    def _add_shared(self, out, x, rows):
+        """out += the shared_ffn's output on the rows x (rows: their Rows8 or None), when there is one."""
+        return out if self.shared_ffn is None else self.shared_ffn.add_to(out, x, self.shared_ffn_gate, rows)
 
-    def _check_shared(self, z):
+    def _check_shared(self, z, rows=None):
         """What the shared_ffn refuses is refused before the layer's work: no step is taken that is not carried out."""
         if self.shared_ffn is not None:
             self.shared_ffn.check_added(z, None, self.shared_ffn_gate)
+        if rows is not None:
+            if self.shared_ffn is None:
+                raise ValueError("MoELayer: 8-bit rows are for a shared_ffn of 8-bit weights")
+            self.shared_ffn.check_rows(rows, z.numel() // self.hidden_size)
 
-    def run_bszN(self, z, sel, rw, path=L.PATH_AUTO):
-        self._check_shared(z)
+    def run_bszN(self, z, sel, rw, path=L.PATH_AUTO, rows=None):
+        """rows: z's Rows8 (RMSNorm.both), for a shared_ffn of 8-bit weights."""
+        self._check_shared(z, rows)
         x = z.view(-1, self.hidden_size)
         if x.dtype != torch.float16 or not x.is_contiguous():
             x = x.half().contiguous()
@@ -164,14 +177,14 @@ class MoELayer:
             self._workspace(need)
             self.out_bszn = ops.moe_forward(self.slot_desc, x, sel, rw, path, self._ws)
             self.slots.stage_restore(staged)
-            return self._add_shared(self.out_bszn, x)
+            return self._add_shared(self.out_bszn, x, rows)
         if self.slots is not None:
             self.out_bszn = self._run_slots(x, sel, rw, path)
-            return self._add_shared(self.out_bszn, x)
+            return self._add_shared(self.out_bszn, x, rows)
         need = L.lib().bmx_moe_workspace(self.desc, x.shape[0], path)
         self._workspace(need)
         self.out_bszn = ops.moe_forward(self.desc, x, sel, rw, path, self._ws)
-        return self._add_shared(self.out_bszn, x)
+        return self._add_shared(self.out_bszn, x, rows)
 
     def _run_slots(self, x, sel, rw, path):
         """Expert products with the slot table: gate / up of the experts resident before this layer's step, then (after
@@ -285,8 +298,9 @@ class MoELayer:
             self.slots.cpu_add(seq, fhs.view(-1, self.hidden_size))
         return fhs
 
-    def forward(self, z, logits=None, path=L.PATH_AUTO):
-        self._check_shared(z)
+    def forward(self, z, logits=None, path=L.PATH_AUTO, rows=None):
+        """rows: z's Rows8 (RMSNorm.both), for a shared_ffn of 8-bit weights."""
+        self._check_shared(z, rows)
         if (logits is not None or self.router_weight is not None) and self.slots is None:
             # the whole call in one library entry (router + dispatch fused at decode sizes; the router projection of z
             # first when no logits are given)
@@ -298,9 +312,25 @@ class MoELayer:
             self._workspace(need)
             out, self.sel, self.w = ops.moe_layer(self.desc, self.router, x, lg, path, self._ws)
             self.out_bszn = out
-            return self._add_shared(out, x)
+            return self._add_shared(out, x, rows)
         bsz = z.shape[0]
         sel, w = self.routing_fn(bsz, None, z, {"logits": logits} if logits is not None else {})
         sel, w, _ = self.layer(self.li, sel, w, z, bsz)
-        out = self.run_bszN(z, sel, w, path)
+        out = self.run_bszN(z, sel, w, path, rows)
         return self.cpu_split_combine(self.combine(out), None, False, None)
+
+    def block(self, x, residual=None, logits=None, path=L.PATH_AUTO):
+        """The layer behind its norm in a model's stream of residuals: r = residual + x (no residual: r = x), out = forward(norm(r)).
+        x [T, H] is what the stream gets before this layer: an attention's fp16 output, or another layer's fp32 out as it is;
+        residual: the stream, fp16 or fp32 [T, H]. Returns (out fp32 [T, H], r): out is the next block's or norm's x, r its residual.
+        One launch does sum, norm and, for a shared_ffn of 8-bit weights, its 8-bit rows. No gradients."""
+        if self.norm is None:
+            raise ValueError("MoELayer.block: the layer has no norm")
+        self.norm._current()
+        self._check_norm(self.norm, self.table)
+        if x.dim() != 2:
+            raise ValueError(f"MoELayer.block: x must be [T, {self.hidden_size}], got {tuple(x.shape)}")
+        self._check_shared(None)
+        self.norm.refuse_grad(x, residual)
+        z, rows, r = self.norm._run(x, residual, True, self.shared_ffn is not None and self.shared_ffn.bits == 8)
+        return self.forward(z, logits, path, rows), x if residual is None else r

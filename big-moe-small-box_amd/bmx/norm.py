@@ -1,0 +1,171 @@
+"""RMSNorm: the root-mean-square norm with the residual's addition that stands before a layer or a feed-forward block, into 16 bits
+(forward and gradients) or into 8-bit rows, on the HIP library. Every call enqueues on torch's current stream of the weight's
+device; nothing synchronises."""
+import torch
+
+from . import _lib as L
+from .ffn import DTYPES, _modes, _tracing, eager_only, forward_ad, rows_of, stream_here
+from .q8 import ROW_DTYPES, Rows8
+
+MOST_H = 32768
+
+
+class RMSNorm:
+    """y = v w / sqrt(mean(v^2) + eps) over the last dimension, v = x, or x + residual as the stream holds it: r = x + residual is
+    summed in fp32 and rounded to residual's type, and the norm is of r.
+
+    weight: [H] fp16, bf16 or fp32, contiguous on a device, H a multiple of 8 to 32,768; dtype: of y, fp16 or bf16 (default the
+    weight's; fp32 weights need it). x and residual [..., H] of dtype or fp32 each, so that a MoELayer's fp32 output can go into a
+    stream of 16 bits. forward(x) -> y; forward(x, residual) -> (y, r). Where autograd records, y and r carry the gradients of x,
+    residual and weight (the rounding of r passes them as they are); the forward pass then keeps r (x without a residual), which must
+    not be changed before the backward pass. Passes with gradients may be captured as GatedFFN's may."""
+
+    def __init__(self, weight, eps=1e-6, dtype=None):
+        self.weight, self.eps, self.dtype = weight, eps, dtype
+        self._check()
+
+    def _check(self):
+        """The weight and options as they are now, and what follows from them."""
+        w, eps, dtype = self.weight, self.eps, self.dtype
+        if not torch.is_tensor(w) or w.dim() != 1 or w.dtype not in ROW_DTYPES or not w.is_cuda:
+            raise ValueError("RMSNorm: weight must be an fp16, bf16 or fp32 device tensor [H]")
+        if w.shape[0] <= 0 or w.shape[0] % 8 or w.shape[0] > MOST_H:
+            raise ValueError(f"RMSNorm: H ({w.shape[0]}) must be a positive multiple of 8, at most {MOST_H}")
+        if not w.is_contiguous() or w.data_ptr() % 16:
+            raise ValueError("RMSNorm: weight must be contiguous and 16-byte aligned")
+        out = w.dtype if dtype is None else dtype
+        if out not in DTYPES or w.dtype not in (out, torch.float32):
+            raise ValueError(f"RMSNorm: y must be fp16 or bf16 and the weight of that type or fp32, got {out} and {w.dtype}")
+        # (what fp32 makes of it: the kernels get it so)
+        if not 2.0 ** -149 <= eps < float("inf"):
+            raise ValueError(f"RMSNorm: eps must be positive and finite, got {eps}")
+        self._out, self.hidden_size, self.device = out, w.shape[0], w.device
+        self._checked = (w, eps, dtype)
+        self._at = (w.data_ptr(), w.dtype, w.shape)
+        self._descs = {}
+
+    def _current(self):
+        """Checks again what was replaced since: an attribute, or what the weight tensor holds (Parameter.data)."""
+        w, eps, dtype = self._checked
+        if not (w is self.weight and eps == self.eps and dtype is self.dtype and (w.data_ptr(), w.dtype, w.shape) == self._at and
+                w.is_contiguous()):
+            self._check()
+
+    def __getstate__(self):
+        """Without the calls' descriptors, which hold addresses: a copy has a weight of its own."""
+        return {**self.__dict__, "_descs": {}, "_at": None}
+
+    def _desc(self, xt, rt):
+        d = self._descs.get((xt, rt))
+        if d is None:
+            d = L.NormDesc(self.hidden_size, DTYPES[self._out], ROW_DTYPES[xt], ROW_DTYPES[rt], ROW_DTYPES[self._at[1]], self.eps,
+                           self._at[0])
+            self._descs[xt, rt] = d
+        return d
+
+    def _rows(self, x, name):
+        if x.dtype is not self._out and x.dtype is not torch.float32:
+            raise ValueError(f"RMSNorm: {name} must be {self._out} or fp32, got {x.dtype}")
+        return rows_of(x, self.hidden_size, x.dtype, self.device, name)
+
+    def _run(self, x, residual, want_y, want_rows):
+        """(y, rows, r), None what is not wanted. Behind _current()."""
+        a = self._rows(x, "RMSNorm: x")
+        b = None
+        if residual is not None:
+            b = self._rows(residual, "RMSNorm: residual")
+            if residual.shape != x.shape:
+                raise ValueError(f"RMSNorm: x {tuple(x.shape)} and residual {tuple(residual.shape)} must be of one shape")
+        s = stream_here(self.device)
+        if s is None:
+            with torch.cuda.device(self.device):
+                return self._run(x, residual, want_y, want_rows)
+        T, H = a.shape
+        y = a.new_empty(x.shape, dtype=self._out) if want_y else None
+        r = b.new_empty(x.shape) if b is not None else None
+        rows = Rows8._empty(T, H, self.device, self._out, x.shape) if want_rows else None
+        if T:
+            rc = L.lib().bmx_rms_norm(self._desc(a.dtype, a.dtype if b is None else b.dtype), a.data_ptr(),
+                                      b.data_ptr() if b is not None else None, T, r.data_ptr() if r is not None else None,
+                                      y.data_ptr() if want_y else None, rows.struct if want_rows else None, s)
+            if rc:
+                L.check(rc, "bmx_rms_norm")
+        return y, rows, r
+
+    def _enter(self, who, x, residual):
+        """Checks that come before any work; whether autograd records."""
+        self._current()
+        if forward_ad._current_level >= 0 or _tracing() or _modes():
+            eager_only(who, x, residual, self.weight)
+        return torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
+                                            (residual is not None and residual.requires_grad))
+
+    def forward(self, x, residual=None):
+        if self._enter("RMSNorm", x, residual):
+            got = _RMSNormFunction.apply(x, residual, self.weight, self)
+            return got if residual is not None else got[0]
+        y, _, r = self._run(x, residual, True, False)
+        return y if residual is None else (y, r)
+
+    __call__ = forward
+
+    def rows8(self, x, residual=None):
+        """The norm in 8 bits for ops.q8_linear and a GatedFFN of 8-bit weights: Rows8, or (Rows8, r) with a residual. The codes are
+        of y before any rounding to 16 bits. No gradients."""
+        self.refuse_grad(x, residual)
+        _, rows, r = self._run(x, residual, False, True)
+        return rows if residual is None else (rows, r)
+
+    def both(self, x, residual=None):
+        """y and its 8-bit rows in one pass: (y, Rows8), or (y, Rows8, r) with a residual. No gradients."""
+        self.refuse_grad(x, residual)
+        y, rows, r = self._run(x, residual, True, True)
+        return (y, rows) if residual is None else (y, rows, r)
+
+    def refuse_grad(self, x, residual):
+        """What the forms without gradients refuse."""
+        if self._enter("RMSNorm", x, residual):
+            raise ValueError("RMSNorm: 8-bit rows have no gradients (torch.no_grad(), or forward)")
+
+
+class _RMSNormFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, norm):
+        y, _, r = norm._run(x.detach(), None if residual is None else residual.detach(), True, False)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(weight, x if r is None else r)
+        ctx.xt, ctx.summed, ctx.eps, ctx.out, ctx.H = x.dtype, r is not None, norm.eps, norm._out, norm.hidden_size
+        return y, r
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy, dr):
+        weight, v = ctx.saved_tensors
+        H, dev, shape = ctx.H, v.device, v.shape
+        if tuple(weight.shape) != (H,) or weight.device != dev or not weight.is_contiguous() or weight.dtype not in (ctx.out, torch.float32):
+            raise RuntimeError("RMSNorm: the weight was replaced between the forward and the backward pass")
+        s = stream_here(dev)
+        if s is None:                           # autograd's threads have a current device of their own
+            with torch.cuda.device(dev):
+                return _RMSNormFunction.backward(ctx, dy, dr)
+        nx, nr, nw, _ = ctx.needs_input_grad
+        rt = v.dtype if ctx.summed else ctx.xt
+        if dy is None:                          # r alone was used (or neither)
+            both = None if dr is None else dr
+            dx = both.to(ctx.xt) if nx and both is not None else None
+            return dx, both if nr else None, torch.zeros_like(weight) if nw else None, None
+        rows = rows_of(v, H, v.dtype, dev, "RMSNorm: the saved rows")
+        g = rows_of(dy, H, ctx.out, dev, "RMSNorm: the gradient of y")
+        more = None if dr is None else rows_of(dr, H, rt, dev, "RMSNorm: the gradient of r")
+        one = ctx.summed and rt == ctx.xt       # x's and residual's gradients are the same values
+        dx = torch.empty(shape, dtype=ctx.xt, device=dev) if nx or (nr and one) else None
+        dres = torch.empty(shape, dtype=rt, device=dev) if nr and not one else None
+        dw = torch.empty_like(weight) if nw else None
+        d, lib, T = L.NormDesc(H, DTYPES[ctx.out], ROW_DTYPES[ctx.xt], ROW_DTYPES[rt], ROW_DTYPES[weight.dtype], ctx.eps,
+                               weight.data_ptr()), L.lib(), rows.shape[0]
+        ptr = lambda t: None if t is None else t.data_ptr()
+        need = lib.bmx_rms_norm_backward_workspace(d, T) if nw else 0
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        L.check(lib.bmx_rms_norm_backward(d, rows.data_ptr(), int(ctx.summed), T, g.data_ptr(), ptr(more), ptr(dx), ptr(dres), ptr(dw),
+                                          ptr(ws), need, s), "bmx_rms_norm_backward")
+        return dx if nx else None, (dx if one else dres) if nr else None, dw, None

@@ -7,6 +7,7 @@ import torch
 from . import _lib as L
 from ._lib import check, lib
 from .ffn import DTYPES, _modes, _tracing, eager_only, forward_ad, rows_of, stream_here
+from .q8 import Rows8, quantize_rows  # noqa: F401 (an operator of this module)
 
 
 def _stream():
@@ -86,6 +87,44 @@ def q4_linear(x, q):
         if rc:
             check(rc, "bmx_q4_linear")
     return y if x.dim() == 2 else y.view(x.shape[:-1] + (q.N,))
+
+
+def q8_linear(x, q):
+    """y [..., N] = x W^T for a Q8Matrix q: x [..., K] fp16 or bf16 on the matrix's device, quantized per token as by quantize_rows, or
+    Rows8. The products' sums are exact, each result is rounded to fp32 three times and once to y's type (x's, or the rows' dtype); a
+    token's results do not depend on the tokens beside it. Enqueued on the current stream of that device."""
+    device = q.device
+    rows = r = None
+    if type(x) is Rows8:
+        rows, dtype = x, x.dtype
+        if x.K != q.K or x.device != device:
+            raise ValueError(f"q8_linear: expected rows of {q.K} codes on {device}, got {x.K} on {x.device}")
+        if _tracing() or _modes():
+            eager_only("q8_linear")
+    else:
+        dtype = x.dtype
+        if dtype not in DTYPES:
+            raise ValueError(f"q8_linear: x must be fp16, bf16 or Rows8, got {dtype}")
+        if x.requires_grad and torch.is_grad_enabled():
+            raise ValueError("q8_linear: 8-bit weights have no gradients (detach x, or torch.no_grad())")
+        if forward_ad._current_level >= 0 or _tracing() or _modes():
+            eager_only("q8_linear", x)
+        r = rows_of(x, q.K, dtype, device, "q8_linear: x")
+    s = stream_here(device)
+    if s is None:
+        with torch.cuda.device(device):
+            return q8_linear(x, q)
+    T = rows.N if r is None else r.shape[0]
+    y = torch.empty((T, q.N), dtype=dtype, device=device)
+    if T:
+        L_ = lib()
+        need = L_.bmx_q8_linear_workspace(q.struct, T)
+        ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        rc = L_.bmx_q8_linear(q.struct, DTYPES[dtype], None if r is None else r.data_ptr(), None if rows is None else rows.struct, T,
+                              y.data_ptr(), ws.data_ptr() if need else None, need, s)
+        if rc:
+            check(rc, "bmx_q8_linear")
+    return y if len(x.shape) == 2 else y.view(x.shape[:-1] + (q.N,))
 
 
 class RoutesBuf:

@@ -85,6 +85,14 @@ __global__ __launch_bounds__(256) void row_gate_k(const uint16_t* __restrict__ x
     if (lane == 0) out[t] = sigmoid_fixed(sum);
 }
 
+int launch_row_gate(const void* x, const void* v, int dtype, int n, int H, float* out, hipStream_t s)
+{
+    const uint16_t *xp = static_cast<const uint16_t*>(x), *vp = static_cast<const uint16_t*>(v);
+    if (dtype == BMX_DT_FP16) hipLaunchKernelGGL((row_gate_k<f16>), dim3((n + 3) / 4), dim3(256), 0, s, xp, vp, n, H, out);
+    else hipLaunchKernelGGL((row_gate_k<bf16>), dim3((n + 3) / 4), dim3(256), 0, s, xp, vp, n, H, out);
+    return check_launch("row_gate");
+}
+
 int launch_product(const GemmArgs& g, int dtype, int epi, hipStream_t s)
 {
     const TilePlan p = plan_for(g.M, g.N, g.K, epi == EPI_GU ? 2 : 1);
@@ -154,7 +162,6 @@ static int block_product(const FfnIn& d, const SkinnyArgs& base, int first, int 
     return launch_product(a, d.dtype, epi, s);
 }
 
-template <class T>
 static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add, const void* gate_vec, const bmx_ffn_saved* sv,
                        char* ws, hipStream_t s)
 {
@@ -172,9 +179,7 @@ static int ffn_forward(const FfnIn& d, const void* x, int n, void* y, float* add
     if (gate_vec)
     {
         float* scale = reinterpret_cast<float*>(ws + p.gate);
-        hipLaunchKernelGGL((row_gate_k<T>), dim3((n + 3) / 4), dim3(256), 0, s, static_cast<const uint16_t*>(x),
-                           static_cast<const uint16_t*>(gate_vec), n, d.H, scale);
-        if ((rc = check_launch("row_gate"))) return rc;
+        if ((rc = launch_row_gate(x, gate_vec, d.dtype, n, d.H, scale, s))) return rc;
         k.scale = scale;
     }
     // y = h Wd^T
@@ -317,8 +322,7 @@ static int forward_call(const char* fn, const Desc* desc, const void* x, int T, 
     if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(d, T).total, fn))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
-    return d.dtype == BMX_DT_FP16 ? ffn_forward<f16>(d, x, T, y, nullptr, nullptr, saved, ws, s)
-                                  : ffn_forward<bf16>(d, x, T, y, nullptr, nullptr, saved, ws, s);
+    return ffn_forward(d, x, T, y, nullptr, nullptr, saved, ws, s);
 }
 
 template <class Desc>
@@ -333,8 +337,7 @@ static int add_call(const char* fn, const Desc* desc, const void* x, int T, cons
     if ((rc = check_ws(workspace, workspace_bytes, ffn_plan(d, T).total, fn))) return rc;
     hipStream_t s = static_cast<hipStream_t>(stream);
     char* ws = static_cast<char*>(workspace);
-    return d.dtype == BMX_DT_FP16 ? ffn_forward<f16>(d, x, T, nullptr, out, gate_vec, nullptr, ws, s)
-                                  : ffn_forward<bf16>(d, x, T, nullptr, out, gate_vec, nullptr, ws, s);
+    return ffn_forward(d, x, T, nullptr, out, gate_vec, nullptr, ws, s);
 }
 
 __global__ __launch_bounds__(256) void zero16_k(u32x4* p, int64_t n)

@@ -1,0 +1,396 @@
+// Root-mean-square norm with the residual's addition: forward into 16 bits, 8-bit rows or both, and its gradients. With
+//   s = x + residual (fp32), r = s rounded to the stream's type, v = r (no residual: v = x),
+//   rstd = 1 / sqrt(mean(v^2) + eps), y = v w rstd
+// the norm is of the sum as the stream holds it, since that is what the next layers add to; y is rounded once. In 8 bits rstd drops
+// out of the codes: code = round(v w 127 / top), scale = top rstd / 127, top = max |v w| (rows8.hpp). Gradients from dy of y and
+// dr of r, g = dy w, c = mean(g v) rstd^2:
+//   dv = rstd (g - v c) + dr,  dx = dresidual = dv,  dw = sum over the rows of dy v rstd
+// (the rounding of s to r passes a gradient as it is). Everything is bound by the bytes of the rows: each is read once and kept in
+// registers, and rstd is computed again from them in the backward pass, which has to read v anyhow.
+#include "rows8.hpp"
+
+namespace bmx {
+
+struct NormArgs {
+    const void *x, *res, *w;        // w null: the rows as they are in 8 bits (quantize_rows), neither weight nor norm
+    void *r, *y;
+    int8_t* codes;
+    float* scale;
+    int64_t ld;                     // of codes
+    int kp;                         // ... columns to write: H up to a multiple of 16
+    int T, H;
+    int xt, rt, wt, yt;             // row types
+    float eps;
+};
+
+// A row by W of a workgroup's NW waves, CH chunks of 8 values a lane
+template <int NW, int W, int CH>
+__global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
+{
+    __shared__ float ssum[NW];
+    __shared__ uint32_t smax[NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
+    const int64_t t = (int64_t)blockIdx.x * (NW / W) + wave / W;
+    const bool on = t < p.T;
+    const int64_t row = (on ? t : p.T - 1) * p.H;
+    float v[CH][8], vw[CH][8];
+    Raw8 x[CH], res[CH], w[CH];
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+    {
+        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        if (h >= p.H) continue;
+        x[c] = load_raw8(p.x, p.xt, row + h);
+        if (p.res) res[c] = load_raw8(p.res, p.rt, row + h);
+        if (p.w) w[c] = load_raw8(p.w, p.wt, h);
+    }
+    float ssq = 0.0f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+    {
+        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        if (h >= p.H) continue;
+        to_f32(x[c], p.xt, v[c]);
+        if (p.res)
+        {
+            float a[8];
+            to_f32(res[c], p.rt, a);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[c][i] += a[i];
+            if (on) store8(p.r, p.rt, row + h, v[c]);
+        }
+        float b[8];
+        if (p.w) to_f32(w[c], p.wt, b);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+        {
+            ssq = __builtin_fmaf(v[c][i], v[c][i], ssq);
+            vw[c][i] = p.w ? v[c][i] * b[i] : v[c][i];
+            top = max(top, mag(vw[c][i]));
+        }
+    }
+    ssq = wave_sum(ssq);
+    if (p.codes) top = wave_max(top);
+    if (W > 1)
+    {
+        if (lane == 0) { ssum[wave] = ssq; smax[wave] = top; }
+        lds_barrier();
+        const int w0 = wave - part;
+        ssq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+        {
+            ssq += ssum[w0 + i];
+            top = max(top, smax[w0 + i]);
+        }
+    }
+    if (!on) return;
+    const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
+    const Top8 q = top8(top);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+    {
+        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        if (p.codes && h < p.kp)
+            *reinterpret_cast<u32x2*>(p.codes + t * p.ld + h) =
+                h < p.H ? u32x2{codes4(vw[c], q), codes4(vw[c] + 4, q)} : u32x2{0, 0};
+        if (p.y && h < p.H)
+        {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = vw[c][i] * rstd;
+            store8(p.y, p.yt, row + h, y);
+        }
+    }
+    if (p.codes && part == 0 && lane == 0) p.scale[t] = p.w ? q.scale * rstd : q.scale;
+}
+
+// Waves of a row: one where there are rows enough to fill the chip with them and a lane holds all of its values, else eight
+static int launch_norm(const NormArgs& a, hipStream_t s)
+{
+    const bool wave = a.T >= 2048;
+    if (a.H <= 2048 && wave) hipLaunchKernelGGL((norm_k<4, 1, 4>), dim3((a.T + 3) / 4), dim3(256), 0, s, a);
+    else if (a.H <= 4096) hipLaunchKernelGGL((norm_k<8, 8, 1>), dim3(a.T), dim3(512), 0, s, a);
+    else if (a.H <= 8192) hipLaunchKernelGGL((norm_k<8, 8, 2>), dim3(a.T), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((norm_k<8, 8, 8>), dim3(a.T), dim3(512), 0, s, a);
+    return check_launch("rms_norm");
+}
+
+// The same for any K and rows at any 2-byte boundary: a workgroup per row, read twice
+__global__ __launch_bounds__(512) void quantize_any_k(const NormArgs p)
+{
+    __shared__ uint32_t smax[8];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t t = blockIdx.x, row = t * p.H;
+    auto value = [&](int h) {
+        if (h >= p.H) return 0.0f;
+        return p.xt == ROW_F32 ? static_cast<const float*>(p.x)[row + h] : value16(p.xt, static_cast<const uint16_t*>(p.x)[row + h]);
+    };
+    uint32_t top = 0;
+    for (int h = threadIdx.x; h < p.H; h += 512) top = max(top, mag(value(h)));
+    top = wave_max(top);
+    if (lane == 0) smax[wave] = top;
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) top = max(top, smax[i]);
+    const Top8 q = top8(top);
+    for (int h = threadIdx.x * 4; h < p.kp; h += 2048)
+    {
+        const float v[4] = {value(h), value(h + 1), value(h + 2), value(h + 3)};
+        *reinterpret_cast<uint32_t*>(p.codes + t * p.ld + h) = codes4(v, q);
+    }
+    if (threadIdx.x == 0) p.scale[t] = q.scale;
+}
+
+int launch_quantize(const void* x, int type, const bmx_q8* out, hipStream_t s)
+{
+    NormArgs a = {};
+    a.x = x; a.xt = type; a.T = out->N; a.H = out->K;
+    a.codes = static_cast<int8_t*>(const_cast<void*>(out->codes));
+    a.scale = const_cast<float*>(out->scale);
+    a.ld = out->ld; a.kp = q8_columns(out->K);
+    if (a.H % 8 == 0 && a.H <= BMX_NORM_MAX_H && reinterpret_cast<uintptr_t>(x) % 16 == 0) return launch_norm(a, s);
+    hipLaunchKernelGGL(quantize_any_k, dim3(a.T), dim3(512), 0, s, a);
+    return check_launch("quantize");
+}
+
+// ---- gradients ----------------------------------------------------------------------------------------------------------
+
+struct NormBackArgs {
+    const void *v, *w, *dy, *dr;    // dr null: no gradient of r
+    void *dx, *dres;                // null: not wanted
+    float* part;                    // [workgroup][H], null: the weight's gradient is not wanted
+    int T, H;
+    int vt, wt, yt, rt, xt;         // row types: v, w, dy, dr and dres, dx
+    float eps;
+};
+
+// A workgroup takes every gridDim.x-th row, the next row's loads on their way while one is summed up, and keeps its rows' sums for the
+// weight's gradient in registers
+template <int NW, int CH>
+__global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
+{
+    __shared__ f32x4 red[2][NW];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    float w[CH][8], dw[CH][8];
+    Raw8 v[CH], dy[CH], dr[CH];
+    auto at = [&](int c) { return (wave * 64 + lane + c * (NW * 64)) * 8; };
+    auto load = [&](int t) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+        {
+            const int64_t i = (int64_t)t * p.H + at(c);
+            if (at(c) >= p.H) continue;
+            v[c] = load_raw8(p.v, p.vt, i);
+            dy[c] = load_raw8(p.dy, p.yt, i);
+            if (p.dr) dr[c] = load_raw8(p.dr, p.rt, i);
+        }
+    };
+    int t = blockIdx.x;
+    load(t);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+    {
+        if (at(c) < p.H) to_f32(load_raw8(p.w, p.wt, at(c)), p.wt, w[c]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
+    }
+    for (int set = 0; t < p.T; t += gridDim.x, set ^= 1)
+    {
+        float a[CH][8], d[CH][8], more[CH][8];
+        float ssq = 0.0f, dot = 0.0f;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+        {
+            if (at(c) >= p.H) continue;
+            to_f32(v[c], p.vt, a[c]);
+            to_f32(dy[c], p.yt, d[c]);
+            if (p.dr) to_f32(dr[c], p.rt, more[c]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                ssq = __builtin_fmaf(a[c][i], a[c][i], ssq);
+                dot = __builtin_fmaf(d[c][i] * w[c][i], a[c][i], dot);
+            }
+        }
+        if (t + (int)gridDim.x < p.T) load(t + gridDim.x);
+        ssq = wave_sum(ssq);
+        dot = wave_sum(dot);
+        if (lane == 0) red[set][wave] = f32x4{ssq, dot, 0.0f, 0.0f};
+        lds_barrier();
+        ssq = dot = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NW; ++i)
+        {
+            const f32x4 one = red[set][i];
+            ssq += one[0];
+            dot += one[1];
+        }
+        const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
+        const float k = __fdiv_rn(dot, (float)p.H) * rstd * rstd;
+#pragma unroll
+        for (int c = 0; c < CH; ++c)
+        {
+            if (at(c) >= p.H) continue;
+            const int64_t at_row = (int64_t)t * p.H + at(c);
+            float o[8], q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+            {
+                o[i] = rstd * (d[c][i] * w[c][i] - a[c][i] * k);
+                if (p.dr) o[i] += more[c][i];
+                q[i] = o[i];
+                dw[c][i] = __builtin_fmaf(d[c][i], a[c][i] * rstd, dw[c][i]);
+            }
+            if (p.dx) store8(p.dx, p.xt, at_row, o);
+            if (p.dres) store8(p.dres, p.rt, at_row, q);
+        }
+    }
+    if (!p.part) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+        if (at(c) < p.H) store8(p.part + (int64_t)blockIdx.x * p.H, ROW_F32, at(c), dw[c]);
+}
+
+// dw: the workgroups' sums of 32 columns, every 64th by a group of 8 lanes, then the groups' in their order
+__global__ __launch_bounds__(512) void norm_weight_k(const float* __restrict__ part, int groups, int H, void* __restrict__ dw, int wt)
+{
+    __shared__ f32x4 red[64][8];
+    const int q = threadIdx.x & 7, g = threadIdx.x >> 3, h = blockIdx.x * 32 + q * 4;
+    f32x4 s = {0, 0, 0, 0};
+    if (h < H)
+#pragma unroll 4
+        for (int i = g; i < groups; i += 64)
+        {
+            const f32x4 v = ldg4f(part + (int64_t)i * H + h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[e] += v[e];
+        }
+    red[g][q] = s;
+    __syncthreads();
+    if (threadIdx.x >= 32) return;
+    const int c = blockIdx.x * 32 + threadIdx.x;
+    if (c >= H) return;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) sum += red[i][threadIdx.x >> 2][threadIdx.x & 3];
+    if (wt == ROW_F32) static_cast<float*>(dw)[c] = sum;
+    else static_cast<uint16_t*>(dw)[c] = (uint16_t)bits16(wt, sum);
+}
+
+constexpr int NORM_BACK_WG = 512;   // workgroups of a backward pass, two on each compute unit
+
+static int norm_back_groups(int T) { return T < NORM_BACK_WG ? T : NORM_BACK_WG; }
+
+static int launch_norm_back(const NormBackArgs& a, hipStream_t s)
+{
+    const dim3 grid(norm_back_groups(a.T));
+    if (a.H <= 4096) hipLaunchKernelGGL((norm_back_k<8, 1>), grid, dim3(512), 0, s, a);
+    else if (a.H <= 8192) hipLaunchKernelGGL((norm_back_k<8, 2>), grid, dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((norm_back_k<8, 8>), grid, dim3(512), 0, s, a);
+    return check_launch("rms_norm_backward");
+}
+
+// ---- argument checks ----------------------------------------------------------------------------------------------------
+
+static bool odd16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; }
+static bool is16(int t) { return t == BMX_DT_FP16 || t == BMX_DT_BF16; }
+
+static int check_norm(const bmx_norm_desc* d, int T, const char* who)
+{
+    if (!d) return set_error(BMX_ERR_ARG, "%s: null descriptor", who);
+    if (d->H <= 0 || d->H % 8 || d->H > BMX_NORM_MAX_H)
+        return set_error(BMX_ERR_ARG, "%s: H (%d) must be a positive multiple of 8, at most %d", who, d->H, BMX_NORM_MAX_H);
+    if (!is16(d->dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", who, d->dtype);
+    for (int t : {d->x_dtype, d->residual_dtype, d->weight_dtype})
+        if (t != d->dtype && t != BMX_DT_FP32)
+            return set_error(BMX_ERR_ARG, "%s: x, residual and weight must be of dtype or fp32, got %d beside %d", who, t, d->dtype);
+    if (!(d->eps > 0.0f)) return set_error(BMX_ERR_ARG, "%s: eps must be positive", who);
+    if (!d->weight || odd16(d->weight)) return set_error(BMX_ERR_ARG, "%s: weight null or not 16-byte aligned", who);
+    if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", who, T);
+    return BMX_OK;
+}
+
+// zeros for the weight's gradient of no rows
+__global__ __launch_bounds__(256) void norm_zero_k(uint32_t* p, int n)
+{
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 0;
+}
+
+}  // namespace bmx
+
+using namespace bmx;
+
+extern "C" {
+
+int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual, int T, void* sum, void* y, const bmx_q8* rows,
+                 bmx_stream_t stream)
+{
+    const char* fn = "bmx_rms_norm";
+    int rc = check_norm(desc, T, fn);
+    if (rc) return rc;
+    if (rows && (rc = check_rows8(rows, T, desc->H, fn))) return rc;
+    if (T == 0) return BMX_OK;
+    if (!x || odd16(x) || odd16(residual) || odd16(sum) || odd16(y))
+        return set_error(BMX_ERR_ARG, "%s: x null, or x, residual, sum or y not 16-byte aligned", fn);
+    if (!residual != !sum) return set_error(BMX_ERR_ARG, "%s: a residual and its sum go together", fn);
+    if (!y && !rows) return set_error(BMX_ERR_ARG, "%s: neither y nor rows is wanted", fn);
+    NormArgs a = {};
+    a.x = x; a.res = residual; a.w = desc->weight; a.r = sum; a.y = y;
+    if (rows)
+    {
+        a.codes = static_cast<int8_t*>(const_cast<void*>(rows->codes));
+        a.scale = const_cast<float*>(rows->scale);
+        a.ld = rows->ld; a.kp = q8_columns(rows->K);
+    }
+    a.T = T; a.H = desc->H;
+    a.xt = desc->x_dtype; a.rt = desc->residual_dtype; a.wt = desc->weight_dtype; a.yt = desc->dtype;
+    a.eps = desc->eps;
+    return launch_norm(a, static_cast<hipStream_t>(stream));
+}
+
+size_t bmx_rms_norm_backward_workspace(const bmx_norm_desc* desc, int T)
+{
+    if (check_norm(desc, T, "bmx_rms_norm_backward_workspace")) return 0;
+    return align_up((size_t)(T ? norm_back_groups(T) : 1) * desc->H * 4, 256);
+}
+
+int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, int T, const void* dy, const void* dr, void* dx,
+                          void* dresidual, void* dweight, void* workspace, size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_rms_norm_backward";
+    int rc = check_norm(desc, T, fn);
+    if (rc) return rc;
+    if (odd16(dweight) || odd16(dx) || odd16(dresidual)) return set_error(BMX_ERR_ARG, "%s: gradients must be 16-byte aligned", fn);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    if (T == 0)
+    {
+        if (!dweight) return BMX_OK;
+        const int n = desc->weight_dtype == BMX_DT_FP32 ? desc->H : desc->H / 2;
+        hipLaunchKernelGGL(norm_zero_k, dim3((n + 255) / 256), dim3(256), 0, s, static_cast<uint32_t*>(dweight), n);
+        return check_launch(fn);
+    }
+    if (!v || !dy || odd16(v) || odd16(dy) || odd16(dr)) return set_error(BMX_ERR_ARG, "%s: v or dy null, or v, dy or dr not 16-byte aligned", fn);
+    if (!summed && (dr || dresidual)) return set_error(BMX_ERR_ARG, "%s: gradients of a residual that was not there", fn);
+    if (!dx && !dresidual && !dweight) return BMX_OK;
+    if (dweight)
+    {
+        const size_t need = bmx_rms_norm_backward_workspace(desc, T);
+        if (!workspace || odd16(workspace)) return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", fn);
+        if (workspace_bytes < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", fn, workspace_bytes, need);
+    }
+    NormBackArgs a = {};
+    a.v = v; a.w = desc->weight; a.dy = dy; a.dr = dr; a.dx = dx; a.dres = dresidual;
+    a.part = dweight ? static_cast<float*>(workspace) : nullptr;
+    a.T = T; a.H = desc->H;
+    a.vt = summed ? desc->residual_dtype : desc->x_dtype;
+    a.wt = desc->weight_dtype; a.yt = desc->dtype; a.rt = desc->residual_dtype; a.xt = desc->x_dtype;
+    a.eps = desc->eps;
+    if ((rc = launch_norm_back(a, s)) || !dweight) return rc;
+    hipLaunchKernelGGL(norm_weight_k, dim3((desc->H + 31) / 32), dim3(512), 0, s, a.part, norm_back_groups(T), desc->H, dweight,
+                       desc->weight_dtype);
+    return check_launch("norm_weight");
+}
+
+}  // extern "C"

@@ -202,6 +202,17 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
     return us * 1.15 < std::max(q4_many_us(N, K, at, products, group, keep), least) ? FEW_DIRECT : MANY;
 }
 
+// ---- 8-bit weights ------------------------------------------------------------------------------------------------------
+
+constexpr int Q8_K = 128;   // columns of a K tile (gemm8_k): as many bytes as gemm16_k's 64, and as much time
+
+// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, else gemm8_k's tiles
+inline bool q8_few(int T) { return T <= 16; }
+inline TilePlan q8_plan(int N, int K, int T, int products)
+{
+    return plan_product((int64_t)N * products, T, (K + Q8_K - 1) / Q8_K, 1, true);
+}
+
 inline int padded(int n) { return (n + 7) / 8 * 8; }
 inline int slices_of(int K) { return (K + SL_K - 1) / SL_K; }
 
@@ -251,6 +262,14 @@ inline size_t product_bytes(int N, int K, int T, int products, int group, bool k
 {
     if (product_path(N, K, T, products, group, keep) != MANY) return skinny_part_bytes(N, K, T, products, group);
     return group ? q4_many_bytes(N, K, T, products, group, keep) : product_part_bytes(N, T, K, products);
+}
+
+// Partial sums of a product in 8 bits
+inline size_t q8_part_bytes(int N, int K, int T, int products)
+{
+    if (q8_few(T)) return 0;
+    const TilePlan p = q8_plan(N, K, T, products);
+    return p.splits > 1 ? (size_t)p.splits * products * T * padded(N) * 4 : 0;
 }
 
 }  // namespace bmx

@@ -1,0 +1,327 @@
+// 8-bit matrices: decoding, the launches of their products (skinny8_k, gemm8_k, planned in product_plan.hpp), single products and the
+// gated feed-forward block on them.
+#include <algorithm>
+
+#include "q8_gemm.hpp"
+
+namespace bmx {
+
+static bool odd16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16; }
+static bool is16(int t) { return t == BMX_DT_FP16 || t == BMX_DT_BF16; }
+
+int check_q8(const bmx_q8* q, const char* who)
+{
+    if (!q) return set_error(BMX_ERR_ARG, "%s: null matrix", who);
+    if (q->N <= 0 || q->N > (1 << 24) || q->K <= 0 || q->K > 131071)
+        return set_error(BMX_ERR_ARG, "%s: N (%d) must be in [1, 2^24], K (%d) in [1, 131071]", who, q->N, q->K);
+    if (q->ld % 16 || q->ld < q8_columns(q->K) || q->ld > (1 << 20))
+        return set_error(BMX_ERR_ARG, "%s: ld (%lld) must be a multiple of 16 from K (%d) up, at most 2^20", who, (long long)q->ld, q->K);
+    if (!q->codes || !q->scale) return set_error(BMX_ERR_ARG, "%s: null codes or scale", who);
+    if (odd16(q->codes) || reinterpret_cast<uintptr_t>(q->scale) % 4)
+        return set_error(BMX_ERR_ARG, "%s: codes must be 16-byte, scale 4-byte aligned", who);
+    return BMX_OK;
+}
+
+int check_rows8(const bmx_q8* rows, int T, int K, const char* who)
+{
+    if (T == 0 && rows) return BMX_OK;
+    if (const int rc = check_q8(rows, who)) return rc;
+    if (rows->N != T || rows->K != K)
+        return set_error(BMX_ERR_ARG, "%s: rows must be %d of %d codes, got %d of %d", who, T, K, rows->N, rows->K);
+    return BMX_OK;
+}
+
+// v = scale code; 16 codes a thread
+__global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int64_t ld, int K,
+                                                    int type, void* __restrict__ out, int64_t pieces)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int per = (K + 15) / 16;
+    const int64_t n = i / per;
+    const int k = (int)(i % per) * 16;
+    const u32x4 c = ldg4(codes + n * ld + k);
+    const float s = scale[n];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+    {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = s * (float)(int8_t)(c[h * 2 + e / 4] >> (8 * (e % 4)));
+        const int64_t o = n * K + k + h * 8;
+        if (K % 8 == 0)
+        {
+            if (k + h * 8 < K) store8(out, type, o, v);
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (k + h * 8 + e < K)
+            {
+                if (type == ROW_F32) static_cast<float*>(out)[o + e] = v[e];
+                else static_cast<uint16_t*>(out)[o + e] = (uint16_t)bits16(type, v[e]);
+            }
+    }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+
+template <bool FUSED, int RT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
+{
+    constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT;
+    const int64_t rows = (a.N + ROWS - 1) / ROWS, blocks = a.T <= 16 ? rows : (rows + 7) / 8 * 8 * ((a.T + 15) / 16);
+    hipLaunchKernelGGL((skinny8_k<FUSED, RT, EPI>), dim3((unsigned)blocks), dim3(S8_W * 64), FUSED ? skinny8_lds(a.T, a.K) : 0, s, a);
+    return check_launch("skinny8");
+}
+
+template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
+{
+    const int bm = EPI == EPI_GU ? TILES[tile].M / 2 : TILES[tile].M;
+    a.tm = (a.N + bm - 1) / bm;
+    a.tn = (a.T + TILES[tile].N - 1) / TILES[tile].N;
+    const dim3 grid((unsigned)(a.tm * a.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * (a.w[1] ? 2 : 1) : 1));
+    switch (tile)
+    {
+        case 0: hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 2, EPI>), grid, dim3(512), 0, s, a); break;
+        case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 2, EPI>), grid, dim3(256), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 3, EPI>), grid, dim3(512), 0, s, a); break;
+        default: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 2, EPI>), grid, dim3(512), 0, s, a);
+    }
+    return check_launch("gemm8");
+}
+
+// A product with one matrix (EPI_STORE, EPI_ADD) or two (EPI_GU, a.w[1]); a.part: q8_part_bytes
+template <int EPI> static int product8(const Q8Args& base, hipStream_t s)
+{
+    Q8Args a = base;
+    if (q8_few(a.T)) return a.xc ? skinny8_rows<false, 1, EPI>(a, s) : skinny8_rows<true, 1, EPI>(a, s);
+    const TilePlan tp = q8_plan(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1);
+    if (tp.splits == 1)
+    {
+        ProductPart part[2];
+        const int n = product_parts(tp, a.N, EPI == EPI_GU ? 2 : 1, part);
+        for (int i = 0; i < n; ++i)
+        {
+            Q8Args g = a;
+            g.from = part[i].from;
+            g.N = part[i].rows;
+            if (const int rc = gemm8_tiles<EPI>(g, part[i].tile, s)) return rc;
+        }
+        return BMX_OK;
+    }
+    a.splits = tp.splits;
+    a.ldp = padded(a.N);
+    if (const int rc = gemm8_tiles<EPI_PART>(a, tp.tile, s)) return rc;
+    const int64_t pieces = (int64_t)a.ldp / 8 * a.T;
+    hipLaunchKernelGGL((finish8_k<EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a);
+    return check_launch("finish8");
+}
+
+// Tokens of a product: codes already (rows), or to be quantized by the product's workgroups themselves, or into ws first
+struct Tokens {
+    const void* x;
+    int type;
+    const bmx_q8* rows;
+};
+
+static bool fused8(const Tokens& in, int T, int K) { return !in.rows && q8_few(T) && skinny8_fused(T, K); }
+static size_t rows8_bytes(int T, int K) { return align_up((size_t)T * q8_columns(K), 256) + align_up((size_t)T * 4, 256); }
+
+static int take_tokens(const Tokens& in, int T, int K, char* ws, Q8Args& a, hipStream_t s)
+{
+    a.T = T;
+    a.K = K;
+    a.x = nullptr;
+    a.xc = nullptr;
+    if (fused8(in, T, K))
+    {
+        a.x = in.x;
+        a.xt = in.type;
+        return BMX_OK;
+    }
+    bmx_q8 q = {T, K, q8_columns(K), ws, reinterpret_cast<float*>(ws + align_up((size_t)T * q8_columns(K), 256))};
+    if (in.rows) q = *in.rows;
+    a.xc = static_cast<const int8_t*>(q.codes);
+    a.sx = q.scale;
+    a.ldx = q.ld;
+    return in.rows ? BMX_OK : launch_quantize(in.x, in.type, &q, s);
+}
+
+static void put_matrix(Q8Args& a, int m, const bmx_q8* w)
+{
+    a.w[m] = static_cast<const int8_t*>(w->codes);
+    a.sw[m] = w->scale;
+    a.ldw = w->ld;
+}
+
+static size_t linear8_ws(const bmx_q8* w, int T, bool rows)
+{
+    const size_t r = rows || (q8_few(T) && skinny8_fused(T, w->K)) ? 0 : rows8_bytes(T, w->K), p = q8_part_bytes(w->N, w->K, T, 1);
+    return r + p;
+}
+
+static int check_ws(const void* ws, size_t have, size_t need, const char* who)
+{
+    if (need && (!ws || odd16(ws))) return set_error(BMX_ERR_ARG, "%s: workspace null or not 16-byte aligned", who);
+    if (have < need) return set_error(BMX_ERR_WORKSPACE, "%s: workspace %zu < %zu", who, have, need);
+    return BMX_OK;
+}
+
+// ---- the block ----------------------------------------------------------------------------------------------------------
+
+struct Ffn8Plan { size_t h, gate, rows, part, total; };
+
+static Ffn8Plan ffn8_plan(const bmx_ffn8_desc* d, int T)
+{
+    Ffn8Plan p;
+    size_t o = 0;
+    auto take = [&](size_t b) { const size_t at = o; o += align_up(b, 256); return at; };
+    const int H = d->gate->K, I = d->gate->N;
+    p.h = take((size_t)T * I * 4);
+    p.gate = take((size_t)T * 4);
+    p.rows = take(std::max(rows8_bytes(T, H), rows8_bytes(T, I)));       // x's, then h's
+    p.part = take(std::max(q8_part_bytes(I, H, T, 2), q8_part_bytes(H, I, T, 1)));
+    p.total = o + 256;
+    return p;
+}
+
+static int ffn8_call(const bmx_ffn8_desc* d, const void* x, const bmx_q8* rows, int T, void* y, float* add, const void* gate_vec,
+                     char* ws, hipStream_t s)
+{
+    const Ffn8Plan p = ffn8_plan(d, T);
+    const int H = d->gate->K, I = d->gate->N;
+    Q8Args a = {};
+    a.act = act_par(d->act, d->act_limit);
+    a.part = reinterpret_cast<int*>(ws + p.part);
+    int rc = take_tokens({x, d->dtype, rows}, T, H, ws + p.rows, a, s);
+    if (rc) return rc;
+    put_matrix(a, 0, d->gate);
+    a.w[1] = static_cast<const int8_t*>(d->up->codes);
+    a.sw[1] = d->up->scale;
+    a.N = a.ldo = I;
+    a.out = ws + p.h;
+    if ((rc = product8<EPI_GU>(a, s))) return rc;
+    if (gate_vec)
+    {
+        a.scale = reinterpret_cast<float*>(ws + p.gate);
+        if ((rc = launch_row_gate(x, gate_vec, d->dtype, T, H, reinterpret_cast<float*>(ws + p.gate), s))) return rc;
+    }
+    if ((rc = take_tokens({ws + p.h, BMX_DT_FP32, nullptr}, T, I, ws + p.rows, a, s))) return rc;
+    put_matrix(a, 0, d->down);
+    a.w[1] = nullptr;
+    a.N = a.ldo = H;
+    a.ot = d->dtype;
+    a.out = add ? static_cast<void*>(add) : y;
+    return add ? product8<EPI_ADD>(a, s) : product8<EPI_STORE>(a, s);
+}
+
+static int check_ffn8(const bmx_ffn8_desc* d, int T, const char* who)
+{
+    if (!d) return set_error(BMX_ERR_ARG, "%s: null descriptor", who);
+    for (const bmx_q8* q : {d->gate, d->up, d->down})
+        if (const int rc = check_q8(q, who)) return rc;
+    const int H = d->gate->K, I = d->gate->N;
+    if (d->up->K != H || d->up->N != I || d->down->K != I || d->down->N != H || d->up->ld != d->gate->ld)
+        return set_error(BMX_ERR_ARG, "%s: gate and up must be [I, H] with rows of one length, down [H, I]", who);
+    if (H % 8 || I % 8) return set_error(BMX_ERR_ARG, "%s: H (%d) and I (%d) must be multiples of 8", who, H, I);
+    if (!is16(d->dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", who, d->dtype);
+    if (d->act < BMX_ACT_SILU || d->act > BMX_ACT_SILU_OAI) return set_error(BMX_ERR_ARG, "%s: unknown activation %d", who, d->act);
+    if (!(d->act_limit >= 0.0f)) return set_error(BMX_ERR_ARG, "%s: act_limit must be 0 (off) or positive", who);
+    if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", who, T);
+    return BMX_OK;
+}
+
+static int ffn8_entry(const char* fn, const bmx_ffn8_desc* d, const void* x, const bmx_q8* rows, int T, void* y, float* add,
+                      const void* gate_vec, void* workspace, size_t workspace_bytes, bmx_stream_t stream)
+{
+    int rc = check_ffn8(d, T, fn);
+    if (rc) return rc;
+    if (rows && (rc = check_rows8(rows, T, d->gate->K, fn))) return rc;
+    if (T == 0) return BMX_OK;
+    const void* out = add ? static_cast<const void*>(add) : y;
+    if (!out || odd16(out) || odd16(x) || odd16(gate_vec))
+        return set_error(BMX_ERR_ARG, "%s: output null, or it, x or gate_vec not 16-byte aligned", fn);
+    if (!x && (!rows || gate_vec)) return set_error(BMX_ERR_ARG, "%s: x is null, and needed without rows and for gate_vec", fn);
+    if ((rc = check_ws(workspace, workspace_bytes, ffn8_plan(d, T).total, fn))) return rc;
+    return ffn8_call(d, x, rows, T, y, add, gate_vec, static_cast<char*>(workspace), static_cast<hipStream_t>(stream));
+}
+
+}  // namespace bmx
+
+using namespace bmx;
+
+extern "C" {
+
+int bmx_q8_quantize(const void* x, int dtype, const bmx_q8* out, bmx_stream_t stream)
+{
+    const char* fn = "bmx_q8_quantize";
+    if (const int rc = check_q8(out, fn)) return rc;
+    if (!is16(dtype) && dtype != BMX_DT_FP32) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    if (!x || reinterpret_cast<uintptr_t>(x) % row_type_bytes(dtype)) return set_error(BMX_ERR_ARG, "%s: x null or not aligned", fn);
+    return launch_quantize(x, dtype, out, static_cast<hipStream_t>(stream));
+}
+
+int bmx_q8_dequant(const bmx_q8* q, int dtype, void* out, bmx_stream_t stream)
+{
+    const char* fn = "bmx_q8_dequant";
+    if (const int rc = check_q8(q, fn)) return rc;
+    if (!is16(dtype) && dtype != BMX_DT_FP32) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    if (!out || odd16(out)) return set_error(BMX_ERR_ARG, "%s: out null or not 16-byte aligned", fn);
+    const int64_t pieces = (int64_t)q->N * ((q->K + 15) / 16), blocks = (pieces + 255) / 256;
+    if (blocks > (1 << 23)) return set_error(BMX_ERR_ARG, "%s: %d x %d values are too many for one call", fn, q->N, q->K);
+    hipLaunchKernelGGL(q8_dequant_k, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const int8_t*>(q->codes), q->scale, q->ld, q->K, dtype, out, pieces);
+    return check_launch(fn);
+}
+
+size_t bmx_q8_linear_workspace(const bmx_q8* w, int T)
+{
+    if (check_q8(w, "bmx_q8_linear_workspace") || T < 0 || T > (1 << 24)) return 0;
+    return linear8_ws(w, T, false);
+}
+
+int bmx_q8_linear(const bmx_q8* w, int dtype, const void* x, const bmx_q8* rows, int T, void* y, void* workspace,
+                  size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_q8_linear";
+    int rc = check_q8(w, fn);
+    if (rc) return rc;
+    if (!is16(dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
+    if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", fn, T);
+    if (rows && (rc = check_rows8(rows, T, w->K, fn))) return rc;
+    if (T == 0) return BMX_OK;
+    if (!x == !rows) return set_error(BMX_ERR_ARG, "%s: x or rows, one of them", fn);
+    if (!y || odd16(y) || odd16(x)) return set_error(BMX_ERR_ARG, "%s: y null, or x or y not 16-byte aligned", fn);
+    if ((rc = check_ws(workspace, workspace_bytes, linear8_ws(w, T, rows), fn))) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    char* ws = static_cast<char*>(workspace);
+    Q8Args a = {};
+    if ((rc = take_tokens({x, dtype, rows}, T, w->K, ws, a, s))) return rc;
+    put_matrix(a, 0, w);
+    a.N = a.ldo = w->N;
+    a.out = y;
+    a.ot = dtype;
+    a.part = reinterpret_cast<int*>(ws + (a.xc && !rows ? rows8_bytes(T, w->K) : 0));
+    return product8<EPI_STORE>(a, s);
+}
+
+size_t bmx_ffn8_workspace(const bmx_ffn8_desc* desc, int T)
+{
+    return check_ffn8(desc, T, "bmx_ffn8_workspace") ? 0 : ffn8_plan(desc, T).total;
+}
+
+int bmx_ffn8_forward(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, int T, void* y, void* workspace,
+                     size_t workspace_bytes, bmx_stream_t stream)
+{
+    return ffn8_entry("bmx_ffn8_forward", desc, x, rows, T, y, nullptr, nullptr, workspace, workspace_bytes, stream);
+}
+
+int bmx_ffn8_add(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, int T, const void* gate_vec, float* out,
+                 void* workspace, size_t workspace_bytes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_ffn8_add";
+    if (T > 0 && !out) return set_error(BMX_ERR_ARG, "%s: out is null", fn);
+    return ffn8_entry(fn, desc, x, rows, T, nullptr, out, gate_vec, workspace, workspace_bytes, stream);
+}
+
+}  // extern "C"

@@ -470,7 +470,7 @@ int bmx_combine(const float* y_rows, const int32_t* inv, const void* w_fp16, con
  * bmx_q4_code_bytes bytes, scale 2 and zero 1 byte for each of bmx_q4_group_count values, written by bmx_q4_pack from a
  * checkpoint's order: codes [N][K / 2] with the even column in a byte's low half, scale and zero [N][K / group]. Device
  * memory, 16-byte aligned. */
-enum bmx_dtype { BMX_DT_FP16 = 0, BMX_DT_BF16 = 1 };
+enum bmx_dtype { BMX_DT_FP16 = 0, BMX_DT_BF16 = 1, BMX_DT_FP32 = 2 /* where a call says so */ };
 typedef struct bmx_q4 {
     int32_t N, K, group, scale_dtype;
     const void *codes, *scale, *zero;
@@ -537,6 +537,67 @@ int bmx_ffn4_add(const bmx_ffn4_desc* desc, const void* x, int T, const void* ga
  * dtype before the products that use it. T = 0: the wanted weight gradients are zeroed. */
 int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_ffn_saved* saved, const void* dy, void* dx,
                      void* dgate, void* dup, void* ddown, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* ---- 8-bit matrices and rows ----
+ * N rows of K whole numbers with a scale each, v[n][k] = scale[n] code[n][k], the form of 8-bit weights with a scale per output
+ * channel (bmx_q8 as a matrix) and of activations with a scale per token (as rows, N tokens). codes int8 [N][ld], ld a multiple of
+ * 16, columns from K up to the next multiple of 16 zeros (read, so they have to be), those behind never read; scale fp32 [N].
+ * Device memory, codes 16-byte aligned. N to 2^24, K to 131,071 (so that a sum of products fits 32 bits whatever the codes). */
+typedef struct bmx_q8 {
+    int32_t N, K;
+    int64_t ld;
+    const void* codes;
+    const float* scale;
+} bmx_q8;
+/* Rows x [out->N][out->K] of dtype (fp32 too), contiguous, into out's codes and scales: top = the row's largest magnitude, code =
+ * round(x 127 / top), scale = top / 127. A row whose magnitudes are all below 2^-110 becomes zeros (codes and scale); one with an
+ * infinity or a NaN codes 0 and scale NaN: every product with it is NaN. */
+int bmx_q8_quantize(const void* x, int dtype, const bmx_q8* out, bmx_stream_t stream);
+/* out [N][K] of dtype (fp32 too), contiguous: each value rounded once. */
+int bmx_q8_dequant(const bmx_q8* q, int dtype, void* out, bmx_stream_t stream);
+/* y [T][N] = x W^T of dtype (fp16 or bf16), 16-byte aligned: y[t][n] = sx[t] scale[n] sum_k code_x code_w, the sum exact, then fp32,
+ * rounded once. The tokens are x [T][K] of dtype, contiguous and 16-byte aligned, quantized as by bmx_q8_quantize; or rows of W's K
+ * (rows->N = T), x NULL. A token's result does not depend on the tokens beside it. The workspace is that of a call of T tokens. */
+size_t bmx_q8_linear_workspace(const bmx_q8* w, int T);
+int bmx_q8_linear(const bmx_q8* w, int dtype, const void* x, const bmx_q8* rows, int T, void* y, void* workspace,
+                  size_t workspace_bytes, bmx_stream_t stream);
+
+/* The gated feed-forward block (bmx_ffn_desc's formulas) on three 8-bit matrices (host pointers; gate, up [I, H], down [H, I], H and
+ * I multiples of 8): forward only. x of dtype, or rows of x (x NULL) as above; g, u and h are fp32, h is quantized per token. */
+typedef struct bmx_ffn8_desc {
+    int32_t dtype, act;
+    float act_limit;
+    int32_t reserved;
+    const bmx_q8 *gate, *up, *down;
+} bmx_ffn8_desc;
+size_t bmx_ffn8_workspace(const bmx_ffn8_desc* desc, int T);
+int bmx_ffn8_forward(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, int T, void* y, void* workspace,
+                     size_t workspace_bytes, bmx_stream_t stream);
+/* out[t] += s_t y[t], as bmx_ffn_add: y is not rounded. With rows the products take those; gate_vec is multiplied with x, which is
+ * then needed too. */
+int bmx_ffn8_add(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, int T, const void* gate_vec, float* out,
+                 void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* ---- root-mean-square norm with the residual's addition ----
+ * With a residual: sum = x + residual in fp32, rounded to residual's type, and v = sum; without: v = x. y = v w / sqrt(mean(v^2) +
+ * eps), rounded once to dtype; rows: the same in 8 bits with a scale per token (rows->N = T, K = H), not through y: code = round(v w
+ * 127 / max |v w|). x, residual and the weight [H] of dtype or fp32, contiguous, 16-byte aligned; H a multiple of 8. sum may be
+ * residual or x, if of its type; y apart from all but x. sum goes with residual; y or rows may be NULL. */
+#define BMX_NORM_MAX_H 32768
+typedef struct bmx_norm_desc {
+    int32_t H, dtype;                              /* dtype: fp16 or bf16 */
+    int32_t x_dtype, residual_dtype, weight_dtype;
+    float eps;
+    const void* weight;                            /* device */
+} bmx_norm_desc;
+int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual, int T, void* sum, void* y, const bmx_q8* rows,
+                 bmx_stream_t stream);
+/* Gradients from v (a forward pass's sum when summed, else its x), dy [T, H] of dtype and dr [T, H] of residual_dtype (the gradient
+ * of sum; NULL: none): dx, dresidual (of x's and residual's type: the same values) and dweight [H] (of the weight's), each NULL when
+ * not wanted. The workspace is for dweight. T = 0: dweight is zeroed. */
+size_t bmx_rms_norm_backward_workspace(const bmx_norm_desc* desc, int T);
+int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, int T, const void* dy, const void* dr, void* dx,
+                          void* dresidual, void* dweight, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
 
 #ifdef __cplusplus
 }
