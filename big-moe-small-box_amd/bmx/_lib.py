@@ -77,7 +77,7 @@ class Ffn4Desc(ctypes.Structure):
 
 
 class Q8(ctypes.Structure):
-    _fields_ = [("N", ctypes.c_int32), ("K", ctypes.c_int32), ("ld", ctypes.c_int64), ("codes", _P), ("scale", _P)]
+    _fields_ = [("N", ctypes.c_int32), ("K", ctypes.c_int32), ("codes", _P), ("scale", _P)]
 
 
 class Ffn8Desc(ctypes.Structure):
@@ -168,6 +168,9 @@ SIGNATURES = {
     "bmx_ffn_forward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, ctypes.POINTER(FfnSaved), _P, _SZ, _P]),
     "bmx_ffn_add": (_I, [ctypes.POINTER(FfnDesc), _P, _I, _P, _P, _P, _SZ, _P]),
     "bmx_ffn_backward": (_I, [ctypes.POINTER(FfnDesc), _P, _I, ctypes.POINTER(FfnSaved), _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "bmx_q8_code_bytes": (_SZ, [_I, _I]),
+    "bmx_q8_pack": (_I, [ctypes.POINTER(Q8), _P, _P]),
+    "bmx_q8_unpack": (_I, [ctypes.POINTER(Q8), _P, _P]),
     "bmx_q8_quantize": (_I, [_P, _I, ctypes.POINTER(Q8), _P]),
     "bmx_q8_dequant": (_I, [ctypes.POINTER(Q8), _I, _P, _P]),
     "bmx_q8_linear_workspace": (_SZ, [ctypes.POINTER(Q8), _I]),

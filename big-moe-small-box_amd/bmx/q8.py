@@ -9,13 +9,13 @@ ROW_DTYPES = {**DTYPES, torch.float32: L.DT_FP32}
 MOST_K = 131071
 
 
-def columns8(K):
-    """Codes of a row as they are kept: K up to a multiple of 16."""
-    return (K + 15) // 16 * 16
+def code_bytes(N, K):
+    """bmx_q8_code_bytes: 16 rows x 64 columns a block."""
+    return (N + 15) // 16 * ((K + 63) // 64) * 1024
 
 
 class _Codes8:
-    """codes int8 [N, columns8(K)], zeros past K, and scale fp32 [N], on one device: what Q8Matrix and Rows8 have in common."""
+    """codes int8 in the kernels' order (bmx_q8) and scale fp32 [N], on one device: what Q8Matrix and Rows8 have in common."""
 
     _fixed = ("N", "K", "device", "codes", "scale", "struct")
 
@@ -29,11 +29,11 @@ class _Codes8:
         raise TypeError(f"{type(self).__name__} cannot be pickled or copied (its struct holds device addresses)")
 
     def _set(self, N, K, codes, scale):
-        struct = L.Q8(N, K, codes.shape[1], codes.data_ptr() or None, scale.data_ptr() or None)
+        struct = L.Q8(N, K, codes.data_ptr() or None, scale.data_ptr() or None)
         self.__dict__.update(N=N, K=K, device=codes.device, codes=codes, scale=scale, struct=struct)
 
     def _given(self, codes, scale, rows):
-        """A user's codes [N, K] and scales [N], copied."""
+        """A user's codes [N, K] and scales [N], copied into the kernels' order."""
         who = type(self).__name__
         if codes.dtype != torch.int8 or codes.dim() != 2 or not codes.is_cuda:
             raise ValueError(f"{who}: codes must be an int8 device tensor [{rows}, K], got {codes.dtype} {tuple(codes.shape)} on {codes.device}")
@@ -43,19 +43,30 @@ class _Codes8:
         if scale.dtype not in ROW_DTYPES or scale.numel() != N or scale.device != codes.device or scale.dim() not in (1, 2):
             raise ValueError(f"{who}: scale must be an fp32, fp16 or bf16 tensor of {N} values on {codes.device}, got {scale.dtype} "
                              f"{tuple(scale.shape)} on {scale.device}")
-        own = codes.new_zeros((N, columns8(K)))
-        own[:, :K] = codes.detach()
-        self._set(N, K, own, scale.detach().reshape(-1).to(torch.float32, copy=True))
+        codes = codes.detach().contiguous()
+        self._set(N, K, torch.empty(code_bytes(N, K), dtype=torch.int8, device=codes.device),
+                  scale.detach().reshape(-1).to(torch.float32, copy=True))
+        self._call("bmx_q8_pack", codes)
+
+    def _call(self, name, *args):
+        """A library call on this and args (tensors by address), on the current stream of its device; nothing for no rows."""
+        if self.N:
+            with torch.cuda.device(self.device):
+                s = torch.cuda.current_stream().cuda_stream
+                L.check(getattr(L.lib(), name)(self.struct, *(a.data_ptr() if torch.is_tensor(a) else a for a in args), s), name)
+
+    def int8(self):
+        """The codes, int8 [N, K]."""
+        out = torch.empty((self.N, self.K), dtype=torch.int8, device=self.device)
+        self._call("bmx_q8_unpack", out)
+        return out
 
     def dequant(self, dtype=torch.float16):
         """The values [N, K] in fp16, bf16 or fp32, each rounded once."""
         if dtype not in ROW_DTYPES:
             raise ValueError(f"{type(self).__name__}.dequant: fp16, bf16 or fp32, got {dtype}")
         out = torch.empty((self.N, self.K), dtype=dtype, device=self.device)
-        if self.N:
-            with torch.cuda.device(self.device):
-                s = torch.cuda.current_stream().cuda_stream
-                L.check(L.lib().bmx_q8_dequant(self.struct, ROW_DTYPES[dtype], out.data_ptr(), s), "bmx_q8_dequant")
+        self._call("bmx_q8_dequant", ROW_DTYPES[dtype], out)
         return out
 
 
@@ -65,7 +76,7 @@ def _quantized(to, x, N, K):
     if s is None:
         with torch.cuda.device(x.device):
             return _quantized(to, x, N, K)
-    to._set(N, K, torch.empty((N, columns8(K)), dtype=torch.int8, device=x.device),
+    to._set(N, K, torch.empty(code_bytes(N, K), dtype=torch.int8, device=x.device),
             torch.empty(N, dtype=torch.float32, device=x.device))
     if N:
         rc = L.lib().bmx_q8_quantize(x.data_ptr(), ROW_DTYPES[x.dtype], to.struct, s)
@@ -114,7 +125,7 @@ class Rows8(_Codes8):
     @classmethod
     def _empty(cls, T, K, device, dtype, shape):
         r = cls.__new__(cls)
-        r._set(T, K, torch.empty((T, columns8(K)), dtype=torch.int8, device=device), torch.empty(T, dtype=torch.float32, device=device))
+        r._set(T, K, torch.empty(code_bytes(T, K), dtype=torch.int8, device=device), torch.empty(T, dtype=torch.float32, device=device))
         r.__dict__.update(dtype=dtype, shape=shape)
         return r
 

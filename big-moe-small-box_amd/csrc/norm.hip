@@ -16,8 +16,7 @@ struct NormArgs {
     void *r, *y;
     int8_t* codes;
     float* scale;
-    int64_t ld;                     // of codes
-    int kp;                         // ... columns to write: H up to a multiple of 16
+    int blocks;                     // q8_blocks(H)
     int T, H;
     int xt, rt, wt, yt;             // row types
     float eps;
@@ -92,8 +91,8 @@ __global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
     for (int c = 0; c < CH; ++c)
     {
         const int h = (part * 64 + lane + c * (W * 64)) * 8;
-        if (p.codes && h < p.kp)
-            *reinterpret_cast<u32x2*>(p.codes + t * p.ld + h) =
+        if (p.codes && h < p.blocks * Q8_COLS)
+            *reinterpret_cast<u32x2*>(p.codes + q8_at(t, h, p.blocks)) =
                 h < p.H ? u32x2{codes4(vw[c], q), codes4(vw[c] + 4, q)} : u32x2{0, 0};
         if (p.y && h < p.H)
         {
@@ -134,10 +133,10 @@ __global__ __launch_bounds__(512) void quantize_any_k(const NormArgs p)
     __syncthreads();
     for (int i = 0; i < 8; ++i) top = max(top, smax[i]);
     const Top8 q = top8(top);
-    for (int h = threadIdx.x * 4; h < p.kp; h += 2048)
+    for (int h = threadIdx.x * 4; h < p.blocks * Q8_COLS; h += 2048)
     {
         const float v[4] = {value(h), value(h + 1), value(h + 2), value(h + 3)};
-        *reinterpret_cast<uint32_t*>(p.codes + t * p.ld + h) = codes4(v, q);
+        *reinterpret_cast<uint32_t*>(p.codes + q8_at(t, h, p.blocks)) = codes4(v, q);
     }
     if (threadIdx.x == 0) p.scale[t] = q.scale;
 }
@@ -148,7 +147,7 @@ int launch_quantize(const void* x, int type, const bmx_q8* out, hipStream_t s)
     a.x = x; a.xt = type; a.T = out->N; a.H = out->K;
     a.codes = static_cast<int8_t*>(const_cast<void*>(out->codes));
     a.scale = const_cast<float*>(out->scale);
-    a.ld = out->ld; a.kp = q8_columns(out->K);
+    a.blocks = q8_blocks(out->K);
     if (a.H % 8 == 0 && a.H <= BMX_NORM_MAX_H && reinterpret_cast<uintptr_t>(x) % 16 == 0) return launch_norm(a, s);
     hipLaunchKernelGGL(quantize_any_k, dim3(a.T), dim3(512), 0, s, a);
     return check_launch("quantize");
@@ -342,7 +341,7 @@ int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual,
     {
         a.codes = static_cast<int8_t*>(const_cast<void*>(rows->codes));
         a.scale = const_cast<float*>(rows->scale);
-        a.ld = rows->ld; a.kp = q8_columns(rows->K);
+        a.blocks = q8_blocks(rows->K);
     }
     a.T = T; a.H = desc->H;
     a.xt = desc->x_dtype; a.rt = desc->residual_dtype; a.wt = desc->weight_dtype; a.yt = desc->dtype;

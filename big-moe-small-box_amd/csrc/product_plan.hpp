@@ -206,8 +206,8 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 
 constexpr int Q8_K = 128;   // columns of a K tile (gemm8_k): as many bytes as gemm16_k's 64, and as much time
 
-// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, else gemm8_k's tiles
-inline bool q8_few(int T) { return T <= 16; }
+// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 80 tokens, else gemm8_k's tiles
+inline bool q8_few(int T) { return T <= 80; }
 inline TilePlan q8_plan(int N, int K, int T, int products)
 {
     return plan_product((int64_t)N * products, T, (K + Q8_K - 1) / Q8_K, 1, true);

@@ -14,8 +14,6 @@ int check_q8(const bmx_q8* q, const char* who)
     if (!q) return set_error(BMX_ERR_ARG, "%s: null matrix", who);
     if (q->N <= 0 || q->N > (1 << 24) || q->K <= 0 || q->K > 131071)
         return set_error(BMX_ERR_ARG, "%s: N (%d) must be in [1, 2^24], K (%d) in [1, 131071]", who, q->N, q->K);
-    if (q->ld % 16 || q->ld < q8_columns(q->K) || q->ld > (1 << 20))
-        return set_error(BMX_ERR_ARG, "%s: ld (%lld) must be a multiple of 16 from K (%d) up, at most 2^20", who, (long long)q->ld, q->K);
     if (!q->codes || !q->scale) return set_error(BMX_ERR_ARG, "%s: null codes or scale", who);
     if (odd16(q->codes) || reinterpret_cast<uintptr_t>(q->scale) % 4)
         return set_error(BMX_ERR_ARG, "%s: codes must be 16-byte, scale 4-byte aligned", who);
@@ -31,47 +29,72 @@ int check_rows8(const bmx_q8* rows, int T, int K, const char* who)
     return BMX_OK;
 }
 
-// v = scale code; 16 codes a thread
-__global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int64_t ld, int K,
-                                                    int type, void* __restrict__ out, int64_t pieces)
+// v = scale code (scale null: the codes themselves); 16 codes a thread, of one row
+__global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int K, int type,
+                                                    void* __restrict__ out, int64_t pieces)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
     const int per = (K + 15) / 16;
     const int64_t n = i / per;
     const int k = (int)(i % per) * 16;
-    const u32x4 c = ldg4(codes + n * ld + k);
-    const float s = scale[n];
+    const u32x4 c = ldg4(codes + q8_at(n, k, q8_blocks(K)));
+    const float s = scale ? scale[n] : 1.0f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int e = 0; e < 16; ++e)
     {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = s * (float)(int8_t)(c[h * 2 + e / 4] >> (8 * (e % 4)));
-        const int64_t o = n * K + k + h * 8;
-        if (K % 8 == 0)
-        {
-            if (k + h * 8 < K) store8(out, type, o, v);
-            continue;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (k + h * 8 + e < K)
-            {
-                if (type == ROW_F32) static_cast<float*>(out)[o + e] = v[e];
-                else static_cast<uint16_t*>(out)[o + e] = (uint16_t)bits16(type, v[e]);
-            }
+        const int8_t code = (int8_t)(c[e / 4] >> (8 * (e % 4)));
+        const int64_t o = n * K + k + e;
+        if (k + e >= K) continue;
+        if (!scale) static_cast<int8_t*>(out)[o] = code;
+        else if (type == ROW_F32) static_cast<float*>(out)[o] = s * (float)code;
+        else static_cast<uint16_t*>(out)[o] = (uint16_t)bits16(type, s * (float)code);
     }
+}
+
+// Row-major codes into blocks: 16 a thread, zeros past K
+__global__ __launch_bounds__(256) void q8_pack_k(const int8_t* __restrict__ in, int K, int8_t* __restrict__ codes, int64_t pieces)
+{
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int per = q8_blocks(K) * (Q8_COLS / 16);
+    const int64_t n = i / per;
+    const int k = (int)(i % per) * 16;
+    u32x4 c = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        if (k + e < K) c[e / 4] |= (uint32_t)(uint8_t)in[n * K + k + e] << (8 * (e % 4));
+    *reinterpret_cast<u32x4*>(codes + q8_at(n, k, q8_blocks(K))) = c;
+}
+
+static int q8_whole(const char* fn, const bmx_q8* q, int per, int64_t* pieces)
+{
+    *pieces = (int64_t)q->N * per;
+    if (*pieces > (int64_t)1 << 31) return set_error(BMX_ERR_ARG, "%s: %d x %d values are too many for one call", fn, q->N, q->K);
+    return BMX_OK;
 }
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
-template <bool FUSED, int RT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
+template <bool FUSED, int TT, int EPI> static int skinny8_launch(const Q8Args& a, hipStream_t s)
 {
-    constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT;
-    const int64_t rows = (a.N + ROWS - 1) / ROWS, blocks = a.T <= 16 ? rows : (rows + 7) / 8 * 8 * ((a.T + 15) / 16);
-    hipLaunchKernelGGL((skinny8_k<FUSED, RT, EPI>), dim3((unsigned)blocks), dim3(S8_W * 64), FUSED ? skinny8_lds(a.T, a.K) : 0, s, a);
+    constexpr int ROWS = EPI == EPI_GU ? 8 : 16;
+    hipLaunchKernelGGL((skinny8_k<FUSED, TT, EPI>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(S8_W * 64),
+                       FUSED ? skinny8_lds(a.T, a.K) : 0, s, a);
     return check_launch("skinny8");
+}
+
+template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
+{
+    if (!a.xc) return skinny8_launch<true, 1, EPI>(a, s);
+    switch ((a.T + 15) / 16)
+    {
+        case 1: return skinny8_launch<false, 1, EPI>(a, s);
+        case 2: return skinny8_launch<false, 2, EPI>(a, s);
+        case 3: return skinny8_launch<false, 3, EPI>(a, s);
+        case 4: return skinny8_launch<false, 4, EPI>(a, s);
+        default: return skinny8_launch<false, 5, EPI>(a, s);
+    }
 }
 
 template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
@@ -82,10 +105,10 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
     const dim3 grid((unsigned)(a.tm * a.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * (a.w[1] ? 2 : 1) : 1));
     switch (tile)
     {
-        case 0: hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 2, EPI>), grid, dim3(512), 0, s, a); break;
-        case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 2, EPI>), grid, dim3(256), 0, s, a); break;
-        case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 3, EPI>), grid, dim3(512), 0, s, a); break;
-        default: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 2, EPI>), grid, dim3(512), 0, s, a);
+        case 0: hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 4, EPI>), grid, dim3(512), 0, s, a); break;
+        case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a); break;
+        case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
+        default: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
     }
     return check_launch("gemm8");
 }
@@ -94,7 +117,7 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
 template <int EPI> static int product8(const Q8Args& base, hipStream_t s)
 {
     Q8Args a = base;
-    if (q8_few(a.T)) return a.xc ? skinny8_rows<false, 1, EPI>(a, s) : skinny8_rows<true, 1, EPI>(a, s);
+    if (q8_few(a.T)) return skinny8_tokens<EPI>(a, s);
     const TilePlan tp = q8_plan(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1);
     if (tp.splits == 1)
     {
@@ -125,7 +148,7 @@ struct Tokens {
 };
 
 static bool fused8(const Tokens& in, int T, int K) { return !in.rows && q8_few(T) && skinny8_fused(T, K); }
-static size_t rows8_bytes(int T, int K) { return align_up((size_t)T * q8_columns(K), 256) + align_up((size_t)T * 4, 256); }
+static size_t rows8_bytes(int T, int K) { return align_up(q8_bytes(T, K), 256) + align_up((size_t)T * 4, 256); }
 
 static int take_tokens(const Tokens& in, int T, int K, char* ws, Q8Args& a, hipStream_t s)
 {
@@ -139,11 +162,10 @@ static int take_tokens(const Tokens& in, int T, int K, char* ws, Q8Args& a, hipS
         a.xt = in.type;
         return BMX_OK;
     }
-    bmx_q8 q = {T, K, q8_columns(K), ws, reinterpret_cast<float*>(ws + align_up((size_t)T * q8_columns(K), 256))};
+    bmx_q8 q = {T, K, ws, reinterpret_cast<float*>(ws + align_up(q8_bytes(T, K), 256))};
     if (in.rows) q = *in.rows;
     a.xc = static_cast<const int8_t*>(q.codes);
     a.sx = q.scale;
-    a.ldx = q.ld;
     return in.rows ? BMX_OK : launch_quantize(in.x, in.type, &q, s);
 }
 
@@ -151,7 +173,6 @@ static void put_matrix(Q8Args& a, int m, const bmx_q8* w)
 {
     a.w[m] = static_cast<const int8_t*>(w->codes);
     a.sw[m] = w->scale;
-    a.ldw = w->ld;
 }
 
 static size_t linear8_ws(const bmx_q8* w, int T, bool rows)
@@ -221,8 +242,8 @@ static int check_ffn8(const bmx_ffn8_desc* d, int T, const char* who)
     for (const bmx_q8* q : {d->gate, d->up, d->down})
         if (const int rc = check_q8(q, who)) return rc;
     const int H = d->gate->K, I = d->gate->N;
-    if (d->up->K != H || d->up->N != I || d->down->K != I || d->down->N != H || d->up->ld != d->gate->ld)
-        return set_error(BMX_ERR_ARG, "%s: gate and up must be [I, H] with rows of one length, down [H, I]", who);
+    if (d->up->K != H || d->up->N != I || d->down->K != I || d->down->N != H)
+        return set_error(BMX_ERR_ARG, "%s: gate and up must be [I, H], down [H, I]", who);
     if (H % 8 || I % 8) return set_error(BMX_ERR_ARG, "%s: H (%d) and I (%d) must be multiples of 8", who, H, I);
     if (!is16(d->dtype)) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", who, d->dtype);
     if (d->act < BMX_ACT_SILU || d->act > BMX_ACT_SILU_OAI) return set_error(BMX_ERR_ARG, "%s: unknown activation %d", who, d->act);
@@ -261,17 +282,44 @@ int bmx_q8_quantize(const void* x, int dtype, const bmx_q8* out, bmx_stream_t st
     return launch_quantize(x, dtype, out, static_cast<hipStream_t>(stream));
 }
 
+size_t bmx_q8_code_bytes(int N, int K) { return N <= 0 || K <= 0 ? 0 : q8_bytes(N, K); }
+
+int bmx_q8_pack(const bmx_q8* q, const void* codes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_q8_pack";
+    int64_t pieces = 0;
+    if (const int rc = check_q8(q, fn)) return rc;
+    if (!codes) return set_error(BMX_ERR_ARG, "%s: codes are null", fn);
+    if (const int rc = q8_whole(fn, q, q8_blocks(q->K) * (Q8_COLS / 16), &pieces)) return rc;
+    hipLaunchKernelGGL(q8_pack_k, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const int8_t*>(codes), q->K, static_cast<int8_t*>(const_cast<void*>(q->codes)), pieces);
+    return check_launch(fn);
+}
+
+static int dequant_call(const char* fn, const bmx_q8* q, const float* scale, int dtype, void* out, bmx_stream_t stream)
+{
+    int64_t pieces = 0;
+    if (const int rc = q8_whole(fn, q, (q->K + 15) / 16, &pieces)) return rc;
+    hipLaunchKernelGGL(q8_dequant_k, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       static_cast<const int8_t*>(q->codes), scale, q->K, dtype, out, pieces);
+    return check_launch(fn);
+}
+
+int bmx_q8_unpack(const bmx_q8* q, void* codes, bmx_stream_t stream)
+{
+    const char* fn = "bmx_q8_unpack";
+    if (const int rc = check_q8(q, fn)) return rc;
+    if (!codes) return set_error(BMX_ERR_ARG, "%s: codes are null", fn);
+    return dequant_call(fn, q, nullptr, 0, codes, stream);
+}
+
 int bmx_q8_dequant(const bmx_q8* q, int dtype, void* out, bmx_stream_t stream)
 {
     const char* fn = "bmx_q8_dequant";
     if (const int rc = check_q8(q, fn)) return rc;
     if (!is16(dtype) && dtype != BMX_DT_FP32) return set_error(BMX_ERR_ARG, "%s: unknown dtype %d", fn, dtype);
     if (!out || odd16(out)) return set_error(BMX_ERR_ARG, "%s: out null or not 16-byte aligned", fn);
-    const int64_t pieces = (int64_t)q->N * ((q->K + 15) / 16), blocks = (pieces + 255) / 256;
-    if (blocks > (1 << 23)) return set_error(BMX_ERR_ARG, "%s: %d x %d values are too many for one call", fn, q->N, q->K);
-    hipLaunchKernelGGL(q8_dequant_k, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const int8_t*>(q->codes), q->scale, q->ld, q->K, dtype, out, pieces);
-    return check_launch(fn);
+    return dequant_call(fn, q, q->scale, dtype, out, stream);
 }
 
 size_t bmx_q8_linear_workspace(const bmx_q8* w, int T)

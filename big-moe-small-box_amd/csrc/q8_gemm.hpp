@@ -1,14 +1,15 @@
 // Products of 8-bit integers: y[t][n] = sx[t] sw[n] sum_k a[t][k] c[n][k], the sum exact in int32 (K <= 131,071), so that a result
-// does not depend on tiles, splits or the tokens beside it. Rows of codes are whole 16-byte chunks with zeros past K.
+// does not depend on tiles, splits or the tokens beside it. Both factors lie in blocks of 16 rows x 64 columns (rows8.hpp).
 //
-// skinny8_k: few tokens, bound by the bytes of W. A workgroup has 16 RT rows of W (half of gate and half of up in the gated product);
-// its eight waves take every eighth 128 columns of them straight from HBM to matrix operands, several steps ahead. Up to four
-// tokens' rows are quantized by each workgroup itself while its first loads of W are on their way, into LDS: one launch instead of two.
+// skinny8_k: to 80 tokens, bound by the bytes of W. A workgroup has 16 rows of W (eight of gate and eight of up in the gated
+// product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
+// ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized by each workgroup itself while
+// its first loads of W are on their way, into LDS: one launch instead of two.
 // v_mfma_i32_16x16x64_i8: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 16 .. + 15; of the
 // result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3.
 //
-// gemm8_k: many tokens, gemm16_k's tiles: an 8-bit row of 128 columns is the 128 bytes of a 16-bit row of 64, and
-// v_mfma_i32_32x32x32_i8 takes the same 16 bytes a lane in the same places as v_mfma_f32_32x32x16, for twice the products.
+// gemm8_k: many tokens, gemm16_k's tiles with v_mfma_i32_32x32x32_i8, in stages of 64 columns: as many bytes as half of gemm16_k's K
+// tile, for as many products.
 #pragma once
 #include "rows8.hpp"
 
@@ -17,22 +18,18 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 namespace bmx {
 
-constexpr int G8_K = 2 * GK;        // columns of a K tile
-constexpr int S8_K = 128;           // columns of a step (skinny8_k)
-constexpr int S8_W = 8;             // waves of a workgroup
+constexpr int S8_W = 8;             // waves of a workgroup (skinny8_k)
 constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup quantizes: 4 a wave
 
 struct Q8Args {
     const int8_t* w[2];             // second: up
     const float* sw[2];
-    int64_t ldw;
     const void* x;                  // rows to quantize (skinny8_k<true>), of row type xt, K values each
     int xt;
     const int8_t* xc;               // or codes
     const float* sx;
-    int64_t ldx;
     int T, N, K;                    // N: rows of W (of each of the two matrices)
-    int from;                       // W's first row: the rows before are another launch's
+    int from;                       // W's first row, a multiple of 16: the rows before are another launch's
     void* out;                      // EPI_STORE: 16 bits of type ot; EPI_ADD: fp32 +=; EPI_GU: h fp32
     int ot, ldo;
     const float* scale;             // EPI_ADD: [T] or null
@@ -43,31 +40,23 @@ struct Q8Args {
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------------
 
-inline bool skinny8_fused(int T, int K) { return K % 8 == 0 && (int64_t)T * ((K + 511) / 512) <= S8_SLOTS; }
-inline size_t skinny8_lds(int T, int K) { return (size_t)T * (round_up(K, S8_K) + 16); }
+inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && T * ((K + 511) / 512) <= S8_SLOTS; }
+inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
-template <bool FUSED, int RT, int EPI>
+// TT: tiles of 16 tokens
+template <bool FUSED, int TT, int EPI>
 __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
 {
     constexpr bool GU = EPI == EPI_GU;
-    constexpr int ROWS = GU ? 8 : 16, D = RT == 1 ? 4 : 2;         // result columns of a tile, steps in flight
+    constexpr int ROWS = GU ? 8 : 16, D = TT == 1 ? 8 : TT <= 3 ? 4 : 3;     // result columns, blocks in flight
+    static_assert(!FUSED || TT == 1, "one tile of tokens quantized here");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
-    // 16 tokens a workgroup; those of one block of rows follow one another on one XCD, so that all but the first find W in its L2
-    int row = blockIdx.x, t0 = 0;
-    if (p.T > 16)
-    {
-        const int tt = (p.T + 15) >> 4, rest = row >> 3;
-        t0 = rest % tt * 16;
-        row = rest / tt * 8 + (row & 7);
-    }
-    const int n0 = row * (ROWS * RT);
-    if (n0 >= p.N) return;
-    const int KP = (p.K + 15) & ~15, KT = (KP + S8_K - 1) / S8_K;
+    const int n0 = blockIdx.x * ROWS, KB = q8_blocks(p.K);
 
     extern __shared__ __attribute__((aligned(16))) char xl[];
     __shared__ uint32_t tops[S8_SLOTS];
     __shared__ float lsx[16];
-    const int xrow = KT * S8_K + 16, spt = (p.K + 511) / 512;      // (rows an odd number of 16 bytes apart: 16 of them on all banks)
+    const int xrow = KB * Q8_COLS + 16, spt = (p.K + 511) / 512;   // (rows an odd number of 16 bytes apart: 16 of them on all banks)
     Raw8 raw[4];
     if (FUSED)
 #pragma unroll
@@ -77,45 +66,33 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
             if (t < p.T && h < p.K) raw[n] = load_raw8(p.x, p.xt, (int64_t)t * p.K + h);
         }
 
-    // this lane's rows of W, and whose (rows past the last load it again)
-    const int mat = GU ? r >> 3 : 0;
-    const int8_t* w[RT];
+    // this lane's row of W, and whose (rows past the last load it again)
+    const int mat = GU ? r >> 3 : 0, n = min(n0 + (GU ? r & 7 : r), p.N - 1);
+    const int8_t* w = p.w[mat] + q8_at(n, q * 16, KB);
+    const int8_t* xr = FUSED ? nullptr : p.xc + q8_at(r, q * 16, KB);
+    struct Step { u32x4 w, x[FUSED ? 1 : TT]; } st[D];
+    auto load = [&](Step& b, int kb) {
+        b.w = ldg4(w + (int64_t)kb * Q8_BLOCK);
+        if (!FUSED)
 #pragma unroll
-    for (int i = 0; i < RT; ++i) w[i] = p.w[mat] + (int64_t)min(n0 + i * ROWS + (GU ? r & 7 : r), p.N - 1) * p.ldw;
-    const int8_t* xr = FUSED ? nullptr : p.xc + (int64_t)min(t0 + r, p.T - 1) * p.ldx;
-    struct Step { u32x4 w[RT][2], x[FUSED ? 1 : 2]; } st[D];
-    auto load = [&](Step& b, int kt) {
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-        {
-            // past the last column the last again, beside zeros of x
-            const int k = kt * S8_K + j * 64 + q * 16, at = min(k, KP - 16);
-#pragma unroll
-            for (int i = 0; i < RT; ++i) b.w[i][j] = ldg4(w[i] + at);
-            if (FUSED) continue;
-            const u32x4 x = ldg4(xr + at);
-            b.x[FUSED ? 0 : j] = k < KP ? x : u32x4{0, 0, 0, 0};
-        }
+            for (int i = 0; i < TT; ++i) b.x[FUSED ? 0 : i] = ldg4(xr + ((int64_t)i * KB + kb) * Q8_BLOCK);
     };
-    i32x4 acc[RT];
+    i32x4 acc[TT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) acc[i] = i32x4{0, 0, 0, 0};
-    auto multiply = [&](const Step& b, int kt) {
+    for (int i = 0; i < TT; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    auto multiply = [&](const Step& b, int kb) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < TT; ++i)
         {
-            const u32x4 x = FUSED ? *reinterpret_cast<const u32x4*>(xl + min(r, p.T - 1) * xrow + kt * S8_K + j * 64 + q * 16)
-                                  : b.x[FUSED ? 0 : j];
-#pragma unroll
-            for (int i = 0; i < RT; ++i)
-                acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, b.w[i][j]), acc[i], 0, 0, 0);
+            const u32x4 x = FUSED ? *reinterpret_cast<const u32x4*>(xl + min(r, p.T - 1) * xrow + kb * Q8_COLS + q * 16) : b.x[FUSED ? 0 : i];
+            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, b.w), acc[i], 0, 0, 0);
         }
     };
 
-    int kt = wave;                                                 // the next step to multiply; D are in flight
+    int kb = wave;                                                 // the next block to multiply; D are in flight
 #pragma unroll
     for (int d = 0; d < D; ++d)
-        if (kt + d * S8_W < KT) load(st[d], kt + d * S8_W);
+        if (kb + d * S8_W < KB) load(st[d], kb + d * S8_W);
     if (FUSED)
     {
         float v[4][8];
@@ -140,35 +117,34 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
             const int s = wave + n * S8_W, t = s / spt, h = s % spt * 512 + lane * 8;
             if (t >= p.T) break;
             const Top8 o = top8(wave_max(lane < spt ? tops[t * spt + lane] : 0u));
-            if (h < KT * S8_K)
-                *reinterpret_cast<u32x2*>(xl + t * xrow + h) = u32x2{codes4(v[n], o), codes4(v[n] + 4, o)};
+            if (h < KB * Q8_COLS) *reinterpret_cast<u32x2*>(xl + t * xrow + h) = u32x2{codes4(v[n], o), codes4(v[n] + 4, o)};
             if (s % spt == 0 && lane == 0) lsx[t] = o.scale;
         }
         lds_barrier();
     }
-    while (kt < KT)
+    while (kb < KB)
     {
 #pragma unroll
         for (int d = 0; d < D; ++d)
         {
-            if (kt >= KT) break;
-            multiply(st[d], kt);
-            if (kt + D * S8_W < KT) load(st[d], kt + D * S8_W);
-            kt += S8_W;
+            if (kb >= KB) break;
+            multiply(st[d], kb);
+            if (kb + D * S8_W < KB) load(st[d], kb + D * S8_W);
+            kb += S8_W;
         }
     }
 
     // join the waves
-    constexpr int V = RT * 256;                                    // (row tile, element, lane)
+    constexpr int V = TT * 256;                                    // (token tile, element, lane)
     __shared__ int part[S8_W][V];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < TT; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) part[wave][(i * 4 + e) * 64 + lane] = acc[i][e];
     __syncthreads();
     for (int i = threadIdx.x; i < V; i += S8_W * 64)
     {
-        const int c = i & 15, tl = ((i >> 4) & 3) * 4 + ((i >> 6) & 3), t = t0 + tl, n = n0 + (i >> 8) * ROWS + c;
+        const int c = i & 15, t = (i >> 8) * 16 + ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + c;
         if (t >= p.T || c >= ROWS || n >= p.N) continue;
         auto sum = [&](int at) {
             int s = part[0][at];
@@ -176,7 +152,7 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
             for (int w = 1; w < S8_W; ++w) s += part[w][at];
             return (float)s;
         };
-        const float sx = FUSED ? lsx[tl] : p.sx[t], s = sum(i) * sx * p.sw[0][n];
+        const float sx = FUSED ? lsx[t] : p.sx[t], s = sum(i) * sx * p.sw[0][n];
         const int64_t o = (int64_t)t * p.ldo + n;
         if (GU) static_cast<float*>(p.out)[o] = act_h(p.act, s, sum(i + 8) * sx * p.sw[1][n]);
         else if (EPI == EPI_ADD)
@@ -190,31 +166,31 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
 
 // ---- many tokens --------------------------------------------------------------------------------------------------------
 
-// What becomes of 8 neighbouring sums (rows m .. m + 7 of W) of token n
-__device__ __forceinline__ void times8(const Q8Args& p, int mat, int n, int m, const int (&s)[8], float (&v)[8])
+// The scales of 8 neighbouring rows of W from row m of p.N (0 behind the last)
+__device__ __forceinline__ void scales8(const Q8Args& p, int mat, int m, float (&w)[8])
 {
-    const float sx = p.sx[n];
     const float* sw = p.sw[mat] + p.from + m;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (float)s[i] * sx * (m + i < p.N ? sw[i] : 0.0f);
+    for (int i = 0; i < 8; ++i) w[i] = m + i < p.N ? sw[i] : 0.0f;
 }
 
-template <int EPI> __device__ __forceinline__ void put8(const Q8Args& p, int n, int m, const int (&s)[8], const int (&u)[8])
+// What becomes of 8 neighbouring sums (rows m .. m + 7 of W, of scales w; u: up's) of token n, of scale sx; k: its factor (EPI_ADD)
+template <int EPI>
+__device__ __forceinline__ void put8(const Q8Args& p, int n, int m, const int (&s)[8], const int (&u)[8], float sx, float k,
+                                     const float (&w)[8], const float (&wu)[8])
 {
     float v[8];
-    times8(p, 0, n, m, s, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)s[i] * sx * w[i];
     const int64_t o = (int64_t)n * p.ldo + p.from + m;
     if (EPI == EPI_GU)
     {
-        float b[8];
-        times8(p, 1, n, m, u, b);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_h(p.act, v[i], b[i]);
+        for (int i = 0; i < 8; ++i) v[i] = act_h(p.act, v[i], (float)u[i] * sx * wu[i]);
         store8(p.out, ROW_F32, o, v);
     }
     else if (EPI == EPI_ADD)
     {
-        const float k = p.scale ? p.scale[n] : 1.0f;
         float* y = static_cast<float*>(p.out) + o;
         const Vals<8> c = load32<8>(y);
 #pragma unroll
@@ -230,18 +206,27 @@ template <int EPI> __device__ __forceinline__ void put8(const Q8Args& p, int n, 
     }
 }
 
-// BM rows of W x BN tokens by WK groups of WM x WN waves, NB buffers of a K tile each; as gemm16_tile, whose comments say why
+// BM rows of W x BN tokens by WK groups of WM x WN waves, NB buffers of a stage of 64 columns each; every group has every WK-th stage.
+// A stage's loads go out NB - 1 stages ahead (two or three microseconds), each a contiguous block; as gemm16_tile otherwise, whose
+// comments say why.
+template <int BM, int BN, int WM, int WN, int WK, int NB> constexpr int gemm8_lds()
+{
+    constexpr int TILES = WK * NB * (BM + BN) * Q8_COLS, TURN = WM * WN * WK * 32 * (BM / WM + 4) * 4;
+    return TILES > TURN ? TILES : TURN;
+}
+
 template <int BM, int BN, int WM, int WN, int WK, int NB, int EPI>
 __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
 {
-    __shared__ __attribute__((aligned(1024))) char lds_all[gemm16_lds<BM, BN, WM, WN, WK, NB>()];
-    constexpr int NT = WM * WN * 64;                               // threads of a group
+    __shared__ __attribute__((aligned(1024))) char lds_all[gemm8_lds<BM, BN, WM, WN, WK, NB>()];
+    constexpr int NW = WM * WN;                                    // waves of a group
     constexpr int MF = BM / WM / 32, NF = BN / WN / 32;            // 32 x 32 fragments of a wave
-    constexpr int ABYTES = BM * G8_K, BBYTES = BN * G8_K;
+    constexpr int ABYTES = BM * Q8_COLS, BUF = (BM + BN) * Q8_COLS, AL = BM / 16 / NW, BL = BN / 16 / NW;    // blocks a wave loads
+    static_assert(AL * NW * 16 == BM && BL * NW * 16 == BN, "whole blocks");
     const int z = blockIdx.z;
     const int lane = threadIdx.x & 63, any = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int group = any / (WM * WN), wave = any % (WM * WN);
-    char* lds = lds_all + group * (NB * (ABYTES + BBYTES));
+    const int group = any / NW, wave = any % NW;
+    const lds_ptr lds = (lds_ptr)lds_all + group * (NB * BUF);
     const int wm = wave / WN, wn = wave % WN;
 
     // an XCD on neighbouring tiles (gemm16_tile)
@@ -255,8 +240,8 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
     const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
     const int tm = g0 + (id % per) % gn, tn = (id % per) / gn;
     const int m0 = EPI == EPI_GU ? tm * (BM / 2) : tm * BM, n0 = tn * BN;
-    const int KP = (p.K + 15) & ~15;
-    int kt = 0, kt_end = (KP + G8_K - 1) / G8_K;
+    const int KB = q8_blocks(p.K);
+    int kt = 0, kt_end = KB;
     const int prod = EPI == EPI_PART ? z / p.splits : 0;
     if (EPI == EPI_PART)
     {
@@ -265,26 +250,41 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
         kt_end = kt + q + (sp < r);
     }
 
-    // the loaders count in 16-bit values: two codes
-    TileLoader<BM, NT, WK, false, EPI == EPI_GU> la;
-    TileLoader<BN, NT, WK, false, false> lb;
-    la.init((int)(p.ldw / 2), wave);
-    lb.init((int)(p.ldx / 2), wave);
-    int loaded = kt + group;                                       // this group's next tile to load
-    la.seek(p.w[prod], p.w[1], p.from + m0, loaded * GK, p.from + p.N, KP / 2, wave);
-    lb.seek(p.xc, nullptr, n0, loaded * GK, p.T, KP / 2, wave);
-    auto tail = [&]() { return KP / 2 - loaded * GK; };
-    auto load_a = [&](lds_ptr to) { la.load(to, wave, tail(), loaded < kt_end); };
+    // this wave's blocks of a stage: NW apart, rows of blocks past the last load it again. EPI_GU: two of gate, two of up in turn
+    const char *ap[AL], *bp[BL];
+    int loaded = kt + group;                                       // this group's next stage to load
+    auto block = [&](const int8_t* m, int rb, int rows) {
+        return reinterpret_cast<const char*>(m) + ((int64_t)min(rb, (rows - 1) / Q8_ROWS) * KB + loaded) * Q8_BLOCK;
+    };
+#pragma unroll
+    for (int j = 0; j < AL; ++j)
+    {
+        const int i = wave + j * NW;
+        ap[j] = EPI == EPI_GU ? block(i & 2 ? p.w[1] : p.w[0], (p.from + m0) / Q8_ROWS + (i >> 2) * 2 + (i & 1), p.from + p.N)
+                              : block(p.w[prod], (p.from + m0) / Q8_ROWS + i, p.from + p.N);
+    }
+#pragma unroll
+    for (int j = 0; j < BL; ++j) bp[j] = block(p.xc, n0 / Q8_ROWS + wave + j * NW, p.T);
+    auto load = [&](lds_ptr to, const char*& from, int place) {
+        // (past the last stage zeros: an empty range, so that the count of loads holds)
+        const __amdgpu_buffer_rsrc_t r =
+            __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from), 0, loaded < kt_end ? Q8_BLOCK : 0, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + place * Q8_BLOCK), 16, lane * 16, 0, 0, 0);
+        from += WK * Q8_BLOCK;
+    };
+    auto load_a = [&](lds_ptr to) {
+#pragma unroll
+        for (int j = 0; j < AL; ++j) load(to, ap[j], wave + j * NW);
+    };
     auto load_b = [&](lds_ptr to) {
-        lb.load(to + ABYTES, wave, tail(), loaded < kt_end);
-        la.next();
-        lb.next();
+#pragma unroll
+        for (int j = 0; j < BL; ++j) load(to + ABYTES, bp[j], wave + j * NW);
         loaded += WK;
     };
     // 32 rows from row0, 32 columns from ks * 32: lane l holds row l % 32, columns (l / 32) * 16 .. + 15
-    auto frag = [&](lds_ptr tile, int row0, int ks) -> i32x4 {
+    auto frag = [&](lds_ptr at, int row0, int ks) -> i32x4 {
         const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
-        return *(__attribute__((address_space(3))) i32x4*)(tile + r * G8_K + ((c ^ swz_along(r)) << 4));
+        return *(__attribute__((address_space(3))) i32x4*)(at + r * Q8_COLS + ((c ^ q8_swz(r)) << 4));
     };
     i32x16 acc[MF][NF];
 #pragma unroll
@@ -294,22 +294,21 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
 
-    constexpr int KS = G8_K / 32;
     i32x4 a[2][MF], b[2][NF];
-    auto read = [&](int set, lds_ptr at, int ks) {
+    auto read = [&](int ks, lds_ptr at) {
 #pragma unroll
-        for (int i = 0; i < MF; ++i) a[set][i] = frag(at, wm * (BM / WM) + i * 32, ks);
+        for (int i = 0; i < MF; ++i) a[ks][i] = frag(at, wm * (BM / WM) + i * 32, ks);
 #pragma unroll
-        for (int j = 0; j < NF; ++j) b[set][j] = frag(at + ABYTES, wn * (BN / WN) + j * 32, ks);
+        for (int j = 0; j < NF; ++j) b[ks][j] = frag(at + ABYTES, wn * (BN / WN) + j * 32, ks);
     };
-    auto products = [&](int set, int from, int to) {
+    auto products = [&](int ks, int from, int to) {
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
             for (int j = 0; j < NF; ++j)
-                if (i >= from && i < to) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[set][i], b[set][j], acc[i][j], 0, 0, 0);
+                if (i >= from && i < to) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks][i], b[ks][j], acc[i][j], 0, 0, 0);
     };
-    constexpr int BEHIND = (la.INSTR + lb.INSTR) * (NB - 2);
+    constexpr int BEHIND = (AL + BL) * (NB - 2);
     static_assert(BEHIND < 64, "vmcnt has 6 bits");
     auto landed = [&]() {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -317,63 +316,69 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     };
-    constexpr bool SPREAD = MF * NF >= 8, IN_STEPS = MF * NF >= 4;
-    static_assert(!SPREAD || NB == 2, "spread loads end early: only a wait for all of them fits");
-    auto tile = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
-        if (!SPREAD) { load_a(to); load_b(to); }
-        read(0, at, 0);
-        products((KS - 1) & 1, 0, MF);
-        if (IN_STEPS) __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int ks = 0; ks < KS - 1; ++ks)
-        {
-            if (SPREAD)
-            {
-                if (loaded < kt_end)
-                {
-                    if (ks == 0) load_a(to);
-                    if (ks == 1) load_b(to);
-                }
-                products(ks & 1, 0, MF / 2);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            read((ks + 1) & 1, at, ks + 1);
-            products(ks & 1, SPREAD ? MF / 2 : 0, MF);
-            if (IN_STEPS) __builtin_amdgcn_sched_barrier(0);
-        }
+    // One stage: the second half of the stage before's products first, so that the wait has products on both sides
+    auto stage = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
+        read(0, at);
+        products(1, 0, MF);
+        __builtin_amdgcn_sched_barrier(0);
+        load_a(to);
+        products(0, 0, MF / 2);
+        __builtin_amdgcn_sched_barrier(0);
+        load_b(to);
+        read(1, at);
+        products(0, MF / 2, MF);
+        __builtin_amdgcn_sched_barrier(0);
     };
-    constexpr int BUF = ABYTES + BBYTES;
 #pragma unroll
     for (int i = 0; i < NB - 1; ++i)
     {
-        load_a((lds_ptr)lds + i * BUF);
-        load_b((lds_ptr)lds + i * BUF);
+        load_a(lds + i * BUF);
+        load_b(lds + i * BUF);
     }
-    // the first tile follows products with zeros
+    // the first stage follows products with zeros
 #pragma unroll
-    for (int i = 0; i < MF; ++i) a[(KS - 1) & 1][i] = i32x4{0, 0, 0, 0};
+    for (int i = 0; i < MF; ++i) a[1][i] = i32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int j = 0; j < NF; ++j) b[(KS - 1) & 1][j] = i32x4{0, 0, 0, 0};
+    for (int j = 0; j < NF; ++j) b[1][j] = i32x4{0, 0, 0, 0};
     int buf = 0, before = NB - 1;
-    for (; kt < kt_end; kt += WK)
+    for (; kt < kt_end; kt += WK)                                  // group 0's stage; the others' may lie past the end: zeros
     {
         landed();
-        tile((lds_ptr)lds + buf * BUF, (lds_ptr)lds + before * BUF);
+        stage(lds + buf * BUF, lds + before * BUF);
         before = buf;
         buf = buf + 1 == NB ? 0 : buf + 1;
     }
-    products((KS - 1) & 1, 0, MF);
+    products(1, 0, MF);
 
-    // results, 32 tokens at a time turned over in LDS (gemm16_tile)
+    // results, 32 tokens at a time turned over in LDS (gemm16_tile). A lane's pieces are the same 8 rows of W of different tokens: their
+    // scales are loaded once, all tokens' before the pieces (loaded for each piece, the epilogue took 25 us of 4,096 x 4,096 x 11,008's
+    // 187)
     constexpr int WROW = BM / WM, LROW = WROW + 4, AREA = WM * WN * 32 * LROW;
+    constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8, MINE = 32 * PIECES / WK, EACH = MINE / 64;
+    static_assert(MINE % 64 == 0 && 64 % PIECES == 0, "whole steps, a lane's pieces in one column");
     int* turn = reinterpret_cast<int*>(lds_all) + wave * (32 * LROW);
-    const int wm0 = EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW;
+    const int c = lane % PIECES * 8, m = (EPI == EPI_GU ? m0 + wm * (WROW / 2) : m0 + wm * WROW) + c;
+    const int nb0 = n0 + wn * (BN / WN) + (group * MINE + lane) / PIECES;     // the lane's first token
+    float w0[8], w1[8], sx[NF][EACH], add[NF][EACH];
+    if (EPI != EPI_PART)
+    {
+        scales8(p, 0, m, w0);
+        if (EPI == EPI_GU) scales8(p, 1, m, w1);
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int e = 0; e < EACH; ++e)
+            {
+                const int n = min(nb0 + j * 32 + e * (64 / PIECES), p.T - 1);
+                sx[j][e] = p.sx[n];
+                add[j][e] = EPI == EPI_ADD && p.scale ? p.scale[n] : 1.0f;
+            }
+    }
     __builtin_amdgcn_s_waitcnt(0x0f70);
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NF; ++j)
     {
-        const int nb = n0 + wn * (BN / WN) + j * 32;
 #pragma unroll
         for (int i = 0; i < MF; ++i)
 #pragma unroll
@@ -382,11 +387,10 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
                     i32x4{acc[i][j][e], acc[i][j][e + 1], acc[i][j][e + 2], acc[i][j][e + 3]};
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        constexpr int PIECES = (EPI == EPI_GU ? WROW / 2 : WROW) / 8, MINE = 32 * PIECES / WK;
-        static_assert(MINE % 64 == 0, "whole steps");
-        for (int q = group * MINE + lane; q < (group + 1) * MINE; q += 64)
+#pragma unroll
+        for (int e = 0; e < EACH; ++e)
         {
-            const int rr = q / PIECES, c = q % PIECES * 8, n = nb + rr, m = wm0 + c;
+            const int rr = (group * MINE + lane) / PIECES + e * (64 / PIECES), n = nb0 + j * 32 + e * (64 / PIECES);
             if (n >= p.T || m >= p.N) continue;
             auto piece = [&](int col, int (&v)[8]) {
 #pragma unroll
@@ -416,7 +420,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
                 to[0] = i32x4{s[0], s[1], s[2], s[3]};
                 to[1] = i32x4{s[4], s[5], s[6], s[7]};
             }
-            else put8<EPI>(p, n, m, s, u);
+            else put8<EPI>(p, n, m, s, u, sx[j][e], add[j][e], w0, w1);
         }
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -432,6 +436,10 @@ __global__ __launch_bounds__(64) void finish8_k(const Q8Args p)
     if (at >= plane) return;
     const int n = (int)(at / p.ldp), m = (int)(at % p.ldp);
     int sum[2][8] = {};
+    float w0[8], w1[8];
+    scales8(p, 0, m, w0);
+    if (EPI == EPI_GU) scales8(p, 1, m, w1);
+    const float sx = p.sx[n], add = EPI == EPI_ADD && p.scale ? p.scale[n] : 1.0f;
     for (int s0 = 0; s0 < p.splits; s0 += B)
     {
         i32x4 v[PRODS][B][2];
@@ -451,7 +459,7 @@ __global__ __launch_bounds__(64) void finish8_k(const Q8Args p)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum[k][i] += v[k][s][i / 4][i % 4];
     }
-    put8<EPI>(p, n, m, sum[0], sum[1]);
+    put8<EPI>(p, n, m, sum[0], sum[1], sx, add, w0, w1);
 }
 
 }  // namespace bmx

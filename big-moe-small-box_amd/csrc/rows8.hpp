@@ -129,8 +129,19 @@ __device__ __forceinline__ uint32_t codes4(const float* v, const Top8& o)
     return lo | hi;
 }
 
-// Columns of a row of K codes that are read: whole 16-byte chunks, zeros past K
-inline int q8_columns(int K) { return (int)round_up(K, 16); }
+// Codes in blocks of 16 rows x 64 columns (bmx_q8): 1 KB, a fragment of v_mfma_i32_16x16x64_i8 or two halves of one of 32x32x32, so that
+// a wave's load is one contiguous piece whatever the row's length. (Row by row a wave's load is 64 bytes of each of 16 rows, for
+// K = 4096 all in one memory channel: 4,096 x 4,096 x 11,008 187 us, in blocks 175.) In a block a row's chunk c of 16 bytes lies at c ^
+// (row / 4 % 4): 16 rows' chunks c on all banks of LDS.
+constexpr int Q8_ROWS = 16, Q8_COLS = 64, Q8_BLOCK = Q8_ROWS * Q8_COLS;
+__host__ __device__ constexpr int q8_blocks(int K) { return (K + Q8_COLS - 1) / Q8_COLS; }     // of a row of blocks
+__host__ __device__ constexpr int q8_swz(int row) { return (row >> 2) & 3; }
+__host__ __device__ constexpr int64_t q8_at(int64_t row, int k, int blocks)
+{
+    return (row / Q8_ROWS * blocks + k / Q8_COLS) * Q8_BLOCK + (row % Q8_ROWS) * Q8_COLS + (((k % Q8_COLS) >> 4) ^ q8_swz((int)(row % Q8_ROWS))) * 16 +
+           k % 16;
+}
+inline size_t q8_bytes(int N, int K) { return (size_t)round_up(N, Q8_ROWS) * q8_blocks(K) * Q8_COLS; }
 
 // Rows x of a row type into out's codes and scales (norm.hip)
 int launch_quantize(const void* x, int type, const bmx_q8* out, hipStream_t s);

@@ -539,16 +539,21 @@ int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_f
                      void* dgate, void* dup, void* ddown, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
 
 /* ---- 8-bit matrices and rows ----
- * N rows of K whole numbers with a scale each, v[n][k] = scale[n] code[n][k], the form of 8-bit weights with a scale per output
- * channel (bmx_q8 as a matrix) and of activations with a scale per token (as rows, N tokens). codes int8 [N][ld], ld a multiple of
- * 16, columns from K up to the next multiple of 16 zeros (read, so they have to be), those behind never read; scale fp32 [N].
- * Device memory, codes 16-byte aligned. N to 2^24, K to 131,071 (so that a sum of products fits 32 bits whatever the codes). */
+ * N rows of K whole numbers (-128 .. 127) with a scale each, v[n][k] = scale[n] code[n][k], the form of 8-bit weights with a scale
+ * per output channel (bmx_q8 as a matrix) and of activations with a scale per token (as rows, N tokens). A bmx_q8 holds the codes in
+ * the kernels' order, bmx_q8_code_bytes bytes: blocks of 16 rows x 64 columns, [row / 16][column / 64], in a block each row's 64
+ * bytes, its four 16-byte chunks c at place c ^ (row / 4 % 4); columns from K up to the next multiple of 64 are 0. scale fp32 [N].
+ * Written by bmx_q8_pack from row-major codes, or by the calls that quantize. Device memory, codes 16-byte aligned. N to 2^24, K to
+ * 131,071 (so that a sum of products fits 32 bits whatever the codes). */
 typedef struct bmx_q8 {
     int32_t N, K;
-    int64_t ld;
     const void* codes;
     const float* scale;
 } bmx_q8;
+size_t bmx_q8_code_bytes(int N, int K);
+/* Row-major int8 codes [N][K] into q's codes (its scales are the caller's to write), and back. */
+int bmx_q8_pack(const bmx_q8* q, const void* codes, bmx_stream_t stream);
+int bmx_q8_unpack(const bmx_q8* q, void* codes, bmx_stream_t stream);
 /* Rows x [out->N][out->K] of dtype (fp32 too), contiguous, into out's codes and scales: top = the row's largest magnitude, code =
  * round(x 127 / top), scale = top / 127. A row whose magnitudes are all below 2^-110 becomes zeros (codes and scale); one with an
  * infinity or a NaN codes 0 and scale NaN: every product with it is NaN. */

@@ -32,10 +32,11 @@ def check_rows(rows, y64, e):
     top = y64.abs().amax(1)
     scale = rows.scale.double()
     assert bool(((scale - top / 127).abs() <= top / 127 * (Q.RSTD + 4 * Q.STEP)).all())
-    codes = rows.codes[:, :rows.K].double()
+    codes = rows.int8().double()
     assert bool((codes.abs().amax(1) == 127).all())
     R.check("rows", codes * scale[:, None], y64, scale[:, None] * (0.5 + 127 * 3 * Q.STEP) + e + y64.abs() * 3 * Q.STEP)
-    assert not bool(rows.codes[:, rows.K:].any())
+    b = rows.codes.view(-1, (rows.K + 63) // 64, 16, 64)            # nothing but zeros behind a row, in whatever order
+    assert int((b != 0).sum((1, 3)).view(-1)[:rows.N].sum()) == int((codes != 0).sum())
 
 
 @pytest.mark.parametrize("dt", sorted(DT))
@@ -65,7 +66,7 @@ def test_types(cuda, x32, r32, w32, dt):
         y1, r1 = n(x, res)
         rows2, r2 = n.rows8(x, res)
         assert torch.equal(y1, y) and torch.equal(r1, r) and torch.equal(r2, r)
-        assert torch.equal(rows2.codes, rows.codes) and torch.equal(rows2.scale, rows.scale)
+        assert torch.equal(rows2.int8(), rows.int8()) and torch.equal(rows2.scale, rows.scale)
 
 
 @pytest.mark.parametrize("dt", sorted(DT))
@@ -80,7 +81,7 @@ def test_rows(cuda, T, H, dt):
     check_rows(rows, *Q.norm(x.double(), w.double(), 1e-6))
     assert rows.shape == x.shape and rows.dtype == x.dtype
     # what the codes stand for
-    assert torch.equal(rows.dequant(F32), rows.codes[:, :H].float() * rows.scale[:, None])
+    assert torch.equal(rows.dequant(F32), rows.int8().float() * rows.scale[:, None])
 
 
 def backward_check(cuda, T, H, dt, x32=False, r32=False, w32=False, residual=True, seed=3, use="both"):
@@ -200,7 +201,7 @@ def test_strides_shapes_and_no_tokens(cuda):
     flat = torch.empty(24 * 136 + 3, device=cuda, dtype=torch.float16)
     off = flat[3:].view(24, 136).copy_(x)
     rows, r5 = n.rows8(off, res)
-    assert torch.equal(r5, r) and torch.equal(rows.codes, n.rows8(x, res)[0].codes)
+    assert torch.equal(r5, r) and torch.equal(rows.int8(), n.rows8(x, res)[0].int8())
     y1 = n(x[0], res[0])[0]
     assert y1.shape == (136,) and torch.equal(y1, y[0])
     # none
@@ -226,8 +227,8 @@ def test_zeros_infinities_and_nan(cuda, dt):
         x[2, 5], x[3, 100], x[4, 263] = float("inf"), float("nan"), float("-inf")
         y, rows, r = bmx.RMSNorm(w).both(x, res)
         keep = [0] + list(range(5, T))
-        assert torch.equal(y[keep], clean[keep]) and torch.equal(rows.codes[keep], crows.codes[keep]) and torch.equal(rows.scale[keep], crows.scale[keep])
-        assert not bool(y[1].any()) and not bool(rows.codes[1:5].any()) and float(rows.scale[1]) == 0.0
+        assert torch.equal(y[keep], clean[keep]) and torch.equal(rows.int8()[keep], crows.int8()[keep]) and torch.equal(rows.scale[keep], crows.scale[keep])
+        assert not bool(y[1].any()) and not bool(rows.int8()[1:5].any()) and float(rows.scale[1]) == 0.0
         v = r.float()
         want = v[2:5] * w.float() / torch.sqrt((v[2:5] ** 2).mean(1, keepdim=True) + 1e-6)
         assert torch.equal(y[2:5].isnan(), want.isnan()) and bool((y[2][:5] == 0).all()) and bool(y[2, 5].isnan()) and bool(y[3].isnan().all())
@@ -245,11 +246,11 @@ def test_largest_and_smallest_values(cuda):
     x[2] *= 1e-30
     y, rows = n.both(x)
     assert not bool(y[0].any()) and float(rows.scale[0]) == 0.0
-    assert not bool(rows.codes[1].any()) and float(rows.scale[1]) == 0.0
+    assert not bool(rows.int8()[1].any()) and float(rows.scale[1]) == 0.0
     for i in (2, 3):
         y64, e = Q.norm(x[i:i + 1].double(), w.double(), 1e-6)
         R.check("y", y[i:i + 1], y64, R.rounded(y64, e, torch.bfloat16))
-        assert int(rows.codes[i].abs().max()) == 127
+        assert int(rows.int8()[i].abs().max()) == 127
 
 
 def test_streams_and_graph(cuda):
@@ -259,7 +260,7 @@ def test_streams_and_graph(cuda):
     x2, res2, _ = make(cuda, 300, 2048, torch.float16, seed=9)
     n = bmx.RMSNorm(w)
     want, want2 = n.both(x, res), n.both(x2, res2)
-    same = lambda a, b: torch.equal(a[0], b[0]) and torch.equal(a[1].codes, b[1].codes) and torch.equal(a[1].scale, b[1].scale) and torch.equal(a[2], b[2])
+    same = lambda a, b: torch.equal(a[0], b[0]) and torch.equal(a[1].int8(), b[1].int8()) and torch.equal(a[1].scale, b[1].scale) and torch.equal(a[2], b[2])
     torch.cuda.synchronize()
     s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
     for _ in range(5):
@@ -323,7 +324,7 @@ def test_more_than_2_to_31_values(cuda):
     x[:-3] = 1.0
     y, rows, r = n.both(x, x)
     want, wrows, wr = n.both(x[-3:].clone(), x[-3:].clone())
-    assert torch.equal(y[-3:], want) and torch.equal(rows.codes[-3:], wrows.codes) and torch.equal(rows.scale[-3:], wrows.scale)
+    assert torch.equal(y[-3:], want) and torch.equal(rows.int8()[-3:], wrows.int8()) and torch.equal(rows.scale[-3:], wrows.scale)
     assert torch.equal(r[-3:], wr)
     del y, rows
     xg = r.requires_grad_()

@@ -28,7 +28,18 @@ def matrix(cuda, N, K, seed, sdt=F32):
 
 
 def values(rows):
-    return rows.codes[:, :rows.K].double() * rows.scale.double()[:, None]
+    return rows.int8().double() * rows.scale.double()[:, None]
+
+
+def check_padding(rows):
+    """In the blocks, zeros behind each row; and the documented order."""
+    N, K = rows.N, rows.K
+    b = rows.codes.view(-1, (K + 63) // 64, 16, 4, 16)
+    c = torch.arange(4, device=b.device)
+    r = torch.arange(16, device=b.device)
+    b = torch.stack([b[:, :, r, c[i] ^ (r // 4) % 4] for i in range(4)], 3)      # chunk c of row r at place c ^ (r / 4 % 4)
+    flat = b.permute(0, 2, 1, 3, 4).reshape(b.shape[0] * 16, -1)
+    assert torch.equal(flat[:N, :K], rows.int8()) and not bool(flat[:N, K:].any())
 
 
 def check_quantized(rows, x):
@@ -37,12 +48,13 @@ def check_quantized(rows, x):
     v = x.double().reshape(-1, x.shape[-1])
     top = v.abs().amax(1, keepdim=True)
     z = torch.where(top > 0, v * 127.0 / top, torch.zeros_like(v))
-    codes = rows.codes[:, :rows.K]
+    codes = rows.int8()
     if x.dtype is F32:
         assert bool(((codes.double() - z).abs() <= 0.5 + 2.0 ** -16).all())
     else:
         assert torch.equal(codes, torch.round(z).to(torch.int8))
-    assert torch.equal(rows.scale, (top / top.new_tensor(127.0)).float().view(-1)) and not bool(rows.codes[:, rows.K:].any())
+    assert torch.equal(rows.scale, (top / top.new_tensor(127.0)).float().view(-1))
+    check_padding(rows)
 
 
 def test_ties(cuda):
@@ -70,10 +82,10 @@ def test_quantize_and_dequant(cuda, T, K, dt):
     q = bmx.Q8Matrix.quantize(x)
     check_quantized(q, x)
     for out in (torch.float16, torch.bfloat16, F32):
-        assert torch.equal(q.dequant(out), (q.codes[:, :K].float() * q.scale[:, None]).to(out))
+        assert torch.equal(q.dequant(out), (q.int8().float() * q.scale[:, None]).to(out))
     if dt is not F32:
         r = bmx.ops.quantize_rows(x)
-        assert torch.equal(r.codes, q.codes) and torch.equal(r.scale, q.scale) and r.dtype == dt and r.shape == (T, K)
+        assert torch.equal(r.int8(), q.int8()) and torch.equal(r.scale, q.scale) and r.dtype == dt and r.shape == (T, K)
 
 
 def test_quantize_layouts_and_rows_of_no_numbers(cuda):
@@ -90,15 +102,27 @@ def test_quantize_layouts_and_rows_of_no_numbers(cuda):
         y[2, 3], y[3, 200], y[4, K - 1] = float("nan"), float("inf"), float("-inf")
         q = bmx.ops.quantize_rows(y)
         check_quantized(bmx.ops.quantize_rows(y[[0, 1, 5]]), y[[0, 1, 5]])
-        assert torch.equal(q.codes[[0, 1, 5]], bmx.ops.quantize_rows(y[[0, 1, 5]]).codes)
-        assert not bool(q.codes[1:5].any()) and bool(q.scale[2:5].isnan().all()) and float(q.scale[1]) == 0.0
+        assert torch.equal(q.int8()[[0, 1, 5]], bmx.ops.quantize_rows(y[[0, 1, 5]]).int8())
+        assert not bool(q.int8()[1:5].any()) and bool(q.scale[2:5].isnan().all()) and float(q.scale[1]) == 0.0
         tiny = torch.full((2, K), 2.0 ** -111, device=cuda, dtype=torch.bfloat16)
         tiny[1, 5] = 2.0 ** -110
         q = bmx.ops.quantize_rows(tiny)
-        assert not bool(q.codes[0].any()) and float(q.scale[0]) == 0.0 and int(q.codes[1, 5]) == 127
+        assert not bool(q.int8()[0].any()) and float(q.scale[0]) == 0.0 and int(q.int8()[1, 5]) == 127
         big = torch.full((1, K), 3e38, device=cuda, dtype=torch.bfloat16)
-        assert bool((bmx.ops.quantize_rows(big).codes[:, :K] == 127).all())
-    assert bmx.ops.quantize_rows(x[:0]).N == 0
+        assert bool((bmx.ops.quantize_rows(big).int8() == 127).all())
+    assert bmx.ops.quantize_rows(x[:0]).N == 0 and bmx.ops.quantize_rows(x[:0]).int8().shape == (0, 264)
+
+
+@pytest.mark.parametrize("N,K", [(1, 1), (16, 64), (17, 65), (40, 15), (15, 130), (100, 4096)])
+def test_given_codes(cuda, N, K):
+    """Every code, in and out again, in rows and matrices; transposed and sliced ones too."""
+    import bmx
+    (c, s), _ = matrix(cuda, N, K, seed=N)
+    for given in (c, c.t().contiguous().t(), torch.cat((c, c), 1)[:, :K]):
+        for kind in (bmx.Q8Matrix, bmx.Rows8):
+            q = kind(given, s)
+            assert torch.equal(q.int8(), c) and torch.equal(q.scale, s)
+            check_padding(q)
 
 
 TOKENS = [1, 2, 3, 4, 5, 7, 15, 16, 17, 31, 33, 64, 65, 77, 128, 129, 200, 257, 300]
@@ -402,7 +426,7 @@ def test_refusals(cuda):
         with pytest.raises(TypeError):
             f(q)
     c.zero_()
-    assert bool(q.codes.any())                         # its own copy
+    assert bool(q.int8().any())                        # its own copy
     x = rand(cuda, 3, 256, dt=torch.float16, seed=1)
     rows = bmx.ops.quantize_rows(x)
     for bad in (x.float(), x.cpu(), x[:, :128], x.long(), bmx.ops.quantize_rows(x[:, :128])):
@@ -418,8 +442,8 @@ def test_refusals(cuda):
         q.dequant(torch.float64)
     for kw in (dict(dtype=F32), dict(shape=(2, 256)), dict(shape=(256, 3))):
         with pytest.raises(ValueError):
-            bmx.Rows8(rows.codes, rows.scale, **kw)
-    assert torch.equal(bmx.ops.q8_linear(bmx.Rows8(rows.codes, rows.scale, shape=(1, 3, 256)), q)[0], bmx.ops.q8_linear(x, q))
+            bmx.Rows8(rows.int8(), rows.scale, **kw)
+    assert torch.equal(bmx.ops.q8_linear(bmx.Rows8(rows.int8(), rows.scale, shape=(1, 3, 256)), q)[0], bmx.ops.q8_linear(x, q))
     down = bmx.Q8Matrix(*matrix(cuda, 256, 48, seed=2)[0])
     ffn = bmx.GatedFFN(q, q, down)
     four = bmx.Q4Matrix.quantize(rand(cuda, 48, 256, dt=torch.float16, seed=3), 64)

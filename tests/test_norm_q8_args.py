@@ -7,14 +7,13 @@ import torch
 
 def q8(**k):
     import bmx
-    v = dict(N=72, K=128, ld=128, codes=256, scale=256)
+    v = dict(N=72, K=128, codes=256, scale=256)
     v.update(k)
     return bmx._lib.Q8(*(v[n] for n, _ in bmx._lib.Q8._fields_))
 
 
 @pytest.mark.parametrize("bad,text", [(dict(N=0), b"N (0)"), (dict(N=-1), b"N (-1)"), (dict(N=(1 << 24) + 1), b"2^24"), (dict(K=0), b"131071"),
-                                      (dict(K=131072, ld=131072), b"131071"), (dict(ld=120), b"ld"), (dict(ld=112), b"ld"), (dict(ld=136), b"ld"),
-                                      (dict(ld=1 << 21), b"ld"), (dict(K=129), b"ld"), (dict(codes=None), b"null"), (dict(scale=None), b"null"),
+                                      (dict(K=131072), b"131071"), (dict(codes=None), b"null"), (dict(scale=None), b"null"),
                                       (dict(codes=264), b"aligned"), (dict(scale=258), b"aligned")])
 def test_matrix_refusals(bad, text):
     import bmx
@@ -22,6 +21,8 @@ def test_matrix_refusals(bad, text):
     q = q8(**bad)
     assert L.bmx_q8_quantize(256, 0, q, None) == E and text in L.bmx_last_error()
     assert L.bmx_q8_dequant(q, 0, 256, None) == E and text in L.bmx_last_error()
+    assert L.bmx_q8_pack(q, 256, None) == E and text in L.bmx_last_error()
+    assert L.bmx_q8_unpack(q, 256, None) == E and text in L.bmx_last_error()
     assert L.bmx_q8_linear_workspace(q, 100) == 0 and text in L.bmx_last_error()
     assert L.bmx_q8_linear(q, 0, 256, None, 4, 256, 256, 1 << 30, None) == E and text in L.bmx_last_error()
     # as rows of a call
@@ -42,7 +43,9 @@ def test_product_call_refusals():
         assert L.bmx_q8_quantize(256, dt, q, None) == E and L.bmx_q8_dequant(q, dt, 256, None) == E
     assert L.bmx_q8_quantize(None, 0, q, None) == E and L.bmx_q8_quantize(257, 0, q, None) == E and L.bmx_q8_quantize(258, 2, q, None) == E
     assert L.bmx_q8_dequant(q, 0, None, None) == E and L.bmx_q8_dequant(q, 0, 264, None) == E
-    assert L.bmx_q8_dequant(q8(N=1 << 24, K=131071, ld=131072), 0, 256, None) == E and b"too many" in L.bmx_last_error()
+    assert L.bmx_q8_dequant(q8(N=1 << 24, K=131071), 0, 256, None) == E and b"too many" in L.bmx_last_error()
+    assert L.bmx_q8_pack(q, None, None) == E and L.bmx_q8_unpack(q, None, None) == E
+    assert L.bmx_q8_code_bytes(72, 128) == 80 * 128 and L.bmx_q8_code_bytes(1, 1) == 1024 and L.bmx_q8_code_bytes(0, 1) == 0
     lin = lambda dt=0, x=256, r=None, T=40, y=256, ws=256, n=1 << 30: L.bmx_q8_linear(q, dt, x, r, T, y, ws, n, None)
     assert lin(dt=2) == E and lin(x=None) == E and lin(r=rows) == E and lin(x=264) == E and lin(y=None) == E and lin(y=264) == E
     assert lin(T=-1) == E and lin(T=(1 << 24) + 1) == E and lin(T=0, x=None, y=None, ws=None, n=0) == 0
@@ -52,11 +55,11 @@ def test_product_call_refusals():
     assert L.bmx_q8_linear_workspace(q, -1) == 0 and L.bmx_q8_linear_workspace(q, 0) == 0
 
     three = lambda a, b, c, **k: bmx._lib.Ffn8Desc(k.get("dtype", 0), k.get("act", 0), k.get("limit", 0.0), 0, *map(ctypes.pointer, (a, b, c)))
-    gu, dn = q8(N=72, K=128), q8(N=128, K=72, ld=80)
+    gu, dn = q8(N=72, K=128), q8(N=128, K=72)
     good = three(gu, gu, dn)
     need = L.bmx_ffn8_workspace(good, 4)
     assert need >= 4 * 72 * 4
-    for d, text in ((three(gu, dn, dn), b"[I, H]"), (three(gu, gu, gu), b"[I, H]"), (three(gu, q8(N=72, K=128, ld=144), dn), b"one length"),
+    for d, text in ((three(gu, dn, dn), b"[I, H]"), (three(gu, gu, gu), b"[I, H]"),
                     (three(gu, gu, dn, dtype=2), b"dtype"), (three(gu, gu, dn, act=4), b"activation"), (three(gu, gu, dn, limit=-1.0), b"act_limit"),
                     (three(gu, gu, dn, limit=float("nan")), b"act_limit"), (three(q8(N=72, K=124), q8(N=72, K=124), q8(N=124, K=72)), b"multiples of 8"),
                     (None, b"null")):
@@ -96,11 +99,11 @@ def test_norm_call_refusals():
     import bmx
     L, E, W = bmx.lib(), bmx._lib.BMX_ERR_ARG, bmx._lib.BMX_ERR_WORKSPACE
     d = norm()
-    rows = q8(N=4, K=64, ld=64)
+    rows = q8(N=4, K=64)
     fwd = lambda x=256, res=None, T=4, r=None, y=256, rows=None: L.bmx_rms_norm(d, x, res, T, r, y, rows, None)
     assert fwd(x=None) == E and fwd(x=264) == E and fwd(res=256) == E and fwd(r=256) == E and fwd(res=264, r=256) == E and fwd(res=256, r=264) == E
     assert fwd(y=None) == E and fwd(y=264) == E and fwd(T=-1) == E and fwd(T=(1 << 24) + 1) == E and fwd(T=0, x=None, y=None) == 0
-    assert fwd(rows=q8(N=3, K=64, ld=64)) == E and fwd(rows=q8(N=4, K=56, ld=64)) == E and fwd(rows=q8(N=4, K=64, ld=48)) == E
+    assert fwd(rows=q8(N=3, K=64)) == E and fwd(rows=q8(N=4, K=56)) == E
     need = L.bmx_rms_norm_backward_workspace(d, 1000)
     assert need >= 512 * 64 * 4 and rows.N == 4
     back = lambda v=256, s=1, T=1000, dy=256, dr=None, dx=256, ds=None, dw=256, ws=256, n=need: L.bmx_rms_norm_backward(
@@ -130,6 +133,6 @@ def test_struct_sizes_are_the_headers():
     """The ctypes structs have the header's layout (natural alignment, 64-bit pointers)."""
     import bmx
     L = bmx._lib
-    assert ctypes.sizeof(L.Q8) == 32 and L.Q8.ld.offset == 8 and L.Q8.scale.offset == 24
+    assert ctypes.sizeof(L.Q8) == 24 and L.Q8.codes.offset == 8 and L.Q8.scale.offset == 16
     assert ctypes.sizeof(L.Ffn8Desc) == 40 and L.Ffn8Desc.gate.offset == 16
     assert ctypes.sizeof(L.NormDesc) == 32 and L.NormDesc.weight.offset == 24
