@@ -7,14 +7,14 @@ from . import _lib as L
 from .ffn import DTYPES, _modes, _tracing, eager_only, forward_ad, rows_of, stream_here
 from .q8 import ROW_DTYPES, Rows8
 
-MOST_H = 32768
+MOST_H = 16384
 
 
 class RMSNorm:
     """y = v w / sqrt(mean(v^2) + eps) over the last dimension, v = x, or x + residual as the stream holds it: r = x + residual is
     summed in fp32 and rounded to residual's type, and the norm is of r.
 
-    weight: [H] fp16, bf16 or fp32, contiguous on a device, H a multiple of 8 to 32,768; dtype: of y, fp16 or bf16 (default the
+    weight: [H] fp16, bf16 or fp32, contiguous on a device, H a multiple of 8 to 16,384; dtype: of y, fp16 or bf16 (default the
     weight's; fp32 weights need it). x and residual [..., H] of dtype or fp32 each, so that a MoELayer's fp32 output can go into a
     stream of 16 bits. forward(x) -> y; forward(x, residual) -> (y, r). Where autograd records, y and r carry the gradients of x,
     residual and weight (the rounding of r passes them as they are); the forward pass then keeps r (x without a residual), which must

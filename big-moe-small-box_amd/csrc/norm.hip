@@ -7,6 +7,8 @@
 //   dv = rstd (g - v c) + dr,  dx = dresidual = dv,  dw = sum over the rows of dy v rstd
 // (the rounding of s to r passes a gradient as it is). Everything is bound by the bytes of the rows: each is read once and kept in
 // registers, and rstd is computed again from them in the backward pass, which has to read v anyhow.
+#include <algorithm>
+
 #include "rows8.hpp"
 
 namespace bmx {
@@ -17,27 +19,34 @@ struct NormArgs {
     int8_t* codes;
     float* scale;
     int blocks;                     // q8_blocks(H)
+    int spread;                     // rows to workgroups by blocks of 16
     int T, H;
     int xt, rt, wt, yt;             // row types
     float eps;
 };
 
-// A row by W of a workgroup's NW waves, CH chunks of 8 values a lane
-template <int NW, int W, int CH>
-__global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
+// A workgroup a row, CH chunks of 8 values a lane. One chunk and as many waves as that takes (16 at most) is the fastest: 8,192 rows of
+// 4,096 with two tensors in and two out 52 us (5.1 TB/s, as a copy), with half the waves and two chunks a lane 56, with one wave a
+// row 96; of 5,120 82 us with five waves, 92 with eight of which most have nothing in their second chunk.
+template <int CH>
+__global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
 {
-    __shared__ float ssum[NW];
-    __shared__ uint32_t smax[NW];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), part = wave % W;
-    const int64_t t = (int64_t)blockIdx.x * (NW / W) + wave / W;
-    const bool on = t < p.T;
-    const int64_t row = (on ? t : p.T - 1) * p.H;
-    float v[CH][8], vw[CH][8];
+    __shared__ float ssum[16];
+    __shared__ uint32_t smax[16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    // With codes, rows of one block of 16 on one XCD (workgroups are dealt to the 8 in turn), whose L2 then joins their 64 bytes of a
+    // block to whole lines
+    int64_t t = blockIdx.x;
+    if (p.spread) t = ((t >> 3) / Q8_ROWS * 8 + (t & 7)) * Q8_ROWS + (t >> 3) % Q8_ROWS;
+    if (t >= p.T) return;
+    const int64_t row = t * p.H;
+    float v[CH][8];                                                // the row, then v w
     Raw8 x[CH], res[CH], w[CH];
+    auto at = [&](int c) { return (int)(threadIdx.x + c * blockDim.x) * 8; };
 #pragma unroll
     for (int c = 0; c < CH; ++c)
     {
-        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        const int h = at(c);
         if (h >= p.H) continue;
         x[c] = load_raw8(p.x, p.xt, row + h);
         if (p.res) res[c] = load_raw8(p.res, p.rt, row + h);
@@ -48,7 +57,7 @@ __global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
 #pragma unroll
     for (int c = 0; c < CH; ++c)
     {
-        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        const int h = at(c);
         if (h >= p.H) continue;
         to_f32(x[c], p.xt, v[c]);
         if (p.res)
@@ -57,7 +66,7 @@ __global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
             to_f32(res[c], p.rt, a);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] += a[i];
-            if (on) store8(p.r, p.rt, row + h, v[c]);
+            store8(p.r, p.rt, row + h, v[c]);
         }
         float b[8];
         if (p.w) to_f32(w[c], p.wt, b);
@@ -65,54 +74,51 @@ __global__ __launch_bounds__(NW * 64) void norm_k(const NormArgs p)
         for (int i = 0; i < 8; ++i)
         {
             ssq = __builtin_fmaf(v[c][i], v[c][i], ssq);
-            vw[c][i] = p.w ? v[c][i] * b[i] : v[c][i];
-            top = max(top, mag(vw[c][i]));
+            if (p.w) v[c][i] *= b[i];
+            top = max(top, mag(v[c][i]));
         }
     }
-    ssq = wave_sum(ssq);
+    if (p.w) ssq = wave_sum(ssq);
     if (p.codes) top = wave_max(top);
-    if (W > 1)
+    if (waves > 1)
     {
         if (lane == 0) { ssum[wave] = ssq; smax[wave] = top; }
         lds_barrier();
-        const int w0 = wave - part;
         ssq = 0.0f;
-#pragma unroll
-        for (int i = 0; i < W; ++i)
+        for (int i = 0; i < waves; ++i)
         {
-            ssq += ssum[w0 + i];
-            top = max(top, smax[w0 + i]);
+            ssq += ssum[i];
+            top = max(top, smax[i]);
         }
     }
-    if (!on) return;
     const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
     const Top8 q = top8(top);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
     {
-        const int h = (part * 64 + lane + c * (W * 64)) * 8;
+        const int h = at(c);
         if (p.codes && h < p.blocks * Q8_COLS)
             *reinterpret_cast<u32x2*>(p.codes + q8_at(t, h, p.blocks)) =
-                h < p.H ? u32x2{codes4(vw[c], q), codes4(vw[c] + 4, q)} : u32x2{0, 0};
+                h < p.H ? u32x2{codes4(v[c], q), codes4(v[c] + 4, q)} : u32x2{0, 0};
         if (p.y && h < p.H)
         {
             float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = vw[c][i] * rstd;
+            for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd;
             store8(p.y, p.yt, row + h, y);
         }
     }
-    if (p.codes && part == 0 && lane == 0) p.scale[t] = p.w ? q.scale * rstd : q.scale;
+    if (p.codes && threadIdx.x == 0) p.scale[t] = p.w ? q.scale * rstd : q.scale;
 }
 
-// Waves of a row: one where there are rows enough to fill the chip with them and a lane holds all of its values, else eight
-static int launch_norm(const NormArgs& a, hipStream_t s)
+static int launch_norm(NormArgs a, hipStream_t s)                  // H <= BMX_NORM_MAX_H
 {
-    const bool wave = a.T >= 2048;
-    if (a.H <= 2048 && wave) hipLaunchKernelGGL((norm_k<4, 1, 4>), dim3((a.T + 3) / 4), dim3(256), 0, s, a);
-    else if (a.H <= 4096) hipLaunchKernelGGL((norm_k<8, 8, 1>), dim3(a.T), dim3(512), 0, s, a);
-    else if (a.H <= 8192) hipLaunchKernelGGL((norm_k<8, 8, 2>), dim3(a.T), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((norm_k<8, 8, 8>), dim3(a.T), dim3(512), 0, s, a);
+    const int chunks = (a.H + 511) / 512;                          // of a wave
+    a.spread = a.codes && a.T >= 8 * Q8_ROWS;
+    const dim3 grid((unsigned)(a.spread ? round_up(a.T, 8 * Q8_ROWS) : a.T));
+    // (two chunks: 12 waves for 11,008 values 155 us, 11 174)
+    if (chunks <= 16) hipLaunchKernelGGL((norm_k<1>), grid, dim3(chunks * 64), 0, s, a);
+    else hipLaunchKernelGGL((norm_k<2>), grid, dim3((unsigned)round_up((chunks + 1) / 2, 4) * 64), 0, s, a);
     return check_launch("rms_norm");
 }
 
@@ -164,16 +170,17 @@ struct NormBackArgs {
     float eps;
 };
 
-// A workgroup takes every gridDim.x-th row, the next row's loads on their way while one is summed up, and keeps its rows' sums for the
-// weight's gradient in registers
-template <int NW, int CH>
-__global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
+// A workgroup takes every gridDim.x-th row and keeps its rows' sums for the weight's gradient in registers, and for rows of one chunk a
+// lane the weight; the next row's loads are then on their way while one is summed up (two chunks do not leave registers for that).
+template <int CH>
+__global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
 {
-    __shared__ f32x4 red[2][NW];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    float w[CH][8], dw[CH][8];
+    constexpr bool ONE = CH == 1;
+    __shared__ f32x2 red[2][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    float w[8], dw[CH][8];
     Raw8 v[CH], dy[CH], dr[CH];
-    auto at = [&](int c) { return (wave * 64 + lane + c * (NW * 64)) * 8; };
+    auto at = [&](int c) { return (int)(threadIdx.x + c * blockDim.x) * 8; };
     auto load = [&](int t) {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
@@ -185,15 +192,14 @@ __global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
             if (p.dr) dr[c] = load_raw8(p.dr, p.rt, i);
         }
     };
+    auto weight = [&](int c) { to_f32(load_raw8(p.w, p.wt, at(c)), p.wt, w); };
     int t = blockIdx.x;
     load(t);
+    if (ONE && at(0) < p.H) weight(0);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
-    {
-        if (at(c) < p.H) to_f32(load_raw8(p.w, p.wt, at(c)), p.wt, w[c]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
-    }
     for (int set = 0; t < p.T; t += gridDim.x, set ^= 1)
     {
         float a[CH][8], d[CH][8], more[CH][8];
@@ -204,24 +210,24 @@ __global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
             if (at(c) >= p.H) continue;
             to_f32(v[c], p.vt, a[c]);
             to_f32(dy[c], p.yt, d[c]);
-            if (p.dr) to_f32(dr[c], p.rt, more[c]);
+            if (ONE && p.dr) to_f32(dr[c], p.rt, more[c]);
+            if (!ONE) weight(c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
             {
                 ssq = __builtin_fmaf(a[c][i], a[c][i], ssq);
-                dot = __builtin_fmaf(d[c][i] * w[c][i], a[c][i], dot);
+                dot = __builtin_fmaf(d[c][i] * w[i], a[c][i], dot);
             }
         }
-        if (t + (int)gridDim.x < p.T) load(t + gridDim.x);
+        if (ONE && t + (int)gridDim.x < p.T) load(t + gridDim.x);
         ssq = wave_sum(ssq);
         dot = wave_sum(dot);
-        if (lane == 0) red[set][wave] = f32x4{ssq, dot, 0.0f, 0.0f};
+        if (lane == 0) red[set][wave] = f32x2{ssq, dot};
         lds_barrier();
         ssq = dot = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NW; ++i)
+        for (int i = 0; i < waves; ++i)
         {
-            const f32x4 one = red[set][i];
+            const f32x2 one = red[set][i];
             ssq += one[0];
             dot += one[1];
         }
@@ -233,10 +239,15 @@ __global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
             if (at(c) >= p.H) continue;
             const int64_t at_row = (int64_t)t * p.H + at(c);
             float o[8], q[8];
+            if (!ONE)
+            {
+                weight(c);
+                if (p.dr) to_f32(dr[c], p.rt, more[c]);
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
             {
-                o[i] = rstd * (d[c][i] * w[c][i] - a[c][i] * k);
+                o[i] = rstd * (d[c][i] * w[i] - a[c][i] * k);
                 if (p.dr) o[i] += more[c][i];
                 q[i] = o[i];
                 dw[c][i] = __builtin_fmaf(d[c][i], a[c][i] * rstd, dw[c][i]);
@@ -244,6 +255,7 @@ __global__ __launch_bounds__(NW * 64) void norm_back_k(const NormBackArgs p)
             if (p.dx) store8(p.dx, p.xt, at_row, o);
             if (p.dres) store8(p.dres, p.rt, at_row, q);
         }
+        if (!ONE && t + (int)gridDim.x < p.T) load(t + gridDim.x);
     }
     if (!p.part) return;
 #pragma unroll
@@ -277,16 +289,16 @@ __global__ __launch_bounds__(512) void norm_weight_k(const float* __restrict__ p
     else static_cast<uint16_t*>(dw)[c] = (uint16_t)bits16(wt, sum);
 }
 
-constexpr int NORM_BACK_WG = 512;   // workgroups of a backward pass, two on each compute unit
-
-static int norm_back_groups(int T) { return T < NORM_BACK_WG ? T : NORM_BACK_WG; }
+// Waves of a row and workgroups of a backward pass: as many as the compute units hold at once, 16 waves each (8,192 rows of 4,096: 512
+// workgroups 66 us, 256 96, 768 79, 1,024 69)
+static int norm_back_waves(int H) { return H <= 8192 ? (H + 511) / 512 : (H + 1023) / 1024; }
+static int norm_back_groups(int T, int H) { return std::min(T, 256 * (16 / norm_back_waves(H))); }
 
 static int launch_norm_back(const NormBackArgs& a, hipStream_t s)
 {
-    const dim3 grid(norm_back_groups(a.T));
-    if (a.H <= 4096) hipLaunchKernelGGL((norm_back_k<8, 1>), grid, dim3(512), 0, s, a);
-    else if (a.H <= 8192) hipLaunchKernelGGL((norm_back_k<8, 2>), grid, dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((norm_back_k<8, 8>), grid, dim3(512), 0, s, a);
+    const dim3 grid(norm_back_groups(a.T, a.H)), block(norm_back_waves(a.H) * 64);
+    if (a.H <= 8192) hipLaunchKernelGGL((norm_back_k<1>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((norm_back_k<2>), grid, block, 0, s, a);
     return check_launch("rms_norm_backward");
 }
 
@@ -352,7 +364,7 @@ int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual,
 size_t bmx_rms_norm_backward_workspace(const bmx_norm_desc* desc, int T)
 {
     if (check_norm(desc, T, "bmx_rms_norm_backward_workspace")) return 0;
-    return align_up((size_t)(T ? norm_back_groups(T) : 1) * desc->H * 4, 256);
+    return align_up((size_t)(T ? norm_back_groups(T, desc->H) : 1) * desc->H * 4, 256);
 }
 
 int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, int T, const void* dy, const void* dr, void* dx,
@@ -387,7 +399,7 @@ int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, 
     a.wt = desc->weight_dtype; a.yt = desc->dtype; a.rt = desc->residual_dtype; a.xt = desc->x_dtype;
     a.eps = desc->eps;
     if ((rc = launch_norm_back(a, s)) || !dweight) return rc;
-    hipLaunchKernelGGL(norm_weight_k, dim3((desc->H + 31) / 32), dim3(512), 0, s, a.part, norm_back_groups(T), desc->H, dweight,
+    hipLaunchKernelGGL(norm_weight_k, dim3((desc->H + 31) / 32), dim3(512), 0, s, a.part, norm_back_groups(T, desc->H), desc->H, dweight,
                        desc->weight_dtype);
     return check_launch("norm_weight");
 }

@@ -19,6 +19,7 @@ inline size_t row_type_bytes(int t) { return t == ROW_F32 ? 4 : 2; }
 
 // 8 values as they lie in memory: the second half for fp32 alone
 struct Raw8 { u32x4 a, b; };
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // values i .. i + 7 of p (16-byte aligned)
 __device__ __forceinline__ Raw8 load_raw8(const void* p, int type, int64_t i)

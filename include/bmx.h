@@ -588,7 +588,7 @@ int bmx_ffn8_add(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, i
  * eps), rounded once to dtype; rows: the same in 8 bits with a scale per token (rows->N = T, K = H), not through y: code = round(v w
  * 127 / max |v w|). x, residual and the weight [H] of dtype or fp32, contiguous, 16-byte aligned; H a multiple of 8. sum may be
  * residual or x, if of its type; y apart from all but x. sum goes with residual; y or rows may be NULL. */
-#define BMX_NORM_MAX_H 32768
+#define BMX_NORM_MAX_H 16384
 typedef struct bmx_norm_desc {
     int32_t H, dtype;                              /* dtype: fp16 or bf16 */
     int32_t x_dtype, residual_dtype, weight_dtype;

@@ -4,9 +4,9 @@ import torch
 import ffn_ref as R
 
 STEP = 2.0 ** -23          # one step of an fp32 value, relative; a rounding is off by half of it
-# A row's sums: a lane's chain (at most 64 values), its wave's six steps and up to eight waves: each value passes fewer than 80
+# A row's sums: a lane's chain (at most 16 values), its wave's six steps and up to 16 waves: each value passes fewer than 40
 # additions. Of a sum of squares, all terms positive, that is its relative error.
-CHAIN = 80 * STEP / 2
+CHAIN = 40 * STEP / 2
 # rstd: half of the sum's, and division by H, sum with eps, root and reciprocal, each within a step
 RSTD = CHAIN / 2 + 4 * STEP
 
@@ -31,8 +31,8 @@ def norm_grads(v, w, eps, dy, dr):
         ev = ev + STEP * (dv.abs() + ev + dr.abs())
         dv = dv + dr
     t = dy * v * rstd
-    # a column: a workgroup's rows one after the other, every 64th workgroup, 64 groups
-    adds = (T + 511) // 512 + 8 + 64
+    # a column: a workgroup's rows one after the other (of 256 workgroups at least), every 64th of at most 4,096 workgroups, 64 groups
+    adds = (T + 255) // 256 + 64 + 64
     return dv, ev, t.sum(0), t.abs().sum(0) * (RSTD + 2 * STEP + adds * STEP)
 
 

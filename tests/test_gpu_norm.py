@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 DT = {"fp16": torch.float16, "bf16": torch.bfloat16}
 F32 = torch.float32
 SIZES = [(1, 8), (2, 24), (3, 512), (1, 520), (5, 1000), (4, 2048), (7, 2056), (1, 4096), (3, 4104), (2, 5120), (33, 768), (513, 136), (2, 8192),
-         (3, 8200), (2, 11008), (1, 32768), (2049, 64), (2050, 2048), (2051, 2064), (2052, 5120)]
+         (3, 8200), (2, 11008), (1, 16384), (2049, 64), (2050, 2048), (2051, 2064), (2052, 5120)]
 
 
 def make(cuda, T, H, dt, x32=False, r32=False, w32=False, seed=1):
@@ -112,7 +112,7 @@ def backward_check(cuda, T, H, dt, x32=False, r32=False, w32=False, residual=Tru
 
 
 @pytest.mark.parametrize("dt", sorted(DT))
-@pytest.mark.parametrize("T,H", SIZES + [(600, 4096), (1100, 520), (1030, 8200)])
+@pytest.mark.parametrize("T,H", SIZES + [(600, 4096), (1100, 520), (1030, 8200), (300, 16384), (4200, 64)])
 def test_gradients(cuda, T, H, dt):
     backward_check(cuda, T, H, DT[dt], seed=T + H)
 
@@ -316,7 +316,7 @@ def test_captured_training_step(cuda):
 def test_more_than_2_to_31_values(cuda):
     """Rows whose values lie past 2^31: the last ones as they are alone."""
     import bmx
-    T, H = 70000, 32768
+    T, H = 140000, 16384
     w = torch.randn(H, device=cuda).half()
     n = bmx.RMSNorm(w)
     x = torch.empty((T, H), device=cuda, dtype=torch.float16)
@@ -360,7 +360,7 @@ def test_replaced_weight_and_options(cuda):
 def test_refusals(cuda):
     import bmx
     x, res, w = make(cuda, 4, 64, torch.float16)
-    for bad in (w[:60].clone(), w.cpu(), w.view(1, 64), w.long(), torch.ones(128, device=cuda).half()[::2], w[:0], torch.ones(32776, device=cuda).half()):
+    for bad in (w[:60].clone(), w.cpu(), w.view(1, 64), w.long(), torch.ones(128, device=cuda).half()[::2], w[:0], torch.ones(16392, device=cuda).half()):
         with pytest.raises(ValueError):
             bmx.RMSNorm(bad)
     for kw in (dict(eps=0.0), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=1e-60), dict(eps=float("inf")), dict(dtype=torch.bfloat16), dict(dtype=F32)):
