@@ -26,7 +26,9 @@ def rows_of(x, K, dtype, device, name):
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
-_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch.cuda.current_device
+_raw_stream = torch._C._cuda_getCurrentRawStream
+# (torch.cuda.current_device behind its check that CUDA runs, which it does where a device tensor is)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def stream_here(device):

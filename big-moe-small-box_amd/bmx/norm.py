@@ -63,31 +63,43 @@ class RMSNorm:
             self._descs[xt, rt] = d
         return d
 
-    def _rows(self, x, name):
-        if x.dtype is not self._out and x.dtype is not torch.float32:
-            raise ValueError(f"RMSNorm: {name} must be {self._out} or fp32, got {x.dtype}")
-        return rows_of(x, self.hidden_size, x.dtype, self.device, name)
+    def _given(self, x, name):
+        """x of [..., H], checked, contiguous and 16-byte aligned (a copy only where it is neither), and its address."""
+        dt, shape = x.dtype, x.shape
+        if (dt is not self._out and dt is not torch.float32) or x.device != self.device or not shape or shape[-1] != self.hidden_size:
+            raise ValueError(f"RMSNorm: expected {name} {self._out} or fp32 [..., {self.hidden_size}] on {self.device}, got {dt} {tuple(shape)} "
+                             f"on {x.device}")
+        p = x.data_ptr()
+        if p & 15 or not x.is_contiguous():
+            x = x.clone(memory_format=torch.contiguous_format)
+            p = x.data_ptr()
+        return x, p
 
     def _run(self, x, residual, want_y, want_rows):
         """(y, rows, r), None what is not wanted. Behind _current()."""
-        a = self._rows(x, "RMSNorm: x")
-        b = None
+        x, xp = self._given(x, "x")
+        H, rp, r, sp = self.hidden_size, None, None, None
         if residual is not None:
-            b = self._rows(residual, "RMSNorm: residual")
+            residual, rp = self._given(residual, "residual")
             if residual.shape != x.shape:
                 raise ValueError(f"RMSNorm: x {tuple(x.shape)} and residual {tuple(residual.shape)} must be of one shape")
         s = stream_here(self.device)
         if s is None:
             with torch.cuda.device(self.device):
                 return self._run(x, residual, want_y, want_rows)
-        T, H = a.shape
-        y = a.new_empty(x.shape, dtype=self._out) if want_y else None
-        r = b.new_empty(x.shape) if b is not None else None
+        T, xt, yp = x.numel() // H, x.dtype, None
+        if residual is not None:
+            r = torch.empty_like(residual)
+            sp, rt = r.data_ptr(), residual.dtype
+        else:
+            rt = xt
+        y = None
+        if want_y:
+            y = torch.empty_like(x) if xt is self._out else torch.empty_like(x, dtype=self._out)
+            yp = y.data_ptr()
         rows = Rows8._empty(T, H, self.device, self._out, x.shape) if want_rows else None
         if T:
-            rc = L.lib().bmx_rms_norm(self._desc(a.dtype, a.dtype if b is None else b.dtype), a.data_ptr(),
-                                      b.data_ptr() if b is not None else None, T, r.data_ptr() if r is not None else None,
-                                      y.data_ptr() if want_y else None, rows.struct if want_rows else None, s)
+            rc = L.lib().bmx_rms_norm(self._desc(xt, rt), xp, rp, T, sp, yp, rows.struct if want_rows else None, s)
             if rc:
                 L.check(rc, "bmx_rms_norm")
         return y, rows, r
@@ -97,8 +109,8 @@ class RMSNorm:
         self._current()
         if forward_ad._current_level >= 0 or _tracing() or _modes():
             eager_only(who, x, residual, self.weight)
-        return torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad or
-                                            (residual is not None and residual.requires_grad))
+        return ((x.requires_grad or self.weight.requires_grad or (residual is not None and residual.requires_grad)) and
+                torch.is_grad_enabled())
 
     def forward(self, x, residual=None):
         if self._enter("RMSNorm", x, residual):
@@ -131,7 +143,7 @@ class RMSNorm:
 class _RMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, norm):
-        y, _, r = norm._run(x.detach(), None if residual is None else residual.detach(), True, False)
+        y, _, r = norm._run(x, residual, True, False)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(weight, x if r is None else r)
         ctx.xt, ctx.summed, ctx.eps, ctx.out, ctx.H = x.dtype, r is not None, norm.eps, norm._out, norm.hidden_size

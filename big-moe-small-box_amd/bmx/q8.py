@@ -9,15 +9,11 @@ ROW_DTYPES = {**DTYPES, torch.float32: L.DT_FP32}
 MOST_K = 131071
 
 
-def code_bytes(N, K):
-    """bmx_q8_code_bytes: 16 rows x 64 columns a block."""
-    return (N + 15) // 16 * ((K + 63) // 64) * 1024
-
-
 class _Codes8:
-    """codes int8 in the kernels' order (bmx_q8) and scale fp32 [N], on one device: what Q8Matrix and Rows8 have in common."""
+    """codes int8 in the kernels' order (bmx_q8) and scale fp32 [N], views of one allocation: what Q8Matrix and Rows8 have in
+    common."""
 
-    _fixed = ("N", "K", "device", "codes", "scale", "struct")
+    _fixed = ("N", "K", "device", "codes", "scale", "struct", "_held")
 
     def __setattr__(self, name, value):
         if name in self._fixed:
@@ -28,9 +24,21 @@ class _Codes8:
         """A copy has codes of its own: made again from this one's, since the struct holds addresses."""
         raise TypeError(f"{type(self).__name__} cannot be pickled or copied (its struct holds device addresses)")
 
-    def _set(self, N, K, codes, scale):
-        struct = L.Q8(N, K, codes.data_ptr() or None, scale.data_ptr() or None)
-        self.__dict__.update(N=N, K=K, device=codes.device, codes=codes, scale=scale, struct=struct)
+    def _make(self, N, K, device):
+        """Codes and behind them scales of one allocation, not yet written."""
+        n = (N + 15) // 16 * ((K + 63) // 64) * 1024
+        held = torch.empty(n + 4 * N, dtype=torch.int8, device=device)
+        p = held.data_ptr()
+        d = self.__dict__
+        d["N"], d["K"], d["device"], d["_held"], d["struct"] = N, K, device, held, L.Q8(N, K, p or None, p + n if p else None)
+
+    @property
+    def codes(self):
+        return self._held[:self._held.numel() - 4 * self.N]
+
+    @property
+    def scale(self):
+        return self._held[self._held.numel() - 4 * self.N:].view(torch.float32)
 
     def _given(self, codes, scale, rows):
         """A user's codes [N, K] and scales [N], copied into the kernels' order."""
@@ -43,10 +51,9 @@ class _Codes8:
         if scale.dtype not in ROW_DTYPES or scale.numel() != N or scale.device != codes.device or scale.dim() not in (1, 2):
             raise ValueError(f"{who}: scale must be an fp32, fp16 or bf16 tensor of {N} values on {codes.device}, got {scale.dtype} "
                              f"{tuple(scale.shape)} on {scale.device}")
-        codes = codes.detach().contiguous()
-        self._set(N, K, torch.empty(code_bytes(N, K), dtype=torch.int8, device=codes.device),
-                  scale.detach().reshape(-1).to(torch.float32, copy=True))
-        self._call("bmx_q8_pack", codes)
+        self._make(N, K, codes.device)
+        self.scale.copy_(scale.detach().reshape(-1))
+        self._call("bmx_q8_pack", codes.detach().contiguous())
 
     def _call(self, name, *args):
         """A library call on this and args (tensors by address), on the current stream of its device; nothing for no rows."""
@@ -76,8 +83,7 @@ def _quantized(to, x, N, K):
     if s is None:
         with torch.cuda.device(x.device):
             return _quantized(to, x, N, K)
-    to._set(N, K, torch.empty(code_bytes(N, K), dtype=torch.int8, device=x.device),
-            torch.empty(N, dtype=torch.float32, device=x.device))
+    to._make(N, K, x.device)
     if N:
         rc = L.lib().bmx_q8_quantize(x.data_ptr(), ROW_DTYPES[x.dtype], to.struct, s)
         if rc:
@@ -125,8 +131,9 @@ class Rows8(_Codes8):
     @classmethod
     def _empty(cls, T, K, device, dtype, shape):
         r = cls.__new__(cls)
-        r._set(T, K, torch.empty(code_bytes(T, K), dtype=torch.int8, device=device), torch.empty(T, dtype=torch.float32, device=device))
-        r.__dict__.update(dtype=dtype, shape=shape)
+        r._make(T, K, device)
+        d = r.__dict__
+        d["dtype"], d["shape"] = dtype, shape
         return r
 
     @classmethod

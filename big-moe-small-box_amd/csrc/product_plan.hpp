@@ -208,6 +208,16 @@ constexpr int Q8_K = 128;   // columns of a K tile (gemm8_k): as many bytes as g
 
 // A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 80 tokens, else gemm8_k's tiles
 inline bool q8_few(int T) { return T <= 80; }
+// skinny8_k: tiles of 16 rows of W per workgroup, 1 or 2. A compute unit reads the tokens once per workgroup and its rows of W, from L2
+// and HBM alike at what its L1 takes, and the unit with the most workgroups is the last to end. us with 1 / 2: 77 tokens 4096 -> 14336
+// 25.3 / 19.4, 2304 -> 5120 9.6 / 7.8, 64 tokens 4096 -> 4096 8.3 / 9.3, 33 tokens 5120 -> 2304 7.8 / 9.0, 2304 -> 5120 7.4 / 6.3; one
+// token 4096 -> 14336 11.7 / 11.2, 14336 -> 4096 11.4 / 12.4.
+inline int q8_few_rows(int N, int T, int products, bool fused)
+{
+    const int64_t tiles = (int64_t)((N + 15) / 16) * products, x = fused ? 0 : (T + 15) / 16;
+    auto cost = [&](int rt) { return ((tiles + rt - 1) / rt + 255) / 256 * (rt + x); };
+    return cost(2) < cost(1) ? 2 : 1;
+}
 inline TilePlan q8_plan(int N, int K, int T, int products)
 {
     return plan_product((int64_t)N * products, T, (K + Q8_K - 1) / Q8_K, 1, true);

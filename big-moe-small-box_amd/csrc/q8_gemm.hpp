@@ -1,7 +1,7 @@
 // Products of 8-bit integers: y[t][n] = sx[t] sw[n] sum_k a[t][k] c[n][k], the sum exact in int32 (K <= 131,071), so that a result
 // does not depend on tiles, splits or the tokens beside it. Both factors lie in blocks of 16 rows x 64 columns (rows8.hpp).
 //
-// skinny8_k: to 80 tokens, bound by the bytes of W. A workgroup has 16 rows of W (eight of gate and eight of up in the gated
+// skinny8_k: to 80 tokens, bound by the bytes of W. A workgroup has 16 or 32 rows of W (half of gate and half of up in the gated
 // product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
 // ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized by each workgroup itself while
 // its first loads of W are on their way, into LDS: one launch instead of two.
@@ -43,12 +43,12 @@ struct Q8Args {
 inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && T * ((K + 511) / 512) <= S8_SLOTS; }
 inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
-// TT: tiles of 16 tokens
-template <bool FUSED, int TT, int EPI>
+// TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each.
+template <bool FUSED, int TT, int RT, int EPI>
 __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
 {
-    constexpr bool GU = EPI == EPI_GU;
-    constexpr int ROWS = GU ? 8 : 16, D = TT == 1 ? 8 : TT <= 3 ? 4 : 3;     // result columns, blocks in flight
+    constexpr bool GU = EPI == EPI_GU, HALF = GU && RT == 1;
+    constexpr int ROWS = GU ? 8 * RT : 16 * RT, D = TT + RT == 2 ? 8 : TT + RT <= 5 ? 4 : 3;     // result columns, blocks in flight
     static_assert(!FUSED || TT == 1, "one tile of tokens quantized here");
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, q = lane >> 4;
     const int n0 = blockIdx.x * ROWS, KB = q8_blocks(p.K);
@@ -66,26 +66,36 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
             if (t < p.T && h < p.K) raw[n] = load_raw8(p.x, p.xt, (int64_t)t * p.K + h);
         }
 
-    // this lane's row of W, and whose (rows past the last load it again)
-    const int mat = GU ? r >> 3 : 0, n = min(n0 + (GU ? r & 7 : r), p.N - 1);
-    const int8_t* w = p.w[mat] + q8_at(n, q * 16, KB);
+    // this lane's rows of W, and whose (rows past the last load it again)
+    const int8_t* w[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+    {
+        const int mat = HALF ? r >> 3 : GU ? i : 0, n = min(n0 + (HALF ? r & 7 : GU ? r : i * 16 + r), p.N - 1);
+        w[i] = p.w[mat] + q8_at(n, q * 16, KB);
+    }
     const int8_t* xr = FUSED ? nullptr : p.xc + q8_at(r, q * 16, KB);
-    struct Step { u32x4 w, x[FUSED ? 1 : TT]; } st[D];
+    struct Step { u32x4 w[RT], x[FUSED ? 1 : TT]; } st[D];
     auto load = [&](Step& b, int kb) {
-        b.w = ldg4(w + (int64_t)kb * Q8_BLOCK);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) b.w[i] = ldg4(w[i] + (int64_t)kb * Q8_BLOCK);
         if (!FUSED)
 #pragma unroll
             for (int i = 0; i < TT; ++i) b.x[FUSED ? 0 : i] = ldg4(xr + ((int64_t)i * KB + kb) * Q8_BLOCK);
     };
-    i32x4 acc[TT];
+    i32x4 acc[RT][TT];
 #pragma unroll
-    for (int i = 0; i < TT; ++i) acc[i] = i32x4{0, 0, 0, 0};
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < TT; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
     auto multiply = [&](const Step& b, int kb) {
 #pragma unroll
-        for (int i = 0; i < TT; ++i)
+        for (int j = 0; j < TT; ++j)
         {
-            const u32x4 x = FUSED ? *reinterpret_cast<const u32x4*>(xl + min(r, p.T - 1) * xrow + kb * Q8_COLS + q * 16) : b.x[FUSED ? 0 : i];
-            acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, b.w), acc[i], 0, 0, 0);
+            const u32x4 x = FUSED ? *reinterpret_cast<const u32x4*>(xl + min(r, p.T - 1) * xrow + kb * Q8_COLS + q * 16) : b.x[FUSED ? 0 : j];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+                acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, x), __builtin_bit_cast(i32x4, b.w[i]), acc[i][j], 0, 0, 0);
         }
     };
 
@@ -135,17 +145,20 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
     }
 
     // join the waves
-    constexpr int V = TT * 256;                                    // (token tile, element, lane)
+    constexpr int V = RT * TT * 256;                               // (row tile, token tile, element, lane)
     __shared__ int part[S8_W][V];
 #pragma unroll
-    for (int i = 0; i < TT; ++i)
+    for (int i = 0; i < RT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) part[wave][(i * 4 + e) * 64 + lane] = acc[i][e];
+        for (int j = 0; j < TT; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) part[wave][((i * TT + j) * 4 + e) * 64 + lane] = acc[i][j][e];
     __syncthreads();
-    for (int i = threadIdx.x; i < V; i += S8_W * 64)
+    constexpr int OUT = GU && RT == 2 ? V / 2 : V;                 // (up's sums lie TT tiles behind gate's)
+    for (int i = threadIdx.x; i < OUT; i += S8_W * 64)
     {
-        const int c = i & 15, t = (i >> 8) * 16 + ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + c;
-        if (t >= p.T || c >= ROWS || n >= p.N) continue;
+        const int c = i & 15, tile = i >> 8, t = tile % TT * 16 + ((i >> 4) & 3) * 4 + ((i >> 6) & 3), n = n0 + tile / TT * 16 + c;
+        if (t >= p.T || (HALF && c >= 8) || n >= p.N) continue;
         auto sum = [&](int at) {
             int s = part[0][at];
 #pragma unroll
@@ -154,7 +167,7 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
         };
         const float sx = FUSED ? lsx[t] : p.sx[t], s = sum(i) * sx * p.sw[0][n];
         const int64_t o = (int64_t)t * p.ldo + n;
-        if (GU) static_cast<float*>(p.out)[o] = act_h(p.act, s, sum(i + 8) * sx * p.sw[1][n]);
+        if (GU) static_cast<float*>(p.out)[o] = act_h(p.act, s, sum(HALF ? i + 8 : i + TT * 256) * sx * p.sw[1][n]);
         else if (EPI == EPI_ADD)
         {
             float* y = static_cast<float*>(p.out) + o;

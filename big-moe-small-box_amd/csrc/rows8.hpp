@@ -85,18 +85,25 @@ __device__ __forceinline__ void store8(void* p, int type, int64_t i, float (&v)[
 // |v| as bits: ordered as the magnitudes, NaN above infinity above all numbers
 __device__ __forceinline__ uint32_t mag(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
+// Sum and maximum over the wave, uniform: exchanges within quads, half rows and rows of 16 lanes, then row 0 into 1 and 2 into 3, rows 0 and 1
+// into 2 and 3; lane 63 holds the result. (DPP moves: through LDS, as __shfl_xor, the six steps take half a microsecond.)
+template <class Op> __device__ __forceinline__ uint32_t wave_all(uint32_t v, Op op)
+{
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xf, 0xf, false));
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x140, 0xf, 0xf, false));
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false));
+    v = op(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false));
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ float wave_sum(float v)
 {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-    return v;
+    return __builtin_bit_cast(float, wave_all(__builtin_bit_cast(uint32_t, v), [](uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }));
 }
-__device__ __forceinline__ uint32_t wave_max(uint32_t v)
-{
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o));
-    return v;
-}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) { return wave_all(v, [](uint32_t a, uint32_t b) { return max(a, b); }); }
 
 // What a row's largest magnitude makes of it: codes are v inv to the nearest whole number, the scale is top / 127
 struct Top8 { float inv, scale, part; };    // part: top / 128
