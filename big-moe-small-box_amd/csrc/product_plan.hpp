@@ -204,23 +204,66 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 
 // ---- 8-bit weights ------------------------------------------------------------------------------------------------------
 
-constexpr int Q8_K = 128;   // columns of a K tile (gemm8_k): as many bytes as gemm16_k's 64, and as much time
+// gemm8_k's tiles, as TILES, us a stage of 64 columns. What bounds the small ones is what a compute unit takes in, about 70 bytes a
+// nanosecond whatever the depth of loads: us of one round of a tile at K 4096, 64 x 64 10.1, 128 x 64 13.4, 128 x 128 17.2, 256 x 128 24.7.
+constexpr int Q8_TILES = 6;
+constexpr Tile TILES8[Q8_TILES] = {
+    {256, 256, 256, 0.70, 0.90, 5.0},      // 8 waves
+    {128, 128, 512, 0.25, 0.52, 3.0},      // 4 waves, two on a compute unit
+    {128, 64, 256, 0.165, 0.18, 3.0},      // 2 groups of 4 waves, each every other stage
+    {128, 128, 256, 0.23, 0.27, 3.0},      // the same
+    {256, 128, 256, 0.44, 0.48, 3.0},      // 8 waves
+    {64, 64, 512, 0.13, 0.215, 2.0},       // 2 groups of 2 waves, two on a compute unit
+};
 
-// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 80 tokens, else gemm8_k's tiles
-inline bool q8_few(int T) { return T <= 80; }
+// Tiles of a product with M x N results and stages of 64 columns, as plan_product: the joining kernel (5 us) and the sums' bytes cost
+// as much, and large tiles go ahead for as many rows of M as fill whole rounds
+inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can_part = true)
+{
+    TilePlan best = {0, 1, 0, 1e30};
+    if (M <= 0 || N <= 0) return {0, 1, 0, 0.0};
+    for (int t = 0; t < Q8_TILES; ++t)
+        for (int s = 1; s <= 16; ++s)
+        {
+            if (s > 1 && (!can_split || stages / s < 8)) break;
+            const Tile& c = TILES8[t];
+            const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * s, full = b / c.slots, rest = b % c.slots;
+            const int each = (stages + s - 1) / s;
+            double us = full * (each * c.full + c.ends);
+            if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
+            if (s > 1) us += 5.0 + (double)M * N * s * 8.0 / 4e6;
+            if (us < best.us) best = {t, s, 0, us};
+        }
+    const int64_t tn = (N + 255) / 256, rounds = (M + 255) / 256 * tn / 256, head = rounds * 256 / tn * 256;
+    if (can_part && head > 0 && head < M)
+    {
+        const TilePlan tail = plan8(M - head, N, stages, false, false);
+        const double us = rounds * (stages * TILES8[0].full + TILES8[0].ends) + tail.us + 2.0;
+        if (us < best.us) best = {tail.tile, 1, head, us};
+    }
+    return best;
+}
+
+inline TilePlan q8_plan(int N, int K, int T, int products) { return plan8((int64_t)N * products, T, (K + 63) / 64, true); }
+
 // skinny8_k: tiles of 16 rows of W per workgroup, 1 or 2. A compute unit reads the tokens once per workgroup and its rows of W, from L2
 // and HBM alike at what its L1 takes, and the unit with the most workgroups is the last to end. us with 1 / 2: 77 tokens 4096 -> 14336
 // 25.3 / 19.4, 2304 -> 5120 9.6 / 7.8, 64 tokens 4096 -> 4096 8.3 / 9.3, 33 tokens 5120 -> 2304 7.8 / 9.0, 2304 -> 5120 7.4 / 6.3; one
-// token 4096 -> 14336 11.7 / 11.2, 14336 -> 4096 11.4 / 12.4.
-inline int q8_few_rows(int N, int T, int products, bool fused)
+// token 4096 -> 14336 11.7 / 11.2, 14336 -> 4096 11.4 / 12.4. A unit of 16 rows or tokens by 1,024 columns takes 0.28 us.
+struct Few8 { int rt; double us; };
+inline Few8 q8_few_rows(int N, int K, int T, int products, bool fused)
 {
     const int64_t tiles = (int64_t)((N + 15) / 16) * products, x = fused ? 0 : (T + 15) / 16;
     auto cost = [&](int rt) { return ((tiles + rt - 1) / rt + 255) / 256 * (rt + x); };
-    return cost(2) < cost(1) ? 2 : 1;
+    const int rt = cost(2) < cost(1) ? 2 : 1;
+    return {rt, 3.0 + cost(rt) * 0.28 * K / 1024};
 }
-inline TilePlan q8_plan(int N, int K, int T, int products)
+
+// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 80 where it is planned sooner (77 tokens
+// 4096 -> 14336 19.4 us, by gemm8_k 17.0; 64 tokens 4096 -> 4096 8.1 / 9.9), else gemm8_k
+inline bool q8_few(int N, int K, int T, int products)
 {
-    return plan_product((int64_t)N * products, T, (K + Q8_K - 1) / Q8_K, 1, true);
+    return T <= 16 || (T <= 80 && q8_few_rows(N, K, T, products, false).us <= q8_plan(N, K, T, products).us);
 }
 
 inline int padded(int n) { return (n + 7) / 8 * 8; }
@@ -277,7 +320,7 @@ inline size_t product_bytes(int N, int K, int T, int products, int group, bool k
 // Partial sums of a product in 8 bits
 inline size_t q8_part_bytes(int N, int K, int T, int products)
 {
-    if (q8_few(T)) return 0;
+    if (q8_few(N, K, T, products)) return 0;
     const TilePlan p = q8_plan(N, K, T, products);
     return p.splits > 1 ? (size_t)p.splits * products * T * padded(N) * 4 : 0;
 }

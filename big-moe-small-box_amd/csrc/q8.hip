@@ -86,7 +86,7 @@ template <bool FUSED, int TT, int RT, int EPI> static int skinny8_launch(const Q
 
 template <bool FUSED, int TT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
 {
-    return q8_few_rows(a.N, a.T, EPI == EPI_GU ? 2 : 1, FUSED) == 2 ? skinny8_launch<FUSED, TT, 2, EPI>(a, s) : skinny8_launch<FUSED, TT, 1, EPI>(a, s);
+    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, FUSED).rt == 2 ? skinny8_launch<FUSED, TT, 2, EPI>(a, s) : skinny8_launch<FUSED, TT, 1, EPI>(a, s);
 }
 
 template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
@@ -104,16 +104,18 @@ template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
 
 template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
 {
-    const int bm = EPI == EPI_GU ? TILES[tile].M / 2 : TILES[tile].M;
+    const int bm = EPI == EPI_GU ? TILES8[tile].M / 2 : TILES8[tile].M;
     a.tm = (a.N + bm - 1) / bm;
-    a.tn = (a.T + TILES[tile].N - 1) / TILES[tile].N;
+    a.tn = (a.T + TILES8[tile].N - 1) / TILES8[tile].N;
     const dim3 grid((unsigned)(a.tm * a.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * (a.w[1] ? 2 : 1) : 1));
     switch (tile)
     {
         case 0: hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 4, EPI>), grid, dim3(512), 0, s, a); break;
         case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a); break;
         case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
-        default: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
+        case 3: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
+        case 4: hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI>), grid, dim3(512), 0, s, a); break;
+        default: hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI>), grid, dim3(256), 0, s, a);
     }
     return check_launch("gemm8");
 }
@@ -122,7 +124,7 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
 template <int EPI> static int product8(const Q8Args& base, hipStream_t s)
 {
     Q8Args a = base;
-    if (q8_few(a.T)) return skinny8_tokens<EPI>(a, s);
+    if (q8_few(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1)) return skinny8_tokens<EPI>(a, s);
     const TilePlan tp = q8_plan(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1);
     if (tp.splits == 1)
     {
@@ -152,7 +154,7 @@ struct Tokens {
     const bmx_q8* rows;
 };
 
-static bool fused8(const Tokens& in, int T, int K) { return !in.rows && q8_few(T) && skinny8_fused(T, K); }
+static bool fused8(const Tokens& in, int T, int K) { return !in.rows && skinny8_fused(T, K); }
 static size_t rows8_bytes(int T, int K) { return align_up(q8_bytes(T, K), 256) + align_up((size_t)T * 4, 256); }
 
 static int take_tokens(const Tokens& in, int T, int K, char* ws, Q8Args& a, hipStream_t s)
@@ -182,7 +184,7 @@ static void put_matrix(Q8Args& a, int m, const bmx_q8* w)
 
 static size_t linear8_ws(const bmx_q8* w, int T, bool rows)
 {
-    const size_t r = rows || (q8_few(T) && skinny8_fused(T, w->K)) ? 0 : rows8_bytes(T, w->K), p = q8_part_bytes(w->N, w->K, T, 1);
+    const size_t r = rows || skinny8_fused(T, w->K) ? 0 : rows8_bytes(T, w->K), p = q8_part_bytes(w->N, w->K, T, 1);
     return r + p;
 }
 
