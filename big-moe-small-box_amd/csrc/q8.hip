@@ -76,29 +76,41 @@ static int q8_whole(const char* fn, const bmx_q8* q, int per, int64_t* pieces)
 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 
-template <bool FUSED, int TT, int RT, int EPI> static int skinny8_launch(const Q8Args& a, hipStream_t s)
+template <int IN, int NS, int TT, int RT, int EPI> static int skinny8_launch(const Q8Args& a, hipStream_t s)
 {
     constexpr int ROWS = (EPI == EPI_GU ? 8 : 16) * RT;
-    hipLaunchKernelGGL((skinny8_k<FUSED, TT, RT, EPI>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(S8_W * 64),
-                       FUSED ? skinny8_lds(a.T, a.K) : 0, s, a);
+    hipLaunchKernelGGL((skinny8_k<IN, NS, TT, RT, EPI>), dim3((unsigned)((a.N + ROWS - 1) / ROWS)), dim3(S8_W * 64),
+                       IN != IN_CODES ? skinny8_lds(a.T, a.K) : 0, s, a);
     return check_launch("skinny8");
 }
 
-template <bool FUSED, int TT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
+template <int IN, int NS, int TT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
 {
-    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, FUSED).rt == 2 ? skinny8_launch<FUSED, TT, 2, EPI>(a, s) : skinny8_launch<FUSED, TT, 1, EPI>(a, s);
+    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, IN != IN_CODES).rt == 2 ? skinny8_launch<IN, NS, TT, 2, EPI>(a, s)
+                                                                                      : skinny8_launch<IN, NS, TT, 1, EPI>(a, s);
+}
+
+template <int IN, int EPI> static int skinny8_fused_rows(const Q8Args& a, hipStream_t s)
+{
+    return skinny8_pieces(a.T, a.K) <= S8_W ? skinny8_rows<IN, 1, 1, EPI>(a, s) : skinny8_rows<IN, 4, 1, EPI>(a, s);
 }
 
 template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
 {
-    if (!a.xc) return skinny8_rows<true, 1, EPI>(a, s);
+    if (!a.xc)
+    {
+        // (a block's x has 16 bits, its h 32)
+        if constexpr (EPI != EPI_GU)
+            if (a.xt == ROW_F32) return skinny8_fused_rows<IN_32, EPI>(a, s);
+        if constexpr (EPI != EPI_ADD) return skinny8_fused_rows<IN_16, EPI>(a, s);
+    }
     switch ((a.T + 15) / 16)
     {
-        case 1: return skinny8_rows<false, 1, EPI>(a, s);
-        case 2: return skinny8_rows<false, 2, EPI>(a, s);
-        case 3: return skinny8_rows<false, 3, EPI>(a, s);
-        case 4: return skinny8_rows<false, 4, EPI>(a, s);
-        default: return skinny8_rows<false, 5, EPI>(a, s);
+        case 1: return skinny8_rows<IN_CODES, 1, 1, EPI>(a, s);
+        case 2: return skinny8_rows<IN_CODES, 1, 2, EPI>(a, s);
+        case 3: return skinny8_rows<IN_CODES, 1, 3, EPI>(a, s);
+        case 4: return skinny8_rows<IN_CODES, 1, 4, EPI>(a, s);
+        default: return skinny8_rows<IN_CODES, 1, 5, EPI>(a, s);
     }
 }
 

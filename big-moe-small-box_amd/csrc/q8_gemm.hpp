@@ -19,7 +19,7 @@ typedef int i32x16 __attribute__((ext_vector_type(16)));
 namespace bmx {
 
 constexpr int S8_W = 8;             // waves of a workgroup (skinny8_k)
-constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup quantizes: 4 a wave
+constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup quantizes, one or four a wave
 
 struct Q8Args {
     const int8_t* w[2];             // second: up
@@ -40,13 +40,19 @@ struct Q8Args {
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------------
 
-inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && T * ((K + 511) / 512) <= S8_SLOTS; }
+inline int skinny8_pieces(int T, int K) { return T * ((K + 511) / 512); }
+inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && skinny8_pieces(T, K) <= S8_SLOTS; }
 inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
 // TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each.
-template <bool FUSED, int TT, int RT, int EPI>
+// IN: the tokens are codes, or 16-bit or fp32 rows to be quantized by pieces of 512 values, NS a wave (with the other type's and three
+// more pieces' code in the kernel a token's call took 0.7 us longer: instructions are fetched from L2 too).
+enum Skinny8In { IN_CODES, IN_16, IN_32 };
+template <int IN, int NS, int TT, int RT, int EPI>
 __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
 {
+    constexpr bool FUSED = IN != IN_CODES;
+    const int xt = IN == IN_32 ? (int)ROW_F32 : p.xt == ROW_BF16 ? (int)ROW_BF16 : (int)ROW_F16;
     constexpr bool GU = EPI == EPI_GU, HALF = GU && RT == 1;
     constexpr int ROWS = GU ? 8 * RT : 16 * RT, D = TT + RT == 2 ? 8 : TT + RT <= 5 ? 4 : 3;     // result columns, blocks in flight
     static_assert(!FUSED || TT == 1, "one tile of tokens quantized here");
@@ -57,13 +63,13 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
     __shared__ uint32_t tops[S8_SLOTS];
     __shared__ float lsx[16];
     const int xrow = KB * Q8_COLS + 16, spt = (p.K + 511) / 512;   // (rows an odd number of 16 bytes apart: 16 of them on all banks)
-    Raw8 raw[4];
+    Raw8 raw[NS];
     if (FUSED)
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NS; ++n)
         {
             const int s = wave + n * S8_W, t = s / spt, h = s % spt * 512 + lane * 8;
-            if (t < p.T && h < p.K) raw[n] = load_raw8(p.x, p.xt, (int64_t)t * p.K + h);
+            if (t < p.T && h < p.K) raw[n] = load_raw8(p.x, xt, (int64_t)t * p.K + h);
         }
 
     // this lane's rows of W, and whose (rows past the last load it again)
@@ -105,16 +111,16 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
         if (kb + d * S8_W < KB) load(st[d], kb + d * S8_W);
     if (FUSED)
     {
-        float v[4][8];
+        float v[NS][8];
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NS; ++n)
         {
             const int s = wave + n * S8_W, t = s / spt, h = s % spt * 512 + lane * 8;
             if (t >= p.T) break;
             uint32_t top = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[n][i] = 0.0f;
-            if (h < p.K) to_f32(raw[n], p.xt, v[n]);
+            if (h < p.K) to_f32(raw[n], xt, v[n]);
 #pragma unroll
             for (int i = 0; i < 8; ++i) top = max(top, mag(v[n][i]));
             top = wave_max(top);
@@ -122,7 +128,7 @@ __global__ __launch_bounds__(S8_W * 64) void skinny8_k(const Q8Args p)
         }
         lds_barrier();
 #pragma unroll
-        for (int n = 0; n < 4; ++n)
+        for (int n = 0; n < NS; ++n)
         {
             const int s = wave + n * S8_W, t = s / spt, h = s % spt * 512 + lane * 8;
             if (t >= p.T) break;
