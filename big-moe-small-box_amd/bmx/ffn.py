@@ -234,7 +234,7 @@ class GatedFFN:
         if s is None:
             with torch.cuda.device(self.device):
                 return self._forward8(x)
-        y = torch.empty(x.shape, dtype=x.dtype, device=self.device)
+        y = torch.empty_like(r) if r is x else torch.empty(x.shape, dtype=x.dtype, device=self.device)
         T = rows.N if r is None else r.shape[0]
         if T:
             d, lib = self._desc(x.dtype), L.lib()

@@ -145,39 +145,43 @@ class _RMSNormFunction(torch.autograd.Function):
     def forward(ctx, x, residual, weight, norm):
         y, _, r = norm._run(x, residual, True, False)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(weight, x if r is None else r)
-        ctx.xt, ctx.summed, ctx.eps, ctx.out, ctx.H = x.dtype, r is not None, norm.eps, norm._out, norm.hidden_size
+        v = x if r is None else r
+        ctx.save_for_backward(weight, v)
+        # (the descriptor holds the weight's address: asked for again below)
+        ctx.desc, ctx.out, ctx.xt, ctx.summed = norm._desc(x.dtype, v.dtype), norm._out, x.dtype, r is not None
         return y, r
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dr):
         weight, v = ctx.saved_tensors
-        H, dev, shape = ctx.H, v.device, v.shape
-        if tuple(weight.shape) != (H,) or weight.device != dev or not weight.is_contiguous() or weight.dtype not in (ctx.out, torch.float32):
+        d, dev, xt, rt, summed = ctx.desc, v.device, ctx.xt, v.dtype, ctx.summed
+        if weight.data_ptr() != d.weight or weight.shape[0] != d.H:
             raise RuntimeError("RMSNorm: the weight was replaced between the forward and the backward pass")
         s = stream_here(dev)
         if s is None:                           # autograd's threads have a current device of their own
             with torch.cuda.device(dev):
                 return _RMSNormFunction.backward(ctx, dy, dr)
         nx, nr, nw, _ = ctx.needs_input_grad
-        rt = v.dtype if ctx.summed else ctx.xt
         if dy is None:                          # r alone was used (or neither)
-            both = None if dr is None else dr
-            dx = both.to(ctx.xt) if nx and both is not None else None
-            return dx, both if nr else None, torch.zeros_like(weight) if nw else None, None
-        rows = rows_of(v, H, v.dtype, dev, "RMSNorm: the saved rows")
-        g = rows_of(dy, H, ctx.out, dev, "RMSNorm: the gradient of y")
-        more = None if dr is None else rows_of(dr, H, rt, dev, "RMSNorm: the gradient of r")
-        one = ctx.summed and rt == ctx.xt       # x's and residual's gradients are the same values
-        dx = torch.empty(shape, dtype=ctx.xt, device=dev) if nx or (nr and one) else None
-        dres = torch.empty(shape, dtype=rt, device=dev) if nr and not one else None
-        dw = torch.empty_like(weight) if nw else None
-        d, lib, T = L.NormDesc(H, DTYPES[ctx.out], ROW_DTYPES[ctx.xt], ROW_DTYPES[rt], ROW_DTYPES[weight.dtype], ctx.eps,
-                               weight.data_ptr()), L.lib(), rows.shape[0]
+            return dr.to(xt) if nx and dr is not None else None, dr if nr else None, torch.zeros_like(weight) if nw else None, None
+        v, dy = _dense(v), _dense(dy)
+        if dr is not None:
+            dr = _dense(dr)
+        one = summed and rt is xt               # x's and residual's gradients are the same values
+        dx = torch.empty_like(v, dtype=xt) if nx or (nr and one) else None
+        dres = torch.empty_like(v) if nr and not one else None
+        lib, T, dw, ws, need = L.lib(), v.numel() // d.H, None, None, 0
+        if nw:
+            dw = torch.empty_like(weight)
+            need = lib.bmx_rms_norm_backward_workspace(d, T)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev)
         ptr = lambda t: None if t is None else t.data_ptr()
-        need = lib.bmx_rms_norm_backward_workspace(d, T) if nw else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-        L.check(lib.bmx_rms_norm_backward(d, rows.data_ptr(), int(ctx.summed), T, g.data_ptr(), ptr(more), ptr(dx), ptr(dres), ptr(dw),
-                                          ptr(ws), need, s), "bmx_rms_norm_backward")
+        L.check(lib.bmx_rms_norm_backward(d, v.data_ptr(), summed, T, dy.data_ptr(), ptr(dr), ptr(dx), ptr(dres), ptr(dw), ptr(ws), need, s),
+                "bmx_rms_norm_backward")
         return dx if nx else None, (dx if one else dres) if nr else None, dw, None
+
+
+def _dense(t):
+    """t contiguous and 16-byte aligned."""
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)

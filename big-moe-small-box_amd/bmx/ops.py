@@ -115,7 +115,7 @@ def q8_linear(x, q):
         with torch.cuda.device(device):
             return q8_linear(x, q)
     T = rows.N if r is None else r.shape[0]
-    y = torch.empty((T, q.N), dtype=dtype, device=device)
+    y = torch.empty((T, q.N), dtype=dtype, device=device) if r is None else r.new_empty((T, q.N))
     if T:
         L_ = lib()
         need = L_.bmx_q8_linear_workspace(q.struct, T)
