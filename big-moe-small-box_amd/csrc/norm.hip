@@ -19,7 +19,6 @@ struct NormArgs {
     int8_t* codes;
     float* scale;
     int blocks;                     // q8_blocks(H)
-    int spread;                     // rows to workgroups by blocks of 16
     int T, H;
     int xt, rt, wt, yt;             // row types
     float eps;
@@ -34,12 +33,7 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
     __shared__ float ssum[16];
     __shared__ uint32_t smax[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    // With codes, rows of one block of 16 on one XCD (workgroups are dealt to the 8 in turn), whose L2 then joins their 64 bytes of a
-    // block to whole lines
-    int64_t t = blockIdx.x;
-    if (p.spread) t = ((t >> 3) / Q8_ROWS * 8 + (t & 7)) * Q8_ROWS + (t >> 3) % Q8_ROWS;
-    if (t >= p.T) return;
-    const int64_t row = t * p.H;
+    const int64_t t = blockIdx.x, row = t * p.H;
     float v[CH][8];                                                // the row, then v w
     Raw8 x[CH], res[CH], w[CH];
     auto at = [&](int c) { return (int)(threadIdx.x + c * blockDim.x) * 8; };
@@ -84,12 +78,9 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
     {
         if (lane == 0) { ssum[wave] = ssq; smax[wave] = top; }
         lds_barrier();
-        ssq = 0.0f;
-        for (int i = 0; i < waves; ++i)
-        {
-            ssq += ssum[i];
-            top = max(top, smax[i]);
-        }
+        // (a lane each: one after the other their LDS reads are as long as the row's loads)
+        if (p.w) ssq = wave_sum(lane < waves ? ssum[lane] : 0.0f);
+        if (p.codes) top = wave_max(lane < waves ? smax[lane] : 0u);
     }
     const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
     const Top8 q = top8(top);
@@ -111,11 +102,10 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
     if (p.codes && threadIdx.x == 0) p.scale[t] = p.w ? q.scale * rstd : q.scale;
 }
 
-static int launch_norm(NormArgs a, hipStream_t s)                  // H <= BMX_NORM_MAX_H
+static int launch_norm(const NormArgs& a, hipStream_t s)                  // H <= BMX_NORM_MAX_H
 {
     const int chunks = (a.H + 511) / 512;                          // of a wave
-    a.spread = a.codes && a.T >= 8 * Q8_ROWS;
-    const dim3 grid((unsigned)(a.spread ? round_up(a.T, 8 * Q8_ROWS) : a.T));
+    const dim3 grid((unsigned)a.T);
     // (two chunks: 12 waves for 11,008 values 155 us, 11 174)
     if (chunks <= 16) hipLaunchKernelGGL((norm_k<1>), grid, dim3(chunks * 64), 0, s, a);
     else hipLaunchKernelGGL((norm_k<2>), grid, dim3((unsigned)round_up((chunks + 1) / 2, 4) * 64), 0, s, a);
@@ -224,13 +214,9 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
         dot = wave_sum(dot);
         if (lane == 0) red[set][wave] = f32x2{ssq, dot};
         lds_barrier();
-        ssq = dot = 0.0f;
-        for (int i = 0; i < waves; ++i)
-        {
-            const f32x2 one = red[set][i];
-            ssq += one[0];
-            dot += one[1];
-        }
+        const f32x2 one = lane < waves ? red[set][lane] : f32x2{0.0f, 0.0f};
+        ssq = wave_sum(one[0]);
+        dot = wave_sum(one[1]);
         const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
         const float k = __fdiv_rn(dot, (float)p.H) * rstd * rstd;
 #pragma unroll
