@@ -1,12 +1,16 @@
 """RMSNorm: the root-mean-square norm with the residual's addition that stands before a layer or a feed-forward block, into 16 bits
 (forward and gradients) or into 8-bit rows, on the HIP library. Every call enqueues on torch's current stream of the weight's
 device; nothing synchronises."""
+import ctypes
+
 import torch
+from torch import empty_like
 
 from . import _lib as L
-from .ffn import DTYPES, _modes, _tracing, eager_only, forward_ad, rows_of, stream_here
+from .ffn import DTYPES, _current_device, _modes, _raw_stream, _tracing, eager_only, forward_ad, stream_here
 from .q8 import ROW_DTYPES, Rows8
 
+F32 = torch.float32
 MOST_H = 16384
 
 
@@ -40,66 +44,62 @@ class RMSNorm:
         if not 2.0 ** -149 <= eps < float("inf"):
             raise ValueError(f"RMSNorm: eps must be positive and finite, got {eps}")
         self._out, self.hidden_size, self.device = out, w.shape[0], w.device
-        self._checked = (w, eps, dtype)
-        self._at = (w.data_ptr(), w.dtype, w.shape)
-        self._descs = {}
+        self._checked = (w, eps, dtype, w.data_ptr(), w.dtype, w.shape[0])
+        self._index, self._descs = w.device.index, {}
 
     def _current(self):
         """Checks again what was replaced since: an attribute, or what the weight tensor holds (Parameter.data)."""
-        w, eps, dtype = self._checked
-        if not (w is self.weight and eps == self.eps and dtype is self.dtype and (w.data_ptr(), w.dtype, w.shape) == self._at and
+        w, eps, dtype, at, wt, H = self._checked
+        if not (w is self.weight and eps == self.eps and dtype is self.dtype and w.data_ptr() == at and w.dtype is wt and w.numel() == H and
                 w.is_contiguous()):
             self._check()
 
     def __getstate__(self):
         """Without the calls' descriptors, which hold addresses: a copy has a weight of its own."""
-        return {**self.__dict__, "_descs": {}, "_at": None}
+        return {**self.__dict__, "_descs": {}, "_checked": (None,) * 6}
 
     def _desc(self, xt, rt):
         d = self._descs.get((xt, rt))
         if d is None:
-            d = L.NormDesc(self.hidden_size, DTYPES[self._out], ROW_DTYPES[xt], ROW_DTYPES[rt], ROW_DTYPES[self._at[1]], self.eps,
-                           self._at[0])
-            self._descs[xt, rt] = d
+            _, _, _, at, wt, H = self._checked
+            d = self._descs[xt, rt] = ctypes.pointer(L.NormDesc(H, DTYPES[self._out], ROW_DTYPES[xt], ROW_DTYPES[rt], ROW_DTYPES[wt], self.eps, at))
         return d
 
     def _given(self, x, name):
         """x of [..., H], checked, contiguous and 16-byte aligned (a copy only where it is neither), and its address."""
-        dt, shape = x.dtype, x.shape
-        if (dt is not self._out and dt is not torch.float32) or x.device != self.device or not shape or shape[-1] != self.hidden_size:
-            raise ValueError(f"RMSNorm: expected {name} {self._out} or fp32 [..., {self.hidden_size}] on {self.device}, got {dt} {tuple(shape)} "
-                             f"on {x.device}")
+        dt, H = x.dtype, self.hidden_size
+        if (dt is not self._out and dt is not F32) or x.get_device() != self._index or not x.dim() or x.size(-1) != H:
+            raise ValueError(f"RMSNorm: expected {name} {self._out} or fp32 [..., {H}] on {self.device}, got {dt} {tuple(x.shape)} on {x.device}")
         p = x.data_ptr()
         if p & 15 or not x.is_contiguous():
             x = x.clone(memory_format=torch.contiguous_format)
             p = x.data_ptr()
         return x, p
 
+    # (a decode token's call is the host's time: 8.6 us, 3.6 of them the launch and 2.4 the two results' allocations)
     def _run(self, x, residual, want_y, want_rows):
         """(y, rows, r), None what is not wanted. Behind _current()."""
         x, xp = self._given(x, "x")
-        H, rp, r, sp = self.hidden_size, None, None, None
+        if _current_device() != self._index:    # (kernels go to the current device)
+            with torch.cuda.device(self.device):
+                return self._run(x, residual, want_y, want_rows)
+        rt = xt = x.dtype
+        rp = sp = yp = y = r = rows = to = None
         if residual is not None:
             residual, rp = self._given(residual, "residual")
             if residual.shape != x.shape:
                 raise ValueError(f"RMSNorm: x {tuple(x.shape)} and residual {tuple(residual.shape)} must be of one shape")
-        s = stream_here(self.device)
-        if s is None:
-            with torch.cuda.device(self.device):
-                return self._run(x, residual, want_y, want_rows)
-        T, xt, yp = x.numel() // H, x.dtype, None
-        if residual is not None:
-            r = torch.empty_like(residual)
-            sp, rt = r.data_ptr(), residual.dtype
-        else:
-            rt = xt
-        y = None
+            rt, r = residual.dtype, empty_like(residual)
+            sp = r.data_ptr()
         if want_y:
-            y = torch.empty_like(x) if xt is self._out else torch.empty_like(x, dtype=self._out)
+            y = empty_like(x) if xt is self._out else empty_like(x, dtype=self._out)
             yp = y.data_ptr()
-        rows = Rows8._empty(T, H, self.device, self._out, x.shape) if want_rows else None
+        T = x.numel() // self.hidden_size
+        if want_rows:
+            rows = Rows8._empty(T, self.hidden_size, self.device, self._out, x.shape)
+            to = rows.struct
         if T:
-            rc = L.lib().bmx_rms_norm(self._desc(xt, rt), xp, rp, T, sp, yp, rows.struct if want_rows else None, s)
+            rc = L.lib().bmx_rms_norm(self._desc(xt, rt), xp, rp, T, sp, yp, to, _raw_stream(self._index))
             if rc:
                 L.check(rc, "bmx_rms_norm")
         return y, rows, r
@@ -148,7 +148,7 @@ class _RMSNormFunction(torch.autograd.Function):
         v = x if r is None else r
         ctx.save_for_backward(weight, v)
         # (the descriptor holds the weight's address: asked for again below)
-        ctx.desc, ctx.out, ctx.xt, ctx.summed = norm._desc(x.dtype, v.dtype), norm._out, x.dtype, r is not None
+        ctx.desc, ctx.xt, ctx.summed = norm._desc(x.dtype, v.dtype), x.dtype, r is not None
         return y, r
 
     @staticmethod
@@ -156,7 +156,8 @@ class _RMSNormFunction(torch.autograd.Function):
     def backward(ctx, dy, dr):
         weight, v = ctx.saved_tensors
         d, dev, xt, rt, summed = ctx.desc, v.device, ctx.xt, v.dtype, ctx.summed
-        if weight.data_ptr() != d.weight or weight.shape[0] != d.H:
+        H = d.contents.H
+        if weight.data_ptr() != d.contents.weight or weight.shape != (H,) or not weight.is_contiguous():
             raise RuntimeError("RMSNorm: the weight was replaced between the forward and the backward pass")
         s = stream_here(dev)
         if s is None:                           # autograd's threads have a current device of their own
@@ -171,7 +172,7 @@ class _RMSNormFunction(torch.autograd.Function):
         one = summed and rt is xt               # x's and residual's gradients are the same values
         dx = torch.empty_like(v, dtype=xt) if nx or (nr and one) else None
         dres = torch.empty_like(v) if nr and not one else None
-        lib, T, dw, ws, need = L.lib(), v.numel() // d.H, None, None, 0
+        lib, T, dw, ws, need = L.lib(), v.numel() // H, None, None, 0
         if nw:
             dw = torch.empty_like(weight)
             need = lib.bmx_rms_norm_backward_workspace(d, T)

@@ -208,7 +208,7 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 // nanosecond whatever the depth of loads: us of one round of a tile at K 4096, 64 x 64 10.1, 128 x 64 13.4, 128 x 128 17.2, 256 x 128 24.7.
 constexpr int Q8_TILES = 6;
 constexpr Tile TILES8[Q8_TILES] = {
-    {256, 256, 256, 0.70, 0.90, 5.0},      // 8 waves
+    {256, 256, 256, 0.70, 0.86, 4.0},      // 8 waves, gemm8_big_k
     {128, 128, 512, 0.25, 0.52, 3.0},      // 4 waves, two on a compute unit
     {128, 64, 256, 0.165, 0.18, 3.0},      // 2 groups of 4 waves, each every other stage
     {128, 128, 256, 0.23, 0.27, 3.0},      // the same

@@ -122,7 +122,10 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
     const dim3 grid((unsigned)(a.tm * a.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * (a.w[1] ? 2 : 1) : 1));
     switch (tile)
     {
-        case 0: hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 4, EPI>), grid, dim3(512), 0, s, a); break;
+        case 0:
+            if constexpr (EPI == EPI_PART) hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 4, EPI>), grid, dim3(512), 0, s, a);
+            else hipLaunchKernelGGL((gemm8_big_k<EPI>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
+            break;
         case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a); break;
         case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
         case 3: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;

@@ -446,6 +446,234 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
     }
 }
 
+// 256 x 256 results by 8 waves, a workgroup one tile after the other (every gridDim.x-th): the stages of its next tile are on their way
+// while a tile's results are turned over and written, in LDS of their own (4 KB a wave). In a launch per tile the chip waits at each
+// tile's two ends, 12 us for a tile of 65 at K 4096 (4,096 x 4,096 x 11,008 174 us, this way 162: 2.28 POP/s).
+constexpr int BIG8 = 256, BIG8_NB = 4, BIG8_RING = BIG8_NB * 2 * BIG8 * Q8_COLS;
+
+template <int EPI>
+__global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
+{
+    constexpr int WN = 4, MF = 4, NF = 2, NB = BIG8_NB, ABYTES = BIG8 * Q8_COLS, BUF = 2 * ABYTES;
+    constexpr bool GU = EPI == EPI_GU;
+    constexpr int ROWS = GU ? BIG8 / 2 : BIG8;                     // rows of W (of each matrix) of a tile
+    __shared__ __attribute__((aligned(1024))) char lds_all[BIG8_RING + 8 * 4096];
+    const lds_ptr lds = (lds_ptr)lds_all;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+    const int KB = q8_blocks(p.K), nwg = p.tm * p.tn;
+
+    // tile `index` of the launch: an XCD on neighbouring tiles (gemm16_tile)
+    struct At { int m0, n0; };
+    auto place = [&](int index) {
+        const int q = nwg / 8, r = nwg % 8, x = index & 7, id = x * q + (x < r ? x : r) + (index >> 3);
+        constexpr int GRP = 8;
+        const int per = GRP * p.tn, g0 = id / per * GRP, gn = min(GRP, p.tm - g0);
+        return At{(g0 + (id % per) % gn) * ROWS, (id % per) / gn * BIG8};
+    };
+
+    // this wave's two blocks of each operand of a stage, and the stages: `left` of the tile whose loads go out, then the next tile's
+    const char *ap[2], *bp[2];
+    int loading = blockIdx.x, left = 0;
+    auto seek = [&]() {
+        if (loading >= nwg) return;
+        const At t = place(loading);
+        auto block = [&](const int8_t* m, int rb, int rows) {
+            return reinterpret_cast<const char*>(m) + (int64_t)min(rb, (rows - 1) / Q8_ROWS) * KB * Q8_BLOCK;
+        };
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+        {
+            const int i = wave + j * 8, rb = (p.from + t.m0) / Q8_ROWS;
+            ap[j] = GU ? block(i & 2 ? p.w[1] : p.w[0], rb + (i >> 2) * 2 + (i & 1), p.from + p.N) : block(p.w[0], rb + i, p.from + p.N);
+            bp[j] = block(p.xc, t.n0 / Q8_ROWS + i, p.T);
+        }
+        left = KB;
+    };
+    auto load = [&](lds_ptr to, const char*& from, int at) {
+        // (behind the last tile zeros: an empty range, so that the count of loads holds)
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(from), 0, left ? Q8_BLOCK : 0, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)(to + at * Q8_BLOCK), 16, lane * 16, 0, 0, 0);
+        from += Q8_BLOCK;
+    };
+    auto load_a = [&](lds_ptr to) {
+        load(to, ap[0], wave);
+        load(to, ap[1], wave + 8);
+    };
+    auto load_b = [&](lds_ptr to) {
+        load(to + ABYTES, bp[0], wave);
+        load(to + ABYTES, bp[1], wave + 8);
+        if (left && --left == 0)
+        {
+            loading += gridDim.x;
+            seek();
+        }
+    };
+    auto frag = [&](lds_ptr at, int row0, int ks) -> i32x4 {
+        const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
+        return *(__attribute__((address_space(3))) i32x4*)(at + r * Q8_COLS + ((c ^ q8_swz(r)) << 4));
+    };
+    i32x16 acc[MF][NF];
+    i32x4 a[2][MF], b[2][NF];
+    auto read = [&](int ks, lds_ptr at) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i) a[ks][i] = frag(at, wm * 128 + i * 32, ks);
+#pragma unroll
+        for (int j = 0; j < NF; ++j) b[ks][j] = frag(at + ABYTES, wn * 64 + j * 32, ks);
+    };
+    auto products = [&](int ks, int from, int to) {
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+                if (i >= from && i < to) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[ks][i], b[ks][j], acc[i][j], 0, 0, 0);
+    };
+    // (the epilogue's loads and stores are counted too: behind one the wait is for more than the stage's loads, never for fewer)
+    constexpr int BEHIND = 4 * (NB - 2);
+    auto landed = [&]() {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (BEHIND & 15) | (BEHIND >> 4) << 14);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    };
+    auto stage = [&](lds_ptr __restrict__ at, lds_ptr __restrict__ to) __attribute__((always_inline)) {
+        read(0, at);
+        products(1, 0, MF);
+        __builtin_amdgcn_sched_barrier(0);
+        load_a(to);
+        products(0, 0, MF / 2);
+        __builtin_amdgcn_sched_barrier(0);
+        load_b(to);
+        read(1, at);
+        products(0, MF / 2, MF);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    seek();
+#pragma unroll
+    for (int i = 0; i < NB - 1; ++i)
+    {
+        load_a(lds + i * BUF);
+        load_b(lds + i * BUF);
+    }
+    int buf = 0, before = NB - 1;
+    char* turn = lds_all + BIG8_RING + wave * 4096;                // 32 tokens x 128 bytes, chunk c of 16 at c ^ (token / 2 % 8)
+    for (int tile = blockIdx.x; tile < nwg; tile += gridDim.x)
+    {
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+        {
+            a[1][i] = i32x4{0, 0, 0, 0};                           // the first stage follows products with zeros
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+        }
+#pragma unroll
+        for (int j = 0; j < NF; ++j) b[1][j] = i32x4{0, 0, 0, 0};
+        for (int k = 0; k < KB; ++k)
+        {
+            landed();
+            stage(lds + buf * BUF, lds + before * BUF);
+            before = buf;
+            buf = buf + 1 == NB ? 0 : buf + 1;
+        }
+        products(1, 0, MF);
+
+        // A lane's sums are token l % 32 and rows g * 8 + (l / 32) * 4 .. + 3 of a fragment: scaled where they are, then turned over 128
+        // bytes of 32 tokens at a time, so that whole pieces of rows are written
+        const At t = place(tile);
+        const int half = lane >> 5, mw = t.m0 + wm * (ROWS / 2), nw = t.n0 + wn * 64;
+        const bool whole = t.m0 + ROWS <= p.N;
+        auto scales = [&](int mat, int m, f32x4 (&w)[4]) {         // of a fragment's rows from m
+            const float* sw = p.sw[mat] + p.from;
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+            {
+                const int at = m + g * 8 + half * 4;
+                if (whole) w[g] = f32x4{sw[at], sw[at + 1], sw[at + 2], sw[at + 3]};
+                else
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[g][e] = at + e < p.N ? sw[at + e] : 0.0f;
+            }
+        };
+        float sx[NF];
+#pragma unroll
+        for (int j = 0; j < NF; ++j) sx[j] = p.sx[min(nw + j * 32 + (lane & 31), p.T - 1)];
+        auto value = [&](const i32x16& s, int g, int e, float x, const f32x4 (&w)[4]) { return (float)s[g * 4 + e] * x * w[g][e]; };
+        constexpr int FR = EPI == EPI_ADD ? 1 : 2;                 // fragments turned over together
+#pragma unroll
+        for (int i = 0; i < MF; i += FR)
+        {
+            f32x4 w[FR][4];
+            const int m = mw + (GU ? i / 2 : i) * 32;
+#pragma unroll
+            for (int f = 0; f < FR; ++f) scales(GU ? f : 0, GU ? m : m + f * 32, w[f]);
+#pragma unroll
+            for (int j = 0; j < NF; ++j)
+            {
+                const int row = lane & 31, swz = (row >> 1) & 7;
+                char* to = turn + row * 128;
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                {
+                    if (EPI == EPI_STORE)
+                    {
+#pragma unroll
+                        for (int f = 0; f < FR; ++f)
+                        {
+                            uint32_t h[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) h[e] = bits16(p.ot, value(acc[i + f][j], g, e, sx[j], w[f]));
+                            *reinterpret_cast<u32x2*>(to + (((f * 4 + g) ^ swz) << 4) + half * 8) = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
+                        }
+                    }
+                    else
+                    {
+                        f32x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v[e] = GU ? act_h(p.act, value(acc[i][j], g, e, sx[j], w[0]), value(acc[GU ? i + 1 : i][j], g, e, sx[j], w[FR - 1]))
+                                      : value(acc[i][j], g, e, sx[j], w[0]);
+                        *reinterpret_cast<f32x4*>(to + (((g * 2 + half) ^ swz) << 4)) = v;
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    const int rr = e * 8 + (lane >> 3), c = lane & 7, n = nw + j * 32 + rr;
+                    const u32x4 v = *reinterpret_cast<const u32x4*>(turn + rr * 128 + ((c ^ ((rr >> 1) & 7)) << 4));
+                    const int at = m + c * (EPI == EPI_STORE ? 8 : 4);
+                    if (n >= p.T || at >= p.N) continue;
+                    const int64_t o = (int64_t)n * p.ldo + p.from + at;
+                    if (EPI == EPI_STORE)
+                    {
+                        uint16_t* y = static_cast<uint16_t*>(p.out) + o;
+                        if (!(p.ldo & 7)) *reinterpret_cast<u32x4*>(y) = v;
+                        else
+#pragma unroll
+                            for (int k = 0; k < 8; ++k)
+                                if (at + k < p.N) y[k] = (uint16_t)(v[k / 2] >> (16 * (k & 1)));
+                    }
+                    else
+                    {
+                        f32x4* y = reinterpret_cast<f32x4*>(static_cast<float*>(p.out) + o);
+                        if (GU) *y = __builtin_bit_cast(f32x4, v);
+                        else
+                        {
+                            const f32x4 d = __builtin_bit_cast(f32x4, v), c0 = ldg4f(reinterpret_cast<const float*>(y));
+                            const float k = p.scale ? p.scale[n] : 1.0f;
+                            *y = f32x4{__builtin_fmaf(k, d[0], c0[0]), __builtin_fmaf(k, d[1], c0[1]), __builtin_fmaf(k, d[2], c0[2]),
+                                       __builtin_fmaf(k, d[3], c0[3])};
+                        }
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            }
+        }
+    }
+}
+
 // The sums over the splits (EPI_PART) and what EPI does with them: 8 values a thread
 template <int EPI>
 __global__ __launch_bounds__(64) void finish8_k(const Q8Args p)

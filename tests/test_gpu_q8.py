@@ -248,6 +248,40 @@ def test_gated_block_of_model_sizes(cuda, T, H, I):
         R.check("y", ffn(x), y64, R.rounded(y64, e, dt))
 
 
+@pytest.mark.parametrize("T,K,N", [(2100, 64, 8190), (4100, 200, 4104), (8300, 40, 8200), (16400, 1030, 2056), (4096, 2048, 4096)])
+def test_many_tiles(cuda, T, K, N):
+    """Several large tiles a workgroup one after the other, of fewer stages than are loaded ahead and of more, ragged at both ends; and
+    the same rows in calls of few tokens."""
+    import bmx
+    given, w = matrix(cuda, N, K, seed=N)
+    q = bmx.Q8Matrix(*given)
+    x = rand(cuda, T, K, dt=torch.bfloat16, seed=T)
+    y = bmx.ops.q8_linear(x, q)
+    check_linear(x, q, w, y)
+    for at in (0, 255, T - 300):
+        assert torch.equal(bmx.ops.q8_linear(x[at:at + 300], q), y[at:at + 300])
+
+
+@pytest.mark.parametrize("T,H,I", [(4100, 2056, 1032), (2300, 4104, 2568), (8200, 136, 4104)])
+def test_gated_block_of_many_tiles(cuda, T, H, I):
+    """Large tiles in both products: forward and added, against 64 bits, and the same as in calls of fewer tokens bit for bit."""
+    import bmx
+    ffn, w = block(cuda, H, I, 3, 7.0)
+    x = rand(cuda, T, H, dt=torch.float16, seed=T)
+    rows = bmx.ops.quantize_rows(x)
+    y64, e = Q.block(values(rows), *w, 3, 7.0)
+    y = ffn(x)
+    R.check("y", y, y64, R.rounded(y64, e, x.dtype))
+    vec = (torch.randn(H, device=cuda) / H ** 0.5).half()
+    base = torch.randn((T, H), device=cuda)
+    out = ffn.add_to(base.clone(), x, vec)
+    s = torch.sigmoid(x.double() @ vec.double())[:, None]
+    want = base.double() + s * y64
+    R.check("out", out, want, s * e + 2.0 ** -22 * (want.abs() + y64.abs()) + H * R.ACC * y64.abs())
+    at = T - 70
+    assert torch.equal(ffn(x[at:]), y[at:]) and torch.equal(ffn.add_to(base[at:].clone(), x[at:], vec), out[at:])
+
+
 @pytest.mark.parametrize("T", [1, 20, 100, 600])
 def test_added_form_and_rows_behind(cuda, T):
     """add_to on a larger buffer: y before its rounding, with and without the gate vector; the rows behind the last token keep their
