@@ -53,6 +53,10 @@ __device__ __forceinline__ float act_h(const ActPar& p, float g, float u)
     return clamp_hi(act_a(p, g, act_f(p, g)), p.La) * (clamp_both(u, p.Lu) + p.add);
 }
 
+// silu without clamps by itself: act_h's value, in half its operations (an 8-bit epilogue of 128 of them a lane waits for nothing else)
+__device__ __forceinline__ bool is_silu(const ActPar& p) { return !p.limited && !p.relu2 && p.c1 == 1.0f && p.c3 == 0.0f; }
+__device__ __forceinline__ float silu_h(float g, float u) { return g * rcp_hw(1.0f + exp_hw(-g)) * u; }
+
 // dh/dg and dh/du at (g, u): a' = f + g f', f' = s (1 - s) (c1 + 3 c3 g^2); 2 f for the squared relu
 __device__ __forceinline__ void act_grad(const ActPar& p, float g, float u, float& hg, float& hu)
 {

@@ -583,7 +583,7 @@ __global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
         // bytes of 32 tokens at a time, so that whole pieces of rows are written
         const At t = place(tile);
         const int half = lane >> 5, mw = t.m0 + wm * (ROWS / 2), nw = t.n0 + wn * 64;
-        const bool whole = t.m0 + ROWS <= p.N;
+        const bool whole = t.m0 + ROWS <= p.N, silu = is_silu(p.act);
         auto scales = [&](int mat, int m, f32x4 (&w)[4]) {         // of a fragment's rows from m
             const float* sw = p.sw[mat] + p.from;
 #pragma unroll
@@ -630,10 +630,14 @@ __global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
                     else
                     {
                         f32x4 v;
+                        auto gate = [&](int e) { return value(acc[i][j], g, e, sx[j], w[0]); };
+                        auto up = [&](int e) { return value(acc[GU ? i + 1 : i][j], g, e, sx[j], w[FR - 1]); };
+                        if (GU && silu)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            v[e] = GU ? act_h(p.act, value(acc[i][j], g, e, sx[j], w[0]), value(acc[GU ? i + 1 : i][j], g, e, sx[j], w[FR - 1]))
-                                      : value(acc[i][j], g, e, sx[j], w[0]);
+                            for (int e = 0; e < 4; ++e) v[e] = silu_h(gate(e), up(e));
+                        else
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = GU ? act_h(p.act, gate(e), up(e)) : gate(e);
                         *reinterpret_cast<f32x4*>(to + (((g * 2 + half) ^ swz) << 4)) = v;
                     }
                 }

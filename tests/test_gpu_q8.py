@@ -118,7 +118,8 @@ def test_given_codes(cuda, N, K):
     """Every code, in and out again, in rows and matrices; transposed and sliced ones too."""
     import bmx
     (c, s), _ = matrix(cuda, N, K, seed=N)
-    for given in (c, c.t().contiguous().t(), torch.cat((c, c), 1)[:, :K]):
+    odd = torch.empty(N * K + 5, dtype=torch.int8, device=cuda)[5:].view(N, K).copy_(c)
+    for given in (c, c.t().contiguous().t(), torch.cat((c, c), 1)[:, :K], odd):
         for kind in (bmx.Q8Matrix, bmx.Rows8):
             q = kind(given, s)
             assert torch.equal(q.int8(), c) and torch.equal(q.scale, s)
