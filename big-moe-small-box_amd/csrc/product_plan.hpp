@@ -209,12 +209,13 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 constexpr int Q8_TILES = 6;
 constexpr Tile TILES8[Q8_TILES] = {
     {256, 256, 256, 0.70, 0.86, 4.0},      // 8 waves, gemm8_big_k
-    {128, 128, 512, 0.25, 0.52, 3.0},      // 4 waves, two on a compute unit
+    {128, 128, 512, 0.29, 0.52, 3.0},      // 4 waves, two on a compute unit
     {128, 64, 256, 0.165, 0.18, 3.0},      // 2 groups of 4 waves, each every other stage
-    {128, 128, 256, 0.23, 0.27, 3.0},      // the same
+    {128, 128, 256, 0.23, 0.28, 3.0},      // the same
     {256, 128, 256, 0.44, 0.48, 3.0},      // 8 waves
     {64, 64, 512, 0.13, 0.215, 2.0},       // 2 groups of 2 waves, two on a compute unit
 };
+constexpr bool splits8(int t) { return t == 2 || t == 3 || t == 5; }      // their K axis can be split: few results, where it pays
 
 // Tiles of a product with M x N results and stages of 64 columns, as plan_product: the joining kernel (5 us) and the sums' bytes cost
 // as much, and large tiles go ahead for as many rows of M as fill whole rounds
@@ -225,7 +226,7 @@ inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can
     for (int t = 0; t < Q8_TILES; ++t)
         for (int s = 1; s <= 16; ++s)
         {
-            if (s > 1 && (!can_split || stages / s < 8)) break;
+            if (s > 1 && (!can_split || !splits8(t) || stages / s < 8)) break;
             const Tile& c = TILES8[t];
             const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * s, full = b / c.slots, rest = b % c.slots;
             const int each = (stages + s - 1) / s;
@@ -246,24 +247,29 @@ inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can
 
 inline TilePlan q8_plan(int N, int K, int T, int products) { return plan8((int64_t)N * products, T, (K + 63) / 64, true); }
 
+constexpr int S8_W = 8;             // waves of a workgroup (skinny8_k)
+constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup quantizes, one or four a wave
+inline int skinny8_pieces(int T, int K) { return T * ((K + 511) / 512); }
+inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && skinny8_pieces(T, K) <= S8_SLOTS; }
+
 // skinny8_k: tiles of 16 rows of W per workgroup, 1 or 2. A compute unit reads the tokens once per workgroup and its rows of W, from L2
 // and HBM alike at what its L1 takes, and the unit with the most workgroups is the last to end. us with 1 / 2: 77 tokens 4096 -> 14336
 // 25.3 / 19.4, 2304 -> 5120 9.6 / 7.8, 64 tokens 4096 -> 4096 8.3 / 9.3, 33 tokens 5120 -> 2304 7.8 / 9.0, 2304 -> 5120 7.4 / 6.3; one
 // token 4096 -> 14336 11.7 / 11.2, 14336 -> 4096 11.4 / 12.4. A unit of 16 rows or tokens by 1,024 columns takes 0.28 us.
 struct Few8 { int rt; double us; };
-inline Few8 q8_few_rows(int N, int K, int T, int products, bool fused)
+inline Few8 q8_few_rows(int N, int K, int T, int products)
 {
-    const int64_t tiles = (int64_t)((N + 15) / 16) * products, x = fused ? 0 : (T + 15) / 16;
+    const int64_t tiles = (int64_t)((N + 15) / 16) * products, x = (T + 15) / 16;
     auto cost = [&](int rt) { return ((tiles + rt - 1) / rt + 255) / 256 * (rt + x); };
     const int rt = cost(2) < cost(1) ? 2 : 1;
     return {rt, 3.0 + cost(rt) * 0.28 * K / 1024};
 }
 
-// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 80 where it is planned sooner (77 tokens
-// 4096 -> 14336 19.4 us, by gemm8_k 17.0; 64 tokens 4096 -> 4096 8.1 / 9.9), else gemm8_k
+// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 64 where it is planned sooner (64 tokens
+// 4096 -> 4096 8.1 us, by gemm8_k 9.9; 77 tokens 4096 -> 14336 19.4 / 17.0), else gemm8_k
 inline bool q8_few(int N, int K, int T, int products)
 {
-    return T <= 16 || (T <= 80 && q8_few_rows(N, K, T, products, false).us <= q8_plan(N, K, T, products).us);
+    return T <= 16 || (T <= 64 && q8_few_rows(N, K, T, products).us <= q8_plan(N, K, T, products).us);
 }
 
 inline int padded(int n) { return (n + 7) / 8 * 8; }

@@ -89,15 +89,16 @@ template <int IN, int NS, int TT, int RT, int EPI> static int skinny8_launch(con
     return check_launch("skinny8");
 }
 
-template <int IN, int NS, int TT, int EPI> static int skinny8_rows(const Q8Args& a, hipStream_t s)
+template <int TT, int EPI> static int skinny8_codes(const Q8Args& a, hipStream_t s)
 {
-    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1, IN != IN_CODES).rt == 2 ? skinny8_launch<IN, NS, TT, 2, EPI>(a, s)
-                                                                                      : skinny8_launch<IN, NS, TT, 1, EPI>(a, s);
+    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1).rt == 2 ? skinny8_launch<IN_CODES, 1, TT, 2, EPI>(a, s)
+                                                                      : skinny8_launch<IN_CODES, 1, TT, 1, EPI>(a, s);
 }
 
-template <int IN, int EPI> static int skinny8_fused_rows(const Q8Args& a, hipStream_t s)
+// (the workgroups that quantize read the tokens once each, whatever their rows of W: 16 of them)
+template <int IN, int EPI> static int skinny8_values(const Q8Args& a, hipStream_t s)
 {
-    return skinny8_pieces(a.T, a.K) <= S8_W ? skinny8_rows<IN, 1, 1, EPI>(a, s) : skinny8_rows<IN, 4, 1, EPI>(a, s);
+    return skinny8_pieces(a.T, a.K) <= S8_W ? skinny8_launch<IN, 1, 1, 1, EPI>(a, s) : skinny8_launch<IN, 4, 1, 1, EPI>(a, s);
 }
 
 template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
@@ -106,16 +107,15 @@ template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
     {
         // (a block's x has 16 bits, its h 32)
         if constexpr (EPI != EPI_GU)
-            if (a.xt == ROW_F32) return skinny8_fused_rows<IN_32, EPI>(a, s);
-        if constexpr (EPI != EPI_ADD) return skinny8_fused_rows<IN_16, EPI>(a, s);
+            if (a.xt == ROW_F32) return skinny8_values<IN_32, EPI>(a, s);
+        if constexpr (EPI != EPI_ADD) return skinny8_values<IN_16, EPI>(a, s);
     }
     switch ((a.T + 15) / 16)
     {
-        case 1: return skinny8_rows<IN_CODES, 1, 1, EPI>(a, s);
-        case 2: return skinny8_rows<IN_CODES, 1, 2, EPI>(a, s);
-        case 3: return skinny8_rows<IN_CODES, 1, 3, EPI>(a, s);
-        case 4: return skinny8_rows<IN_CODES, 1, 4, EPI>(a, s);
-        default: return skinny8_rows<IN_CODES, 1, 5, EPI>(a, s);
+        case 1: return skinny8_codes<1, EPI>(a, s);
+        case 2: return skinny8_codes<2, EPI>(a, s);
+        case 3: return skinny8_codes<3, EPI>(a, s);
+        default: return skinny8_codes<4, EPI>(a, s);
     }
 }
 
@@ -125,18 +125,18 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
     a.tm = (a.N + bm - 1) / bm;
     a.tn = (a.T + TILES8[tile].N - 1) / TILES8[tile].N;
     const dim3 grid((unsigned)(a.tm * a.tn), 1, (unsigned)(EPI == EPI_PART ? a.splits * (a.w[1] ? 2 : 1) : 1));
-    switch (tile)
+    if constexpr (EPI != EPI_PART)
     {
-        case 0:
-            if constexpr (EPI == EPI_PART) hipLaunchKernelGGL((gemm8_k<256, 256, 2, 4, 1, 4, EPI>), grid, dim3(512), 0, s, a);
-            else hipLaunchKernelGGL((gemm8_big_k<EPI>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
-            break;
-        case 1: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a); break;
-        case 2: hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
-        case 3: hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a); break;
-        case 4: hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI>), grid, dim3(512), 0, s, a); break;
-        default: hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI>), grid, dim3(256), 0, s, a);
+        if (tile == 0)
+            hipLaunchKernelGGL((gemm8_big_k<EPI>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
+        else if (tile == 1)
+            hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a);
+        else if (tile == 4)
+            hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI>), grid, dim3(512), 0, s, a);
     }
+    if (tile == 2) hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
+    if (tile == 3) hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
+    if (tile == 5) hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI>), grid, dim3(256), 0, s, a);
     return check_launch("gemm8");
 }
 

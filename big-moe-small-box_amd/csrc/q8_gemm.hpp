@@ -1,7 +1,7 @@
 // Products of 8-bit integers: y[t][n] = sx[t] sw[n] sum_k a[t][k] c[n][k], the sum exact in int32 (K <= 131,071), so that a result
 // does not depend on tiles, splits or the tokens beside it. Both factors lie in blocks of 16 rows x 64 columns (rows8.hpp).
 //
-// skinny8_k: to 80 tokens, bound by the bytes of W. A workgroup has 16 or 32 rows of W (half of gate and half of up in the gated
+// skinny8_k: to 64 tokens, bound by the bytes of W. A workgroup has 16 or 32 rows of W (half of gate and half of up in the gated
 // product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
 // ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized by each workgroup itself while
 // its first loads of W are on their way, into LDS: one launch instead of two.
@@ -17,9 +17,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x16 __attribute__((ext_vector_type(16)));
 
 namespace bmx {
-
-constexpr int S8_W = 8;             // waves of a workgroup (skinny8_k)
-constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup quantizes, one or four a wave
 
 struct Q8Args {
     const int8_t* w[2];             // second: up
@@ -40,8 +37,6 @@ struct Q8Args {
 
 // ---- few tokens ---------------------------------------------------------------------------------------------------------
 
-inline int skinny8_pieces(int T, int K) { return T * ((K + 511) / 512); }
-inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && skinny8_pieces(T, K) <= S8_SLOTS; }
 inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
 // TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each.
