@@ -59,11 +59,11 @@ class GatedFFN:
     bits x may be fp16 or bf16, and there are no gradients. act: ACT_SILU, ACT_GELU (tanh), ACT_RELU2 or ACT_SILU_OAI; act_limit:
     the activation's clamp (0: none), both as MoELayer's.
 
-    forward(x) -> y, x [..., H] of the weights' type (8-bit weights: or Rows8, as RMSNorm.rows8 gives them). Where autograd records (x or a weight requires grad), y carries the
-    gradients of x and of the three weights; the forward pass then keeps x, g and u (fp32 [T, I]) and h (16 bits). Passes
-    with gradients may be captured into a graph through torch.autograd.grad; with backward(), which accumulates into the
-    leaves, only while no eager result of the same leaves is alive (torch's accumulation belongs to the stream that the
-    leaf was first used on)."""
+    forward(x) -> y, x [..., H] of the weights' type (8-bit weights: or Rows8, as RMSNorm.rows8 gives them). Where autograd
+    records (x or a weight requires grad), y carries the gradients of x and of the three weights; the forward pass then keeps
+    x, g and u (fp32 [T, I]) and h (16 bits). Passes with gradients may be captured into a graph through torch.autograd.grad;
+    with backward(), which accumulates into the leaves, only while no eager result of the same leaves is alive (torch's
+    accumulation belongs to the stream that the leaf was first used on)."""
 
     def __init__(self, gate, up, down, act=L.ACT_SILU, act_limit=0.0):
         self.gate, self.up, self.down = gate, up, down

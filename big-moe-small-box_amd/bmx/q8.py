@@ -21,7 +21,6 @@ class _Codes8:
         super().__setattr__(name, value)
 
     def __reduce_ex__(self, protocol):
-        """A copy has codes of its own: made again from this one's, since the struct holds addresses."""
         raise TypeError(f"{type(self).__name__} cannot be pickled or copied (its struct holds device addresses)")
 
     def _make(self, N, K, device):

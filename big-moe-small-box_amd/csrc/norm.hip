@@ -24,16 +24,22 @@ struct NormArgs {
     float eps;
 };
 
+// A launch's axis holds fewer than 2^32 threads: rows past 2^20 on the second
+constexpr int ROW_BITS = 20;
+static dim3 row_grid(int T) { return dim3((unsigned)std::min(T, 1 << ROW_BITS), (unsigned)(((int64_t)T + (1 << ROW_BITS) - 1) >> ROW_BITS)); }
+__device__ __forceinline__ int64_t row_here() { return (int64_t)blockIdx.y << ROW_BITS | blockIdx.x; }
+
 // A workgroup a row, CH chunks of 8 values a lane. One chunk and as many waves as that takes (16 at most) is the fastest: 8,192 rows of
 // 4,096 with two tensors in and two out 52 us (5.1 TB/s, as a copy), with half the waves and two chunks a lane 56, with one wave a
-// row 96; of 5,120 82 us with five waves, 92 with eight of which most have nothing in their second chunk.
+// row 96; of 5,120 76 us with its ten waves, 82 with five, 92 with eight of which most have nothing in their second chunk.
 template <int CH>
 __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
 {
     __shared__ float ssum[16];
     __shared__ uint32_t smax[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t t = blockIdx.x, row = t * p.H;
+    const int64_t t = row_here(), row = t * p.H;
+    if (t >= p.T) return;
     float v[CH][8];                                                // the row, then v w
     Raw8 x[CH], res[CH], w[CH];
     auto at = [&](int c) { return (int)(threadIdx.x + c * blockDim.x) * 8; };
@@ -105,7 +111,7 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
 static int launch_norm(const NormArgs& a, hipStream_t s)                  // H <= BMX_NORM_MAX_H
 {
     const int chunks = (a.H + 511) / 512;                          // of a wave
-    const dim3 grid((unsigned)a.T);
+    const dim3 grid = row_grid(a.T);
     // (two chunks: 12 waves for 11,008 values 155 us, 11 174)
     if (chunks <= 16) hipLaunchKernelGGL((norm_k<1>), grid, dim3(chunks * 64), 0, s, a);
     else hipLaunchKernelGGL((norm_k<2>), grid, dim3((unsigned)round_up((chunks + 1) / 2, 4) * 64), 0, s, a);
@@ -117,7 +123,8 @@ __global__ __launch_bounds__(512) void quantize_any_k(const NormArgs p)
 {
     __shared__ uint32_t smax[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t t = blockIdx.x, row = t * p.H;
+    const int64_t t = row_here(), row = t * p.H;
+    if (t >= p.T) return;
     auto value = [&](int h) {
         if (h >= p.H) return 0.0f;
         return p.xt == ROW_F32 ? static_cast<const float*>(p.x)[row + h] : value16(p.xt, static_cast<const uint16_t*>(p.x)[row + h]);
@@ -145,7 +152,7 @@ int launch_quantize(const void* x, int type, const bmx_q8* out, hipStream_t s)
     a.scale = const_cast<float*>(out->scale);
     a.blocks = q8_blocks(out->K);
     if (a.H % 8 == 0 && a.H <= BMX_NORM_MAX_H && reinterpret_cast<uintptr_t>(x) % 16 == 0) return launch_norm(a, s);
-    hipLaunchKernelGGL(quantize_any_k, dim3(a.T), dim3(512), 0, s, a);
+    hipLaunchKernelGGL(quantize_any_k, row_grid(a.T), dim3(512), 0, s, a);
     return check_launch("quantize");
 }
 

@@ -9,7 +9,7 @@
 // result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3.
 //
 // gemm8_k: many tokens, gemm16_k's tiles with v_mfma_i32_32x32x32_i8, in stages of 64 columns: as many bytes as half of gemm16_k's K
-// tile, for as many products.
+// tile, for as many products. gemm8_big_k: its largest tile, a workgroup one after the other.
 #pragma once
 #include "rows8.hpp"
 
@@ -21,7 +21,7 @@ namespace bmx {
 struct Q8Args {
     const int8_t* w[2];             // second: up
     const float* sw[2];
-    const void* x;                  // rows to quantize (skinny8_k<true>), of row type xt, K values each
+    const void* x;                  // rows to quantize (skinny8_k), of row type xt, K values each
     int xt;
     const int8_t* xc;               // or codes
     const float* sx;

@@ -44,3 +44,25 @@ def test_gated_block(cuda, T, H, I):
         want = base[:T].double() + s * y64
         R.check("out", out[:T], want, s * e + 2.0 ** -22 * (want.abs() + y64.abs()) + H * R.ACC * y64.abs())
         assert out.dtype is F32 and torch.equal(out[T:], base[T:])
+
+
+@pytest.mark.parametrize("T,K", [((1 << 23) + 5, 3), ((1 << 20) + 37, 8)])
+def test_more_rows_than_an_axis_of_a_launch_holds(cuda, T, K):
+    """2^23 workgroups of 512 threads are more than 2^32 threads; the first form with rows at any boundary, the second the norm's."""
+    import bmx
+    x = torch.randn((T, K), device=cuda).half()
+    rows = bmx.ops.quantize_rows(x)
+    top = x.abs().amax(1).float()
+    assert torch.equal(rows.scale, (top.double() / 127.0).float())
+    want = torch.round(x.double() * 127.0 / x.abs().amax(1, keepdim=True).double())
+    assert torch.equal(rows.int8().double(), want)
+    if K % 8 == 0:
+        norm = bmx.RMSNorm(torch.ones(K, device=cuda).half())
+        y, rows, r = norm.both(x, x)
+        v = r.double()
+        y64 = v / (v.square().mean(1, keepdim=True) + 1e-6).sqrt()
+        # (before its rounding y is off by its sum of 8 squares and six operations, under 2^-20; fp16 numbers below 2^-14 lie 2^-24
+        # apart whatever their size, which a bound relative to y64 does not hold: a rounding there is off by up to 2^-25)
+        assert torch.equal(r, x + x)
+        R.check("y", y, y64, R.rounded(y64, 2.0 ** -20 * y64.abs(), y.dtype))
+        assert torch.equal(rows.int8().double(), torch.round(v * 127.0 / v.abs().amax(1, keepdim=True)))
