@@ -29,28 +29,31 @@ constexpr int ROW_BITS = 20;
 static dim3 row_grid(int T) { return dim3((unsigned)std::min(T, 1 << ROW_BITS), (unsigned)(((int64_t)T + (1 << ROW_BITS) - 1) >> ROW_BITS)); }
 __device__ __forceinline__ int64_t row_here() { return (int64_t)blockIdx.y << ROW_BITS | blockIdx.x; }
 
-// A workgroup a row, CH chunks of 8 values a lane. One chunk and as many waves as that takes (16 at most) is the fastest: 8,192 rows of
-// 4,096 with two tensors in and two out 52 us (5.1 TB/s, as a copy), with half the waves and two chunks a lane 56, with one wave a
-// row 96; of 5,120 76 us with its ten waves, 82 with five, 92 with eight of which most have nothing in their second chunk.
-template <int CH>
+// A workgroup a row, CH chunks of 8 values a lane: one to 4,096 values, two past them (8,192 rows of 5,120: ten waves of one chunk 72 us,
+// five of two 62). NORM false: the rows as they are in 8 bits alone. WIDE: some tensor is fp32, and a chunk's registers hold any type;
+// 16 bits alone need half of them (8,192 rows of 4,096, two tensors in and two out: 44 us, 6.0 TB/s; with any type's 50, of 16,384 190
+// and 271), and the quantizing form no sums and weight (4,096 x 4,096 12.6 us, with them 17.5).
+template <int CH, bool NORM, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
 {
+    auto type = [](int t) { return !WIDE ? t == ROW_BF16 ? (int)ROW_BF16 : (int)ROW_F16 : NORM ? t : (int)ROW_F32; };
+    const int xt = type(p.xt), rt = type(p.rt), wt = type(p.wt), yt = p.yt == ROW_BF16 ? (int)ROW_BF16 : (int)ROW_F16;
     __shared__ float ssum[16];
     __shared__ uint32_t smax[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int64_t t = row_here(), row = t * p.H;
     if (t >= p.T) return;
     float v[CH][8];                                                // the row, then v w
-    Raw8 x[CH], res[CH], w[CH];
+    Raw8 x[CH], res[CH], w;
     auto at = [&](int c) { return (int)(threadIdx.x + c * blockDim.x) * 8; };
 #pragma unroll
     for (int c = 0; c < CH; ++c)
     {
         const int h = at(c);
         if (h >= p.H) continue;
-        x[c] = load_raw8(p.x, p.xt, row + h);
-        if (p.res) res[c] = load_raw8(p.res, p.rt, row + h);
-        if (p.w) w[c] = load_raw8(p.w, p.wt, h);
+        x[c] = load_raw8(p.x, xt, row + h);
+        if (NORM && p.res) res[c] = load_raw8(p.res, rt, row + h);
+        if (NORM && CH == 1) w = load_raw8(p.w, wt, h);
     }
     float ssq = 0.0f;
     uint32_t top = 0;
@@ -59,62 +62,81 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
     {
         const int h = at(c);
         if (h >= p.H) continue;
-        to_f32(x[c], p.xt, v[c]);
-        if (p.res)
+        to_f32(x[c], xt, v[c]);
+        if (NORM && p.res)
         {
             float a[8];
-            to_f32(res[c], p.rt, a);
+            to_f32(res[c], rt, a);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[c][i] += a[i];
-            store8(p.r, p.rt, row + h, v[c]);
+            store8(p.r, rt, row + h, v[c]);
         }
         float b[8];
-        if (p.w) to_f32(w[c], p.wt, b);
+        if (NORM)
+        {
+            if (CH > 1) w = load_raw8(p.w, wt, h);
+            to_f32(w, wt, b);
+        }
 #pragma unroll
         for (int i = 0; i < 8; ++i)
         {
-            ssq = __builtin_fmaf(v[c][i], v[c][i], ssq);
-            if (p.w) v[c][i] *= b[i];
+            if (NORM)
+            {
+                ssq = __builtin_fmaf(v[c][i], v[c][i], ssq);
+                v[c][i] *= b[i];
+            }
             top = max(top, mag(v[c][i]));
         }
+        if (NORM && CH > 1) __builtin_amdgcn_sched_barrier(0);     // (else all chunks' weights are loaded at once: 74 registers)
     }
-    if (p.w) ssq = wave_sum(ssq);
-    if (p.codes) top = wave_max(top);
+    const bool codes = !NORM || p.codes;
+    if (NORM) ssq = wave_sum(ssq);
+    if (codes) top = wave_max(top);
     if (waves > 1)
     {
         if (lane == 0) { ssum[wave] = ssq; smax[wave] = top; }
         lds_barrier();
         // (a lane each: one after the other their LDS reads are as long as the row's loads)
-        if (p.w) ssq = wave_sum(lane < waves ? ssum[lane] : 0.0f);
-        if (p.codes) top = wave_max(lane < waves ? smax[lane] : 0u);
+        if (NORM) ssq = wave_sum(lane < waves ? ssum[lane] : 0.0f);
+        if (codes) top = wave_max(lane < waves ? smax[lane] : 0u);
     }
-    const float rstd = __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps));
+    const float rstd = NORM ? __fdiv_rn(1.0f, __builtin_sqrtf(__fdiv_rn(ssq, (float)p.H) + p.eps)) : 1.0f;
     const Top8 q = top8(top);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
     {
         const int h = at(c);
-        if (p.codes && h < p.blocks * Q8_COLS)
+        if (codes && h < p.blocks * Q8_COLS)
             *reinterpret_cast<u32x2*>(p.codes + q8_at(t, h, p.blocks)) =
                 h < p.H ? u32x2{codes4(v[c], q), codes4(v[c] + 4, q)} : u32x2{0, 0};
-        if (p.y && h < p.H)
+        if (NORM && p.y && h < p.H)
         {
             float y[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) y[i] = v[c][i] * rstd;
-            store8(p.y, p.yt, row + h, y);
+            store8(p.y, yt, row + h, y);
         }
     }
-    if (p.codes && threadIdx.x == 0) p.scale[t] = p.w ? q.scale * rstd : q.scale;
+    if (codes && threadIdx.x == 0) p.scale[t] = NORM ? q.scale * rstd : q.scale;
 }
 
 static int launch_norm(const NormArgs& a, hipStream_t s)                  // H <= BMX_NORM_MAX_H
 {
     const int chunks = (a.H + 511) / 512;                          // of a wave
-    const dim3 grid = row_grid(a.T);
-    // (two chunks: 12 waves for 11,008 values 155 us, 11 174)
-    if (chunks <= 16) hipLaunchKernelGGL((norm_k<1>), grid, dim3(chunks * 64), 0, s, a);
-    else hipLaunchKernelGGL((norm_k<2>), grid, dim3((unsigned)round_up((chunks + 1) / 2, 4) * 64), 0, s, a);
+    const bool wide = a.xt == ROW_F32 || a.rt == ROW_F32 || a.wt == ROW_F32;
+    const dim3 grid = row_grid(a.T), one(chunks * 64), two((chunks + 1) / 2 * 64);
+    if (!a.w)
+    {
+        if (wide) hipLaunchKernelGGL((norm_k<2, false, true>), grid, two, 0, s, a);
+        else hipLaunchKernelGGL((norm_k<2, false, false>), grid, two, 0, s, a);
+    }
+    else if (chunks <= 8)
+    {
+        if (wide) hipLaunchKernelGGL((norm_k<1, true, true>), grid, one, 0, s, a);
+        else hipLaunchKernelGGL((norm_k<1, true, false>), grid, one, 0, s, a);
+    }
+    else if (wide) hipLaunchKernelGGL((norm_k<2, true, true>), grid, two, 0, s, a);
+    else hipLaunchKernelGGL((norm_k<2, true, false>), grid, two, 0, s, a);
     return check_launch("rms_norm");
 }
 
@@ -168,11 +190,15 @@ struct NormBackArgs {
 };
 
 // A workgroup takes every gridDim.x-th row and keeps its rows' sums for the weight's gradient in registers, and for rows of one chunk a
-// lane the weight; the next row's loads are then on their way while one is summed up (two chunks do not leave registers for that).
-template <int CH>
+// lane the weight; the next row's loads are on their way while one is summed up. WIDE: some tensor is fp32. (Of 16 bits alone a chunk
+// takes half the registers, and 24 waves of one chunk fit a compute unit: 8,192 rows of 4,096 with the forward pass 94 us, as WIDE 117;
+// 4,096 of 16,384 206 and 384.) Two chunks of any type leave no registers for loads ahead and for what the first pass made of a row: AHEAD
+// false makes it again.
+template <int CH, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
 {
-    constexpr bool ONE = CH == 1;
+    constexpr bool AHEAD = CH == 1 || !WIDE;
+    const int yt = p.yt == ROW_BF16 ? (int)ROW_BF16 : (int)ROW_F16, vt = WIDE ? p.vt : yt, wt = WIDE ? p.wt : yt, xt = WIDE ? p.xt : yt;
     __shared__ f32x2 red[2][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     float w[8], dw[CH][8];
@@ -184,15 +210,15 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
         {
             const int64_t i = (int64_t)t * p.H + at(c);
             if (at(c) >= p.H) continue;
-            v[c] = load_raw8(p.v, p.vt, i);
-            dy[c] = load_raw8(p.dy, p.yt, i);
-            if (p.dr) dr[c] = load_raw8(p.dr, p.rt, i);
+            v[c] = load_raw8(p.v, vt, i);
+            dy[c] = load_raw8(p.dy, yt, i);
+            if (AHEAD && p.dr) dr[c] = load_raw8(p.dr, vt, i);
         }
     };
-    auto weight = [&](int c) { to_f32(load_raw8(p.w, p.wt, at(c)), p.wt, w); };
+    auto weight = [&](int c) { to_f32(load_raw8(p.w, wt, at(c)), p.wt, w); };
     int t = blockIdx.x;
     load(t);
-    if (ONE && at(0) < p.H) weight(0);
+    if (CH == 1 && at(0) < p.H) weight(0);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -205,18 +231,19 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
         for (int c = 0; c < CH; ++c)
         {
             if (at(c) >= p.H) continue;
-            to_f32(v[c], p.vt, a[c]);
-            to_f32(dy[c], p.yt, d[c]);
-            if (ONE && p.dr) to_f32(dr[c], p.rt, more[c]);
-            if (!ONE) weight(c);
+            to_f32(v[c], vt, a[c]);
+            to_f32(dy[c], yt, d[c]);
+            if (AHEAD && p.dr) to_f32(dr[c], vt, more[c]);
+            if (CH > 1) weight(c);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
             {
                 ssq = __builtin_fmaf(a[c][i], a[c][i], ssq);
                 dot = __builtin_fmaf(d[c][i] * w[i], a[c][i], dot);
             }
+            if (CH > 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (ONE && t + (int)gridDim.x < p.T) load(t + gridDim.x);
+        if (AHEAD && t + (int)gridDim.x < p.T) load(t + gridDim.x);
         ssq = wave_sum(ssq);
         dot = wave_sum(dot);
         if (lane == 0) red[set][wave] = f32x2{ssq, dot};
@@ -232,10 +259,14 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
             if (at(c) >= p.H) continue;
             const int64_t at_row = (int64_t)t * p.H + at(c);
             float o[8], q[8];
-            if (!ONE)
+            if (CH > 1) weight(c);
+            if (!AHEAD)
             {
-                weight(c);
-                if (p.dr) to_f32(dr[c], p.rt, more[c]);
+                asm volatile("" : "+v"(v[c].a), "+v"(v[c].b), "+v"(dy[c].a));     // (not to be kept from the first pass)
+                dy[c].b = dy[c].a;
+                to_f32(v[c], vt, a[c]);
+                to_f32(dy[c], yt, d[c]);
+                if (p.dr) to_f32(load_raw8(p.dr, vt, at_row), vt, more[c]);
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -245,10 +276,11 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
                 q[i] = o[i];
                 dw[c][i] = __builtin_fmaf(d[c][i], a[c][i] * rstd, dw[c][i]);
             }
-            if (p.dx) store8(p.dx, p.xt, at_row, o);
-            if (p.dres) store8(p.dres, p.rt, at_row, q);
+            if (p.dx) store8(p.dx, xt, at_row, o);
+            if (p.dres) store8(p.dres, vt, at_row, q);
+            if (CH > 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (!ONE && t + (int)gridDim.x < p.T) load(t + gridDim.x);
+        if (!AHEAD && t + (int)gridDim.x < p.T) load(t + gridDim.x);
     }
     if (!p.part) return;
 #pragma unroll
@@ -282,16 +314,21 @@ __global__ __launch_bounds__(512) void norm_weight_k(const float* __restrict__ p
     else static_cast<uint16_t*>(dw)[c] = (uint16_t)bits16(wt, sum);
 }
 
-// Waves of a row and workgroups of a backward pass: as many as the compute units hold at once, 16 waves each (8,192 rows of 4,096: 512
-// workgroups 66 us, 256 96, 768 79, 1,024 69)
+// Waves of a row and workgroups of a backward pass: as many as the compute units hold at once (8,192 rows of 4,096: 16 waves a unit
+// 98 us with the forward pass, 24 94, 32 96)
 static int norm_back_waves(int H) { return H <= 8192 ? (H + 511) / 512 : (H + 1023) / 1024; }
-static int norm_back_groups(int T, int H) { return std::min(T, 256 * (16 / norm_back_waves(H))); }
+static int norm_back_groups(int T, int H, bool wide) { return std::min(T, 256 * ((H <= 8192 && !wide ? 24 : 16) / norm_back_waves(H))); }
 
-static int launch_norm_back(const NormBackArgs& a, hipStream_t s)
+static int launch_norm_back(const NormBackArgs& a, int groups, bool wide, hipStream_t s)
 {
-    const dim3 grid(norm_back_groups(a.T, a.H)), block(norm_back_waves(a.H) * 64);
-    if (a.H <= 8192) hipLaunchKernelGGL((norm_back_k<1>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((norm_back_k<2>), grid, block, 0, s, a);
+    const dim3 grid(groups), block(norm_back_waves(a.H) * 64);
+    if (a.H <= 8192)
+    {
+        if (wide) hipLaunchKernelGGL((norm_back_k<1, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((norm_back_k<1, false>), grid, block, 0, s, a);
+    }
+    else if (wide) hipLaunchKernelGGL((norm_back_k<2, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((norm_back_k<2, false>), grid, block, 0, s, a);
     return check_launch("rms_norm_backward");
 }
 
@@ -357,7 +394,7 @@ int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual,
 size_t bmx_rms_norm_backward_workspace(const bmx_norm_desc* desc, int T)
 {
     if (check_norm(desc, T, "bmx_rms_norm_backward_workspace")) return 0;
-    return align_up((size_t)(T ? norm_back_groups(T, desc->H) : 1) * desc->H * 4, 256);
+    return align_up((size_t)(T ? norm_back_groups(T, desc->H, false) : 1) * desc->H * 4, 256);
 }
 
 int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, int T, const void* dy, const void* dr, void* dx,
@@ -391,9 +428,10 @@ int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, 
     a.vt = summed ? desc->residual_dtype : desc->x_dtype;
     a.wt = desc->weight_dtype; a.yt = desc->dtype; a.rt = desc->residual_dtype; a.xt = desc->x_dtype;
     a.eps = desc->eps;
-    if ((rc = launch_norm_back(a, s)) || !dweight) return rc;
-    hipLaunchKernelGGL(norm_weight_k, dim3((desc->H + 31) / 32), dim3(512), 0, s, a.part, norm_back_groups(T, desc->H), desc->H, dweight,
-                       desc->weight_dtype);
+    const bool wide = a.vt == ROW_F32 || a.wt == ROW_F32 || a.xt == ROW_F32;
+    const int groups = norm_back_groups(T, desc->H, wide);
+    if ((rc = launch_norm_back(a, groups, wide, s)) || !dweight) return rc;
+    hipLaunchKernelGGL(norm_weight_k, dim3((desc->H + 31) / 32), dim3(512), 0, s, a.part, groups, desc->H, dweight, desc->weight_dtype);
     return check_launch("norm_weight");
 }
 

@@ -124,6 +124,13 @@ def test_gradients_of_types(cuda, x32, r32, w32, dt):
     backward_check(cuda, 21, 136, DT[dt], x32, r32, w32, residual=False)
 
 
+@pytest.mark.parametrize("x32,r32,w32", [(True, False, False), (False, True, False), (False, False, True), (True, True, True)])
+@pytest.mark.parametrize("T,H", [(600, 8456), (1100, 4104)])
+def test_gradients_of_types_over_several_rows_a_workgroup(cuda, T, H, x32, r32, w32):
+    backward_check(cuda, T, H, torch.bfloat16, x32, r32, w32)
+    backward_check(cuda, T, H, torch.float16, x32, r32, w32, residual=False)
+
+
 @pytest.mark.parametrize("use", ["y", "r"])
 def test_gradients_of_one_output(cuda, use):
     backward_check(cuda, 37, 264, torch.float16, use=use)
