@@ -119,7 +119,7 @@ template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
     }
 }
 
-template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
+template <int EPI, int OT> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
 {
     const int bm = EPI == EPI_GU ? TILES8[tile].M / 2 : TILES8[tile].M;
     a.tm = (a.N + bm - 1) / bm;
@@ -128,15 +128,15 @@ template <int EPI> static int gemm8_tiles(Q8Args a, int tile, hipStream_t s)
     if constexpr (EPI != EPI_PART)
     {
         if (tile == 0)
-            hipLaunchKernelGGL((gemm8_big_k<EPI>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
+            hipLaunchKernelGGL((gemm8_big_k<EPI, OT>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
         else if (tile == 1)
-            hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI>), grid, dim3(256), 0, s, a);
+            hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI, OT>), grid, dim3(256), 0, s, a);
         else if (tile == 4)
-            hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI>), grid, dim3(512), 0, s, a);
+            hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI, OT>), grid, dim3(512), 0, s, a);
     }
-    if (tile == 2) hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
-    if (tile == 3) hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI>), grid, dim3(512), 0, s, a);
-    if (tile == 5) hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI>), grid, dim3(256), 0, s, a);
+    if (tile == 2) hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
+    if (tile == 3) hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
+    if (tile == 5) hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI, OT>), grid, dim3(256), 0, s, a);
     return check_launch("gemm8");
 }
 
@@ -155,13 +155,15 @@ template <int EPI> static int product8(const Q8Args& base, hipStream_t s)
             Q8Args g = a;
             g.from = part[i].from;
             g.N = part[i].rows;
-            if (const int rc = gemm8_tiles<EPI>(g, part[i].tile, s)) return rc;
+            const int rc = EPI != EPI_STORE || a.ot == ROW_F16 ? gemm8_tiles<EPI, ROW_F16>(g, part[i].tile, s)
+                                                               : gemm8_tiles<EPI, EPI == EPI_STORE ? ROW_BF16 : ROW_F16>(g, part[i].tile, s);
+            if (rc) return rc;
         }
         return BMX_OK;
     }
     a.splits = tp.splits;
     a.ldp = padded(a.N);
-    if (const int rc = gemm8_tiles<EPI_PART>(a, tp.tile, s)) return rc;
+    if (const int rc = gemm8_tiles<EPI_PART, ROW_F16>(a, tp.tile, s)) return rc;
     const int64_t pieces = (int64_t)a.ldp / 8 * a.T;
     hipLaunchKernelGGL((finish8_k<EPI>), dim3((unsigned)((pieces + 63) / 64)), dim3(64), 0, s, a);
     return check_launch("finish8");

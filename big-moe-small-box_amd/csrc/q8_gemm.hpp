@@ -188,17 +188,24 @@ __device__ __forceinline__ void scales8(const Q8Args& p, int mat, int m, float (
     for (int i = 0; i < 8; ++i) w[i] = m + i < p.N ? sw[i] : 0.0f;
 }
 
-// What becomes of 8 neighbouring sums (rows m .. m + 7 of W, of scales w; u: up's) of token n, of scale sx; k: its factor (EPI_ADD)
-template <int EPI>
+// What becomes of 8 neighbouring sums (rows m .. m + 7 of W, of scales w; u: up's) of token n, of scale sx; k: its factor (EPI_ADD).
+// OT: EPI_STORE's type, or ANY_OT: p.ot, what a launch says (known to the kernel, 4,096 x 4,096 x 11,008 175 -> 167 us)
+constexpr int ANY_OT = -1;
+template <int EPI, int OT>
 __device__ __forceinline__ void put8(const Q8Args& p, int n, int m, const int (&s)[8], const int (&u)[8], float sx, float k,
                                      const float (&w)[8], const float (&wu)[8])
 {
+    const int ot = OT == ANY_OT ? p.ot : OT;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = (float)s[i] * sx * w[i];
     const int64_t o = (int64_t)n * p.ldo + p.from + m;
     if (EPI == EPI_GU)
     {
+        if (is_silu(p.act))                                
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = silu_h(v[i], (float)u[i] * sx * wu[i]);
+        else
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = act_h(p.act, v[i], (float)u[i] * sx * wu[i]);
         store8(p.out, ROW_F32, o, v);
@@ -211,12 +218,12 @@ __device__ __forceinline__ void put8(const Q8Args& p, int n, int m, const int (&
         for (int i = 0; i < 8; ++i) v[i] = __builtin_fmaf(k, v[i], c.v[i]);
         store8(y, ROW_F32, 0, v);
     }
-    else if (!(p.ldo & 7)) store8(p.out, p.ot, o, v);
+    else if (!(p.ldo & 7)) store8(p.out, ot, o, v);
     else
     {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (m + i < p.N) static_cast<uint16_t*>(p.out)[o + i] = (uint16_t)bits16(p.ot, v[i]);
+            if (m + i < p.N) static_cast<uint16_t*>(p.out)[o + i] = (uint16_t)bits16(ot, v[i]);
     }
 }
 
@@ -229,7 +236,7 @@ template <int BM, int BN, int WM, int WN, int WK, int NB> constexpr int gemm8_ld
     return TILES > TURN ? TILES : TURN;
 }
 
-template <int BM, int BN, int WM, int WN, int WK, int NB, int EPI>
+template <int BM, int BN, int WM, int WN, int WK, int NB, int EPI, int OT>
 __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
 {
     __shared__ __attribute__((aligned(1024))) char lds_all[gemm8_lds<BM, BN, WM, WN, WK, NB>()];
@@ -434,7 +441,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
                 to[0] = i32x4{s[0], s[1], s[2], s[3]};
                 to[1] = i32x4{s[4], s[5], s[6], s[7]};
             }
-            else put8<EPI>(p, n, m, s, u, sx[j][e], add[j][e], w0, w1);
+            else put8<EPI, OT>(p, n, m, s, u, sx[j][e], add[j][e], w0, w1);
         }
         if (WK > 1) __syncthreads();
         else __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -446,7 +453,7 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
 // tile's two ends, 12 us for a tile of 65 at K 4096 (4,096 x 4,096 x 11,008 174 us, this way 162: 2.28 POP/s).
 constexpr int BIG8 = 256, BIG8_NB = 4, BIG8_RING = BIG8_NB * 2 * BIG8 * Q8_COLS;
 
-template <int EPI>
+template <int EPI, int OT>
 __global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
 {
     constexpr int WN = 4, MF = 4, NF = 2, NB = BIG8_NB, ABYTES = BIG8 * Q8_COLS, BUF = 2 * ABYTES;
@@ -618,7 +625,7 @@ __global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
                         {
                             uint32_t h[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) h[e] = bits16(p.ot, value(acc[i + f][j], g, e, sx[j], w[f]));
+                            for (int e = 0; e < 4; ++e) h[e] = bits16(OT, value(acc[i + f][j], g, e, sx[j], w[f]));
                             *reinterpret_cast<u32x2*>(to + (((f * 4 + g) ^ swz) << 4) + half * 8) = u32x2{h[0] | h[1] << 16, h[2] | h[3] << 16};
                         }
                     }
@@ -705,7 +712,7 @@ __global__ __launch_bounds__(64) void finish8_k(const Q8Args p)
 #pragma unroll
                     for (int i = 0; i < 8; ++i) sum[k][i] += v[k][s][i / 4][i % 4];
     }
-    put8<EPI>(p, n, m, sum[0], sum[1], sx, add, w0, w1);
+    put8<EPI, ANY_OT>(p, n, m, sum[0], sum[1], sx, add, w0, w1);
 }
 
 }  // namespace bmx
