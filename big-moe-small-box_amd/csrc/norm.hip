@@ -24,10 +24,16 @@ struct NormArgs {
     float eps;
 };
 
-// A launch's axis holds fewer than 2^32 threads: rows past 2^20 on the second
+// A launch's axis holds fewer than 2^32 threads: rows past 2^20 on the second. Of whole 128 rows an XCD has 16 neighbours (workgroups go to
+// the XCDs in turn), whose codes share lines of memory: written on eight XCDs a line goes out in eight parts (4,096 rows of 11,008 62 us,
+// this way 44).
 constexpr int ROW_BITS = 20;
 static dim3 row_grid(int T) { return dim3((unsigned)std::min(T, 1 << ROW_BITS), (unsigned)(((int64_t)T + (1 << ROW_BITS) - 1) >> ROW_BITS)); }
-__device__ __forceinline__ int64_t row_here() { return (int64_t)blockIdx.y << ROW_BITS | blockIdx.x; }
+__device__ __forceinline__ int64_t row_here(int T)
+{
+    const int64_t i = (int64_t)blockIdx.y << ROW_BITS | blockIdx.x, g = i & ~(int64_t)127;
+    return g + 128 <= T ? g + (i & 7) * 16 + (i >> 3 & 15) : i;
+}
 
 // A workgroup a row, CH chunks of 8 values a lane: one to 4,096 values, two past them (8,192 rows of 5,120: ten waves of one chunk 72 us,
 // five of two 62). NORM false: the rows as they are in 8 bits alone. WIDE: some tensor is fp32, and a chunk's registers hold any type;
@@ -41,7 +47,7 @@ __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
     __shared__ float ssum[16];
     __shared__ uint32_t smax[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
-    const int64_t t = row_here(), row = t * p.H;
+    const int64_t t = row_here(p.T), row = t * p.H;
     if (t >= p.T) return;
     float v[CH][8];                                                // the row, then v w
     Raw8 x[CH], res[CH], w;
@@ -145,7 +151,7 @@ __global__ __launch_bounds__(512) void quantize_any_k(const NormArgs p)
 {
     __shared__ uint32_t smax[8];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t t = row_here(), row = t * p.H;
+    const int64_t t = row_here(p.T), row = t * p.H;
     if (t >= p.T) return;
     auto value = [&](int h) {
         if (h >= p.H) return 0.0f;

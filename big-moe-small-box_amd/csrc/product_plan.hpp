@@ -252,24 +252,31 @@ constexpr int S8_SLOTS = 32;        // pieces of 512 values that a workgroup qua
 inline int skinny8_pieces(int T, int K) { return T * ((K + 511) / 512); }
 inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && skinny8_pieces(T, K) <= S8_SLOTS; }
 
-// skinny8_k: tiles of 16 rows of W per workgroup, 1 or 2. A compute unit reads the tokens once per workgroup and its rows of W, from L2
-// and HBM alike at what its L1 takes, and the unit with the most workgroups is the last to end. us with 1 / 2: 77 tokens 4096 -> 14336
-// 25.3 / 19.4, 2304 -> 5120 9.6 / 7.8, 64 tokens 4096 -> 4096 8.3 / 9.3, 33 tokens 5120 -> 2304 7.8 / 9.0, 2304 -> 5120 7.4 / 6.3; one
-// token 4096 -> 14336 11.7 / 11.2, 14336 -> 4096 11.4 / 12.4. A unit of 16 rows or tokens by 1,024 columns takes 0.28 us.
+// skinny8_k, tiles of 16 rows of W per workgroup, 1 or 2 (to 80 tokens): a workgroup takes in its rows of W and the tokens; us for 1,024
+// columns of 16 of them are 0.07 alone and 0.20 when every compute unit has a workgroup (of 32 rows, more of them from HBM: 0.13 and
+// 0.26), and of more workgroups than units some have one more, which is the last to end. us with 1 / 2: 77 tokens 5120 -> 4608 12.7 / 9.9
+// (by gemm8_k 10.6), 64 tokens 2304 -> 5120 5.9 / 5.3, 4096 -> 4096 6.7 / 7.5, 4096 -> 1536 5.3 / 6.6
+constexpr int S8_MOST = 128;
 struct Few8 { int rt; double us; };
 inline Few8 q8_few_rows(int N, int K, int T, int products)
 {
-    const int64_t tiles = (int64_t)((N + 15) / 16) * products, x = (T + 15) / 16;
-    auto cost = [&](int rt) { return ((tiles + rt - 1) / rt + 255) / 256 * (rt + x); };
-    const int rt = cost(2) < cost(1) ? 2 : 1;
-    return {rt, 3.0 + cost(rt) * 0.28 * K / 1024};
+    auto us = [&](int rt) {
+        const double w = (double)(((N + 15) / 16 * products + rt - 1) / rt) / 256;
+        const int whole = (int)w;
+        const double rounds = w > whole ? whole + 0.5 + 0.5 * (w - whole) : w, first = rt == 1 ? 0.07 : 0.13;
+        return 2.6 + (rt + (T + 15) / 16) * (K / 1024.0) * (w <= 1.0 ? first + 0.13 * w : (first + 0.13) * rounds);
+    };
+    const int rt = T <= 80 && us(2) < us(1) ? 2 : 1;
+    return {rt, us(rt)};
 }
 
-// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 64 where it is planned sooner (64 tokens
-// 4096 -> 4096 8.1 us, by gemm8_k 9.9; 77 tokens 4096 -> 14336 19.4 / 17.0), else gemm8_k
+// A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 128 where it is planned sooner than gemm8_k
+// (33 tokens 5120 -> 2304 5.5 us, by gemm8_k 8.2; 96 tokens 8.2 / 11.6; 64 tokens 4096 -> 11008 13.6 / 11.0), which reads W no faster than
+// HBM does
 inline bool q8_few(int N, int K, int T, int products)
 {
-    return T <= 16 || (T <= 64 && q8_few_rows(N, K, T, products).us <= q8_plan(N, K, T, products).us);
+    if (T <= 16 || T > S8_MOST) return T <= 16;
+    return q8_few_rows(N, K, T, products).us <= std::max(q8_plan(N, K, T, products).us, 1.0 + (double)N * K * products / 5.0e6);
 }
 
 inline int padded(int n) { return (n + 7) / 8 * 8; }

@@ -29,16 +29,26 @@ int check_rows8(const bmx_q8* rows, int T, int K, const char* who)
     return BMX_OK;
 }
 
+// Piece i of the blocks' 16 codes each: of row n, columns k .. k + 15. A wave has a block: one piece of the codes, 64 columns of 16 rows
+struct Piece8 { int64_t n; int k; };
+__device__ __forceinline__ Piece8 piece8(int64_t i, int blocks)
+{
+    const int64_t b = i >> 6;
+    const int j = (int)i & 63;
+    return {b / blocks * Q8_ROWS + (j & 15), (int)(b % blocks) * Q8_COLS + (j >> 4) * 16};
+}
+
 // v = scale code (scale null: the codes themselves); 16 codes a thread, of one row
-__global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int K, int type,
+__global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int N, int K, int type,
                                                     void* __restrict__ out, int64_t pieces)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
-    const int per = (K + 15) / 16;
-    const int64_t n = i / per;
-    const int k = (int)(i % per) * 16;
-    const u32x4 c = ldg4(codes + q8_at(n, k, q8_blocks(K)));
+    const Piece8 at = piece8(i, q8_blocks(K));
+    const int64_t n = at.n;
+    const int k = at.k;
+    if (n >= N || k >= K) return;
+    const u32x4 c = ldg4(codes + i * 16);
     const float s = scale ? scale[n] : 1.0f;
 #pragma unroll
     for (int e = 0; e < 16; ++e)
@@ -53,13 +63,15 @@ __global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ c
 }
 
 // Row-major codes into blocks: 16 a thread, zeros past K
-__global__ __launch_bounds__(256) void q8_pack_k(const int8_t* __restrict__ in, int K, bool whole, int8_t* __restrict__ codes, int64_t pieces)
+__global__ __launch_bounds__(256) void q8_pack_k(const int8_t* __restrict__ in, int N, int K, bool whole, int8_t* __restrict__ codes,
+                                                 int64_t pieces)
 {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
-    const int per = q8_blocks(K) * (Q8_COLS / 16);
-    const int64_t n = i / per;
-    const int k = (int)(i % per) * 16;
+    const Piece8 at = piece8(i, q8_blocks(K));
+    const int64_t n = at.n;
+    const int k = at.k;
+    if (n >= N) return;
     u32x4 c = {0, 0, 0, 0};
     if (whole)                                                     // rows of whole aligned pieces (54 -> 15 us for 4096 x 11008)
     {
@@ -69,12 +81,12 @@ __global__ __launch_bounds__(256) void q8_pack_k(const int8_t* __restrict__ in, 
 #pragma unroll
         for (int e = 0; e < 16; ++e)
             if (k + e < K) c[e / 4] |= (uint32_t)(uint8_t)in[n * K + k + e] << (8 * (e % 4));
-    *reinterpret_cast<u32x4*>(codes + q8_at(n, k, q8_blocks(K))) = c;
+    *reinterpret_cast<u32x4*>(codes + i * 16) = c;
 }
 
-static int q8_whole(const char* fn, const bmx_q8* q, int per, int64_t* pieces)
+static int q8_whole(const char* fn, const bmx_q8* q, int64_t* pieces)
 {
-    *pieces = (int64_t)q->N * per;
+    *pieces = (int64_t)(q8_bytes(q->N, q->K) / 16);
     if (*pieces > (int64_t)1 << 31) return set_error(BMX_ERR_ARG, "%s: %d x %d values are too many for one call", fn, q->N, q->K);
     return BMX_OK;
 }
@@ -91,11 +103,12 @@ template <int IN, int NS, int TT, int RT, int EPI> static int skinny8_launch(con
 
 template <int TT, int EPI> static int skinny8_codes(const Q8Args& a, hipStream_t s)
 {
-    return q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1).rt == 2 ? skinny8_launch<IN_CODES, 1, TT, 2, EPI>(a, s)
-                                                                      : skinny8_launch<IN_CODES, 1, TT, 1, EPI>(a, s);
+    if constexpr (TT <= 5)
+        if (q8_few_rows(a.N, a.K, a.T, EPI == EPI_GU ? 2 : 1).rt == 2) return skinny8_launch<IN_CODES, 1, TT, 2, EPI>(a, s);
+    return skinny8_launch<IN_CODES, 1, TT, 1, EPI>(a, s);
 }
 
-// (the workgroups that quantize read the tokens once each, whatever their rows of W: 16 of them)
+// (the workgroups that quantize take 16 rows of W: what they read of the tokens is little)
 template <int IN, int EPI> static int skinny8_values(const Q8Args& a, hipStream_t s)
 {
     return skinny8_pieces(a.T, a.K) <= S8_W ? skinny8_launch<IN, 1, 1, 1, EPI>(a, s) : skinny8_launch<IN, 4, 1, 1, EPI>(a, s);
@@ -115,7 +128,11 @@ template <int EPI> static int skinny8_tokens(const Q8Args& a, hipStream_t s)
         case 1: return skinny8_codes<1, EPI>(a, s);
         case 2: return skinny8_codes<2, EPI>(a, s);
         case 3: return skinny8_codes<3, EPI>(a, s);
-        default: return skinny8_codes<4, EPI>(a, s);
+        case 4: return skinny8_codes<4, EPI>(a, s);
+        case 5: return skinny8_codes<5, EPI>(a, s);
+        case 6: return skinny8_codes<6, EPI>(a, s);
+        case 7: return skinny8_codes<7, EPI>(a, s);
+        default: return skinny8_codes<8, EPI>(a, s);
     }
 }
 
@@ -319,18 +336,18 @@ int bmx_q8_pack(const bmx_q8* q, const void* codes, bmx_stream_t stream)
     int64_t pieces = 0;
     if (const int rc = check_q8(q, fn)) return rc;
     if (!codes) return set_error(BMX_ERR_ARG, "%s: codes are null", fn);
-    if (const int rc = q8_whole(fn, q, q8_blocks(q->K) * (Q8_COLS / 16), &pieces)) return rc;
+    if (const int rc = q8_whole(fn, q, &pieces)) return rc;
     hipLaunchKernelGGL(q8_pack_k, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const int8_t*>(codes), q->K, q->K % 16 == 0 && !odd16(codes), static_cast<int8_t*>(const_cast<void*>(q->codes)), pieces);
+                       static_cast<const int8_t*>(codes), q->N, q->K, q->K % 16 == 0 && !odd16(codes), static_cast<int8_t*>(const_cast<void*>(q->codes)), pieces);
     return check_launch(fn);
 }
 
 static int dequant_call(const char* fn, const bmx_q8* q, const float* scale, int dtype, void* out, bmx_stream_t stream)
 {
     int64_t pieces = 0;
-    if (const int rc = q8_whole(fn, q, (q->K + 15) / 16, &pieces)) return rc;
+    if (const int rc = q8_whole(fn, q, &pieces)) return rc;
     hipLaunchKernelGGL(q8_dequant_k, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const int8_t*>(q->codes), scale, q->K, dtype, out, pieces);
+                       static_cast<const int8_t*>(q->codes), scale, q->N, q->K, dtype, out, pieces);
     return check_launch(fn);
 }
 

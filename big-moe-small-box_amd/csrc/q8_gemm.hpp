@@ -1,8 +1,8 @@
 // Products of 8-bit integers: y[t][n] = sx[t] sw[n] sum_k a[t][k] c[n][k], the sum exact in int32 (K <= 131,071), so that a result
 // does not depend on tiles, splits or the tokens beside it. Both factors lie in blocks of 16 rows x 64 columns (rows8.hpp).
 //
-// skinny8_k: to 64 tokens, bound by the bytes of W. A workgroup has 16 or 32 rows of W (half of gate and half of up in the gated
-// product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
+// skinny8_k: to 128 tokens, bound by the bytes of W and by what a compute unit takes in. A workgroup has 16 or 32 rows of W (half of
+// gate and half of up in the gated product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
 // ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized by each workgroup itself while
 // its first loads of W are on their way, into LDS: one launch instead of two.
 // v_mfma_i32_16x16x64_i8: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 16 .. + 15; of the
@@ -39,8 +39,7 @@ struct Q8Args {
 
 inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
-// TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each.
-// IN: the tokens are codes, or 16-bit or fp32 rows to be quantized by pieces of 512 values, NS a wave (with the other type's and three
+// TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each. IN: the tokens are codes, or 16-bit or fp32 rows to be quantized by pieces of 512 values, NS a wave (with the other type's and three
 // more pieces' code in the kernel a token's call took 0.7 us longer: instructions are fetched from L2 too).
 enum Skinny8In { IN_CODES, IN_16, IN_32 };
 template <int IN, int NS, int TT, int RT, int EPI>
@@ -303,9 +302,9 @@ __global__ __launch_bounds__(WM * WN * WK * 64) void gemm8_k(const Q8Args p)
         loaded += WK;
     };
     // 32 rows from row0, 32 columns from ks * 32: lane l holds row l % 32, columns (l / 32) * 16 .. + 15
+    const int frag_at = (lane >> 4 & 1) * Q8_BLOCK + (lane >> 5) * Q8_CHUNK + (lane & 15) * 16;
     auto frag = [&](lds_ptr at, int row0, int ks) -> i32x4 {
-        const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
-        return *(__attribute__((address_space(3))) i32x4*)(at + r * Q8_COLS + ((c ^ q8_swz(r)) << 4));
+        return *(__attribute__((address_space(3))) i32x4*)(at + row0 * Q8_COLS + ks * 2 * Q8_CHUNK + frag_at);
     };
     i32x16 acc[MF][NF];
 #pragma unroll
@@ -510,9 +509,9 @@ __global__ __launch_bounds__(512) void gemm8_big_k(const Q8Args p)
             seek();
         }
     };
+    const int frag_at = (lane >> 4 & 1) * Q8_BLOCK + (lane >> 5) * Q8_CHUNK + (lane & 15) * 16;
     auto frag = [&](lds_ptr at, int row0, int ks) -> i32x4 {
-        const int r = row0 + (lane & 31), c = ks * 2 + (lane >> 5);
-        return *(__attribute__((address_space(3))) i32x4*)(at + r * Q8_COLS + ((c ^ q8_swz(r)) << 4));
+        return *(__attribute__((address_space(3))) i32x4*)(at + row0 * Q8_COLS + ks * 2 * Q8_CHUNK + frag_at);
     };
     i32x16 acc[MF][NF];
     i32x4 a[2][MF], b[2][NF];

@@ -137,17 +137,16 @@ __device__ __forceinline__ uint32_t codes4(const float* v, const Top8& o)
     return lo | hi;
 }
 
-// Codes in blocks of 16 rows x 64 columns (bmx_q8): 1 KB, a fragment of v_mfma_i32_16x16x64_i8 or two halves of one of 32x32x32, so that
-// a wave's load is one contiguous piece whatever the row's length. (Row by row a wave's load is 64 bytes of each of 16 rows, for
-// K = 4096 all in one memory channel: 4,096 x 4,096 x 11,008 187 us, in blocks 175.) In a block a row's chunk c of 16 bytes lies at c ^
-// (row / 4 % 4): 16 rows' chunks c on all banks of LDS.
-constexpr int Q8_ROWS = 16, Q8_COLS = 64, Q8_BLOCK = Q8_ROWS * Q8_COLS;
+// Codes in blocks of 16 rows x 64 columns (bmx_q8): 1 KB, in the order in which v_mfma_i32_16x16x64_i8's lanes hold it (or two halves of
+// one of 32x32x32): chunk c of 16 columns of row r at c * 256 + r * 16, so that a wave's load is one contiguous piece whatever the row's
+// length. (Row by row a wave's load is 64 bytes of each of 16 rows, for K = 4096 all in one memory channel: 4,096 x 4,096 x 11,008 187 us,
+// in blocks 175. In blocks of rows of 64 bytes a compute unit takes fragments in at 74 bytes a nanosecond, this way at 115 to 140, since
+// its L1 gives 64 neighbouring bytes to four lanes at a time.)
+constexpr int Q8_ROWS = 16, Q8_COLS = 64, Q8_BLOCK = Q8_ROWS * Q8_COLS, Q8_CHUNK = Q8_ROWS * 16;
 __host__ __device__ constexpr int q8_blocks(int K) { return (K + Q8_COLS - 1) / Q8_COLS; }     // of a row of blocks
-__host__ __device__ constexpr int q8_swz(int row) { return (row >> 2) & 3; }
 __host__ __device__ constexpr int64_t q8_at(int64_t row, int k, int blocks)
 {
-    return (row / Q8_ROWS * blocks + k / Q8_COLS) * Q8_BLOCK + (row % Q8_ROWS) * Q8_COLS + (((k % Q8_COLS) >> 4) ^ q8_swz((int)(row % Q8_ROWS))) * 16 +
-           k % 16;
+    return (row / Q8_ROWS * blocks + k / Q8_COLS) * Q8_BLOCK + (k % Q8_COLS >> 4) * Q8_CHUNK + (row % Q8_ROWS) * 16 + k % 16;
 }
 inline size_t q8_bytes(int N, int K) { return (size_t)round_up(N, Q8_ROWS) * q8_blocks(K) * Q8_COLS; }
 

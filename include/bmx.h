@@ -541,8 +541,8 @@ int bmx_ffn_backward(const bmx_ffn_desc* desc, const void* x, int T, const bmx_f
 /* ---- 8-bit matrices and rows ----
  * N rows of K whole numbers (-128 .. 127) with a scale each, v[n][k] = scale[n] code[n][k], the form of 8-bit weights with a scale
  * per output channel (bmx_q8 as a matrix) and of activations with a scale per token (as rows, N tokens). A bmx_q8 holds the codes in
- * the kernels' order, bmx_q8_code_bytes bytes: blocks of 16 rows x 64 columns, [row / 16][column / 64], in a block each row's 64
- * bytes, its four 16-byte chunks c at place c ^ (row / 4 % 4); columns from K up to the next multiple of 64 are 0. scale fp32 [N].
+ * the kernels' order, bmx_q8_code_bytes bytes: blocks of 16 rows x 64 columns, [row / 16][column / 64], in a block the column's
+ * chunk of 16, then the row: [column / 16 % 4][row % 16][column % 16]; columns from K up to the next multiple of 64 are 0. scale fp32 [N].
  * Written by bmx_q8_pack from row-major codes, or by the calls that quantize. Device memory, codes 16-byte aligned. N to 2^24, K to
  * 131,071 (so that a sum of products fits 32 bits whatever the codes). */
 typedef struct bmx_q8 {

@@ -35,8 +35,8 @@ def check_rows(rows, y64, e):
     codes = rows.int8().double()
     assert bool((codes.abs().amax(1) == 127).all())
     R.check("rows", codes * scale[:, None], y64, scale[:, None] * (0.5 + 127 * 3 * Q.STEP) + e + y64.abs() * 3 * Q.STEP)
-    b = rows.codes.view(-1, (rows.K + 63) // 64, 16, 64)            # nothing but zeros behind a row, in whatever order
-    assert int((b != 0).sum((1, 3)).view(-1)[:rows.N].sum()) == int((codes != 0).sum())
+    b = rows.codes.view(-1, (rows.K + 63) // 64, 4, 16, 16)         # nothing but zeros behind a row: chunks of 16 columns, of 16 rows each
+    assert int((b != 0).sum((1, 2, 4)).view(-1)[:rows.N].sum()) == int((codes != 0).sum())
 
 
 @pytest.mark.parametrize("dt", sorted(DT))

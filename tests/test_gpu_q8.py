@@ -34,10 +34,7 @@ def values(rows):
 def check_padding(rows):
     """In the blocks, zeros behind each row; and the documented order."""
     N, K = rows.N, rows.K
-    b = rows.codes.view(-1, (K + 63) // 64, 16, 4, 16)
-    c = torch.arange(4, device=b.device)
-    r = torch.arange(16, device=b.device)
-    b = torch.stack([b[:, :, r, c[i] ^ (r // 4) % 4] for i in range(4)], 3)      # chunk c of row r at place c ^ (r / 4 % 4)
+    b = rows.codes.view(-1, (K + 63) // 64, 4, 16, 16).transpose(2, 3)           # [16 rows][64 columns]: chunks of 16 columns, of all rows each
     flat = b.permute(0, 2, 1, 3, 4).reshape(b.shape[0] * 16, -1)
     assert torch.equal(flat[:N, :K], rows.int8()) and not bool(flat[:N, K:].any())
 
