@@ -271,7 +271,7 @@ inline Few8 q8_few_rows(int N, int K, int T, int products)
 }
 
 // A product of T tokens with an N x K matrix (or two, side by side): skinny8_k to 16 tokens, to 128 where it is planned sooner than gemm8_k
-// (33 tokens 5120 -> 2304 5.5 us, by gemm8_k 8.2; 96 tokens 8.2 / 11.6; 64 tokens 4096 -> 11008 13.6 / 11.0), which reads W no faster than
+// (33 tokens 5120 -> 2304 5.6 us, by gemm8_k 8.4; 96 tokens 8.1 / 10.9; 64 tokens 4096 -> 11008 12.7 / 11.0), which reads W no faster than
 // HBM does
 inline bool q8_few(int N, int K, int T, int products)
 {
