@@ -204,8 +204,9 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 
 // ---- 8-bit weights ------------------------------------------------------------------------------------------------------
 
-// gemm8_k's tiles, as TILES, us a stage of 64 columns. What bounds the small ones is what a compute unit takes in, about 70 bytes a
-// nanosecond whatever the depth of loads: us of one round of a tile at K 4096, 64 x 64 10.1, 128 x 64 13.4, 128 x 128 17.2, 256 x 128 24.7.
+// gemm8_k's tiles, as TILES, us a stage of 64 columns; one round at K 4096: 64 x 64 10.1, 128 x 64 13.4, 128 x 128 17.2, 256 x 128 24.7.
+// Matrix units busy over a whole launch: 128 x 128 0.50, 256 x 128 0.63, 256 x 256 0.80; LDS a third in each, and a compute unit takes in
+// 50 to 74 of the 120 bytes a nanosecond that L2 gives it, whatever the depth of loads: the small ones wait at each stage's barrier.
 constexpr int Q8_TILES = 6;
 constexpr Tile TILES8[Q8_TILES] = {
     {256, 256, 256, 0.70, 0.86, 4.0},      // 8 waves, gemm8_big_k
