@@ -221,7 +221,7 @@ __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
             if (AHEAD && p.dr) dr[c] = load_raw8(p.dr, vt, i);
         }
     };
-    auto weight = [&](int c) { to_f32(load_raw8(p.w, wt, at(c)), p.wt, w); };
+    auto weight = [&](int c) { to_f32(load_raw8(p.w, wt, at(c)), wt, w); };
     int t = blockIdx.x;
     load(t);
     if (CH == 1 && at(0) < p.H) weight(0);
