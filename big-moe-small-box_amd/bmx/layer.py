@@ -328,8 +328,8 @@ class MoELayer:
             raise ValueError("MoELayer.block: the layer has no norm")
         self.norm._current()
         self._check_norm(self.norm, self.table)
-        if x.dim() != 2:
-            raise ValueError(f"MoELayer.block: x must be [T, {self.hidden_size}], got {tuple(x.shape)}")
+        if x.dim() != 2 or not x.shape[0]:
+            raise ValueError(f"MoELayer.block: x must be [T, {self.hidden_size}] of a token or more, got {tuple(x.shape)}")
         self._check_shared(None)
         self.norm.refuse_grad(x, residual)
         z, rows, r = self.norm._run(x, residual, True, self.shared_ffn is not None and self.shared_ffn.bits == 8)

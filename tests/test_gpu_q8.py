@@ -426,6 +426,7 @@ def test_a_layer_refuses_before_its_work(cuda):
     layer = bmx.MoELayer(tab, 4, shared_ffn=ffn, norm=norm, slots=slots)
     steps, rows = list(slots.seq), bmx.ops.quantize_rows(x)
     for f in (lambda: layer.forward(x[:4], lg[:4], rows=rows), lambda: layer.block(x.view(5, 1, 256), None, lg), lambda: layer.block(x, x[:3], lg),
+              lambda: layer.block(x[:0], None, lg[:0]),
               lambda: layer.block(x.bfloat16(), None, lg), lambda: layer.block(x.clone().requires_grad_(), None, lg),
               lambda: bmx.MoELayer(tab, 4, slots=slots).forward(x, lg, rows=rows)):
         with pytest.raises(ValueError):
