@@ -204,22 +204,31 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 
 // ---- 8-bit weights ------------------------------------------------------------------------------------------------------
 
-// gemm8_k's tiles, as TILES, us a stage of 64 columns; one round at K 4096: 64 x 64 10.1, 128 x 64 13.4, 128 x 128 17.2, 256 x 128 24.7.
+// gemm8_k's tiles, as TILES, us a stage of 64 columns and the ends of a launch (130 to 2,048 tokens, 768 to 11,008 columns: within 10 %).
 // Matrix units busy over a whole launch: 128 x 128 0.50, 256 x 128 0.63, 256 x 256 0.80; LDS a third in each, and a compute unit takes in
 // 50 to 74 of the 120 bytes a nanosecond that L2 gives it, whatever the depth of loads: the small ones wait at each stage's barrier.
 constexpr int Q8_TILES = 6;
 constexpr Tile TILES8[Q8_TILES] = {
-    {256, 256, 256, 0.70, 0.86, 4.0},      // 8 waves, gemm8_big_k
-    {128, 128, 512, 0.29, 0.52, 3.0},      // 4 waves, two on a compute unit
-    {128, 64, 256, 0.165, 0.18, 3.0},      // 2 groups of 4 waves, each every other stage
-    {128, 128, 256, 0.23, 0.28, 3.0},      // the same
-    {256, 128, 256, 0.44, 0.48, 3.0},      // 8 waves
-    {64, 64, 512, 0.13, 0.215, 2.0},       // 2 groups of 2 waves, two on a compute unit
+    {256, 256, 256, 0.50, 0.82, 7.3},      // 8 waves, gemm8_big_k
+    {128, 128, 512, 0.17, 0.50, 5.5},      // 4 waves, two on a compute unit
+    {128, 64, 256, 0.13, 0.15, 4.0},       // 2 groups of 4 waves, each every other stage
+    {128, 128, 256, 0.155, 0.26, 5.5},     // the same
+    {256, 128, 256, 0.265, 0.467, 6.5},    // 8 waves
+    {64, 64, 512, 0.081, 0.18, 3.6},       // 2 groups of 2 waves, two on a compute unit
 };
-constexpr bool splits8(int t) { return t == 2 || t == 3 || t == 5; }      // their K axis can be split: few results, where it pays
+constexpr int Q8_SPLIT = 5;         // the tile whose K axis can be split: it pays for few results
 
-// Tiles of a product with M x N results and stages of 64 columns, as plan_product: the joining kernel (5 us) and the sums' bytes cost
-// as much, and large tiles go ahead for as many rows of M as fill whole rounds
+// us of a stage of a tile with n of its workgroups at once: alone's with few, and more the more compute units have one (128 x 128 0.163,
+// 0.19, 0.206 and 0.27 with 64, 160, 192 and 256); with a second one on some, full's
+inline double stage8(const Tile& c, int64_t n)
+{
+    const double w = (double)n / 256, one = c.slots == 256 ? c.full : c.full / 2;
+    return n <= 256 ? c.alone + (one - c.alone) * w * w : c.full;
+}
+
+// Tiles of a product with M x N results and stages of 64 columns, as plan_product: the joining kernel (4.5 us) and the sums' bytes cost
+// as much (130 tokens 11008 -> 256 16.2 us, split 8.6; 11008 -> 4096 18.0, in two 25), and large tiles go ahead for as many rows of M as
+// fill whole rounds
 inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can_part = true)
 {
     TilePlan best = {0, 1, 0, 1e30};
@@ -227,13 +236,13 @@ inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can
     for (int t = 0; t < Q8_TILES; ++t)
         for (int s = 1; s <= 16; ++s)
         {
-            if (s > 1 && (!can_split || !splits8(t) || stages / s < 8)) break;
+            if (s > 1 && (!can_split || t != Q8_SPLIT || stages / s < 8)) break;
             const Tile& c = TILES8[t];
             const int64_t b = (M + c.M - 1) / c.M * ((N + c.N - 1) / c.N) * s, full = b / c.slots, rest = b % c.slots;
             const int each = (stages + s - 1) / s;
             double us = full * (each * c.full + c.ends);
-            if (rest) us += each * (rest <= 256 ? c.alone : c.full) + c.ends;
-            if (s > 1) us += 5.0 + (double)M * N * s * 8.0 / 4e6;
+            if (rest) us += each * stage8(c, rest) + c.ends;
+            if (s > 1) us += 4.5 + (double)M * N * s * 8.0 / 4e6;
             if (us < best.us) best = {t, s, 0, us};
         }
     const int64_t tn = (N + 255) / 256, rounds = (M + 255) / 256 * tn / 256, head = rounds * 256 / tn * 256;

@@ -148,12 +148,14 @@ template <int EPI, int OT> static int gemm8_tiles(Q8Args a, int tile, hipStream_
             hipLaunchKernelGGL((gemm8_big_k<EPI, OT>), dim3(std::min(grid.x, (unsigned)TILES8[0].slots)), dim3(512), 0, s, a);
         else if (tile == 1)
             hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 1, 4, EPI, OT>), grid, dim3(256), 0, s, a);
+        else if (tile == 2)
+            hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
+        else if (tile == 3)
+            hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
         else if (tile == 4)
             hipLaunchKernelGGL((gemm8_k<256, 128, 4, 2, 1, 4, EPI, OT>), grid, dim3(512), 0, s, a);
     }
-    if (tile == 2) hipLaunchKernelGGL((gemm8_k<128, 64, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
-    if (tile == 3) hipLaunchKernelGGL((gemm8_k<128, 128, 2, 2, 2, 4, EPI, OT>), grid, dim3(512), 0, s, a);
-    if (tile == 5) hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI, OT>), grid, dim3(256), 0, s, a);
+    if (tile == Q8_SPLIT) hipLaunchKernelGGL((gemm8_k<64, 64, 1, 2, 2, 4, EPI, OT>), grid, dim3(256), 0, s, a);
     return check_launch("gemm8");
 }
 
