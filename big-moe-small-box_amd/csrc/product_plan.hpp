@@ -263,7 +263,7 @@ inline int skinny8_pieces(int T, int K) { return T * ((K + 511) / 512); }
 inline bool skinny8_fused(int T, int K) { return T <= 16 && K % 8 == 0 && skinny8_pieces(T, K) <= S8_SLOTS; }
 
 // skinny8_k, tiles of 16 rows of W per workgroup, 1 or 2 (to 80 tokens): a workgroup takes in its rows of W and the tokens; us for 1,024
-// columns of 16 of them are 0.07 alone and 0.20 when every compute unit has a workgroup (of 32 rows, more of them from HBM: 0.13 and
+// columns of 16 of them are 0.10 alone and 0.20 when every compute unit has a workgroup (of 32 rows, more of them from HBM: 0.13 and
 // 0.26), and of more workgroups than units some have one more, which is the last to end. us with 1 / 2: 77 tokens 5120 -> 4608 12.7 / 9.9
 // (by gemm8_k 10.6), 64 tokens 2304 -> 5120 5.9 / 5.3, 4096 -> 4096 6.7 / 7.5, 4096 -> 1536 5.3 / 6.6
 constexpr int S8_MOST = 128;
@@ -273,8 +273,8 @@ inline Few8 q8_few_rows(int N, int K, int T, int products)
     auto us = [&](int rt) {
         const double w = (double)(((N + 15) / 16 * products + rt - 1) / rt) / 256;
         const int whole = (int)w;
-        const double rounds = w > whole ? whole + 0.5 + 0.5 * (w - whole) : w, first = rt == 1 ? 0.07 : 0.13;
-        return 2.6 + (rt + (T + 15) / 16) * (K / 1024.0) * (w <= 1.0 ? first + 0.13 * w : (first + 0.13) * rounds);
+        const double rounds = w > whole ? whole + 0.5 + 0.5 * (w - whole) : w, first = rt == 1 ? 0.10 : 0.13;
+        return 2.6 + (rt + (T + 15) / 16) * (K / 1024.0) * first * (w <= 1.0 ? 1.0 + w : 2.0 * rounds);
     };
     const int rt = T <= 80 && us(2) < us(1) ? 2 : 1;
     return {rt, us(rt)};
