@@ -66,3 +66,23 @@ def test_more_rows_than_an_axis_of_a_launch_holds(cuda, T, K):
         assert torch.equal(r, x + x)
         R.check("y", y, y64, R.rounded(y64, 2.0 ** -20 * y64.abs(), y.dtype))
         assert torch.equal(rows.int8().double(), torch.round(v * 127.0 / v.abs().amax(1, keepdim=True)))
+
+
+def test_more_than_2_to_31_codes(cuda):
+    """A matrix, and tokens, whose codes lie past 32 bits: the last rows' results are those of a matrix of them alone, bit for bit."""
+    import bmx
+    n, K, few = 540000, 4096, 70
+    codes = torch.randint(-128, 128, (n, K), device=cuda, dtype=torch.int8)
+    scale = (torch.rand(n, device=cuda) + 0.2) / 4096
+    big, last = bmx.Q8Matrix(codes, scale), bmx.Q8Matrix(codes[-few:].contiguous(), scale[-few:].contiguous())
+    assert torch.equal(big.int8()[-few:], codes[-few:])
+    rows = bmx.Rows8(codes, scale, torch.bfloat16)
+    del codes
+    for T in (1, 16, 40, 130, 300):
+        x = rand(cuda, T, K, dt=torch.bfloat16, seed=T)
+        assert torch.equal(bmx.ops.q8_linear(x, big)[:, -few:], bmx.ops.q8_linear(x, last))
+    del big
+    tail = bmx.Rows8(last.int8(), last.scale, torch.bfloat16)
+    for N in (8, 70, 300):
+        q = bmx.Q8Matrix.quantize(torch.randn((N, K), device=cuda) / 64)
+        assert torch.equal(bmx.ops.q8_linear(rows, q)[-few:], bmx.ops.q8_linear(tail, q))
