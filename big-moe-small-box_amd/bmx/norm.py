@@ -148,17 +148,23 @@ class _RMSNormFunction(torch.autograd.Function):
         v = x if r is None else r
         ctx.save_for_backward(weight, v)
         # (the descriptor holds the weight's address: asked for again below)
-        ctx.desc, ctx.xt, ctx.summed = norm._desc(x.dtype, v.dtype), x.dtype, r is not None
+        ctx.desc, ctx.weight, ctx.device = norm._desc(x.dtype, v.dtype), weight, norm.device
+        ctx.xt, ctx.vt, ctx.summed, ctx.shape = x.dtype, v.dtype, r is not None, v.shape
         return y, r
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dr):
         weight, v = ctx.saved_tensors
-        d, dev, xt, rt, summed = ctx.desc, v.device, ctx.xt, v.dtype, ctx.summed
+        d, dev, xt, rt, summed = ctx.desc, ctx.device, ctx.xt, ctx.vt, ctx.summed
         H = d.contents.H
-        if weight.data_ptr() != d.contents.weight or weight.shape != (H,) or not weight.is_contiguous():
-            raise RuntimeError("RMSNorm: the weight was replaced between the forward and the backward pass")
+        # (what hooks give back of the weight lies elsewhere; the weight itself does where its data was replaced)
+        if weight.shape != (H,) or ROW_DTYPES.get(weight.dtype) != d.contents.weight_dtype or weight.device != dev or \
+                (weight is ctx.weight and (weight.data_ptr() != d.contents.weight or not weight.is_contiguous())):
+            raise RuntimeError("RMSNorm: the weight was replaced between the forward and the backward pass, or hooks gave its saved value back "
+                               f"as {weight.dtype} {tuple(weight.shape)} on {weight.device}")
+        if v.dtype is not rt or v.device != dev or v.shape != ctx.shape:
+            raise RuntimeError(f"RMSNorm: hooks gave the saved rows back as {v.dtype} {tuple(v.shape)} on {v.device}")
         s = stream_here(dev)
         if s is None:                           # autograd's threads have a current device of their own
             with torch.cuda.device(dev):
@@ -166,7 +172,10 @@ class _RMSNormFunction(torch.autograd.Function):
         nx, nr, nw, _ = ctx.needs_input_grad
         if dy is None:                          # r alone was used (or neither)
             return dr.to(xt) if nx and dr is not None else None, dr if nr else None, torch.zeros_like(weight) if nw else None, None
-        v, dy = _dense(v), _dense(dy)
+        v, dy, weight = _dense(v), _dense(dy), _dense(weight)
+        if weight.data_ptr() != d.contents.weight:
+            c = d.contents
+            d = L.NormDesc(c.H, c.dtype, c.x_dtype, c.residual_dtype, c.weight_dtype, c.eps, weight.data_ptr())
         if dr is not None:
             dr = _dense(dr)
         one = summed and rt is xt               # x's and residual's gradients are the same values
