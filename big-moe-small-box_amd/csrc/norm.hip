@@ -358,6 +358,30 @@ static int check_norm(const bmx_norm_desc* d, int T, const char* who)
     return BMX_OK;
 }
 
+// Outputs on inputs or on each other. A row's workgroup reads it whole before it writes: an output of the same type may lie where
+// the input lies, but for another type, or rows further on, it would be on rows that other workgroups have yet to read.
+struct Place { const void* at; size_t bytes; };
+static bool meet(const Place& a, const Place& b)
+{
+    const uintptr_t p = reinterpret_cast<uintptr_t>(a.at), q = reinterpret_cast<uintptr_t>(b.at);
+    return p && q && p < q + b.bytes && q < p + a.bytes;
+}
+static bool norm_overlaps(const NormArgs& a)
+{
+    const size_t n = (size_t)a.T * a.H, r = n * row_type_bytes(a.rt);
+    const Place x = {a.x, n * row_type_bytes(a.xt)}, res = {a.res, r}, w = {a.w, a.H * row_type_bytes(a.wt)}, sum = {a.r, r},
+                y = {a.y, n * row_type_bytes(a.yt)}, codes = {a.codes, q8_bytes(a.T, a.H)}, scale = {a.scale, (size_t)a.T * 4};
+    if (meet(sum, x) && !(sum.at == x.at && a.rt == a.xt)) return true;
+    if (meet(sum, res) && sum.at != res.at) return true;
+    if (meet(y, x) && !(y.at == x.at && a.yt == a.xt)) return true;
+    if (meet(y, res) || meet(y, sum) || meet(codes, scale)) return true;
+    for (const Place& o : {sum, y})
+        if (meet(o, w) || meet(o, codes) || meet(o, scale)) return true;
+    for (const Place& i : {x, res, w})
+        if (meet(i, codes) || meet(i, scale)) return true;
+    return false;
+}
+
 // zeros for the weight's gradient of no rows
 __global__ __launch_bounds__(256) void norm_zero_k(uint32_t* p, int n)
 {
@@ -394,6 +418,7 @@ int bmx_rms_norm(const bmx_norm_desc* desc, const void* x, const void* residual,
     a.T = T; a.H = desc->H;
     a.xt = desc->x_dtype; a.rt = desc->residual_dtype; a.wt = desc->weight_dtype; a.yt = desc->dtype;
     a.eps = desc->eps;
+    if (norm_overlaps(a)) return set_error(BMX_ERR_ARG, "%s: sum, y or rows overlap an input or each other", fn);
     return launch_norm(a, static_cast<hipStream_t>(stream));
 }
 

@@ -586,8 +586,9 @@ int bmx_ffn8_add(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, i
 /* ---- root-mean-square norm with the residual's addition ----
  * With a residual: sum = x + residual in fp32, rounded to residual's type, and v = sum; without: v = x. y = v w / sqrt(mean(v^2) +
  * eps), rounded once to dtype; rows: the same in 8 bits with a scale per token (rows->N = T, K = H), not through y: code = round(v w
- * 127 / max |v w|). x, residual and the weight [H] of dtype or fp32, contiguous, 16-byte aligned; H a multiple of 8. sum may be
- * residual or x, if of its type; y apart from all but x. sum goes with residual; y or rows may be NULL. */
+ * 127 / max |v w|). x, residual and the weight [H] of dtype or fp32, contiguous, 16-byte aligned; H a multiple of 8. sum goes with
+ * residual; y or rows may be NULL. In place: sum may be residual, or x if x is of residual's type; y may be x if x is of dtype and
+ * sum is not there. Outputs that overlap inputs or each other in another way are refused. */
 #define BMX_NORM_MAX_H 16384
 typedef struct bmx_norm_desc {
     int32_t H, dtype;                              /* dtype: fp16 or bf16 */
