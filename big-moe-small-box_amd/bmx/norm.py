@@ -41,7 +41,7 @@ class RMSNorm:
         if out not in DTYPES or w.dtype not in (out, torch.float32):
             raise ValueError(f"RMSNorm: y must be fp16 or bf16 and the weight of that type or fp32, got {out} and {w.dtype}")
         # (what fp32 makes of it: the kernels get it so)
-        if not 2.0 ** -149 <= eps < float("inf"):
+        if not 2.0 ** -149 <= eps <= torch.finfo(F32).max:
             raise ValueError(f"RMSNorm: eps must be positive and finite, got {eps}")
         self._out, self.hidden_size, self.device = out, w.shape[0], w.device
         self._checked = (w, eps, dtype, w.data_ptr(), w.dtype, w.shape[0])

@@ -8,6 +8,7 @@
 // (the rounding of s to r passes a gradient as it is). Everything is bound by the bytes of the rows: each is read once and kept in
 // registers, and rstd is computed again from them in the backward pass, which has to read v anyhow.
 #include <algorithm>
+#include <cfloat>
 
 #include "rows8.hpp"
 
@@ -352,7 +353,7 @@ static int check_norm(const bmx_norm_desc* d, int T, const char* who)
     for (int t : {d->x_dtype, d->residual_dtype, d->weight_dtype})
         if (t != d->dtype && t != BMX_DT_FP32)
             return set_error(BMX_ERR_ARG, "%s: x, residual and weight must be of dtype or fp32, got %d beside %d", who, t, d->dtype);
-    if (!(d->eps > 0.0f)) return set_error(BMX_ERR_ARG, "%s: eps must be positive", who);
+    if (!(d->eps > 0.0f && d->eps <= FLT_MAX)) return set_error(BMX_ERR_ARG, "%s: eps must be positive and finite", who);
     if (!d->weight || odd16(d->weight)) return set_error(BMX_ERR_ARG, "%s: weight null or not 16-byte aligned", who);
     if (T < 0 || T > (1 << 24)) return set_error(BMX_ERR_ARG, "%s: T (%d) outside [0, 2^24]", who, T);
     return BMX_OK;
