@@ -117,8 +117,10 @@ __device__ __forceinline__ Top8 top8(uint32_t top)
 
 // Four codes: adding 1.5 * 2^23 leaves the whole number n nearest to v inv in the low bits, as a two's complement byte. Rows of
 // 16-bit values hold true ties, v = top / 2 first of all (63.5, about one in each row), which inv's rounding would send up or down;
-// 127 v - n top, scaled by 2^-7 and exact for them, says so, and the even neighbour is taken. Their other values are at least 2^-12
-// from a border, further than v inv is off (2^-17): their codes are those of the exact quotients. (Another code here and there in x
+// 127 v - n top, scaled by 2^-7 and exact for them, says so, and the even neighbour is taken. The codes of their other values are those
+// of the exact quotients too: with v = a 2^-d and top = b, significands as whole numbers below 2^11, 127 v / top is |254 a - m b 2^d|
+// / (b 2^(d + 1)) from the border m / 2 (m odd), where the upper part is 1 at least, and 2 for d > 0: 2^-12 or 2^-(11 + d). v inv is below
+// 2^(8 - d) (127 for d = 0) and off by half a step of inv, less than 2^-17 or 2^-(16 + d). (Another code here and there in x
 // moves one h in a hundred to its neighbour behind the next quantization: a block's error against 64 bits was 0.0053 of the norm for
 // it, 0.0017 without.) inv 0 stands for rows of zeros, and for rows that hold a NaN or an infinity: codes 0 whatever they hold.
 __device__ __forceinline__ uint32_t codes4(const float* v, const Top8& o)
