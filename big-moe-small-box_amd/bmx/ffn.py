@@ -125,7 +125,7 @@ class GatedFFN:
     @staticmethod
     def _check_tensors(gate, up, down):
         if not all(torch.is_tensor(w) for w in (gate, up, down)):
-            raise ValueError("GatedFFN: three tensors or three Q4Matrix")
+            raise ValueError("GatedFFN: three tensors, three Q4Matrix or three Q8Matrix")
         if gate.dim() != 2 or gate.dtype not in DTYPES:
             raise ValueError(f"GatedFFN: gate must be fp16 or bf16 [I, H], got {gate.dtype} {tuple(gate.shape)}")
         I, H = gate.shape

@@ -192,7 +192,7 @@ struct NormBackArgs {
     void *dx, *dres;                // null: not wanted
     float* part;                    // [workgroup][H], null: the weight's gradient is not wanted
     int T, H;
-    int vt, wt, yt, rt, xt;         // row types: v, w, dy, dr and dres, dx
+    int vt, wt, yt, xt;             // row types: v, dr and dres (of a sum v the residual's), w, dy, dx
     float eps;
 };
 
@@ -458,7 +458,7 @@ int bmx_rms_norm_backward(const bmx_norm_desc* desc, const void* v, int summed, 
     a.part = dweight ? static_cast<float*>(workspace) : nullptr;
     a.T = T; a.H = desc->H;
     a.vt = summed ? desc->residual_dtype : desc->x_dtype;
-    a.wt = desc->weight_dtype; a.yt = desc->dtype; a.rt = desc->residual_dtype; a.xt = desc->x_dtype;
+    a.wt = desc->weight_dtype; a.yt = desc->dtype; a.xt = desc->x_dtype;
     a.eps = desc->eps;
     const bool wide = a.vt == ROW_F32 || a.wt == ROW_F32 || a.xt == ROW_F32;
     const int groups = norm_back_groups(T, desc->H, wide);

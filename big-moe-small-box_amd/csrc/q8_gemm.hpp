@@ -2,9 +2,9 @@
 // does not depend on tiles, splits or the tokens beside it. Both factors lie in blocks of 16 rows x 64 columns (rows8.hpp).
 //
 // skinny8_k: to 128 tokens, bound by the bytes of W and by what a compute unit takes in. A workgroup has 16 or 32 rows of W (half of
-// gate and half of up in the gated product) and all tokens; its eight waves take every eighth block of columns straight from HBM to matrix operands, several blocks
-// ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized by each workgroup itself while
-// its first loads of W are on their way, into LDS: one launch instead of two.
+// gate and half of up in the gated product) and all tokens; its eight waves take every eighth block of columns straight from HBM to
+// matrix operands, several blocks ahead, with the tokens' blocks of the same columns from the caches. Few tokens' rows are quantized
+// by each workgroup itself while its first loads of W are on their way, into LDS: one launch instead of two.
 // v_mfma_i32_16x16x64_i8: A = 16 tokens, B = 16 rows of W: lane l holds token / row l % 16 and columns (l / 16) * 16 .. + 15; of the
 // result column (row of W) l % 16 and tokens (l / 16) * 4 .. + 3.
 //
@@ -39,7 +39,8 @@ struct Q8Args {
 
 inline size_t skinny8_lds(int T, int K) { return (size_t)T * (q8_blocks(K) * Q8_COLS + 16); }
 
-// TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each. IN: the tokens are codes, or 16-bit or fp32 rows to be quantized by pieces of 512 values, NS a wave (with the other type's and three
+// TT: tiles of 16 tokens; RT: tiles of 16 rows of W. In the gated product RT 1 is eight rows of gate and eight of up, RT 2 16 of each.
+// IN: the tokens are codes, or 16-bit or fp32 rows to be quantized by pieces of 512 values, NS a wave (with the other type's and three
 // more pieces' code in the kernel a token's call took 0.7 us longer: instructions are fetched from L2 too).
 enum Skinny8In { IN_CODES, IN_16, IN_32 };
 template <int IN, int NS, int TT, int RT, int EPI>
