@@ -39,7 +39,8 @@ __device__ __forceinline__ int64_t row_here(int T)
 // A workgroup a row, CH chunks of 8 values a lane: one to 4,096 values, two past them (8,192 rows of 5,120: ten waves of one chunk 72 us,
 // five of two 62). NORM false: the rows as they are in 8 bits alone. WIDE: some tensor is fp32, and a chunk's registers hold any type;
 // 16 bits alone need half of them (8,192 rows of 4,096, two tensors in and two out: 44 us, 6.0 TB/s; with any type's 50, of 16,384 190
-// and 271), and the quantizing form no sums and weight (4,096 x 4,096 a fourth less: 13.4 us).
+// and 271), and the quantizing form no sums and weight (4,096 x 4,096 a fourth less: 13.0 us). fp32
+// rows into a stream of 16 bits: 8,192 of 5,120 78 us, 5.4 TB/s.
 template <int CH, bool NORM, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_k(const NormArgs p)
 {
@@ -147,7 +148,8 @@ static int launch_norm(const NormArgs& a, hipStream_t s)                  // H <
     return check_launch("rms_norm");
 }
 
-// The same for any K and rows at any 2-byte boundary: a workgroup per row, read twice
+// The same for any K and rows at any 2-byte boundary: a workgroup per row, read twice, a value a lane at a time: loads issued, not bytes,
+// bound it (4,096 rows of 18,432 in fp32 152 us, in bf16 148; of 16,384 norm_k takes 65 for fp32's)
 __global__ __launch_bounds__(512) void quantize_any_k(const NormArgs p)
 {
     __shared__ uint32_t smax[8];
@@ -198,9 +200,9 @@ struct NormBackArgs {
 
 // A workgroup takes every gridDim.x-th row and keeps its rows' sums for the weight's gradient in registers, and for rows of one chunk a
 // lane the weight; the next row's loads are on their way while one is summed up. WIDE: some tensor is fp32. (Of 16 bits alone a chunk
-// takes half the registers, and 24 waves of one chunk fit a compute unit: 8,192 rows of 4,096 with the forward pass 94 us, as WIDE 117;
-// 4,096 of 16,384 206 and 384.) Two chunks of any type leave no registers for loads ahead and for what the first pass made of a row: AHEAD
-// false makes it again.
+// takes half the registers, and 24 waves of one chunk fit a compute unit: 8,192 rows of 4,096 with the forward pass 100 us, with an fp32
+// weight and so WIDE 114; 4,096 of 16,384 223 and 264.) Two chunks of any type leave no registers for loads ahead and for what the first
+// pass made of a row: AHEAD false makes it again.
 template <int CH, bool WIDE>
 __global__ __launch_bounds__(1024) void norm_back_k(const NormBackArgs p)
 {

@@ -205,8 +205,10 @@ inline ProductPath product_path(int N, int K, int T, int products, int group, bo
 // ---- 8-bit weights ------------------------------------------------------------------------------------------------------
 
 // gemm8_k's tiles, as TILES, us a stage of 64 columns and the ends of a launch (130 to 2,048 tokens, 768 to 11,008 columns: within 10 %).
-// Matrix units busy over a whole launch: 128 x 128 0.50, 256 x 128 0.63, 256 x 256 0.80; LDS a third in each, and a compute unit takes in
-// 50 to 74 of the 120 bytes a nanosecond that L2 gives it, whatever the depth of loads: the small ones wait at each stage's barrier.
+// Matrix units busy over a whole launch: 128 x 128 0.45, 256 x 128 0.63, 256 x 256 0.74 to 0.80; LDS 0.25 to 0.35, and a compute unit takes
+// in 50 to 74 of the 120 bytes a nanosecond that L2 gives it, whatever the depth of loads: the small ones wait at each stage's barrier.
+// Against every other kernel, tile and split at 152 sizes of 17 to 2,048 tokens the plan is 1 % over the best on the geometric mean, 15 %
+// at the worst (200 tokens 14336 -> 256 in 14 shares 11.5 us, in 8 10.0).
 constexpr int Q8_TILES = 6;
 constexpr Tile TILES8[Q8_TILES] = {
     {256, 256, 256, 0.50, 0.82, 7.3},      // 8 waves, gemm8_big_k
@@ -227,7 +229,7 @@ inline double stage8(const Tile& c, int64_t n)
 }
 
 // Tiles of a product with M x N results and stages of 64 columns, as plan_product: the joining kernel (4.5 us) and the sums' bytes cost
-// as much (130 tokens 11008 -> 256 16.2 us, split 8.6; 11008 -> 4096 18.0, in two 25), and large tiles go ahead for as many rows of M as
+// as much (130 tokens 11008 -> 256 16.2 us, split 8.5; 11008 -> 4096 18.0, in two 25), and large tiles go ahead for as many rows of M as
 // fill whole rounds
 inline TilePlan plan8(int64_t M, int64_t N, int stages, bool can_split, bool can_part = true)
 {

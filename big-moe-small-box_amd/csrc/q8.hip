@@ -38,7 +38,8 @@ __device__ __forceinline__ Piece8 piece8(int64_t i, int blocks)
     return {b / blocks * Q8_ROWS + (j & 15), (int)(b % blocks) * Q8_COLS + (j >> 4) * 16};
 }
 
-// v = scale code (scale null: the codes themselves); 16 codes a thread, of one row
+// v = scale code (scale null: the codes themselves); 16 codes a thread, of one row. For checks and conversions, in no model's call: each
+// value is a store of its own (4096 x 11008 to fp16 111 us, 1.2 TB/s; the codes 89)
 __global__ __launch_bounds__(256) void q8_dequant_k(const int8_t* __restrict__ codes, const float* __restrict__ scale, int N, int K, int type,
                                                     void* __restrict__ out, int64_t pieces)
 {

@@ -588,7 +588,8 @@ int bmx_ffn8_add(const bmx_ffn8_desc* desc, const void* x, const bmx_q8* rows, i
  * eps), rounded once to dtype; rows: the same in 8 bits with a scale per token (rows->N = T, K = H), not through y: code = round(v w
  * 127 / max |v w|). x, residual and the weight [H] of dtype or fp32, contiguous, 16-byte aligned; H a multiple of 8. sum goes with
  * residual; y or rows may be NULL. In place: sum may be residual, or x if x is of residual's type; y may be x if x is of dtype and
- * sum is not there. Outputs that overlap inputs or each other in another way are refused. */
+ * sum is not there. Outputs that overlap inputs or each other in another way are refused. eps is positive and finite. Squares are
+ * summed in fp32: a row whose sum overflows (a norm past 1.8e19) has y 0 and scale 0. */
 #define BMX_NORM_MAX_H 16384
 typedef struct bmx_norm_desc {
     int32_t H, dtype;                              /* dtype: fp16 or bf16 */
